@@ -177,6 +177,12 @@ def _cache(g, lead, pages, c):
     return kv[0], kv[1], sc[0], sc[1]
 
 
+def _handle(s):
+    """The framework's handle of the cache, which a program keeps as long as the cache."""
+    if own:
+        s["kv"] = _ops().KVCacheInt8(*s["cache"])
+
+
 def _parents(g, b, t, tree):
     if tree == "chain":
         p = torch.arange(t, device="cuda") - 1
@@ -291,6 +297,8 @@ def prepare(c, seed):
         s["q"] = qz if c["drafts"] else None
         s["u"] = torch.rand((b, t), generator=g, device="cuda")
         s["e"] = torch.empty((b, v), device="cuda").exponential_(generator=g)
+    if "cache" in s:
+        _handle(s)
     return s
 
 
@@ -308,19 +316,19 @@ def _own(s, c):
         q, k, v = s["qkv"].split([c["hq"], c["hk"], c["hk"]], dim=2)
         out = {}
         if c["rot"]:
-            out["q"] = ops.rotary_kv_write_int8(q, k, v, s["pos"], s["plan"], s["cache"], s["table"], s["start"])
+            out["q"] = ops.rotary_kv_write_int8(q, k, v, s["pos"], s["plan"], s["kv"], s["table"], s["start"])
         else:
-            ops.kv_write_int8(k, v, s["cache"], s["table"], s["start"])
-        out["k"], out["v"] = ops.kv_read_int8(s["cache"], s["table"], s["start"], c["t"], dtype=DT[c["dt"]])
+            ops.kv_write_int8(k, v, s["kv"], s["table"], s["start"])
+        out["k"], out["v"] = ops.kv_read_int8(s["kv"], s["table"], s["start"], c["t"], dtype=DT[c["dt"]])
         out["ks"], out["vs"] = s["cache"][2:]
         return out
     if op == "read":
-        return ops.kv_read_int8(s["cache"], s["table"], None, c["ctx"], lens=s["lens"], dtype=DT[c["dt"]])
+        return ops.kv_read_int8(s["kv"], s["table"], None, c["ctx"], lens=s["lens"], dtype=DT[c["dt"]])
     if op == "move":
-        ops.kv_move_int8(s["cache"], s["table"], s["start"], s["path"], s["n"])
-        return ops.kv_read_int8(s["cache"], s["table"], s["start"], c["t"], dtype=DT[c["dt"]])
+        ops.kv_move_int8(s["kv"], s["table"], s["start"], s["path"], s["n"])
+        return ops.kv_read_int8(s["kv"], s["table"], s["start"], c["t"], dtype=DT[c["dt"]])
     if op == "attention":
-        return ops.tree_attention_int8(s["q"], s["cache"], s["table"], s["lens"], s["mask"])
+        return ops.tree_attention_int8(s["q"], s["kv"], s["table"], s["lens"], s["mask"])
     return ops.verify_tree(s["p"], s["tokens"], s["parents"], s["u"], s["e"], draft_probs=s["q"])
 
 
