@@ -83,6 +83,22 @@ SIGNATURES = {
                                          _I64, _I64, _I64, _P, _c.c_size_t, _P]),
     "bw_quantize_kv_int8": (_c.c_int, [_P, _I64, _I64, _I64, _P, _I64, _P, _P]),
     "bw_dequantize_kv_int8": (_c.c_int, [_P, _I64, _P, _I64, _I64, _P, _I64, _P]),
+    "bw_rotary": (_c.c_int, [_P, _I64, _I64, _I64, _c.c_int, _P, _I64, _I64, _I64, _c.c_int, _P, _P, _c.c_int, _I64,
+                             _I64, _I64, _P, _c.c_int, _P, _c.c_float, _I64, _c.c_int, _P]),
+    "bw_rotary_kv_write_int8": (_c.c_int, [_P, _I64, _I64, _I64, _c.c_int, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64,
+                                           _P, _c.c_int, _I64, _I64, _P, _c.c_int, _P, _c.c_float, _I64, _c.c_int,
+                                           _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _P]),
+    "bw_kv_read_int8": (_c.c_int, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _I64,
+                                   _P, _P, _c.c_int, _P]),
+    "bw_kv_move_int8": (_c.c_int, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _P,
+                                   _I64, _I64, _P]),
+    "bw_tree_positions": (_c.c_int, [_P, _I64, _P, _I64, _I64, _P, _P, _P]),
+    "bw_tree_attention_int8_workspace_size": (_c.c_size_t, [_I64, _I64, _I64, _I64, _I64]),
+    "bw_tree_attention_int8_workspace_zeroed_bytes": (_c.c_size_t, [_I64, _I64, _I64, _I64, _I64]),
+    "bw_tree_attention_int8": (_c.c_int, [_P, _I64, _I64, _I64, _c.c_int, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64,
+                                          _P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _c.c_float, _P, _c.c_size_t,
+                                          _P]),
+    "bw_verify_tree": (_c.c_int, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _P, _P]),
     "bw_set_wait_limit_ns": (_c.c_int, [_c.c_uint64]),
     "bw_get_wait_limit_ns": (_c.c_int, [_c.POINTER(_c.c_uint64)]),
     "bw_trace_enable": (_c.c_int, [_P, _c.c_size_t]),

@@ -1,0 +1,422 @@
+// Rotary positions and the paged int8 KV cache: rotate, quantise as written, read back, move.
+//
+// Rotation.  Pair i of a head's first `rot` elements turns by the angle theta = pos * f_i:
+//   (a, b) -> m (a cos theta - b sin theta, a sin theta + b cos theta)
+// with pairs (i, i + rot/2) (half) or (2i, 2i + 1) (interleaved).  f_i comes as a 64-bit fixed-point
+// number of turns per position, round(f_i / 2 pi * 2^64), so pos * step modulo 2^64 is the angle's
+// fraction of a turn with no range reduction and no rounding: at position 131071 a fp32 product
+// pos * f_i is off by up to 4e-3 radians, this by 2e-7 (the fraction's own rounding to fp32).
+// No sine table is read; the sines cost one sincospi per pair and token.
+//
+// Quantisation.  One fp32 scale per token and head, s = max|x| / 127 (NaN ignored, 0 for a row of
+// zeros), code = clamp(rne(x / s), +-127) with the IEEE quotient (NaN -> 0).  Rotated keys are
+// quantised from their 32-bit values: rounding them to 16 bits first would add an error of the
+// order of a bf16 ulp to codes of 1/127 of the row's maximum.
+#include <stdio.h>
+
+#include "kv_cache.cuh"
+#include "quant_math.cuh"
+
+namespace bw {
+
+int check_kv_cache(const KvCache& c, int64_t b, const char* op) {
+  if (c.pages < 0 || c.heads < 1 || c.page < 1 || c.d < 1 || c.d > kKvMaxDim)
+    return fail(BW_ERR_INVALID_ARGUMENT, "%s: need pages >= 0, heads >= 1, page >= 1 and 1 <= d <= %d", op, kKvMaxDim);
+  if (c.table_cols < 0 || c.table_ld < c.table_cols)
+    return fail(BW_ERR_INVALID_ARGUMENT, "%s: table row stride too small", op);
+  if (c.pages > 0 && (!c.k || !c.v || !c.ks || !c.vs)) return fail(BW_ERR_INVALID_ARGUMENT, "%s: null cache pointer", op);
+  if (b > 0 && c.table_cols > 0 && !c.table) return fail(BW_ERR_INVALID_ARGUMENT, "%s: null table", op);
+  return BW_OK;
+}
+
+// ---------------------------------------------------------------------------
+// rotation and quantised write
+// ---------------------------------------------------------------------------
+struct RowSet {  // [b, t, heads, d] with unit stride in d
+  const void* p;
+  int64_t sb, st, sh;
+  int heads;
+};
+
+struct RotArgs {
+  RowSet q, k, v;      // v only where a cache is written
+  void* q_out;         // contiguous [b, t, heads, d]
+  void* k_out;         // the same, where no cache is written
+  int64_t b, t;
+  int d, rot, interleaved;
+  float mag;
+  const void* pos;     // [b, t], 32 or 64 bits
+  int pos64;
+  const unsigned long long* step;  // [rot / 2] turns per position, 2^-64 each
+  KvCache cache;
+  const int* start;    // [b] first slot
+  const int* counts;   // [b] tokens of a sequence, or null: all t
+};
+
+__device__ __forceinline__ void turn(int64_t pos, unsigned long long step, float mag, float& co, float& si) {
+  const unsigned long long ph = static_cast<unsigned long long>(pos) * step;
+  // the top 32 bits as a signed fraction of half a turn in [-1, 1)
+  const float t = static_cast<float>(static_cast<int>(ph >> 32)) * 0x1p-31f;
+  sincospif(t, &si, &co);
+  co *= mag;
+  si *= mag;
+}
+
+__device__ __forceinline__ int64_t position_of(const RotArgs& a, int64_t tok) {
+  return a.pos64 ? static_cast<const int64_t*>(a.pos)[tok] : static_cast<int64_t>(static_cast<const int*>(a.pos)[tok]);
+}
+
+// Element e of a row, rotated if the row turns.
+template <typename T>
+__device__ __forceinline__ float row_value(const RotArgs& a, const T* x, int e, bool turns, int64_t pos) {
+  if (!turns || e >= a.rot) return to_f32(x[e]);
+  const int half = a.rot / 2;
+  const int i = a.interleaved ? e >> 1 : (e < half ? e : e - half);
+  const bool second = a.interleaved ? (e & 1) : (e >= half);
+  const int other = a.interleaved ? (e ^ 1) : (second ? e - half : e + half);
+  float co, si;
+  turn(pos, a.step[i], a.mag, co, si);
+  const float x0 = to_f32(x[e]), x1 = to_f32(x[other]);
+  return second ? x1 * si + x0 * co : x0 * co - x1 * si;
+}
+
+// Any layout: one warp per (token, head) row.
+template <typename T, bool WRITE>
+__global__ void __launch_bounds__(256) rotary_rows_kernel(const __grid_constant__ RotArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int64_t per_tok = a.q.heads + a.k.heads + a.v.heads;
+  const int64_t rows = a.b * a.t * per_tok;
+  for (int64_t r = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; r < rows;
+       r += (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 5) {
+    const int64_t tok = r / per_tok;
+    int h = static_cast<int>(r - tok * per_tok);
+    const int64_t b = tok / a.t, t = tok - b * a.t;
+    const int which = h < a.q.heads ? 0 : (h < a.q.heads + a.k.heads ? 1 : 2);
+    h -= which == 0 ? 0 : (which == 1 ? a.q.heads : a.q.heads + a.k.heads);
+    const RowSet& s = which == 0 ? a.q : (which == 1 ? a.k : a.v);
+    const T* x = static_cast<const T*>(s.p) + b * s.sb + t * s.st + h * s.sh;
+    const bool turns = which < 2 && a.rot > 0;
+    const int64_t pos = turns ? position_of(a, tok) : 0;
+    if (!WRITE || which == 0) {
+      T* y = static_cast<T*>(which == 0 ? a.q_out : a.k_out) + (tok * s.heads + h) * a.d;
+      for (int e = lane; e < a.d; e += 32) y[e] = from_f32<T>(row_value<T>(a, x, e, turns, pos));
+      continue;
+    }
+    if (a.counts != nullptr && t >= a.counts[b]) continue;
+    const int64_t row0 = kv_row(a.cache, b, static_cast<int64_t>(a.start[b]) + t);
+    if (row0 < 0) continue;
+    const int64_t row = row0 + static_cast<int64_t>(h) * a.cache.page;
+    float v[kKvMaxDim / 32];
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < kKvMaxDim / 32; ++i) {
+      const int e = lane + 32 * i;
+      v[i] = e < a.d ? row_value<T>(a, x, e, turns, pos) : 0.f;
+      m = fmaxf(m, fabsf(v[i]));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float sc = __fdiv_rn(m, 127.0f);
+    const float rcp = __frcp_rn(sc);
+    int8_t* q = (which == 1 ? a.cache.k : a.cache.v) + row * a.d;
+#pragma unroll
+    for (int i = 0; i < kKvMaxDim / 32; ++i) {
+      const int e = lane + 32 * i;
+      if (e < a.d) q[e] = quant_fast<BW_DTYPE_F32>(v[i], sc, rcp);
+    }
+    if (lane == 0) (which == 1 ? a.cache.ks : a.cache.vs)[row] = sc;
+  }
+}
+
+template <typename T>
+static int launch_rotary(const RotArgs& a, bool write, cudaStream_t st) {
+  const int64_t rows = a.b * a.t * (a.q.heads + a.k.heads + a.v.heads);
+  if (rows == 0) return BW_OK;
+  const int64_t blocks = (rows + 7) / 8;
+  const int grid = static_cast<int>(blocks < 16L * num_sms() ? blocks : 16L * num_sms());
+  if (write) rotary_rows_kernel<T, true><<<grid, 256, 0, st>>>(a);
+  else rotary_rows_kernel<T, false><<<grid, 256, 0, st>>>(a);
+  return check_launch("rotary_rows_kernel");
+}
+
+static int check_rows(const RowSet& s, int64_t b, int64_t t, int d, const char* name, const char* op) {
+  if (s.heads < 0) return fail(BW_ERR_INVALID_ARGUMENT, "%s: need %s heads >= 0", op, name);
+  if (s.heads > 0 && b > 0 && t > 0 && !s.p) return fail(BW_ERR_INVALID_ARGUMENT, "%s: null pointer (%s)", op, name);
+  if (s.sb < 0 || s.st < 0 || s.sh < 0) return fail(BW_ERR_INVALID_ARGUMENT, "%s: negative stride (%s)", op, name);
+  return BW_OK;
+}
+
+static int check_rot(const RotArgs& a, int dtype, const char* op) {
+  if (dtype != BW_DTYPE_F16 && dtype != BW_DTYPE_BF16)
+    return fail(BW_ERR_INVALID_ARGUMENT, "%s: inputs must be fp16 or bf16 (dtype %d)", op, dtype);
+  if (a.b < 0 || a.t < 0 || a.d < 1 || a.d > kKvMaxDim)
+    return fail(BW_ERR_INVALID_ARGUMENT, "%s: need b, t >= 0 and 1 <= d <= %d", op, kKvMaxDim);
+  if (a.b > INT32_MAX || a.t > INT32_MAX) return fail(BW_ERR_INVALID_ARGUMENT, "%s: dimension too large", op);
+  if (a.rot < 0 || a.rot > a.d || a.rot % 2) return fail(BW_ERR_INVALID_ARGUMENT, "%s: need an even rot <= d", op);
+  if (int s = check_rows(a.q, a.b, a.t, a.d, "q", op)) return s;
+  if (int s = check_rows(a.k, a.b, a.t, a.d, "k", op)) return s;
+  if (int s = check_rows(a.v, a.b, a.t, a.d, "v", op)) return s;
+  if (a.rot > 0 && a.b > 0 && a.t > 0 && (!a.pos || !a.step))
+    return fail(BW_ERR_INVALID_ARGUMENT, "%s: null pointer (positions or steps)", op);
+  return BW_OK;
+}
+
+// ---------------------------------------------------------------------------
+// read back
+// ---------------------------------------------------------------------------
+struct ReadArgs {
+  KvCache c;
+  int64_t layers, layer_rows;  // rows of one layer in codes and scales
+  int64_t b, n;
+  const int* start;  // [b] or null: 0
+  const int* lens;   // [b] or null: n
+  void* k_out;       // [layers, b, n, heads, d]
+  void* v_out;
+};
+
+// Any layout: one warp per (layer, sequence, slot, head) row of k and of v.
+template <typename T>
+__global__ void __launch_bounds__(256) kv_read_rows_kernel(const __grid_constant__ ReadArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int64_t rows = a.layers * a.b * a.n * a.c.heads;
+  for (int64_t r = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; r < rows;
+       r += (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 5) {
+    const int64_t tok = r / a.c.heads, h = r - tok * a.c.heads;
+    const int64_t lb = tok / a.n, i = tok - lb * a.n;
+    const int64_t layer = lb / a.b, b = lb - layer * a.b;
+    int64_t row = -1;
+    if (a.lens == nullptr || i < a.lens[b]) row = kv_row(a.c, b, (a.start != nullptr ? a.start[b] : 0) + i);
+    if (row >= 0) row += layer * a.layer_rows + h * a.c.page;
+    const float ks = row >= 0 ? a.c.ks[row] : 0.f, vs = row >= 0 ? a.c.vs[row] : 0.f;
+    T* ko = static_cast<T*>(a.k_out) + r * a.c.d;
+    T* vo = static_cast<T*>(a.v_out) + r * a.c.d;
+    for (int e = lane; e < a.c.d; e += 32) {
+      ko[e] = from_f32<T>(row >= 0 ? static_cast<float>(a.c.k[row * a.c.d + e]) * ks : 0.f);
+      vo[e] = from_f32<T>(row >= 0 ? static_cast<float>(a.c.v[row * a.c.d + e]) * vs : 0.f);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// move accepted nodes
+// ---------------------------------------------------------------------------
+// One CTA per (sequence, head, layer): the accepted rows are all read before the first is written
+// (a node's slot may be another one's target), so the order of `path` does not matter.
+__global__ void __launch_bounds__(256) kv_move_kernel(const __grid_constant__ KvCache c, int64_t layer_rows, int t,
+                                                      const int* __restrict__ start, const int* __restrict__ path,
+                                                      int64_t path_ld, const int* __restrict__ taken) {
+  __shared__ int8_t buf[2][kTreeMaxNodes * kKvMaxDim];
+  __shared__ float sc[2][kTreeMaxNodes];
+  __shared__ int64_t src[kTreeMaxNodes], dst[kTreeMaxNodes];
+  const int64_t b = blockIdx.x, h = blockIdx.y, layer = blockIdx.z;
+  int n = taken[b];
+  n = n < t - 1 ? n : t - 1;
+  if (n <= 0) return;
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const int node = path[b * path_ld + i];
+    int64_t s = -1, d = -1;
+    if (node >= 0 && node < t) {
+      s = kv_row(c, b, static_cast<int64_t>(start[b]) + node);
+      d = kv_row(c, b, static_cast<int64_t>(start[b]) + 1 + i);
+    }
+    const bool ok = s >= 0 && d >= 0 && s != d;
+    src[i] = ok ? layer * layer_rows + h * c.page + s : -1;
+    dst[i] = ok ? layer * layer_rows + h * c.page + d : -1;
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < n * c.d; e += blockDim.x) {
+    const int i = e / c.d, j = e - i * c.d;
+    if (src[i] < 0) continue;
+    buf[0][e] = c.k[src[i] * c.d + j];
+    buf[1][e] = c.v[src[i] * c.d + j];
+    if (j == 0) {
+      sc[0][i] = c.ks[src[i]];
+      sc[1][i] = c.vs[src[i]];
+    }
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < n * c.d; e += blockDim.x) {
+    const int i = e / c.d, j = e - i * c.d;
+    if (src[i] < 0) continue;
+    c.k[dst[i] * c.d + j] = buf[0][e];
+    c.v[dst[i] * c.d + j] = buf[1][e];
+    if (j == 0) {
+      c.ks[dst[i]] = sc[0][i];
+      c.vs[dst[i]] = sc[1][i];
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// a draft tree's masks and positions
+// ---------------------------------------------------------------------------
+// parent[i] < i for a node of the tree; node 0 is the root.  Any other parent takes a node out of
+// the tree: it sees nothing and stands at its sequence's own position.
+__global__ void __launch_bounds__(kTreeMaxNodes) tree_positions_kernel(const int* __restrict__ parents, int64_t ld,
+                                                                       const int* __restrict__ ctx, int t,
+                                                                       unsigned long long* __restrict__ mask,
+                                                                       int* __restrict__ pos) {
+  __shared__ int up[kTreeMaxNodes];
+  const int64_t b = blockIdx.x;
+  const int i = threadIdx.x;
+  if (i < t) up[i] = parents[b * ld + i];
+  __syncthreads();
+  if (i >= t) return;
+  unsigned long long bits = 0;
+  int at = i;
+  while (at > 0 && up[at] >= 0 && up[at] < at) {  // strictly descending: ends
+    bits |= 1ull << at;
+    at = up[at];
+  }
+  bits = at == 0 ? bits | 1ull : 0ull;
+  mask[b * t + i] = bits;
+  pos[b * t + i] = (ctx != nullptr ? ctx[b] : 0) + (bits ? __popcll(bits) - 1 : 0);
+}
+
+static KvCache make_cache(void* k, void* v, float* ks, float* vs, int64_t pages, int64_t heads, int64_t page, int64_t d,
+                          const int* table, int64_t table_ld, int64_t table_cols) {
+  KvCache c;
+  c.k = static_cast<int8_t*>(k);
+  c.v = static_cast<int8_t*>(v);
+  c.ks = ks;
+  c.vs = vs;
+  c.pages = pages;
+  // out of int range: 0, which check_kv_cache refuses
+  c.heads = heads > 0 && heads <= 65535 ? static_cast<int>(heads) : 0;
+  c.page = page > 0 && page <= (1 << 24) ? static_cast<int>(page) : 0;
+  c.d = d > 0 && d <= kKvMaxDim ? static_cast<int>(d) : 0;
+  c.table = table;
+  c.table_ld = table_ld;
+  c.table_cols = table_cols >= 0 && table_cols <= INT32_MAX ? static_cast<int>(table_cols) : -1;
+  return c;
+}
+
+}  // namespace bw
+
+extern "C" int bw_rotary(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int hq, const void* k, int64_t k_sb,
+                         int64_t k_st, int64_t k_sh, int hk, void* q_out, void* k_out, int dtype, int64_t b, int64_t t,
+                         int64_t d, const void* positions, int positions64, const uint64_t* steps, float magnitude,
+                         int64_t rot, int interleaved, void* stream) {
+  using namespace bw;
+  RotArgs a = {};
+  a.q = {q, q_sb, q_st, q_sh, hq};
+  a.k = {k, k_sb, k_st, k_sh, hk};
+  a.q_out = q_out;
+  a.k_out = k_out;
+  a.b = b;
+  a.t = t;
+  a.d = d > 0 && d <= kKvMaxDim ? static_cast<int>(d) : 0;
+  a.rot = rot >= 0 && rot <= kKvMaxDim ? static_cast<int>(rot) : -1;
+  a.interleaved = interleaved;
+  a.mag = magnitude;
+  a.pos = positions;
+  a.pos64 = positions64;
+  a.step = reinterpret_cast<const unsigned long long*>(steps);
+  if (int s = check_rot(a, dtype, "rotary")) return s;
+  if (b == 0 || t == 0) return BW_OK;
+  if ((hq > 0 && !q_out) || (hk > 0 && !k_out)) return fail(BW_ERR_INVALID_ARGUMENT, "rotary: null output pointer");
+  if (int s = require_sm100()) return s;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == BW_DTYPE_BF16 ? launch_rotary<__nv_bfloat16>(a, false, st) : launch_rotary<__half>(a, false, st);
+}
+
+extern "C" int bw_rotary_kv_write_int8(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int hq, const void* k,
+                                       int64_t k_sb, int64_t k_st, int64_t k_sh, const void* v, int64_t v_sb,
+                                       int64_t v_st, int64_t v_sh, void* q_out, int dtype, int64_t b, int64_t t,
+                                       const void* positions, int positions64, const uint64_t* steps, float magnitude,
+                                       int64_t rot, int interleaved, int8_t* cache_k, int8_t* cache_v, float* k_scale,
+                                       float* v_scale, int64_t pages, int64_t heads, int64_t page, int64_t d,
+                                       const int32_t* table, int64_t table_ld, int64_t table_cols,
+                                       const int32_t* start, const int32_t* counts, void* stream) {
+  using namespace bw;
+  RotArgs a = {};
+  a.cache = make_cache(cache_k, cache_v, k_scale, v_scale, pages, heads, page, d, table, table_ld, table_cols);
+  if (int s = check_kv_cache(a.cache, b, "kv_write_int8")) return s;
+  a.q = {q, q_sb, q_st, q_sh, hq};
+  a.k = {k, k_sb, k_st, k_sh, a.cache.heads};
+  a.v = {v, v_sb, v_st, v_sh, a.cache.heads};
+  a.q_out = q_out;
+  a.b = b;
+  a.t = t;
+  a.d = a.cache.d;
+  a.rot = rot >= 0 && rot <= kKvMaxDim ? static_cast<int>(rot) : -1;
+  a.interleaved = interleaved;
+  a.mag = magnitude;
+  a.pos = positions;
+  a.pos64 = positions64;
+  a.step = reinterpret_cast<const unsigned long long*>(steps);
+  a.start = start;
+  a.counts = counts;
+  if (int s = check_rot(a, dtype, "kv_write_int8")) return s;
+  if (b == 0 || t == 0) return BW_OK;
+  if (!start || (hq > 0 && !q_out)) return fail(BW_ERR_INVALID_ARGUMENT, "kv_write_int8: null pointer");
+  if (int s = require_sm100()) return s;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == BW_DTYPE_BF16 ? launch_rotary<__nv_bfloat16>(a, true, st) : launch_rotary<__half>(a, true, st);
+}
+
+extern "C" int bw_kv_read_int8(const int8_t* cache_k, const int8_t* cache_v, const float* k_scale,
+                               const float* v_scale, int64_t layers, int64_t pages, int64_t heads, int64_t page,
+                               int64_t d, const int32_t* table, int64_t table_ld, int64_t table_cols,
+                               const int32_t* start, const int32_t* lens, int64_t b, int64_t n, void* k_out,
+                               void* v_out, int dtype, void* stream) {
+  using namespace bw;
+  ReadArgs a = {};
+  a.c = make_cache(const_cast<int8_t*>(cache_k), const_cast<int8_t*>(cache_v), const_cast<float*>(k_scale),
+                   const_cast<float*>(v_scale), pages, heads, page, d, table, table_ld, table_cols);
+  if (int s = check_kv_cache(a.c, b, "kv_read_int8")) return s;
+  if (layers < 0 || b < 0 || n < 0 || layers > INT32_MAX || b > INT32_MAX || n > INT32_MAX)
+    return fail(BW_ERR_INVALID_ARGUMENT, "kv_read_int8: need 0 <= layers, b, n < 2^31");
+  if (dtype != BW_DTYPE_F16 && dtype != BW_DTYPE_BF16)
+    return fail(BW_ERR_INVALID_ARGUMENT, "kv_read_int8: outputs must be fp16 or bf16 (dtype %d)", dtype);
+  if (layers == 0 || b == 0 || n == 0) return BW_OK;
+  if (!k_out || !v_out) return fail(BW_ERR_INVALID_ARGUMENT, "kv_read_int8: null pointer");
+  a.layers = layers;
+  a.layer_rows = pages * heads * page;
+  a.b = b;
+  a.n = n;
+  a.start = start;
+  a.lens = lens;
+  a.k_out = k_out;
+  a.v_out = v_out;
+  if (int s = require_sm100()) return s;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int64_t blocks = (layers * b * n * heads + 7) / 8;
+  const int grid = static_cast<int>(blocks < 16L * num_sms() ? blocks : 16L * num_sms());
+  if (dtype == BW_DTYPE_BF16) kv_read_rows_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a);
+  else kv_read_rows_kernel<__half><<<grid, 256, 0, st>>>(a);
+  return check_launch("kv_read_rows_kernel");
+}
+
+extern "C" int bw_kv_move_int8(int8_t* cache_k, int8_t* cache_v, float* k_scale, float* v_scale, int64_t layers,
+                               int64_t pages, int64_t heads, int64_t page, int64_t d, const int32_t* table,
+                               int64_t table_ld, int64_t table_cols, const int32_t* start, const int32_t* path,
+                               int64_t path_ld, const int32_t* taken, int64_t b, int64_t t, void* stream) {
+  using namespace bw;
+  const KvCache c = make_cache(cache_k, cache_v, k_scale, v_scale, pages, heads, page, d, table, table_ld, table_cols);
+  if (int s = check_kv_cache(c, b, "kv_move_int8")) return s;
+  if (layers < 0 || layers > 65535 || b < 0 || b > INT32_MAX)
+    return fail(BW_ERR_INVALID_ARGUMENT, "kv_move_int8: need 0 <= layers < 65536 and 0 <= b < 2^31");
+  if (t < 0 || t > kTreeMaxNodes || path_ld < t)
+    return fail(BW_ERR_INVALID_ARGUMENT, "kv_move_int8: need 0 <= t <= %d and a path row stride >= t", kTreeMaxNodes);
+  if (layers == 0 || b == 0 || t <= 1) return BW_OK;
+  if (!start || !path || !taken) return fail(BW_ERR_INVALID_ARGUMENT, "kv_move_int8: null pointer");
+  if (int s = require_sm100()) return s;
+  const dim3 grid(static_cast<unsigned>(b), static_cast<unsigned>(heads), static_cast<unsigned>(layers));
+  kv_move_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(c, pages * heads * page, static_cast<int>(t),
+                                                                      start, path, path_ld, taken);
+  return check_launch("kv_move_kernel");
+}
+
+extern "C" int bw_tree_positions(const int32_t* parents, int64_t parents_ld, const int32_t* ctx_lens, int64_t b,
+                                 int64_t t, uint64_t* mask, int32_t* positions, void* stream) {
+  using namespace bw;
+  if (b < 0 || b > INT32_MAX || t < 0 || t > kTreeMaxNodes || parents_ld < t)
+    return fail(BW_ERR_INVALID_ARGUMENT, "tree_positions: need 0 <= t <= %d and a row stride >= t", kTreeMaxNodes);
+  if (b == 0 || t == 0) return BW_OK;
+  if (!parents || !mask || !positions) return fail(BW_ERR_INVALID_ARGUMENT, "tree_positions: null pointer");
+  if (int s = require_sm100()) return s;
+  tree_positions_kernel<<<static_cast<unsigned>(b), kTreeMaxNodes, 0, static_cast<cudaStream_t>(stream)>>>(
+      parents, parents_ld, ctx_lens, static_cast<int>(t), reinterpret_cast<unsigned long long*>(mask), positions);
+  return check_launch("tree_positions_kernel");
+}

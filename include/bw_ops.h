@@ -295,6 +295,115 @@ int bw_dequantize_kv_int8(const int8_t* q, int64_t ldq, const float* scale, int6
                           void* x, int64_t ldx, void* stream);
 
 /*
+ * Speculative decoding over a paged int8 KV cache.  No counterpart in the reference's operators
+ * (its n-gram speculation, src/blackwell_inference/spec/ngram.py:25-197, runs a model's own cache).
+ *
+ * The cache: k, v int8 codes [layers][pages][heads][page][d], k_scale, v_scale fp32
+ * [layers][pages][heads][page], contiguous; value = code * scale; d <= 256.  Slot s of sequence b is
+ * row s % page of page table[b][s / page] (int32, row stride table_ld).  A slot past the table's
+ * table_cols columns, or whose entry is no page of the cache, does not exist: it is not written,
+ * reads as zero and is not attended to.  Two sequences may share a page that is only read.
+ * Strided inputs [b, t, heads, d] have unit stride in d; strides are in elements.
+ */
+
+/*
+ * Rotary positions: q_out, k_out [b, t, heads, d] contiguous = q, k with pair i of the first `rot`
+ * elements of each head turned by positions[b, t] * f_i radians and scaled by `magnitude`, and the
+ * other elements copied.  Pairs are (2i, 2i+1) if interleaved, else (i, i + rot/2).
+ *   dtype      F16 | BF16 (32-bit arithmetic, rounded once)
+ *   positions  [b, t] int32, or int64 if positions64
+ *   steps      [rot/2] turns per position in units of 2^-64: round(f_i / 2pi * 2^64) mod 2^64
+ *   hk == 0: no keys.  An output may be its own input where that is contiguous.
+ */
+int bw_rotary(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int hq, const void* k, int64_t k_sb,
+              int64_t k_st, int64_t k_sh, int hk, void* q_out, void* k_out, int dtype, int64_t b, int64_t t,
+              int64_t d, const void* positions, int positions64, const uint64_t* steps, float magnitude,
+              int64_t rot, int interleaved, void* stream);
+
+/*
+ * Write new keys and values into the cache, quantised per token and head: token i of sequence b
+ * (i < counts[b]; counts == NULL: i < t) goes to slot start[b] + i, with
+ *   scale = max|x| / 127 (fp32; NaN ignored, 0 for a row of zeros),
+ *   code = clamp(rne(x / scale), -127, 127) (IEEE fp32 quotient, NaN -> 0).
+ * rot > 0: q and k are first rotated as by bw_rotary; q_out [b, t, hq, d] gets the rotated q of all
+ * t tokens and the rotated k is quantised from its 32-bit values.  rot == 0: hq > 0 copies q.
+ */
+int bw_rotary_kv_write_int8(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int hq, const void* k,
+                            int64_t k_sb, int64_t k_st, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_st,
+                            int64_t v_sh, void* q_out, int dtype, int64_t b, int64_t t, const void* positions,
+                            int positions64, const uint64_t* steps, float magnitude, int64_t rot, int interleaved,
+                            int8_t* cache_k, int8_t* cache_v, float* k_scale, float* v_scale, int64_t pages,
+                            int64_t heads, int64_t page, int64_t d, const int32_t* table, int64_t table_ld,
+                            int64_t table_cols, const int32_t* start, const int32_t* counts, void* stream);
+
+/*
+ * Read slots start[b] + i, i < n, back as values: k_out, v_out [layers, b, n, heads, d] in dtype
+ * (F16 | BF16) = dt(code * scale).  start == NULL: 0.  Slots i >= lens[b] (lens given) are zeros.
+ */
+int bw_kv_read_int8(const int8_t* cache_k, const int8_t* cache_v, const float* k_scale, const float* v_scale,
+                    int64_t layers, int64_t pages, int64_t heads, int64_t page, int64_t d, const int32_t* table,
+                    int64_t table_ld, int64_t table_cols, const int32_t* start, const int32_t* lens, int64_t b,
+                    int64_t n, void* k_out, void* v_out, int dtype, void* stream);
+
+/*
+ * After a verification: in every layer, the rows of the accepted nodes path[b, 0 .. taken[b]) of a
+ * tree of t nodes written at slots start[b] + node go to slots start[b] + 1, start[b] + 2, ...  All
+ * of a sequence's rows are read before one is written, so any order of nodes is allowed.  A node
+ * outside [0, t) is skipped.  t <= 64.
+ */
+int bw_kv_move_int8(int8_t* cache_k, int8_t* cache_v, float* k_scale, float* v_scale, int64_t layers, int64_t pages,
+                    int64_t heads, int64_t page, int64_t d, const int32_t* table, int64_t table_ld,
+                    int64_t table_cols, const int32_t* start, const int32_t* path, int64_t path_ld,
+                    const int32_t* taken, int64_t b, int64_t t, void* stream);
+
+/*
+ * Masks and positions of draft trees: node 0 is the root, parents[b, i] < i the parent of node i;
+ * any other parent (or one outside the tree) takes a node out of it.  mask[b, i]: bit j is set if
+ * node j is node i or an ancestor of it (0 for a node out of the tree); positions[b, i] =
+ * ctx_lens[b] + depth (ctx_lens == NULL: depth).  t <= 64.
+ */
+int bw_tree_positions(const int32_t* parents, int64_t parents_ld, const int32_t* ctx_lens, int64_t b, int64_t t,
+                      uint64_t* mask, int32_t* positions, void* stream);
+
+/*
+ * Attention of t nodes a sequence over its cache: out [b, t, hq, d] contiguous, in q's dtype,
+ *   out_i = sum_j w_ij v_j / sum_j w_ij,  w_ij = exp(softmax_scale * q_i . k_j)
+ * over the slots j < ctx_lens[b] and the slots ctx_lens[b] + n of the nodes n named by bit n of
+ * mask[b, i] (mask == NULL: nodes 0 .. i).  counts[b] (NULL: t) limits a sequence's nodes: later
+ * ones are not seen and give zeros, and so does a node that sees nothing.  hq is a multiple of
+ * heads (query head h reads key head h / (hq / heads)); t <= 64; t == 1 is ordinary decoding.
+ * Scores, weights' sums and outputs accumulate in fp32.
+ * Workspace: bw_tree_attention_int8_workspace_size bytes, 256-byte aligned; its first
+ * bw_tree_attention_int8_workspace_zeroed_bytes zero before the first call (every call leaves them
+ * zero; after a device timeout zero them again).  Calls that share a workspace must not overlap.
+ */
+size_t bw_tree_attention_int8_workspace_size(int64_t b, int64_t t, int64_t hq, int64_t heads, int64_t d);
+size_t bw_tree_attention_int8_workspace_zeroed_bytes(int64_t b, int64_t t, int64_t hq, int64_t heads, int64_t d);
+int bw_tree_attention_int8(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int dtype, void* out,
+                           const int8_t* cache_k, const int8_t* cache_v, const float* k_scale, const float* v_scale,
+                           int64_t pages, int64_t heads, int64_t page, int64_t d, const int32_t* table,
+                           int64_t table_ld, int64_t table_cols, const int32_t* ctx_lens, const uint64_t* mask,
+                           const int32_t* counts, int64_t b, int64_t t, int64_t hq, float softmax_scale,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Verify drafted tokens: tokens[b, i] is node i's token (node 0, the root, is the last committed
+ * token), target[b, i, :] the target model's probabilities of the token after node i, draft[b, i, :]
+ * the distribution from which node i's children were drawn (draft == NULL: drafts without one, as
+ * from a lookup).  From the root, a node's children (parents[b, i] == node) are tried in index order
+ * with w = target and Z = 1: child i with token x is taken if accept_u[b, i] * draft(x) * Z < w(x);
+ * else w = max(w - Z draft, 0) (draft == NULL: draft(x) = 1 and w(x) = 0) and Z = sum w.  Where no
+ * child is taken the walk ends with the token argmax_v w(v) / sample_e[b, v] over w(v) > 0 (lowest
+ * token on ties; w = target if no w(v) > 0; token 0 if none is still).  With accept_u uniform on
+ * [0, 1) and sample_e exponential the tokens are distributed as the target's own.
+ *   n_accepted [b]; path [b, t]: accepted nodes, then -1; out_tokens [b, t]: their tokens, the last
+ *   token, then -1.  A drafted token outside [0, v) is never taken.  t <= 64.
+ */
+int bw_verify_tree(const float* target, const float* draft, const int64_t* tokens, const int32_t* parents,
+                   const float* accept_u, const float* sample_e, int64_t b, int64_t t, int64_t v,
+                   int32_t* n_accepted, int32_t* path, int64_t* out_tokens, void* stream);
+
+/*
  * Device-side status of the current device: BW_OK, or BW_ERR_DEVICE_TIMEOUT
  * if a kernel's bounded wait expired since the last clear.  Synchronises
  * `stream`.  If `detail` is non-NULL it receives the failing wait site id.
