@@ -60,15 +60,17 @@ def status(device=None, clear: bool = False) -> int:
 def check(device=None, op: str = "blackwell_ops") -> None:
     """Raise ``DeviceTimeoutError`` if a bounded wait of a kernel on ``device`` ran out.
 
-    Clears the status and re-zeroes the cached GEMM and requantisation workspaces first,
+    Clears the status and re-zeroes the cached GEMM, requantisation and attention workspaces first,
     so the next call starts clean.  Synchronises the device's current stream."""
     site = status(device, clear=True)
     if site:
         from .cuda import reset_workspaces as reset_requant
+        from .decode import reset_workspaces as reset_attention
         from .kernels.int8_gemm import reset_workspaces
 
         reset_workspaces()
         reset_requant()
+        reset_attention()
         torch.cuda.synchronize(_dev(device))
         err = DeviceTimeoutError(BW_ERR_DEVICE_TIMEOUT, op)
         err.site = site

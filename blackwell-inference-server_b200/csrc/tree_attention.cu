@@ -6,6 +6,9 @@
 // weights; a row that sees nothing (or only scores of -inf) gives zeros.
 #include <stdio.h>
 
+#include <mutex>
+#include <type_traits>
+
 #include "kv_cache.cuh"
 
 namespace bw {
@@ -106,17 +109,906 @@ __global__ void __launch_bounds__(32 * kRowWarps) attn_rows_kernel(const __grid_
   }
 }
 
-}  // namespace bw
+// ---------------------------------------------------------------------------
+// tensor-core kernel (head dimensions 64 and 128)
+//
+// A tile is 128 slots of one sequence and key head; the R query rows of a CTA are the (node, query
+// head of the group) pairs that read that head.  Both products put the 128-row side on the cache, so
+// one query row costs the tensor core no more than sixteen:
+//   S^T [128 slots x R]  = K [128 x D] (TMEM, dequantised) . Q^T (shared memory)
+//   O^T [D x 2R]        += V^T [D x 128] (shared memory, dequantised) . [P_hi | P_lo] [128 x 2R]
+// Codes are exact in 16 bits, so the products see the cache's values without a rounding; the scales
+// ks_j and vs_j multiply the scores and the weights in fp32.  A weight w vs_j goes in as the sum of
+// two bf16 numbers (hi = bf16(x), lo = bf16(x - hi), 2^-17 of x left out): fp16 would be one number
+// but cannot hold w vs_j for every scale, one bf16 alone loses 2^-9.
+//
+// Softmax: one thread holds one slot's R scores, so the exponentials need no exchange; what is
+// shared is each row's reference m.  m moves only when a score exceeds it by more than 8 (in powers
+// of two): a vote decides, and only then are the row maxima taken over the 128 slots, the sums l and
+// the accumulators rescaled.  Weights stay under 2^8, sums and accumulators are fp32.
+//
+// Work: the (sequence, key head, tile) units, laid end to end, are split evenly over the CTAs, so
+// ragged lengths balance; with more rows than R, neighbouring CTAs take the row blocks of one range
+// at the same time, and the second reads the cache from L2.  A (sequence, head) cut by a range end
+// is joined by its last CTA (a ticket) from the pieces in the workspace, in range order, so results
+// do not depend on timing.
+//
+// One CTA per SM, 19 warps: 0 TMA (one box per page), 1 issues K.Q, 18 issues V.P, 2-5 dequantise K
+// into TMEM (thread = slot), 6-9 dequantise V into shared memory and load Q, 10-17 two softmax groups
+// of half the rows each.
+// ---------------------------------------------------------------------------
+constexpr int kTile = 128;
+constexpr int kAttnThreads = 19 * 32;
+constexpr int kAttnMaxBatch = 1024;  // sequences of one launch (their unit ranges lie in shared memory)
+constexpr size_t kAttnCounterBytes = 4096;
+enum AttnSite : int { kSiteAtTma = 80, kSiteAtDrain, kSiteAtK, kSiteAtV, kSiteAtQk, kSiteAtPv, kSiteAtSoft, kSiteAtFinal };
 
-extern "C" size_t bw_tree_attention_int8_workspace_size(int64_t b, int64_t t, int64_t hq, int64_t hk, int64_t d) {
-  (void)b, (void)t, (void)hq, (void)hk, (void)d;
-  return 0;
+template <int D, int R>
+struct ACfg {
+  static constexpr int RC = R / 2;                     // rows of a softmax group
+  static constexpr int KV = kTile * D;                 // bytes of one K or V tile of codes
+  static constexpr int VB = (D / 64) * kTile * 128;    // a V tile in bf16
+  static constexpr int ZB = D == 64 ? kTile * 128 : 0; // zeros: the rows 64 .. 127 of V^T
+  static constexpr int PB = (2 * R + 63) / 64 * kTile * 128;
+  static constexpr int QB = R * D * 2;
+  static constexpr int NQ = R == 64 ? 1 : 2;           // Q buffers
+  static constexpr int OFF_VB = 0;
+  static constexpr int OFF_Z = OFF_VB + 2 * VB;
+  static constexpr int OFF_P = OFF_Z + ZB;
+  static constexpr int OFF_Q = OFF_P + 2 * PB;
+  static constexpr int OFF_RING = OFF_Q + NQ * QB;
+  static constexpr int CTRL = 512 + 2 * 4 * 32 * 4 * 2 + 2 * 2 * 32 * 4 + 2 * 16 * 32 * 4 + 2 * 64 * 8 +
+                              (kAttnMaxBatch + 1) * 4 + 64;
+  static constexpr int ROOM = 227 * 1024 - 1024 - OFF_RING - CTRL;
+  static constexpr int ST = ROOM / (2 * KV) < 6 ? ROOM / (2 * KV) : 6;  // stages of a K and a V tile
+  static constexpr int OFF_CTRL = OFF_RING + 2 * ST * KV;
+  static constexpr int SMEM = OFF_CTRL + CTRL + 1024;
+  static constexpr int A_COLS = D / 2;                 // TMEM columns of a K tile
+  static constexpr int S_COL = 2 * A_COLS;
+  static constexpr int O_COL = S_COL + 2 * R;
+  static constexpr int COLS = O_COL + 2 * R <= 256 ? 256 : 512;
+  static_assert(ST >= 2, "at least two stages");
+  static_assert(QB % 1024 == 0 && KV % 1024 == 0, "swizzled tiles are 1024-byte aligned");
+};
+
+struct TileArgs {
+  AttnArgs a;
+  int64_t b0;      // first sequence of this launch
+  int nb;          // its sequences
+  int rts;         // row blocks
+  int groups;      // CTAs per row block
+  int qvec;        // q rows are 16-byte aligned
+  float* pieces;   // [grid][2][R][D] fp32 accumulators, then [R] m, [R] l each
+  int* counters;   // [grid][2]
+};
+
+// The units of one CTA's range, one (sequence, head) segment after another.
+struct AttnSeg {
+  int b, h;        // sequence of this launch, key head
+  int kt0, n_kt;   // first tile, tiles
+  int tiles;       // tiles of the whole (sequence, head)
+  int u0;          // its first unit
+  int slot;        // 0: the range's first segment
+};
+struct AttnWalk {
+  int x, end, b;
+  bool first;
+  __device__ __forceinline__ AttnWalk(const int* pre, int nb, int x0, int x1) : x(x0), end(x1), first(true) {
+    int lo = 0, hi = nb - 1;  // the last b with pre[b] <= x
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (pre[mid] <= x) lo = mid;
+      else hi = mid - 1;
+    }
+    b = lo;
+  }
+  __device__ __forceinline__ bool next(const int* pre, int heads, AttnSeg& s) {
+    if (x >= end) return false;
+    while (pre[b + 1] <= x) ++b;
+    s.b = b;
+    s.tiles = (pre[b + 1] - pre[b]) / heads;
+    const int rel = x - pre[b];
+    s.h = rel / s.tiles;
+    s.kt0 = rel - s.h * s.tiles;
+    s.u0 = x - s.kt0;
+    s.n_kt = min(s.tiles - s.kt0, end - x);
+    s.slot = first ? 0 : 1;
+    first = false;
+    x += s.n_kt;
+    return true;
+  }
+};
+
+// Range starts of `groups` CTAs over `units` (units >= groups), and the CTA that holds unit x.
+__host__ __device__ __forceinline__ int range_start(int c, int units, int groups) {
+  return static_cast<int>(static_cast<int64_t>(units) * c / groups);
+}
+__host__ __device__ __forceinline__ int range_owner(int x, int units, int groups) {
+  int c = static_cast<int>(static_cast<int64_t>(x) * groups / units);
+  while (c + 1 < groups && range_start(c + 1, units, groups) <= x) ++c;
+  while (c > 0 && range_start(c, units, groups) > x) --c;
+  return c;
 }
 
-extern "C" size_t bw_tree_attention_int8_workspace_zeroed_bytes(int64_t b, int64_t t, int64_t hq, int64_t hk,
+__device__ __forceinline__ int seq_nodes(const AttnArgs& a, int64_t b) {
+  const int n = a.counts != nullptr ? a.counts[b] : a.t;
+  return n < 0 ? 0 : (n < a.t ? n : a.t);
+}
+__device__ __forceinline__ int64_t seq_ctx(const AttnArgs& a, int64_t b) { return a.ctx[b] > 0 ? a.ctx[b] : 0; }
+
+// 16 codes -> 16 fp16 or bf16 values.
+template <bool BF16>
+__device__ __forceinline__ void codes16(const uint4& v, uint32_t* o) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (BF16) i8x4_to_bf16x4(w[i], o[2 * i], o[2 * i + 1]);
+    else i8x4_to_f16x4(w[i], o[2 * i], o[2 * i + 1]);
+  }
+}
+
+// Maximum or sum over a warp of each of N per-thread values: value c ends in the lanes
+// [c * 32 / N, (c + 1) * 32 / N).
+template <int N, bool MAX>
+__device__ __forceinline__ float warp_columns(float (&v)[N], int lane) {
+  int o = 16;
+#pragma unroll
+  for (int n = N; n > 1; n >>= 1, o >>= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int i = 0; i < n / 2; ++i) {
+      const float send = up ? v[i] : v[i + n / 2];
+      const float keep = up ? v[i + n / 2] : v[i];
+      const float got = __shfl_xor_sync(0xffffffffu, send, o);
+      v[i] = MAX ? fmaxf(keep, got) : keep + got;
+    }
+  }
+#pragma unroll
+  for (; o > 0; o >>= 1) {
+    const float got = __shfl_xor_sync(0xffffffffu, v[0], o);
+    v[0] = MAX ? fmaxf(v[0], got) : v[0] + got;
+  }
+  return v[0];
+}
+
+template <int D, int R, typename T>
+__global__ void __launch_bounds__(kAttnThreads, 1)
+    attn_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                     const __grid_constant__ TileArgs ta) {
+  using C = ACfg<D, R>;
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int RC = C::RC;
+  constexpr int ST = C::ST;
+  const AttnArgs& a = ta.a;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sVB = smem + C::OFF_VB;
+  uint8_t* sP = smem + C::OFF_P;
+  uint8_t* sQ = smem + C::OFF_Q;
+  uint8_t* sK = smem + C::OFF_RING;
+  uint8_t* sV = sK + ST * C::KV;
+  uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + C::OFF_CTRL);
+  uint64_t* kempty = kfull + ST;
+  uint64_t* vfull = kempty + ST;
+  uint64_t* vempty = vfull + ST;
+  uint64_t* afull = vempty + ST;      // 2: K dequantised in TMEM
+  uint64_t* aempty = afull + 2;
+  uint64_t* vbfull = aempty + 2;      // 2: V dequantised
+  uint64_t* vbempty = vbfull + 2;
+  uint64_t* sfull = vbempty + 2;      // 2: scores
+  uint64_t* sempty = sfull + 2;
+  uint64_t* pfull = sempty + 2;       // 2: weights
+  uint64_t* pempty = pfull + 2;       //    (and the accumulator holds the tile's contribution)
+  uint64_t* qfull = pempty + 2;       // 2: Q and the row masks of a segment
+  uint64_t* qempty = qfull + 2;
+  uint64_t* final_bar = qempty + 2;   // 2
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(final_bar + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* wred = reinterpret_cast<float*>(smem + C::OFF_CTRL + 512);  // [2 groups][2][4 warps][32]
+  float* refs = wred + 2 * 2 * 4 * 32;                               // [2 groups][2][32]: m, its factor
+  float* ftab = refs + 2 * 2 * 32;                                   // [2 groups][16][32]
+  unsigned long long* rmask = reinterpret_cast<unsigned long long*>(ftab + 2 * 16 * 32);  // [2][64]
+  int* pre = reinterpret_cast<int*>(rmask + 2 * 64);                 // [nb + 1] first unit of a sequence
+  static_assert((4 * 6 + 18) * 8 + 8 <= 512, "barriers");
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int grp = a.hq / a.c.heads;  // query heads of a key head
+  const int heads = a.c.heads;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(&kfull[s], 1);
+      mbar_init(&kempty[s], 4);
+      mbar_init(&vfull[s], 1);
+      mbar_init(&vempty[s], 4);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&afull[i], 4);
+      mbar_init(&aempty[i], 1);
+      mbar_init(&vbfull[i], 4);
+      mbar_init(&vbempty[i], 1);
+      mbar_init(&sfull[i], 1);
+      mbar_init(&sempty[i], 8);
+      mbar_init(&pfull[i], 8);
+      mbar_init(&pempty[i], 1);
+      mbar_init(&qfull[i], 4);
+      mbar_init(&qempty[i], 9);  // the last K.Q of the segment, and the softmax warps
+      mbar_init(&final_bar[i], 1);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, C::COLS);
+    tmem_relinquish();
+  }
+  if constexpr (C::ZB > 0) {
+    for (int i = threadIdx.x; i < C::ZB / 16; i += kAttnThreads)
+      reinterpret_cast<uint4*>(smem + C::OFF_Z)[i] = make_uint4(0u, 0u, 0u, 0u);
+    fence_proxy_async_smem();
+  }
+  pdl_wait();  // lengths, tables, masks, q and the cache may come from the preceding kernel
+  // units before each sequence; one at least, so that every output row is written
+  if (warp == 0) {
+    const int64_t room = static_cast<int64_t>(a.c.table_cols) * a.c.page;
+    int base = 0;
+    for (int i0 = 0; i0 < ta.nb; i0 += 32) {
+      int n = 0;
+      if (i0 + lane < ta.nb) {
+        int64_t keys = seq_ctx(a, ta.b0 + i0 + lane) + seq_nodes(a, ta.b0 + i0 + lane);
+        keys = keys < room ? keys : room;
+        n = static_cast<int>(keys > 0 ? (keys + kTile - 1) / kTile : 1) * heads;
+      }
+      int sum = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int got = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += got;
+      }
+      if (i0 + lane < ta.nb) pre[i0 + lane] = base + sum - n;
+      base += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (lane == 0) pre[ta.nb] = base;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int units = pre[ta.nb];
+  const int groups = min(ta.groups, units);
+  const int gi = blockIdx.x / ta.rts, rt = blockIdx.x - gi * ta.rts;
+  const int x0 = gi < groups ? range_start(gi, units, groups) : 0;
+  const int x1 = gi < groups ? range_start(gi + 1, units, groups) : 0;  // an empty range: nothing to do
+
+  if (warp == 0) {
+    // ---------------- TMA: one box of K and one of V per page of the tile ----------------
+    const int box = min(a.c.page, kTile);  // rows of a box
+    const int per = kTile / box;           // boxes of a tile
+    const uint64_t pol = ta.rts > 1 ? l2_policy_evict_normal() : l2_policy_evict_first();
+    int it = 0;
+    bool ok = true;
+    AttnWalk wk(pre, ta.nb, x0, x1);
+    AttnSeg sg;
+    while (ok && wk.next(pre, heads, sg)) {
+      const int64_t b = ta.b0 + sg.b;
+      const int64_t keys = seq_ctx(a, b) + seq_nodes(a, b);
+      for (int i = 0; i < sg.n_kt; ++i, ++it) {
+        const int64_t slot = static_cast<int64_t>(sg.kt0 + i) * kTile + lane * box;
+        int64_t row = -1;
+        if (lane < per && slot < keys) row = kv_row(a.c, b, slot);
+        if (row >= 0) row += static_cast<int64_t>(sg.h) * a.c.page;
+        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, row >= 0)) * box * D;
+        const int s = it % ST;
+        if (it >= ST && !mbar_wait(&kempty[s], ((it / ST) & 1) ^ 1, abort_flag, kSiteAtTma)) ok = false;
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) mbar_arrive_expect_tx(&kfull[s], bytes);
+        __syncwarp();
+        if (row >= 0) tma_load_2d(sK + s * C::KV + lane * box * D, &tm_k, &kfull[s], 0, static_cast<int>(row), pol);
+        if (it >= ST && !mbar_wait(&vempty[s], ((it / ST) & 1) ^ 1, abort_flag, kSiteAtTma)) ok = false;
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          // this tile's K is on its way and no V follows it
+          mbar_wait(&kfull[s], (it / ST) & 1, nullptr, kSiteAtDrain);
+          break;
+        }
+        if (lane == 0) mbar_arrive_expect_tx(&vfull[s], bytes);
+        __syncwarp();
+        if (row >= 0) tma_load_2d(sV + s * C::KV + lane * box * D, &tm_v, &vfull[s], 0, static_cast<int>(row), pol);
+      }
+    }
+    if (!ok)  // wait (bounded) for the copies still in flight into this CTA's shared memory
+      for (int j = (it > ST ? it - ST : 0); j < it; ++j) {
+        mbar_wait(&kfull[j % ST], (j / ST) & 1, nullptr, kSiteAtDrain);
+        mbar_wait(&vfull[j % ST], (j / ST) & 1, nullptr, kSiteAtDrain);
+      }
+  } else if (warp == 1) {
+    // ---------------- K . Q ----------------
+    if (lane == 0) {
+      constexpr uint32_t idesc = make_idesc_f16(128, R, BF16, false);
+      int it = 0, seg = 0;
+      bool ok = true;
+      AttnWalk wk(pre, ta.nb, x0, x1);
+      AttnSeg sg;
+      for (; ok && wk.next(pre, heads, sg); ++seg) {
+        const int qb = seg % C::NQ;
+        const uint32_t q_base = smem_u32(sQ + qb * C::QB);
+        if (!mbar_wait(&qfull[qb], (seg / C::NQ) & 1, abort_flag, kSiteAtQk)) break;
+        for (int i = 0; i < sg.n_kt; ++i, ++it) {
+          const int t = it & 1;
+          const uint32_t ph = (it >> 1) & 1;
+          if (!mbar_wait(&afull[t], ph, abort_flag, kSiteAtQk) || !mbar_wait(&sempty[t], ph ^ 1, abort_flag, kSiteAtQk)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint64_t bd = make_sdesc(q_base + (kk >> 2) * R * 128 + (kk & 3) * 32, 16, 1024, kLayoutSW128);
+            umma_f16_ts(tmem + C::S_COL + t * R, tmem + t * C::A_COLS + kk * 8, bd, idesc, kk > 0);
+          }
+          umma_commit(&sfull[t]);
+          umma_commit(&aempty[t]);
+        }
+        if (ok) umma_commit(&qempty[qb]);
+      }
+      umma_commit(&final_bar[0]);  // every MMA issued here has completed before TMEM is released
+      mbar_wait(&final_bar[0], 0, nullptr, kSiteAtFinal);
+    }
+  } else if (warp == 18) {
+    // ---------------- V . P ----------------
+    if (lane == 0) {
+      constexpr uint32_t idesc = make_idesc_f16(128, 2 * R, true, true, true);
+      int it = 0;
+      bool ok = true;
+      AttnWalk wk(pre, ta.nb, x0, x1);
+      AttnSeg sg;
+      while (ok && wk.next(pre, heads, sg)) {
+        for (int i = 0; i < sg.n_kt; ++i, ++it) {
+          const int t = it & 1;
+          const uint32_t ph = (it >> 1) & 1;
+          if (!mbar_wait(&vbfull[t], ph, abort_flag, kSiteAtPv) || !mbar_wait(&pfull[t], ph, abort_flag, kSiteAtPv)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t v_base = smem_u32(sVB + t * C::VB);
+          const uint32_t p_base = smem_u32(sP + t * C::PB);
+          // the second 64 rows of V^T: the next panel, or zeros
+          const uint32_t lbo = D == 128 ? kTile * 128 : smem_u32(smem + C::OFF_Z) - v_base;
+#pragma unroll
+          for (int kk = 0; kk < kTile / 16; ++kk) {
+            const uint64_t ad = make_sdesc(v_base + kk * 2048, lbo, 1024, kLayoutSW128);
+            const uint64_t bd = make_sdesc(p_base + kk * 2048, kTile * 128, 1024, kLayoutSW128);
+            umma_f16(tmem + C::O_COL, ad, bd, idesc, i > 0 || kk > 0);
+          }
+          umma_commit(&pempty[t]);
+          umma_commit(&vbempty[t]);
+        }
+      }
+      umma_commit(&final_bar[1]);
+      mbar_wait(&final_bar[1], 0, nullptr, kSiteAtFinal);
+    }
+  } else if (warp < 6) {
+    // ---------------- K codes -> TMEM (thread = slot) ----------------
+    const int q = warp & 3;
+    const int row = q * 32 + lane;
+    const uint32_t dst = tmem + (static_cast<uint32_t>(q * 32) << 16);
+    const int total = x1 - x0;
+    for (int it = 0; it < total; ++it) {
+      const int s = it % ST, t = it & 1;
+      if (!mbar_wait(&kfull[s], (it / ST) & 1, abort_flag, kSiteAtK)) break;
+      // D = 128: 128-byte rows, 128-byte swizzle; D = 64: 64-byte rows, 64-byte swizzle (16-byte
+      // chunk index exclusive-or bits 7, 8 of the address)
+      const uint8_t* src = sK + s * C::KV + row * D;
+      const int sw = D == 128 ? (row & 7) : ((row >> 1) & 3);
+      uint4 raw[D / 16];
+      uint32_t dep = 0;
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) raw[c] = *reinterpret_cast<const uint4*>(src + ((c ^ sw) << 4));
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) dep |= raw[c].x | raw[c].y | raw[c].z | raw[c].w;
+      asm volatile("" ::"r"(dep));  // every load is complete before the slot is released
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&kempty[s]);
+      if (!mbar_wait(&aempty[t], ((it >> 1) & 1) ^ 1, abort_flag, kSiteAtK)) break;
+      tc_fence_after();
+#pragma unroll
+      for (int p = 0; p < D / 64; ++p) {
+        uint32_t o[32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) codes16<BF16>(raw[4 * p + c], o + 8 * c);
+        tmem_st32(dst + t * C::A_COLS + p * 32, o);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&afull[t]);
+    }
+  } else if (warp < 10) {
+    // ---------------- V codes -> shared memory; Q and the row masks of each segment ----------------
+    const int w = warp - 6;
+    int it = 0, seg = 0;
+    bool ok = true;
+    AttnWalk wk(pre, ta.nb, x0, x1);
+    AttnSeg sg;
+    for (; ok && wk.next(pre, heads, sg); ++seg) {
+      const int64_t b = ta.b0 + sg.b;
+      {
+        const int qb = seg % C::NQ;
+        if (!mbar_wait(&qempty[qb], ((seg / C::NQ) & 1) ^ 1, abort_flag, kSiteAtV)) break;
+        const int nodes = seq_nodes(a, b);
+        const int tid = w * 32 + lane;
+        for (int e = tid; e < R * (D / 8); e += 128) {
+          const int r = e / (D / 8), c = e - r * (D / 8);
+          const int n = (rt * R + r) / grp, g = (rt * R + r) - n * grp;
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (n < a.t) {
+            const T* x = static_cast<const T*>(a.q) + b * a.q_sb + n * a.q_st + (sg.h * grp + g) * a.q_sh + c * 8;
+            if (ta.qvec) {
+              v = *reinterpret_cast<const uint4*>(x);
+            } else {
+              const unsigned short* y = reinterpret_cast<const unsigned short*>(x);
+              v = make_uint4(y[0] | (static_cast<uint32_t>(y[1]) << 16), y[2] | (static_cast<uint32_t>(y[3]) << 16),
+                             y[4] | (static_cast<uint32_t>(y[5]) << 16), y[6] | (static_cast<uint32_t>(y[7]) << 16));
+            }
+          }
+          *reinterpret_cast<uint4*>(sQ + qb * C::QB + (c >> 3) * R * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+        }
+        for (int r = tid; r < R; r += 128) {
+          const int n = (rt * R + r) / grp;
+          rmask[qb * 64 + r] = n < a.t ? node_mask(a, b, n, nodes) : 0ull;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&qfull[qb]);
+      }
+      for (int i = 0; i < sg.n_kt; ++i, ++it) {
+        const int s = it % ST, t = it & 1;
+        if (!mbar_wait(&vfull[s], (it / ST) & 1, abort_flag, kSiteAtV)) {
+          ok = false;
+          break;
+        }
+        if constexpr (D == 128) {
+          // A group of 8 slots per step.  The eight lanes of one shared-memory phase take four chunks
+          // of two slots whose numbers differ in bits 0 and 2, so neither the swizzled read (16-byte
+          // chunks c) nor the write (chunks 2c, 2c + 1 of a bf16 row) meets a bank twice.
+          const int x = lane >> 3;
+          const int tok8 = lane & 4 ? x ^ 5 : x;
+          uint4 raw[8];
+          uint32_t dep = 0;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int tok = (w + 4 * (k >> 1)) * 8 + tok8;
+            const int c = (k & 1) * 4 + (lane & 3);
+            raw[k] = *reinterpret_cast<const uint4*>(sV + s * C::KV + tok * 128 + ((c ^ tok8) << 4));
+            dep |= raw[k].x | raw[k].y | raw[k].z | raw[k].w;
+          }
+          asm volatile("" ::"r"(dep));
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&vempty[s]);
+          if (!mbar_wait(&vbempty[t], ((it >> 1) & 1) ^ 1, abort_flag, kSiteAtV)) {
+            ok = false;
+            break;
+          }
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int tok = (w + 4 * (k >> 1)) * 8 + tok8;
+            uint32_t o[8];
+            codes16<true>(raw[k], o);
+            uint8_t* dst = sVB + t * C::VB + (k & 1) * kTile * 128 + tok * 128;
+            const int c2 = (lane & 3) * 2;
+            *reinterpret_cast<uint4*>(dst + ((c2 ^ tok8) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+            *reinterpret_cast<uint4*>(dst + (((c2 + 1) ^ tok8) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+          }
+        } else {
+          uint4 raw[4];
+          uint32_t dep = 0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int tok = k * 32 + w * 8 + (lane >> 2), c = lane & 3;
+            raw[k] = *reinterpret_cast<const uint4*>(sV + s * C::KV + tok * 64 + ((c ^ ((tok >> 1) & 3)) << 4));
+            dep |= raw[k].x | raw[k].y | raw[k].z | raw[k].w;
+          }
+          asm volatile("" ::"r"(dep));
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&vempty[s]);
+          if (!mbar_wait(&vbempty[t], ((it >> 1) & 1) ^ 1, abort_flag, kSiteAtV)) {
+            ok = false;
+            break;
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int tok = k * 32 + w * 8 + (lane >> 2), c2 = (lane & 3) * 2;
+            uint32_t o[8];
+            codes16<true>(raw[k], o);
+            uint8_t* dst = sVB + t * C::VB + tok * 128;
+            *reinterpret_cast<uint4*>(dst + ((c2 ^ (tok & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+            *reinterpret_cast<uint4*>(dst + (((c2 + 1) ^ (tok & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&vbfull[t]);
+      }
+    }
+  } else {
+    // ---------------- softmax: thread = slot for the scores, = head dimension for the output ----------------
+    const int g = (warp - 10) >> 2;    // rows [g RC, (g + 1) RC) of the block
+    const int w = (warp - 10) & 3;
+    const int q = warp & 3;            // TMEM lanes of this warp
+    const int row = q * 32 + lane;
+    const int tid = w * 32 + lane;
+    const int bar = 1 + g;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(q * 32) << 16);
+    float* gmax = wred + g * 2 * 4 * 32;
+    float* gsum = gmax + 4 * 32;
+    float* mref = refs + g * 2 * 32;
+    float* fac = mref + 32;
+    float* tab = ftab + g * 16 * 32;
+    int it = 0, seg = 0;
+    bool ok = true;
+    AttnWalk wk(pre, ta.nb, x0, x1);
+    AttnSeg sg;
+    for (; ok && wk.next(pre, heads, sg); ++seg) {
+      const int64_t b = ta.b0 + sg.b;
+      const int64_t ctx = seq_ctx(a, b);
+      const int nodes = seq_nodes(a, b);
+      const int64_t keys = ctx + nodes;
+      const int qb = seg % C::NQ;
+      const bool got_q = mbar_wait(&qfull[qb], (seg / C::NQ) & 1, abort_flag, kSiteAtSoft);
+      if (tid < RC) mref[tid] = -INFINITY;
+      if (named_bar_any(bar, 128, !got_q)) break;
+      const unsigned long long* masks = rmask + qb * 64 + g * RC;
+      float l[RC];
+#pragma unroll
+      for (int c = 0; c < RC; ++c) l[c] = 0.f;
+      for (int i = 0; i < sg.n_kt; ++i, ++it) {
+        const int t = it & 1;
+        const uint32_t ph = (it >> 1) & 1;
+        const int64_t j0 = static_cast<int64_t>(sg.kt0 + i) * kTile;
+        const int64_t j = j0 + row;
+        float ks = 0.f, vs = 0.f;
+        bool there = false;
+        if (j < keys) {
+          int64_t kr = kv_row(a.c, b, j);
+          if (kr >= 0) {
+            kr += static_cast<int64_t>(sg.h) * a.c.page;
+            ks = a.c.ks[kr] * a.scale_log2;
+            vs = a.c.vs[kr];
+            there = true;
+          }
+        }
+        // a node's slot is seen by the rows whose mask names it, a context slot by all
+        const int node = j >= ctx ? static_cast<int>(j - ctx) : -1;
+        const bool masked = !there || node >= 0;
+        bool fine = mbar_wait(&sfull[t], ph, abort_flag, kSiteAtSoft);
+        tc_fence_after();
+        float s[RC];
+#pragma unroll
+        for (int c = 0; c < RC; c += 8) tmem_ld8(lanes + C::S_COL + t * R + g * RC + c, reinterpret_cast<uint32_t*>(s) + c);
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sempty[t]);
+        bool over = false;
+        if (masked) {
+#pragma unroll
+          for (int c = 0; c < RC; ++c) {
+            const bool see = there && (node < 0 || ((masks[c] >> node) & 1));
+            s[c] = see ? s[c] * ks : -INFINITY;
+            over |= s[c] > mref[c] + 8.f;
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < RC; ++c) {
+            s[c] *= ks;
+            over |= s[c] > mref[c] + 8.f;
+          }
+        }
+        if (named_bar_any(bar, 128, over || !fine)) {
+          // new references: the rows' maxima over the tile
+          float v[RC];
+#pragma unroll
+          for (int c = 0; c < RC; ++c) v[c] = s[c];
+          const float top = warp_columns<RC, true>(v, lane);
+          if (lane % (32 / RC) == 0) gmax[w * 32 + lane / (32 / RC)] = top;
+          // (the barrier also takes the group's decision to give up)
+          if (named_bar_any(bar, 128, !fine || *abort_flag)) {
+            ok = false;
+            break;
+          }
+          if (tid < RC) {
+            const float old = mref[tid];
+            const float m = fmaxf(fmaxf(fmaxf(gmax[tid], gmax[32 + tid]), fmaxf(gmax[64 + tid], gmax[96 + tid])), old);
+            mref[tid] = m;
+            fac[tid] = m == old ? 1.f : exp2f(old - m);
+          }
+          // the accumulator is still: the last tile's V . P is complete, the next waits for this one's weights
+          if (i > 0) fine = mbar_wait(&pempty[t ^ 1], ((it - 1) >> 1) & 1, abort_flag, kSiteAtSoft);
+          if (named_bar_any(bar, 128, !fine)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < RC; ++c) l[c] *= fac[c];
+          if (i > 0) {
+#pragma unroll
+            for (int c = 0; c < 2 * RC; c += 8) {  // hi, then lo
+              const uint32_t at = lanes + C::O_COL + (c < RC ? g * RC + c : R + g * RC + c - RC);
+              uint32_t o[8];
+              tmem_ld8(at, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fac[(c + e) % RC]);
+              tmem_st8(at, o);
+            }
+            tmem_st_wait();
+            tc_fence_before();
+          }
+        }
+        // weights
+        if (!mbar_wait(&pempty[t], ph ^ 1, abort_flag, kSiteAtSoft)) *abort_flag = 1;
+        uint8_t* prow = sP + t * C::PB + row * 128;
+#pragma unroll
+        for (int c0 = 0; c0 < RC; c0 += 8) {
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float x[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int c = c0 + 2 * e + k;
+              const float m = mref[c];
+              const float p = exp2f(s[c] - (m == -INFINITY ? 0.f : m));
+              l[c] += p;
+              x[k] = s[c] == -INFINITY ? 0.f : p * vs;  // what is not seen adds nothing, whatever its scale
+            }
+            const __nv_bfloat162 h = __floats2bfloat162_rn(x[0], x[1]);
+            hi[e] = *reinterpret_cast<const uint32_t*>(&h);
+            const __nv_bfloat162 r = __floats2bfloat162_rn(x[0] - __uint_as_float(hi[e] << 16),
+                                                           x[1] - __uint_as_float(hi[e] & 0xFFFF0000u));
+            lo[e] = *reinterpret_cast<const uint32_t*>(&r);
+          }
+          const int nh = g * RC + c0, nl = R + nh;  // columns of P
+          *reinterpret_cast<uint4*>(prow + (nh >> 6) * kTile * 128 + ((((nh & 63) >> 3) ^ (row & 7)) << 4)) =
+              make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<uint4*>(prow + (nl >> 6) * kTile * 128 + ((((nl & 63) >> 3) ^ (row & 7)) << 4)) =
+              make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&pfull[t]);
+      }
+      if (!ok) break;
+      // ---- the segment's end: sums of the weights, output or piece ----
+      bool fine = mbar_wait(&pempty[(it - 1) & 1], ((it - 1) >> 1) & 1, abort_flag, kSiteAtSoft);
+      {
+        const float sum = warp_columns<RC, false>(l, lane);
+        if (lane % (32 / RC) == 0) gsum[w * 32 + lane / (32 / RC)] = sum;
+      }
+      if (named_bar_any(bar, 128, !fine || *abort_flag)) break;
+      tc_fence_after();
+      if (lane == 0) mbar_arrive(&qempty[qb]);  // the masks are read no more
+      const bool mine = row < D;                 // this thread's head dimension
+      float o[RC];
+#pragma unroll
+      for (int c = 0; c < RC; c += 8) {
+        uint32_t hi[8], lo[8];
+        tmem_ld8(lanes + C::O_COL + g * RC + c, hi);
+        tmem_ld8(lanes + C::O_COL + R + g * RC + c, lo);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[c + e] = __uint_as_float(hi[e]) + __uint_as_float(lo[e]);
+      }
+      tc_fence_before();
+      float den[RC];
+#pragma unroll
+      for (int c = 0; c < RC; ++c) den[c] = ((gsum[c] + gsum[32 + c]) + gsum[64 + c]) + gsum[96 + c];
+      const int c_first = range_owner(sg.u0, units, groups);
+      const int c_last = range_owner(sg.u0 + sg.tiles - 1, units, groups);
+      bool emit = true;
+      if (c_last > c_first) {
+        constexpr int PIECE = R * D + 2 * R;
+        float* piece = ta.pieces + (static_cast<int64_t>(blockIdx.x) * 2 + sg.slot) * PIECE;
+        if (mine) {
+#pragma unroll
+          for (int c = 0; c < RC; ++c) piece[(g * RC + c) * D + row] = o[c];
+        }
+        if (tid < RC) piece[R * D + g * RC + tid] = mref[tid];
+        if (tid < RC) piece[R * D + R + g * RC + tid] = ((gsum[tid] + gsum[32 + tid]) + gsum[64 + tid]) + gsum[96 + tid];
+        __threadfence();
+        named_bar_sync(bar, 128);
+        int* cnt = ta.counters + (c_first * ta.rts + rt) * 2 + g;
+        if (tid == 0) {
+          const int old = atomicAdd(cnt, 1);
+          const bool last = old == c_last - c_first;
+          if (last) *cnt = 0;
+          fac[0] = last ? 1.f : 0.f;
+        }
+        named_bar_sync(bar, 128);
+        emit = fac[0] != 0.f;
+        if (emit) {
+          __threadfence();
+          // piece p of the (sequence, head): CTA c_first + p's first segment, unless it started before
+          auto piece_of = [&](int p) {
+            const int c = c_first + p;
+            const int slot = range_start(c, units, groups) >= sg.u0 ? 0 : 1;
+            return ta.pieces + (static_cast<int64_t>(c * ta.rts + rt) * 2 + slot) * PIECE;
+          };
+          const int n = c_last - c_first + 1;
+          constexpr int SUB = 128 / RC;  // threads of one row
+          const int c = tid % RC, sub = tid / RC;
+          float m = -INFINITY;
+          for (int p = sub; p < n; p += SUB) m = fmaxf(m, __ldcg(piece_of(p) + R * D + g * RC + c));
+          tab[tid] = m;
+          named_bar_sync(bar, 128);
+          m = tab[c];
+          for (int k = 1; k < SUB; ++k) m = fmaxf(m, tab[c + k * RC]);
+          named_bar_sync(bar, 128);
+          float sum = 0.f;
+          for (int p = sub; p < n; p += SUB) {
+            const float* pp = piece_of(p) + R * D + g * RC + c;
+            const float pm = __ldcg(pp);
+            sum += pm == -INFINITY ? __ldcg(pp + R) : __ldcg(pp + R) * exp2f(pm - m);
+          }
+          tab[tid] = sum;
+          named_bar_sync(bar, 128);
+#pragma unroll
+          for (int e = 0; e < RC; ++e) {
+            float x = tab[e];
+            for (int k = 1; k < SUB; ++k) x += tab[e + k * RC];
+            den[e] = x;
+            o[e] = 0.f;
+          }
+          for (int p0 = 0; p0 < n; p0 += 16) {  // 16 pieces' factors at a time
+            named_bar_sync(bar, 128);
+            for (int e = tid; e < 16 * RC; e += 128) {
+              const int p = p0 + e / RC;
+              // (this thread's row of e is c: 128 is a multiple of RC)
+              float f = 0.f;
+              if (p < n) {
+                const float pm = __ldcg(piece_of(p) + R * D + g * RC + c);
+                f = pm == -INFINITY ? 1.f : exp2f(pm - m);
+              }
+              tab[e] = f;
+            }
+            named_bar_sync(bar, 128);
+            if (mine) {
+              const int n2 = min(16, n - p0);
+              for (int p = 0; p < n2; ++p) {
+                const float* pp = piece_of(p0 + p) + g * RC * D + row;
+#pragma unroll
+                for (int e = 0; e < RC; ++e) o[e] += tab[p * RC + e] * __ldcg(pp + e * D);
+              }
+            }
+          }
+          named_bar_sync(bar, 128);
+        }
+      }
+      if (emit && mine) {
+#pragma unroll
+        for (int c = 0; c < RC; ++c) {
+          const int r = rt * R + g * RC + c;
+          const int n = r / grp, gh = r - n * grp;
+          if (n < a.t) {
+            const float x = den[c] == 0.f || n >= nodes ? 0.f : o[c] / den[c];
+            static_cast<T*>(a.o)[((b * a.t + n) * a.hq + sg.h * grp + gh) * static_cast<int64_t>(D) + row] = from_f32<T>(x);
+          }
+        }
+      }
+      // mref, fac and gsum are free for the next segment once everyone is here
+      named_bar_sync(bar, 128);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, C::COLS);
+}
+
+// Row blocks: the smallest R that holds all rows, 64 at most.
+static int rows_per_cta(int64_t rows) { return rows <= 16 ? 16 : (rows <= 32 ? 32 : 64); }
+
+struct TilePlan {
+  int r, rts, groups, grid;
+  size_t bytes;
+};
+static TilePlan tile_plan(int64_t t, int64_t grp, int64_t d) {
+  TilePlan p;
+  p.r = rows_per_cta(t * grp);
+  p.rts = static_cast<int>((t * grp + p.r - 1) / p.r);
+  p.groups = num_sms() / p.rts > 1 ? num_sms() / p.rts : 1;
+  p.grid = p.groups * p.rts;
+  const size_t counters = (static_cast<size_t>(p.grid) * 2 * sizeof(int) + kAttnCounterBytes - 1) / kAttnCounterBytes *
+                          kAttnCounterBytes;
+  p.bytes = counters + static_cast<size_t>(p.grid) * 2 * (p.r * d + 2 * p.r) * sizeof(float);
+  return p;
+}
+// A tile is made of whole pages or lies inside one.
+static bool tile_dims(int64_t d, int64_t page) {
+  return (d == 64 || d == 128) && page >= 16 && page % 16 == 0 && (kTile % page == 0 || page % kTile == 0);
+}
+
+template <int D, int R, typename T>
+static int launch_tiles(const AttnArgs& a, const TilePlan& p, void* ws, bool qvec, cudaStream_t st) {
+  using C = ACfg<D, R>;
+  static std::once_flag once[64];
+  static cudaError_t attr_err[64];
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev)) return check_cuda(e, "cudaGetDevice");
+  dev &= 63;
+  std::call_once(once[dev], [&] {
+    attr_err[dev] = cudaFuncSetAttribute(attn_tile_kernel<D, R, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  });
+  if (int s = check_cuda(attr_err[dev], "cudaFuncSetAttribute(attn_tile_kernel)")) return s;
+  CUtensorMap tk, tv;
+  const uint64_t rows = static_cast<uint64_t>(a.c.pages) * a.c.heads * a.c.page;
+  const uint32_t box = a.c.page < kTile ? a.c.page : kTile;
+  const CUtensorMapSwizzle swz = D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+  if (int s = make_tmap_2d(&tk, a.c.k, CU_TENSOR_MAP_DATA_TYPE_UINT8, rows, D, D, box, D, swz)) return s;
+  if (int s = make_tmap_2d(&tv, a.c.v, CU_TENSOR_MAP_DATA_TYPE_UINT8, rows, D, D, box, D, swz)) return s;
+  TileArgs ta = {};
+  ta.a = a;
+  ta.rts = p.rts;
+  ta.groups = p.groups;
+  ta.qvec = qvec;
+  ta.counters = static_cast<int*>(ws);
+  ta.pieces = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + p.bytes -
+                                       static_cast<size_t>(p.grid) * 2 * (R * D + 2 * R) * sizeof(float));
+  for (int64_t b0 = 0; b0 < a.b; b0 += kAttnMaxBatch) {
+    ta.b0 = b0;
+    ta.nb = static_cast<int>(a.b - b0 < kAttnMaxBatch ? a.b - b0 : kAttnMaxBatch);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.grid);
+    cfg.blockDim = dim3(kAttnThreads);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (int s = check_cuda(cudaLaunchKernelEx(&cfg, attn_tile_kernel<D, R, T>, tk, tv, ta),
+                           "cudaLaunchKernelEx(attn_tile_kernel)"))
+      return s;
+  }
+  return BW_OK;
+}
+
+template <int D, int R>
+static int launch_tiles_dt(const AttnArgs& a, const TilePlan& p, void* ws, bool qvec, int dtype, cudaStream_t st) {
+  return dtype == BW_DTYPE_BF16 ? launch_tiles<D, R, __nv_bfloat16>(a, p, ws, qvec, st)
+                                : launch_tiles<D, R, __half>(a, p, ws, qvec, st);
+}
+template <int D>
+static int launch_tiles_d(const AttnArgs& a, const TilePlan& p, void* ws, bool qvec, int dtype, cudaStream_t st) {
+  switch (p.r) {
+    case 16: return launch_tiles_dt<D, 16>(a, p, ws, qvec, dtype, st);
+    case 32: return launch_tiles_dt<D, 32>(a, p, ws, qvec, dtype, st);
+    default: return launch_tiles_dt<D, 64>(a, p, ws, qvec, dtype, st);
+  }
+}
+
+}  // namespace bw
+
+extern "C" size_t bw_tree_attention_int8_workspace_size(int64_t b, int64_t t, int64_t hq, int64_t heads, int64_t d) {
+  if (b <= 0 || t <= 0 || t > bw::kTreeMaxNodes || heads <= 0 || hq < heads || hq > 65535 || (d != 64 && d != 128))
+    return 0;
+  return bw::tile_plan(t, hq / heads, d).bytes;
+}
+
+extern "C" size_t bw_tree_attention_int8_workspace_zeroed_bytes(int64_t b, int64_t t, int64_t hq, int64_t heads,
                                                                 int64_t d) {
-  (void)b, (void)t, (void)hq, (void)hk, (void)d;
-  return 0;
+  const size_t all = bw_tree_attention_int8_workspace_size(b, t, hq, heads, d);
+  if (all == 0) return 0;
+  const bw::TilePlan p = bw::tile_plan(t, hq / heads, d);
+  return all - static_cast<size_t>(p.grid) * 2 * (p.r * d + 2 * p.r) * sizeof(float);
 }
 
 extern "C" int bw_tree_attention_int8(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int dtype, void* out,
@@ -127,7 +1019,6 @@ extern "C" int bw_tree_attention_int8(const void* q, int64_t q_sb, int64_t q_st,
                                       int64_t t, int64_t hq, float softmax_scale, void* workspace,
                                       size_t workspace_bytes, void* stream) {
   using namespace bw;
-  (void)workspace, (void)workspace_bytes;
   AttnArgs a = {};
   a.c.k = const_cast<int8_t*>(cache_k);
   a.c.v = const_cast<int8_t*>(cache_v);
@@ -164,6 +1055,20 @@ extern "C" int bw_tree_attention_int8(const void* q, int64_t q_sb, int64_t q_st,
   a.hq = static_cast<int>(hq);
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // the tensor-core kernel's units are counted in 32 bits, its cache rows addressed in them
+  const int64_t units = b * heads * ((table_cols * page + kTile - 1) / kTile + 1);
+  if (tile_dims(d, page) && units < INT32_MAX && pages > 0 && pages * heads * page < INT32_MAX &&
+      reinterpret_cast<uintptr_t>(cache_k) % 16 == 0 && reinterpret_cast<uintptr_t>(cache_v) % 16 == 0) {
+    const TilePlan p = tile_plan(t, hq / heads, d);
+    if (workspace == nullptr || workspace_bytes < p.bytes)
+      return fail(BW_ERR_WORKSPACE, "tree_attention_int8: workspace of %zu bytes required, %zu given", p.bytes,
+                  workspace_bytes);
+    if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
+      return fail(BW_ERR_WORKSPACE, "tree_attention_int8: workspace must be 256-byte aligned");
+    const bool qvec = reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_sb % 8 == 0 && q_st % 8 == 0 && q_sh % 8 == 0;
+    return d == 128 ? launch_tiles_d<128>(a, p, workspace, qvec, dtype, st)
+                    : launch_tiles_d<64>(a, p, workspace, qvec, dtype, st);
+  }
   const dim3 grid(static_cast<unsigned>(hq), static_cast<unsigned>(t), static_cast<unsigned>(b));
   if (dtype == BW_DTYPE_BF16) attn_rows_kernel<__nv_bfloat16><<<grid, 32 * kRowWarps, 0, st>>>(a);
   else attn_rows_kernel<__half><<<grid, 32 * kRowWarps, 0, st>>>(a);
