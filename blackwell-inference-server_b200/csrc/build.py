@@ -3,7 +3,8 @@
     python blackwell-inference-server_b200/csrc/build.py [--verbose]
 
 Compiles every ``*.cu`` here with nvcc for ``-gencode arch=compute_100a,code=sm_100a``
-(relocatable device code, so the kernels share one device status word), links
+(relocatable device code, so the kernels share one device status word; one file is a
+whole program and gets the word's address), links
 them into ``blackwell_ops/_lib/libbw_ops.so`` next to the Python package, and
 skips objects whose sources and headers are unchanged.  No ``--use_fast_math``:
 the quantiser and merge must use IEEE division and round-to-nearest-even.
@@ -26,7 +27,10 @@ OBJ_DIR = CSRC / "_build"
 INCLUDE = CSRC.parent.parent / "include"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-CFLAGS = ["-O3", "-std=c++17", "-lineinfo", "-rdc=true", "-Xcompiler", "-fPIC,-O2", "-I", str(INCLUDE)]
+CFLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-O2", "-I", str(INCLUDE)]
+# Compiled on its own: ptxas ignores setmaxnreg in relocatable device code.  Such a file defines
+# BW_WHOLE_PROGRAM and gets the shared status word's address from the host.
+WHOLE_PROGRAM = {"tree_attention.cu"}
 
 
 def nvcc() -> str:
@@ -58,7 +62,8 @@ def build(verbose: bool = False, ptxas_verbose: bool = False) -> Path:
         obj = OBJ_DIR / (src.stem + ".o")
         if not _stale(obj, src) and not ptxas_verbose:
             return obj, ""
-        cmd = [cc, *ARCH, *CFLAGS, *extra, "-c", str(src), "-o", str(obj)]
+        rdc = [] if src.name in WHOLE_PROGRAM else ["-rdc=true"]
+        cmd = [cc, *ARCH, *CFLAGS, *rdc, *extra, "-c", str(src), "-o", str(obj)]
         if verbose:
             print(" ".join(cmd), flush=True)
         r = subprocess.run(cmd, capture_output=True, text=True)

@@ -72,6 +72,25 @@ int require_sm100() {
 
 int dtype_size(int dtype) { return dtype == BW_DTYPE_F32 ? 4 : 2; }
 
+int device_wait_ptrs(int** status, const long long** limit) {
+  static int* st[64];
+  static long long* lim[64];
+  static cudaError_t err[64];
+  static std::once_flag once[64];
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev)) return check_cuda(e, "cudaGetDevice");
+  dev &= 63;
+  std::call_once(once[dev], [dev] {
+    err[dev] = cudaGetSymbolAddress(reinterpret_cast<void**>(&st[dev]), g_status);
+    if (err[dev] == cudaSuccess)
+      err[dev] = cudaGetSymbolAddress(reinterpret_cast<void**>(&lim[dev]), g_wait_limit_cycles);
+  });
+  if (int s = check_cuda(err[dev], "cudaGetSymbolAddress")) return s;
+  *status = st[dev];
+  *limit = lim[dev];
+  return BW_OK;
+}
+
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);

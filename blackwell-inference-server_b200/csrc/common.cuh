@@ -31,6 +31,10 @@ constexpr size_t kGemmCounterBytes = kGemmCounterSlots * sizeof(int);
 // ---------------------------------------------------------------------------
 // device status word (first failure wins) and the wait limit
 // ---------------------------------------------------------------------------
+// A file compiled as a whole program (BW_WHOLE_PROGRAM: no relocatable device code, without which
+// ptxas ignores setmaxnreg) cannot name another file's device variables: its kernels get their
+// addresses from the host (device_wait_ptrs) and wait with mbar_wait_at.
+#ifndef BW_WHOLE_PROGRAM
 extern __device__ int g_status;  // 0 = ok, else wait-site id
 // Bound of every spin wait, in SM cycles: the limit in ns x 2.5 (no SM clock is
 // above 2.5 GHz, so a wait never gives up before the limit).  Set per device by
@@ -41,6 +45,7 @@ __device__ __forceinline__ long long wait_limit_cycles() {
 }
 
 __device__ __forceinline__ void record_timeout(int site) { atomicCAS(&g_status, 0, site); }
+#endif
 
 // ---------------------------------------------------------------------------
 // device-side phase trace (off unless bw_trace_enable gave a buffer)
@@ -51,6 +56,7 @@ __device__ __forceinline__ void record_timeout(int site) { atomicCAS(&g_status, 
 // (stamp 0 = phase not reached).  The host groups records by gridid (one
 // launch) and reads the phases; nothing is written while tracing is off.
 // ---------------------------------------------------------------------------
+#ifndef BW_WHOLE_PROGRAM
 struct TraceState {
   unsigned long long* buf;  // null: tracing off
   unsigned int records;     // capacity
@@ -81,6 +87,7 @@ __device__ __forceinline__ uint64_t globaltimer_now();
 __device__ __forceinline__ void trace_stamp(unsigned long long* rec, int e) {
   if (rec != nullptr) rec[3 + e] = globaltimer_now();
 }
+#endif
 
 // Acquire load at GPU scope (a flag another CTA publishes with a release or a fence).
 __device__ __forceinline__ int ld_acquire_gpu(const int* p) {
@@ -148,6 +155,7 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 // records `site`) if it did not within the wait limit (measured with the SM
 // cycle counter, assuming at most 2.5 GHz so the bound is never shorter), or if
 // another thread of the CTA has already flagged an abort through `abort_flag`.
+#ifndef BW_WHOLE_PROGRAM
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int site) {
   if (mbar_try_wait(bar, parity)) return true;
   const long long limit = wait_limit_cycles();
@@ -159,6 +167,32 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
       if (clock64() - t0 > limit) {
         record_timeout(site);
         if (abort_flag != nullptr) *abort_flag = 1;
+        return false;
+      }
+    }
+  }
+}
+#endif
+
+// The same with the status word and the limit (SM cycles) at given addresses.
+struct WaitControl {
+  volatile int abort;     // a role of the CTA has given up
+  int* status;
+  const long long* limit;
+};
+__device__ __forceinline__ bool mbar_wait_at(uint64_t* bar, uint32_t parity, WaitControl* w, int site,
+                                             bool heed_abort = true) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  long long limit = -1;
+  for (uint32_t i = 1;; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 63u) == 0u) {
+      if (heed_abort && w->abort) return false;
+      if (limit < 0) limit = *static_cast<const volatile long long*>(w->limit);
+      if (clock64() - t0 > limit) {
+        atomicCAS(w->status, 0, site);
+        w->abort = 1;
         return false;
       }
     }
@@ -203,6 +237,7 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t pa
       : "memory");
   return ok != 0;
 }
+#ifndef BW_WHOLE_PROGRAM
 __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
                                                   int site) {
   const long long limit = wait_limit_cycles();
@@ -216,6 +251,8 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
     }
   }
 }
+
+#endif
 
 // ---------------------------------------------------------------------------
 // named barriers
@@ -386,6 +423,15 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
                : "memory");
 }
 
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
 // 32 lanes x 32 bit, 16 consecutive columns per thread.
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
@@ -495,4 +541,6 @@ int dtype_size(int dtype);
 int make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dt, uint64_t rows, uint64_t cols,
                  uint64_t ld_bytes, uint32_t box_rows, uint32_t box_cols, CUtensorMapSwizzle swz);
 int num_sms();
+// Device addresses of the current device's status word and wait limit.
+int device_wait_ptrs(int** status, const long long** limit);
 }  // namespace bw

@@ -9,6 +9,7 @@
 #include <mutex>
 #include <type_traits>
 
+#define BW_WHOLE_PROGRAM
 #include "kv_cache.cuh"
 
 namespace bw {
@@ -133,12 +134,18 @@ __global__ void __launch_bounds__(32 * kRowWarps) attn_rows_kernel(const __grid_
 // is joined by its last CTA (a ticket) from the pieces in the workspace, in range order, so results
 // do not depend on timing.
 //
-// One CTA per SM, 19 warps: 0 TMA (one box per page), 1 issues K.Q, 18 issues V.P, 2-5 dequantise K
-// into TMEM (thread = slot), 6-9 dequantise V into shared memory and load Q, 10-17 two softmax groups
-// of half the rows each.
+// One CTA per SM, five warpgroups: 0 TMA (one box per page) and scales, 1 issues K.Q, 2 issues V.P;
+// 4-7 dequantise K into TMEM (thread = slot); 8-11 dequantise V into shared memory and load Q; 12-15
+// and 16-19 are two softmax groups of half the rows each.
 // ---------------------------------------------------------------------------
 constexpr int kTile = 128;
-constexpr int kAttnThreads = 19 * 32;
+constexpr int kAttnThreads = 20 * 32;
+// Registers of a thread of the five warpgroups after setmaxnreg: their sum is five times the 96 that
+// a thread of 640 has at launch.
+constexpr int kRegsIssue = 56, kRegsK = 88, kRegsV = 80, kRegsSoft = 128;
+static_assert(kRegsIssue + kRegsK + kRegsV + 2 * kRegsSoft == 5 * 96, "register split");
+constexpr int kScaleStages = 4;   // tiles whose scales are on their way or in use
+constexpr float kLowest = -3.0e38f;  // a row's reference before any score: finite, so differences are
 constexpr int kAttnMaxBatch = 1024;  // sequences of one launch (their unit ranges lie in shared memory)
 constexpr size_t kAttnCounterBytes = 4096;
 enum AttnSite : int { kSiteAtTma = 80, kSiteAtDrain, kSiteAtK, kSiteAtV, kSiteAtQk, kSiteAtPv, kSiteAtSoft, kSiteAtFinal };
@@ -157,7 +164,8 @@ struct ACfg {
   static constexpr int OFF_P = OFF_Z + ZB;
   static constexpr int OFF_Q = OFF_P + 2 * PB;
   static constexpr int OFF_RING = OFF_Q + NQ * QB;
-  static constexpr int CTRL = 512 + 2 * 4 * 32 * 4 * 2 + 2 * 2 * 32 * 4 + 2 * 16 * 32 * 4 + 2 * 64 * 8 +
+  static constexpr int SCALES = kScaleStages * (2 * kTile * 4 + 16);
+  static constexpr int CTRL = 640 + SCALES + 2 * 4 * 32 * 4 * 2 + 2 * 2 * 32 * 4 + (2 * 128 + 32) * 4 + 2 * 64 * 8 +
                               (kAttnMaxBatch + 1) * 4 + 64;
   static constexpr int ROOM = 227 * 1024 - 1024 - OFF_RING - CTRL;
   static constexpr int ST = ROOM / (2 * KV) < 6 ? ROOM / (2 * KV) : 6;  // stages of a K and a V tile
@@ -180,6 +188,8 @@ struct TileArgs {
   int qvec;        // q rows are 16-byte aligned
   float* pieces;   // [grid][2][R][D] fp32 accumulators, then [R] m, [R] l each
   int* counters;   // [grid][2]
+  int* status;     // where a wait that runs out is recorded, and its limit
+  const long long* limit;
 };
 
 // The units of one CTA's range, one (sequence, head) segment after another.
@@ -235,6 +245,29 @@ __device__ __forceinline__ int seq_nodes(const AttnArgs& a, int64_t b) {
   return n < 0 ? 0 : (n < a.t ? n : a.t);
 }
 __device__ __forceinline__ int64_t seq_ctx(const AttnArgs& a, int64_t b) { return a.ctx[b] > 0 ? a.ctx[b] : 0; }
+
+template <int N>
+__device__ __forceinline__ void setmaxnreg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void setmaxnreg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// 2^x to 2 ulps; 0 for -inf and below the normal range.
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 16 bytes global -> shared without registers; zeros, and nothing read, if !have.
+__device__ __forceinline__ void cp_async16_zfill(void* dst, const void* src, bool have) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(have ? 16 : 0)
+               : "memory");
+}
+// One arrival on `bar` when this thread's copies so far are complete.
+__device__ __forceinline__ void cp_async_arrive_noinc(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // 16 codes -> 16 fp16 or bf16 values.
 template <bool BF16>
@@ -301,15 +334,19 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   uint64_t* pempty = pfull + 2;       //    (and the accumulator holds the tile's contribution)
   uint64_t* qfull = pempty + 2;       // 2: Q and the row masks of a segment
   uint64_t* qempty = qfull + 2;
-  uint64_t* final_bar = qempty + 2;   // 2
+  uint64_t* scfull = qempty + 2;      // scales of a tile
+  uint64_t* scempty = scfull + kScaleStages;
+  uint64_t* final_bar = scempty + kScaleStages;  // 2
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(final_bar + 2);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float* wred = reinterpret_cast<float*>(smem + C::OFF_CTRL + 512);  // [2 groups][2][4 warps][32]
+  WaitControl* ctl = reinterpret_cast<WaitControl*>(tmem_slot + 2);
+  float* sScale = reinterpret_cast<float*>(smem + C::OFF_CTRL + 640);  // [stages][2][128]: ks, vs
+  uint32_t* sPages = reinterpret_cast<uint32_t*>(sScale + kScaleStages * 2 * kTile);  // [stages]: pages that exist
+  float* wred = reinterpret_cast<float*>(smem + C::OFF_CTRL + 640 + C::SCALES);  // [2 groups][2][4 warps][32]
   float* refs = wred + 2 * 2 * 4 * 32;                               // [2 groups][2][32]: m, its factor
-  float* ftab = refs + 2 * 2 * 32;                                   // [2 groups][16][32]
-  unsigned long long* rmask = reinterpret_cast<unsigned long long*>(ftab + 2 * 16 * 32);  // [2][64]
+  float* ftab = refs + 2 * 2 * 32;                                   // [2 groups][128], 32 zeros
+  unsigned long long* rmask = reinterpret_cast<unsigned long long*>(ftab + 2 * 128 + 32);  // [2][64]
   int* pre = reinterpret_cast<int*>(rmask + 2 * 64);                 // [nb + 1] first unit of a sequence
-  static_assert((4 * 6 + 18) * 8 + 8 <= 512, "barriers");
+  static_assert((4 * 6 + 22 + 2 * kScaleStages) * 8 + 8 + sizeof(WaitControl) <= 640, "barriers");
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -336,7 +373,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       mbar_init(&qempty[i], 9);  // the last K.Q of the segment, and the softmax warps
       mbar_init(&final_bar[i], 1);
     }
-    *abort_flag = 0;
+    for (int i = 0; i < kScaleStages; ++i) {
+      mbar_init(&scfull[i], 33);  // each lane's copies, and the page word
+      mbar_init(&scempty[i], 8);
+    }
+    ctl->abort = 0;
+    for (int i = 0; i < 32; ++i) ftab[2 * 128 + i] = 0.f;
+    ctl->status = ta.status;
+    ctl->limit = ta.limit;
     fence_mbar_init();
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
@@ -383,50 +427,88 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   const int x0 = gi < groups ? range_start(gi, units, groups) : 0;
   const int x1 = gi < groups ? range_start(gi + 1, units, groups) : 0;  // an empty range: nothing to do
 
-  if (warp == 0) {
-    // ---------------- TMA: one box of K and one of V per page of the tile ----------------
-    const int box = min(a.c.page, kTile);  // rows of a box
-    const int per = kTile / box;           // boxes of a tile
+  if (warp < 4) setmaxnreg_dec<kRegsIssue>();
+  if (warp == 0 || warp == 3) {
+    // ---------------- warp 0: K and V by TMA, one box per page of the tile; warp 3: the scales ----------------
+    const int box = min(a.c.page, kTile);           // rows of a box
+    const int per = kTile / box;                    // boxes of a tile
+    const int tiles_pp = max(a.c.page / kTile, 1);  // tiles of a page
     const uint64_t pol = ta.rts > 1 ? l2_policy_evict_normal() : l2_policy_evict_first();
-    int it = 0;
-    bool ok = true;
+    // lane i looks up the page of box i (of the box its four slots' scales lie in) one tile ahead
+    const int my_box = warp == 0 ? lane : lane * 4 / box;
     AttnWalk wk(pre, ta.nb, x0, x1);
     AttnSeg sg;
-    while (ok && wk.next(pre, heads, sg)) {
-      const int64_t b = ta.b0 + sg.b;
-      const int64_t keys = seq_ctx(a, b) + seq_nodes(a, b);
-      for (int i = 0; i < sg.n_kt; ++i, ++it) {
-        const int64_t slot = static_cast<int64_t>(sg.kt0 + i) * kTile + lane * box;
-        int64_t row = -1;
-        if (lane < per && slot < keys) row = kv_row(a.c, b, slot);
-        if (row >= 0) row += static_cast<int64_t>(sg.h) * a.c.page;
-        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, row >= 0)) * box * D;
+    sg.n_kt = 0;
+    int i_seg = 0;
+    int64_t keys = 0;
+    const int* table = nullptr;
+    int pg = -1;       // the looked-up page, not yet checked against the cache
+    int pg_row = 0;    // first row of the box (or four slots) in its (page, head)
+    auto look_up = [&]() {
+      if (i_seg == sg.n_kt) {
+        if (!wk.next(pre, heads, sg)) return;
+        i_seg = 0;
+        const int64_t room = static_cast<int64_t>(a.c.table_cols) * a.c.page;
+        keys = seq_ctx(a, ta.b0 + sg.b) + seq_nodes(a, ta.b0 + sg.b);
+        keys = keys < room ? keys : room;
+        table = a.c.table + (ta.b0 + sg.b) * a.c.table_ld;
+      }
+      const int kt = sg.kt0 + i_seg++;
+      const int pi = tiles_pp > 1 ? kt / tiles_pp : kt * per + my_box;
+      pg_row = sg.h * a.c.page + (tiles_pp > 1 ? (kt - pi * tiles_pp) * kTile : 0) + (warp == 3 ? lane * 4 % box : 0);
+      pg = -1;
+      if (my_box < per && static_cast<int64_t>(kt) * kTile + my_box * box < keys) pg = table[pi];
+    };
+    const int total = x1 - x0;
+    if (total > 0) look_up();
+    const int page_rows = heads * a.c.page;
+    bool ok = true;
+    int it = 0;
+    for (; it < total; ++it) {
+      const bool have = pg >= 0 && pg < a.c.pages;
+      const int row = have ? pg * page_rows + pg_row : 0;
+      if (it + 1 < total) look_up();
+      const uint32_t boxes = __ballot_sync(0xffffffffu, have);
+      if (warp == 0) {
+        const uint32_t bytes = __popc(boxes) * box * D;
         const int s = it % ST;
-        if (it >= ST && !mbar_wait(&kempty[s], ((it / ST) & 1) ^ 1, abort_flag, kSiteAtTma)) ok = false;
+        if (it >= ST) ok = mbar_wait_at(&kempty[s], ((it / ST) & 1) ^ 1, ctl, kSiteAtTma);
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
           break;
         }
         if (lane == 0) mbar_arrive_expect_tx(&kfull[s], bytes);
         __syncwarp();
-        if (row >= 0) tma_load_2d(sK + s * C::KV + lane * box * D, &tm_k, &kfull[s], 0, static_cast<int>(row), pol);
-        if (it >= ST && !mbar_wait(&vempty[s], ((it / ST) & 1) ^ 1, abort_flag, kSiteAtTma)) ok = false;
+        if (have) tma_load_2d(sK + s * C::KV + lane * box * D, &tm_k, &kfull[s], 0, row, pol);
+        if (it >= ST) ok = mbar_wait_at(&vempty[s], ((it / ST) & 1) ^ 1, ctl, kSiteAtTma);
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
-          // this tile's K is on its way and no V follows it
-          mbar_wait(&kfull[s], (it / ST) & 1, nullptr, kSiteAtDrain);
+          mbar_wait_at(&kfull[s], (it / ST) & 1, ctl, kSiteAtDrain, false);  // this tile's K has no V behind it
           break;
         }
         if (lane == 0) mbar_arrive_expect_tx(&vfull[s], bytes);
         __syncwarp();
-        if (row >= 0) tma_load_2d(sV + s * C::KV + lane * box * D, &tm_v, &vfull[s], 0, static_cast<int>(row), pol);
+        if (have) tma_load_2d(sV + s * C::KV + lane * box * D, &tm_v, &vfull[s], 0, row, pol);
+      } else {
+        const int sc = it % kScaleStages;
+        if (it >= kScaleStages) ok = mbar_wait_at(&scempty[sc], ((it / kScaleStages) & 1) ^ 1, ctl, kSiteAtTma);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        float* dst = sScale + sc * 2 * kTile + lane * 4;
+        cp_async16_zfill(dst, a.c.ks + row, have);
+        cp_async16_zfill(dst + kTile, a.c.vs + row, have);
+        cp_async_arrive_noinc(&scfull[sc]);
+        if (lane == 0) {
+          sPages[sc] = boxes;  // bit l: slots 4 l .. 4 l + 3 exist
+          mbar_arrive(&scfull[sc]);
+        }
       }
     }
-    if (!ok)  // wait (bounded) for the copies still in flight into this CTA's shared memory
+    if (warp == 0 && !ok)  // wait (bounded) for the copies still in flight into this CTA's shared memory
       for (int j = (it > ST ? it - ST : 0); j < it; ++j) {
-        mbar_wait(&kfull[j % ST], (j / ST) & 1, nullptr, kSiteAtDrain);
-        mbar_wait(&vfull[j % ST], (j / ST) & 1, nullptr, kSiteAtDrain);
+        mbar_wait_at(&kfull[j % ST], (j / ST) & 1, ctl, kSiteAtDrain, false);
+        mbar_wait_at(&vfull[j % ST], (j / ST) & 1, ctl, kSiteAtDrain, false);
       }
+    if (warp == 3) cp_async_wait_all();
   } else if (warp == 1) {
     // ---------------- K . Q ----------------
     if (lane == 0) {
@@ -438,11 +520,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       for (; ok && wk.next(pre, heads, sg); ++seg) {
         const int qb = seg % C::NQ;
         const uint32_t q_base = smem_u32(sQ + qb * C::QB);
-        if (!mbar_wait(&qfull[qb], (seg / C::NQ) & 1, abort_flag, kSiteAtQk)) break;
+        if (!mbar_wait_at(&qfull[qb], (seg / C::NQ) & 1, ctl, kSiteAtQk)) break;
         for (int i = 0; i < sg.n_kt; ++i, ++it) {
           const int t = it & 1;
           const uint32_t ph = (it >> 1) & 1;
-          if (!mbar_wait(&afull[t], ph, abort_flag, kSiteAtQk) || !mbar_wait(&sempty[t], ph ^ 1, abort_flag, kSiteAtQk)) {
+          if (!mbar_wait_at(&afull[t], ph, ctl, kSiteAtQk) || !mbar_wait_at(&sempty[t], ph ^ 1, ctl, kSiteAtQk)) {
             ok = false;
             break;
           }
@@ -458,9 +540,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         if (ok) umma_commit(&qempty[qb]);
       }
       umma_commit(&final_bar[0]);  // every MMA issued here has completed before TMEM is released
-      mbar_wait(&final_bar[0], 0, nullptr, kSiteAtFinal);
+      mbar_wait_at(&final_bar[0], 0, ctl, kSiteAtFinal, false);
     }
-  } else if (warp == 18) {
+  } else if (warp == 2) {
     // ---------------- V . P ----------------
     if (lane == 0) {
       constexpr uint32_t idesc = make_idesc_f16(128, 2 * R, true, true, true);
@@ -472,7 +554,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         for (int i = 0; i < sg.n_kt; ++i, ++it) {
           const int t = it & 1;
           const uint32_t ph = (it >> 1) & 1;
-          if (!mbar_wait(&vbfull[t], ph, abort_flag, kSiteAtPv) || !mbar_wait(&pfull[t], ph, abort_flag, kSiteAtPv)) {
+          if (!mbar_wait_at(&vbfull[t], ph, ctl, kSiteAtPv) || !mbar_wait_at(&pfull[t], ph, ctl, kSiteAtPv)) {
             ok = false;
             break;
           }
@@ -492,47 +574,47 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         }
       }
       umma_commit(&final_bar[1]);
-      mbar_wait(&final_bar[1], 0, nullptr, kSiteAtFinal);
+      mbar_wait_at(&final_bar[1], 0, ctl, kSiteAtFinal, false);
     }
-  } else if (warp < 6) {
+  } else if (warp < 8) {
     // ---------------- K codes -> TMEM (thread = slot) ----------------
     const int q = warp & 3;
     const int row = q * 32 + lane;
     const uint32_t dst = tmem + (static_cast<uint32_t>(q * 32) << 16);
+    setmaxnreg_dec<kRegsK>();
     const int total = x1 - x0;
     for (int it = 0; it < total; ++it) {
       const int s = it % ST, t = it & 1;
-      if (!mbar_wait(&kfull[s], (it / ST) & 1, abort_flag, kSiteAtK)) break;
+      if (!mbar_wait_at(&kfull[s], (it / ST) & 1, ctl, kSiteAtK)) break;
       // D = 128: 128-byte rows, 128-byte swizzle; D = 64: 64-byte rows, 64-byte swizzle (16-byte
       // chunk index exclusive-or bits 7, 8 of the address)
       const uint8_t* src = sK + s * C::KV + row * D;
       const int sw = D == 128 ? (row & 7) : ((row >> 1) & 3);
-      uint4 raw[D / 16];
+      if (!mbar_wait_at(&aempty[t], ((it >> 1) & 1) ^ 1, ctl, kSiteAtK)) break;
+      tc_fence_after();
       uint32_t dep = 0;
-#pragma unroll
-      for (int c = 0; c < D / 16; ++c) raw[c] = *reinterpret_cast<const uint4*>(src + ((c ^ sw) << 4));
-#pragma unroll
-      for (int c = 0; c < D / 16; ++c) dep |= raw[c].x | raw[c].y | raw[c].z | raw[c].w;
-      asm volatile("" ::"r"(dep));  // every load is complete before the slot is released
+#pragma unroll 1
+      for (int c = 0; c < D / 16; c += 2) {
+        const uint4 r0 = *reinterpret_cast<const uint4*>(src + ((c ^ sw) << 4));
+        const uint4 r1 = *reinterpret_cast<const uint4*>(src + (((c + 1) ^ sw) << 4));
+        uint32_t o[16];
+        codes16<BF16>(r0, o);
+        codes16<BF16>(r1, o + 8);
+        tmem_st16(dst + t * C::A_COLS + c * 8, o);
+        dep |= o[7] | o[15];
+      }
+      asm volatile("" ::"r"(dep));  // the last loads are complete before the slot is released
       __syncwarp();
       if (lane == 0) mbar_arrive(&kempty[s]);
-      if (!mbar_wait(&aempty[t], ((it >> 1) & 1) ^ 1, abort_flag, kSiteAtK)) break;
-      tc_fence_after();
-#pragma unroll
-      for (int p = 0; p < D / 64; ++p) {
-        uint32_t o[32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) codes16<BF16>(raw[4 * p + c], o + 8 * c);
-        tmem_st32(dst + t * C::A_COLS + p * 32, o);
-      }
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&afull[t]);
     }
-  } else if (warp < 10) {
+  } else if (warp < 12) {
+    setmaxnreg_dec<kRegsV>();
     // ---------------- V codes -> shared memory; Q and the row masks of each segment ----------------
-    const int w = warp - 6;
+    const int w = warp - 8;
     int it = 0, seg = 0;
     bool ok = true;
     AttnWalk wk(pre, ta.nb, x0, x1);
@@ -541,7 +623,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       const int64_t b = ta.b0 + sg.b;
       {
         const int qb = seg % C::NQ;
-        if (!mbar_wait(&qempty[qb], ((seg / C::NQ) & 1) ^ 1, abort_flag, kSiteAtV)) break;
+        if (!mbar_wait_at(&qempty[qb], ((seg / C::NQ) & 1) ^ 1, ctl, kSiteAtV)) break;
         const int nodes = seq_nodes(a, b);
         const int tid = w * 32 + lane;
         for (int e = tid; e < R * (D / 8); e += 128) {
@@ -570,68 +652,55 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       }
       for (int i = 0; i < sg.n_kt; ++i, ++it) {
         const int s = it % ST, t = it & 1;
-        if (!mbar_wait(&vfull[s], (it / ST) & 1, abort_flag, kSiteAtV)) {
+        if (!mbar_wait_at(&vfull[s], (it / ST) & 1, ctl, kSiteAtV)) {
           ok = false;
           break;
         }
-        if constexpr (D == 128) {
-          // A group of 8 slots per step.  The eight lanes of one shared-memory phase take four chunks
-          // of two slots whose numbers differ in bits 0 and 2, so neither the swizzled read (16-byte
-          // chunks c) nor the write (chunks 2c, 2c + 1 of a bf16 row) meets a bank twice.
-          const int x = lane >> 3;
-          const int tok8 = lane & 4 ? x ^ 5 : x;
-          uint4 raw[8];
-          uint32_t dep = 0;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int tok = (w + 4 * (k >> 1)) * 8 + tok8;
-            const int c = (k & 1) * 4 + (lane & 3);
-            raw[k] = *reinterpret_cast<const uint4*>(sV + s * C::KV + tok * 128 + ((c ^ tok8) << 4));
-            dep |= raw[k].x | raw[k].y | raw[k].z | raw[k].w;
-          }
-          asm volatile("" ::"r"(dep));
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&vempty[s]);
-          if (!mbar_wait(&vbempty[t], ((it >> 1) & 1) ^ 1, abort_flag, kSiteAtV)) {
-            ok = false;
-            break;
-          }
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int tok = (w + 4 * (k >> 1)) * 8 + tok8;
-            uint32_t o[8];
-            codes16<true>(raw[k], o);
-            uint8_t* dst = sVB + t * C::VB + (k & 1) * kTile * 128 + tok * 128;
-            const int c2 = (lane & 3) * 2;
-            *reinterpret_cast<uint4*>(dst + ((c2 ^ tok8) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-            *reinterpret_cast<uint4*>(dst + (((c2 + 1) ^ tok8) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
-          }
-        } else {
-          uint4 raw[4];
-          uint32_t dep = 0;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int tok = k * 32 + w * 8 + (lane >> 2), c = lane & 3;
-            raw[k] = *reinterpret_cast<const uint4*>(sV + s * C::KV + tok * 64 + ((c ^ ((tok >> 1) & 3)) << 4));
-            dep |= raw[k].x | raw[k].y | raw[k].z | raw[k].w;
-          }
-          asm volatile("" ::"r"(dep));
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&vempty[s]);
-          if (!mbar_wait(&vbempty[t], ((it >> 1) & 1) ^ 1, abort_flag, kSiteAtV)) {
-            ok = false;
-            break;
-          }
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int tok = k * 32 + w * 8 + (lane >> 2), c2 = (lane & 3) * 2;
-            uint32_t o[8];
-            codes16<true>(raw[k], o);
-            uint8_t* dst = sVB + t * C::VB + tok * 128;
-            *reinterpret_cast<uint4*>(dst + ((c2 ^ (tok & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-            *reinterpret_cast<uint4*>(dst + (((c2 + 1) ^ (tok & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
-          }
+        if (!mbar_wait_at(&vbempty[t], ((it >> 1) & 1) ^ 1, ctl, kSiteAtV)) {
+          ok = false;
+          break;
         }
+        const uint8_t* src = sV + s * C::KV;
+        uint8_t* dst = sVB + t * C::VB;
+        uint32_t dep = 0;
+        // One 16-byte chunk of codes -> chunks 2 (c % 4), 2 (c % 4) + 1 of a bf16 row of panel c / 4.
+        // Two chunks a step, few steps unrolled: five roles share the instruction cache, and with the
+        // loops of the dequantisers unrolled in full half of all issue slots waited for it.
+        // D = 128: the eight lanes of one shared-memory phase take four chunks of two slots whose
+        // numbers differ in bits 0 and 2, so neither the swizzled read (chunks c) nor the write meets a
+        // bank twice.
+        const int tok8 = D == 128 ? (lane & 4 ? (lane >> 3) ^ 5 : lane >> 3) : lane >> 2;
+        const int c4 = lane & 3;
+        const int w0 = (((2 * c4) ^ tok8) << 4), w1 = (((2 * c4 + 1) ^ tok8) << 4);
+#pragma unroll 1
+        for (int k = 0; k < kTile / 32; k += D == 128 ? 1 : 2) {
+          uint4 r0, r1;
+          uint8_t *d0, *d1;
+          if constexpr (D == 128) {  // one slot, both halves of its row
+            const int tok = (w + 4 * k) * 8 + tok8;
+            r0 = *reinterpret_cast<const uint4*>(src + tok * 128 + ((c4 ^ tok8) << 4));
+            r1 = *reinterpret_cast<const uint4*>(src + tok * 128 + (((c4 + 4) ^ tok8) << 4));
+            d0 = dst + tok * 128;
+            d1 = d0 + kTile * 128;
+          } else {  // two slots
+            const int tok = k * 32 + w * 8 + tok8;
+            r0 = *reinterpret_cast<const uint4*>(src + tok * 64 + ((c4 ^ ((tok8 >> 1) & 3)) << 4));
+            r1 = *reinterpret_cast<const uint4*>(src + (tok + 32) * 64 + ((c4 ^ ((tok8 >> 1) & 3)) << 4));
+            d0 = dst + tok * 128;
+            d1 = d0 + 32 * 128;
+          }
+          uint32_t o[16];
+          codes16<true>(r0, o);
+          codes16<true>(r1, o + 8);
+          *reinterpret_cast<uint4*>(d0 + w0) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(d0 + w1) = make_uint4(o[4], o[5], o[6], o[7]);
+          *reinterpret_cast<uint4*>(d1 + w0) = make_uint4(o[8], o[9], o[10], o[11]);
+          *reinterpret_cast<uint4*>(d1 + w1) = make_uint4(o[12], o[13], o[14], o[15]);
+          dep |= o[7] | o[15];
+        }
+        asm volatile("" ::"r"(dep));  // the last loads are complete before the slot is released
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&vempty[s]);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&vbfull[t]);
@@ -639,9 +708,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     }
   } else {
     // ---------------- softmax: thread = slot for the scores, = head dimension for the output ----------------
-    const int g = (warp - 10) >> 2;    // rows [g RC, (g + 1) RC) of the block
-    const int w = (warp - 10) & 3;
-    const int q = warp & 3;            // TMEM lanes of this warp
+    setmaxnreg_inc<kRegsSoft>();
+    const int g = (warp - 12) >> 2;    // rows [g RC, (g + 1) RC) of the block
+    const int w = warp & 3;
+    const int q = w;                   // TMEM lanes of this warp
     const int row = q * 32 + lane;
     const int tid = w * 32 + lane;
     const int bar = 1 + g;
@@ -650,7 +720,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     float* gsum = gmax + 4 * 32;
     float* mref = refs + g * 2 * 32;
     float* fac = mref + 32;
-    float* tab = ftab + g * 16 * 32;
+    float* tab = ftab + g * 128;
+    const float* zeros = ftab + 2 * 128;
     int it = 0, seg = 0;
     bool ok = true;
     AttnWalk wk(pre, ta.nb, x0, x1);
@@ -661,8 +732,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       const int nodes = seq_nodes(a, b);
       const int64_t keys = ctx + nodes;
       const int qb = seg % C::NQ;
-      const bool got_q = mbar_wait(&qfull[qb], (seg / C::NQ) & 1, abort_flag, kSiteAtSoft);
-      if (tid < RC) mref[tid] = -INFINITY;
+      const bool got_q = mbar_wait_at(&qfull[qb], (seg / C::NQ) & 1, ctl, kSiteAtSoft);
+      if (tid < RC) mref[tid] = kLowest;
       if (named_bar_any(bar, 128, !got_q)) break;
       const unsigned long long* masks = rmask + qb * 64 + g * RC;
       float l[RC];
@@ -671,66 +742,68 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       for (int i = 0; i < sg.n_kt; ++i, ++it) {
         const int t = it & 1;
         const uint32_t ph = (it >> 1) & 1;
-        const int64_t j0 = static_cast<int64_t>(sg.kt0 + i) * kTile;
-        const int64_t j = j0 + row;
-        float ks = 0.f, vs = 0.f;
-        bool there = false;
-        if (j < keys) {
-          int64_t kr = kv_row(a.c, b, j);
-          if (kr >= 0) {
-            kr += static_cast<int64_t>(sg.h) * a.c.page;
-            ks = a.c.ks[kr] * a.scale_log2;
-            vs = a.c.vs[kr];
-            there = true;
-          }
-        }
+        const int64_t j = static_cast<int64_t>(sg.kt0 + i) * kTile + row;
+        const int sc = it % kScaleStages;
+        bool fine = mbar_wait_at(&scfull[sc], (it / kScaleStages) & 1, ctl, kSiteAtSoft);
+        const float ks = sScale[sc * 2 * kTile + row] * a.scale_log2;
+        const float vs = sScale[sc * 2 * kTile + kTile + row];
+        const bool there = j < keys && ((sPages[sc] >> (row >> 2)) & 1);
         // a node's slot is seen by the rows whose mask names it, a context slot by all
         const int node = j >= ctx ? static_cast<int>(j - ctx) : -1;
         const bool masked = !there || node >= 0;
-        bool fine = mbar_wait(&sfull[t], ph, abort_flag, kSiteAtSoft);
+        fine = mbar_wait_at(&sfull[t], ph, ctl, kSiteAtSoft) && fine;
         tc_fence_after();
-        float s[RC];
+        // x = score - reference, in powers of two; -inf where the row does not see the slot.  A vote
+        // over the group: does any score exceed its row's reference by more than 8?  Then once more
+        // from 0 for the rows' maxima, and again from the new references.
+        float x[RC];
+        int pass = 0;
+#pragma unroll 1
+        for (;; ++pass) {
+          const float* m = pass == 1 ? zeros : mref;
 #pragma unroll
-        for (int c = 0; c < RC; c += 8) tmem_ld8(lanes + C::S_COL + t * R + g * RC + c, reinterpret_cast<uint32_t*>(s) + c);
-        tmem_ld_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sempty[t]);
-        bool over = false;
-        if (masked) {
+          for (int c = 0; c < RC; c += 8)
+            tmem_ld8(lanes + C::S_COL + t * R + g * RC + c, reinterpret_cast<uint32_t*>(x) + c);
+          tmem_ld_wait();
+          const float2 k2 = make_float2(ks, ks);
 #pragma unroll
-          for (int c = 0; c < RC; ++c) {
-            const bool see = there && (node < 0 || ((masks[c] >> node) & 1));
-            s[c] = see ? s[c] * ks : -INFINITY;
-            over |= s[c] > mref[c] + 8.f;
+          for (int c = 0; c < RC; c += 4) {
+            const float4 r = *reinterpret_cast<const float4*>(m + c);
+            const float2 a01 = __ffma2_rn(make_float2(x[c], x[c + 1]), k2, make_float2(-r.x, -r.y));
+            const float2 a23 = __ffma2_rn(make_float2(x[c + 2], x[c + 3]), k2, make_float2(-r.z, -r.w));
+            x[c] = a01.x;
+            x[c + 1] = a01.y;
+            x[c + 2] = a23.x;
+            x[c + 3] = a23.y;
           }
-        } else {
+          if (masked) {
 #pragma unroll
-          for (int c = 0; c < RC; ++c) {
-            s[c] *= ks;
-            over |= s[c] > mref[c] + 8.f;
+            for (int c = 0; c < RC; ++c)
+              if (!there || !((masks[c] >> node) & 1)) x[c] = -INFINITY;
           }
-        }
-        if (named_bar_any(bar, 128, over || !fine)) {
-          // new references: the rows' maxima over the tile
-          float v[RC];
+          if (pass == 2) break;
+          if (pass == 0) {
+            float top = x[0];
 #pragma unroll
-          for (int c = 0; c < RC; ++c) v[c] = s[c];
-          const float top = warp_columns<RC, true>(v, lane);
+            for (int c = 1; c < RC; ++c) top = fmaxf(top, x[c]);
+            if (!named_bar_any(bar, 128, top > 8.f || !fine)) break;
+            continue;
+          }
+          const float top = warp_columns<RC, true>(x, lane);
           if (lane % (32 / RC) == 0) gmax[w * 32 + lane / (32 / RC)] = top;
           // (the barrier also takes the group's decision to give up)
-          if (named_bar_any(bar, 128, !fine || *abort_flag)) {
+          if (named_bar_any(bar, 128, !fine || ctl->abort)) {
             ok = false;
             break;
           }
           if (tid < RC) {
             const float old = mref[tid];
-            const float m = fmaxf(fmaxf(fmaxf(gmax[tid], gmax[32 + tid]), fmaxf(gmax[64 + tid], gmax[96 + tid])), old);
-            mref[tid] = m;
-            fac[tid] = m == old ? 1.f : exp2f(old - m);
+            const float best = fmaxf(fmaxf(fmaxf(gmax[tid], gmax[32 + tid]), fmaxf(gmax[64 + tid], gmax[96 + tid])), old);
+            mref[tid] = best;
+            fac[tid] = exp2_approx(old - best);
           }
           // the accumulator is still: the last tile's V . P is complete, the next waits for this one's weights
-          if (i > 0) fine = mbar_wait(&pempty[t ^ 1], ((it - 1) >> 1) & 1, abort_flag, kSiteAtSoft);
+          if (i > 0) fine = mbar_wait_at(&pempty[t ^ 1], ((it - 1) >> 1) & 1, ctl, kSiteAtSoft);
           if (named_bar_any(bar, 128, !fine)) {
             ok = false;
             break;
@@ -739,41 +812,46 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 #pragma unroll
           for (int c = 0; c < RC; ++c) l[c] *= fac[c];
           if (i > 0) {
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < 2 * RC; c += 8) {  // hi, then lo
               const uint32_t at = lanes + C::O_COL + (c < RC ? g * RC + c : R + g * RC + c - RC);
+              const float* f = fac + c % RC;
               uint32_t o[8];
               tmem_ld8(at, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fac[(c + e) % RC]);
+              for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f[e]);
               tmem_st8(at, o);
             }
             tmem_st_wait();
-            tc_fence_before();
           }
         }
+        if (!ok) break;
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&sempty[t]);
+          mbar_arrive(&scempty[sc]);
+        }
         // weights
-        if (!mbar_wait(&pempty[t], ph ^ 1, abort_flag, kSiteAtSoft)) *abort_flag = 1;
+        if (!mbar_wait_at(&pempty[t], ph ^ 1, ctl, kSiteAtSoft)) ctl->abort = 1;
         uint8_t* prow = sP + t * C::PB + row * 128;
 #pragma unroll
         for (int c0 = 0; c0 < RC; c0 += 8) {
           uint32_t hi[4], lo[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            float x[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const int c = c0 + 2 * e + k;
-              const float m = mref[c];
-              const float p = exp2f(s[c] - (m == -INFINITY ? 0.f : m));
-              l[c] += p;
-              x[k] = s[c] == -INFINITY ? 0.f : p * vs;  // what is not seen adds nothing, whatever its scale
-            }
-            const __nv_bfloat162 h = __floats2bfloat162_rn(x[0], x[1]);
+            const int c = c0 + 2 * e;
+            const float2 p = make_float2(exp2_approx(x[c]), exp2_approx(x[c + 1]));
+            const float2 l2 = __fadd2_rn(make_float2(l[c], l[c + 1]), p);
+            l[c] = l2.x;
+            l[c + 1] = l2.y;
+            const float2 v = __fmul2_rn(p, make_float2(vs, vs));
+            const __nv_bfloat162 h = __float22bfloat162_rn(v);
             hi[e] = *reinterpret_cast<const uint32_t*>(&h);
-            const __nv_bfloat162 r = __floats2bfloat162_rn(x[0] - __uint_as_float(hi[e] << 16),
-                                                           x[1] - __uint_as_float(hi[e] & 0xFFFF0000u));
+            const float2 left = __fadd2_rn(v, make_float2(-__uint_as_float(hi[e] << 16),
+                                                          -__uint_as_float(hi[e] & 0xFFFF0000u)));
+            const __nv_bfloat162 r = __float22bfloat162_rn(left);
             lo[e] = *reinterpret_cast<const uint32_t*>(&r);
           }
           const int nh = g * RC + c0, nl = R + nh;  // columns of P
@@ -782,59 +860,81 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           *reinterpret_cast<uint4*>(prow + (nl >> 6) * kTile * 128 + ((((nl & 63) >> 3) ^ (row & 7)) << 4)) =
               make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
+        // What is not seen adds nothing, whatever its scale (0 times one that is not finite is not 0).
+        if (masked && !(fabsf(vs) <= 3.402823466e38f)) {
+#pragma unroll 1
+          for (int c = 0; c < RC; ++c) {
+            if (there && ((masks[c] >> node) & 1)) continue;
+            const int nh = g * RC + c, nl = R + nh;
+            *reinterpret_cast<unsigned short*>(prow + (nh >> 6) * kTile * 128 + ((((nh & 63) >> 3) ^ (row & 7)) << 4) + (nh & 7) * 2) = 0;
+            *reinterpret_cast<unsigned short*>(prow + (nl >> 6) * kTile * 128 + ((((nl & 63) >> 3) ^ (row & 7)) << 4) + (nl & 7) * 2) = 0;
+          }
+        }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&pfull[t]);
       }
       if (!ok) break;
       // ---- the segment's end: sums of the weights, output or piece ----
-      bool fine = mbar_wait(&pempty[(it - 1) & 1], ((it - 1) >> 1) & 1, abort_flag, kSiteAtSoft);
+      bool fine = mbar_wait_at(&pempty[(it - 1) & 1], ((it - 1) >> 1) & 1, ctl, kSiteAtSoft);
       {
         const float sum = warp_columns<RC, false>(l, lane);
         if (lane % (32 / RC) == 0) gsum[w * 32 + lane / (32 / RC)] = sum;
       }
-      if (named_bar_any(bar, 128, !fine || *abort_flag)) break;
+      if (named_bar_any(bar, 128, !fine || ctl->abort)) break;
       tc_fence_after();
       if (lane == 0) mbar_arrive(&qempty[qb]);  // the masks are read no more
       const bool mine = row < D;                 // this thread's head dimension
-      float o[RC];
+      if (tid < RC) fac[tid] = ((gsum[tid] + gsum[32 + tid]) + gsum[64 + tid]) + gsum[96 + tid];  // sum of the weights
+      named_bar_sync(bar, 128);
+      // eight rows' values of this thread's head dimension, divided by their sums, to the output
+      auto emit = [&](int c0, const float (&o)[8]) {
 #pragma unroll
-      for (int c = 0; c < RC; c += 8) {
-        uint32_t hi[8], lo[8];
-        tmem_ld8(lanes + C::O_COL + g * RC + c, hi);
-        tmem_ld8(lanes + C::O_COL + R + g * RC + c, lo);
-        tmem_ld_wait();
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o[c + e] = __uint_as_float(hi[e]) + __uint_as_float(lo[e]);
-      }
-      tc_fence_before();
-      float den[RC];
-#pragma unroll
-      for (int c = 0; c < RC; ++c) den[c] = ((gsum[c] + gsum[32 + c]) + gsum[64 + c]) + gsum[96 + c];
+        for (int e = 0; e < 8; ++e) {
+          const int r = rt * R + g * RC + c0 + e;
+          const int n = r / grp, gh = r - n * grp;
+          if (mine && n < a.t) {
+            const float den = fac[c0 + e];
+            const float y = den == 0.f || n >= nodes ? 0.f : o[e] / den;
+            static_cast<T*>(a.o)[((b * a.t + n) * a.hq + sg.h * grp + gh) * static_cast<int64_t>(D) + row] = from_f32<T>(y);
+          }
+        }
+      };
+      constexpr int PIECE = R * D + 2 * R;
       const int c_first = range_owner(sg.u0, units, groups);
       const int c_last = range_owner(sg.u0 + sg.tiles - 1, units, groups);
-      bool emit = true;
-      if (c_last > c_first) {
-        constexpr int PIECE = R * D + 2 * R;
-        float* piece = ta.pieces + (static_cast<int64_t>(blockIdx.x) * 2 + sg.slot) * PIECE;
-        if (mine) {
+      const bool split = c_last > c_first;
+      float* piece = ta.pieces + (static_cast<int64_t>(blockIdx.x) * 2 + sg.slot) * PIECE;
+#pragma unroll 1
+      for (int c0 = 0; c0 < RC; c0 += 8) {
+        uint32_t hi[8], lo[8];
+        float o[8];
+        tmem_ld8(lanes + C::O_COL + g * RC + c0, hi);
+        tmem_ld8(lanes + C::O_COL + R + g * RC + c0, lo);
+        tmem_ld_wait();
 #pragma unroll
-          for (int c = 0; c < RC; ++c) piece[(g * RC + c) * D + row] = o[c];
+        for (int e = 0; e < 8; ++e) o[e] = __uint_as_float(hi[e]) + __uint_as_float(lo[e]);
+        if (!split) {
+          emit(c0, o);
+        } else if (mine) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) piece[(g * RC + c0 + e) * D + row] = o[e];
         }
+      }
+      tc_fence_before();
+      if (split) {
         if (tid < RC) piece[R * D + g * RC + tid] = mref[tid];
-        if (tid < RC) piece[R * D + R + g * RC + tid] = ((gsum[tid] + gsum[32 + tid]) + gsum[64 + tid]) + gsum[96 + tid];
+        if (tid < RC) piece[R * D + R + g * RC + tid] = fac[tid];
         __threadfence();
         named_bar_sync(bar, 128);
-        int* cnt = ta.counters + (c_first * ta.rts + rt) * 2 + g;
         if (tid == 0) {
-          const int old = atomicAdd(cnt, 1);
-          const bool last = old == c_last - c_first;
+          int* cnt = ta.counters + (c_first * ta.rts + rt) * 2 + g;
+          const bool last = atomicAdd(cnt, 1) == c_last - c_first;
           if (last) *cnt = 0;
-          fac[0] = last ? 1.f : 0.f;
+          gmax[0] = last ? 1.f : 0.f;
         }
         named_bar_sync(bar, 128);
-        emit = fac[0] != 0.f;
-        if (emit) {
+        if (gmax[0] != 0.f) {
           __threadfence();
           // piece p of the (sequence, head): CTA c_first + p's first segment, unless it started before
           auto piece_of = [&](int p) {
@@ -845,7 +945,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           const int n = c_last - c_first + 1;
           constexpr int SUB = 128 / RC;  // threads of one row
           const int c = tid % RC, sub = tid / RC;
-          float m = -INFINITY;
+          float m = kLowest;
           for (int p = sub; p < n; p += SUB) m = fmaxf(m, __ldcg(piece_of(p) + R * D + g * RC + c));
           tab[tid] = m;
           named_bar_sync(bar, 128);
@@ -855,51 +955,37 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           float sum = 0.f;
           for (int p = sub; p < n; p += SUB) {
             const float* pp = piece_of(p) + R * D + g * RC + c;
-            const float pm = __ldcg(pp);
-            sum += pm == -INFINITY ? __ldcg(pp + R) : __ldcg(pp + R) * exp2f(pm - m);
+            sum += __ldcg(pp + R) * exp2_approx(__ldcg(pp) - m);
           }
           tab[tid] = sum;
+          if (tid < RC) mref[tid] = m;
           named_bar_sync(bar, 128);
-#pragma unroll
-          for (int e = 0; e < RC; ++e) {
-            float x = tab[e];
-            for (int k = 1; k < SUB; ++k) x += tab[e + k * RC];
-            den[e] = x;
-            o[e] = 0.f;
+          if (tid < RC) {
+            for (int k = 1; k < SUB; ++k) sum += tab[tid + k * RC];
+            fac[tid] = sum;
           }
-          for (int p0 = 0; p0 < n; p0 += 16) {  // 16 pieces' factors at a time
-            named_bar_sync(bar, 128);
-            for (int e = tid; e < 16 * RC; e += 128) {
-              const int p = p0 + e / RC;
-              // (this thread's row of e is c: 128 is a multiple of RC)
-              float f = 0.f;
-              if (p < n) {
-                const float pm = __ldcg(piece_of(p) + R * D + g * RC + c);
-                f = pm == -INFINITY ? 1.f : exp2f(pm - m);
-              }
-              tab[e] = f;
-            }
-            named_bar_sync(bar, 128);
-            if (mine) {
-              const int n2 = min(16, n - p0);
-              for (int p = 0; p < n2; ++p) {
-                const float* pp = piece_of(p0 + p) + g * RC * D + row;
+#pragma unroll 1
+          for (int c0 = 0; c0 < RC; c0 += 8) {
+            float o[8];
 #pragma unroll
-                for (int e = 0; e < RC; ++e) o[e] += tab[p * RC + e] * __ldcg(pp + e * D);
+            for (int e = 0; e < 8; ++e) o[e] = 0.f;
+            for (int p0 = 0; p0 < n; p0 += 16) {
+              named_bar_sync(bar, 128);
+              // the factors of 16 pieces and 8 rows, one a thread
+              const int p = p0 + (tid >> 3), e = c0 + (tid & 7);
+              tab[tid] = p < n ? exp2_approx(__ldcg(piece_of(p) + R * D + g * RC + e) - mref[e]) : 0.f;
+              named_bar_sync(bar, 128);
+              if (mine) {
+                const int n2 = min(16, n - p0);
+#pragma unroll 4
+                for (int k = 0; k < n2; ++k) {
+                  const float* pp = piece_of(p0 + k) + (g * RC + c0) * D + row;
+#pragma unroll
+                  for (int q8 = 0; q8 < 8; ++q8) o[q8] += tab[k * 8 + q8] * __ldcg(pp + q8 * D);
+                }
               }
             }
-          }
-          named_bar_sync(bar, 128);
-        }
-      }
-      if (emit && mine) {
-#pragma unroll
-        for (int c = 0; c < RC; ++c) {
-          const int r = rt * R + g * RC + c;
-          const int n = r / grp, gh = r - n * grp;
-          if (n < a.t) {
-            const float x = den[c] == 0.f || n >= nodes ? 0.f : o[c] / den[c];
-            static_cast<T*>(a.o)[((b * a.t + n) * a.hq + sg.h * grp + gh) * static_cast<int64_t>(D) + row] = from_f32<T>(x);
+            emit(c0, o);
           }
         }
       }
@@ -959,6 +1045,7 @@ static int launch_tiles(const AttnArgs& a, const TilePlan& p, void* ws, bool qve
   ta.groups = p.groups;
   ta.qvec = qvec;
   ta.counters = static_cast<int*>(ws);
+  if (int s = device_wait_ptrs(&ta.status, &ta.limit)) return s;
   ta.pieces = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + p.bytes -
                                        static_cast<size_t>(p.grid) * 2 * (R * D + 2 * R) * sizeof(float));
   for (int64_t b0 = 0; b0 < a.b; b0 += kAttnMaxBatch) {
@@ -1058,7 +1145,8 @@ extern "C" int bw_tree_attention_int8(const void* q, int64_t q_sb, int64_t q_st,
   // the tensor-core kernel's units are counted in 32 bits, its cache rows addressed in them
   const int64_t units = b * heads * ((table_cols * page + kTile - 1) / kTile + 1);
   if (tile_dims(d, page) && units < INT32_MAX && pages > 0 && pages * heads * page < INT32_MAX &&
-      reinterpret_cast<uintptr_t>(cache_k) % 16 == 0 && reinterpret_cast<uintptr_t>(cache_v) % 16 == 0) {
+      (reinterpret_cast<uintptr_t>(cache_k) | reinterpret_cast<uintptr_t>(cache_v) |
+       reinterpret_cast<uintptr_t>(k_scale) | reinterpret_cast<uintptr_t>(v_scale)) % 16 == 0) {
     const TilePlan p = tile_plan(t, hq / heads, d);
     if (workspace == nullptr || workspace_bytes < p.bytes)
       return fail(BW_ERR_WORKSPACE, "tree_attention_int8: workspace of %zu bytes required, %zu given", p.bytes,
