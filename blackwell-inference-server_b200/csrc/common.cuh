@@ -174,7 +174,9 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
 }
 #endif
 
-// The same with the status word and the limit (SM cycles) at given addresses.
+// The same with the status word and the limit (SM cycles) at given addresses: mbar_wait_at, for the one
+// thread or warp of a CTA that watches the time, and mbar_wait_or_abort, a few instructions, for the roles
+// that leave when it has set `abort`.
 struct WaitControl {
   volatile int abort;     // a role of the CTA has given up
   int* status;
@@ -182,21 +184,28 @@ struct WaitControl {
 };
 __device__ __forceinline__ bool mbar_wait_at(uint64_t* bar, uint32_t parity, WaitControl* w, int site,
                                              bool heed_abort = true) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const long long t0 = clock64();
-  long long limit = -1;
-  for (uint32_t i = 1;; ++i) {
+  long long t0 = 0;
+#pragma unroll 1
+  for (uint32_t i = 0;; ++i) {
     if (mbar_try_wait(bar, parity)) return true;
     if ((i & 63u) == 0u) {
+      const long long now = clock64();
+      if (i == 0u) t0 = now;
       if (heed_abort && w->abort) return false;
-      if (limit < 0) limit = *static_cast<const volatile long long*>(w->limit);
-      if (clock64() - t0 > limit) {
+      if (now - t0 > *static_cast<const volatile long long*>(w->limit)) {
         atomicCAS(w->status, 0, site);
         w->abort = 1;
         return false;
       }
     }
   }
+}
+
+__device__ __forceinline__ bool mbar_wait_or_abort(uint64_t* bar, uint32_t parity, WaitControl* w) {
+#pragma unroll 1
+  while (!mbar_try_wait(bar, parity))
+    if (w->abort) return false;
+  return true;
 }
 
 // ---------------------------------------------------------------------------

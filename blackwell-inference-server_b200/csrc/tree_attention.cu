@@ -142,17 +142,23 @@ constexpr int kTile = 128;
 constexpr int kAttnThreads = 20 * 32;
 // Registers of a thread of the five warpgroups after setmaxnreg: their sum is five times the 96 that
 // a thread of 640 has at launch.
-constexpr int kRegsIssue = 56, kRegsK = 88, kRegsV = 80, kRegsSoft = 128;
+constexpr int kRegsIssue = 72, kRegsK = 80, kRegsV = 72, kRegsSoft = 128;
 static_assert(kRegsIssue + kRegsK + kRegsV + 2 * kRegsSoft == 5 * 96, "register split");
 constexpr int kScaleStages = 4;   // tiles whose scales are on their way or in use
 constexpr float kLowest = -3.0e38f;  // a row's reference before any score: finite, so differences are
 constexpr int kAttnMaxBatch = 1024;  // sequences of one launch (their unit ranges lie in shared memory)
 constexpr size_t kAttnCounterBytes = 4096;
-enum AttnSite : int { kSiteAtTma = 80, kSiteAtDrain, kSiteAtK, kSiteAtV, kSiteAtQk, kSiteAtPv, kSiteAtSoft, kSiteAtFinal };
+enum AttnSite : int { kSiteAtTma = 401, kSiteAtDrain = 402, kSiteAtDone = 403, kSiteAtFinal = 404 };
 
 template <int D, int R>
 struct ACfg {
-  static constexpr int RC = R / 2;                     // rows of a softmax group
+  // The two softmax groups take alternate tiles with all rows, each with its own references, sums and
+  // accumulators, joined at a segment's end (few rows: a tile's softmax is a chain of latencies), or
+  // half the rows of every tile (many rows: throughput, and registers for half of them).
+  static constexpr bool ALT = R <= 32;
+  static constexpr int RC = ALT ? R : R / 2;           // rows of a softmax group
+  static constexpr int RH = R / 2;                     // rows of a group at a segment's end
+  static constexpr int GW = ALT ? 4 : 8;               // softmax warps of a tile
   static constexpr int KV = kTile * D;                 // bytes of one K or V tile of codes
   static constexpr int VB = (D / 64) * kTile * 128;    // a V tile in bf16
   static constexpr int ZB = D == 64 ? kTile * 128 : 0; // zeros: the rows 64 .. 127 of V^T
@@ -165,7 +171,7 @@ struct ACfg {
   static constexpr int OFF_Q = OFF_P + 2 * PB;
   static constexpr int OFF_RING = OFF_Q + NQ * QB;
   static constexpr int SCALES = kScaleStages * (2 * kTile * 4 + 16);
-  static constexpr int CTRL = 640 + SCALES + 2 * 4 * 32 * 4 * 2 + 2 * 2 * 32 * 4 + (2 * 128 + 32) * 4 + 2 * 64 * 8 +
+  static constexpr int CTRL = 640 + SCALES + 2 * 4 * 32 * 4 * 2 + 2 * 3 * 32 * 4 + 4 * 64 * 4 + (2 * 128 + 32) * 4 + 2 * 64 * 8 + 64 * 4 +
                               (kAttnMaxBatch + 1) * 4 + 64;
   static constexpr int ROOM = 227 * 1024 - 1024 - OFF_RING - CTRL;
   static constexpr int ST = ROOM / (2 * KV) < 6 ? ROOM / (2 * KV) : 6;  // stages of a K and a V tile
@@ -174,7 +180,7 @@ struct ACfg {
   static constexpr int A_COLS = D / 2;                 // TMEM columns of a K tile
   static constexpr int S_COL = 2 * A_COLS;
   static constexpr int O_COL = S_COL + 2 * R;
-  static constexpr int COLS = O_COL + 2 * R <= 256 ? 256 : 512;
+  static constexpr int COLS = O_COL + (ALT ? 4 : 2) * R <= 256 ? 256 : 512;
   static_assert(ST >= 2, "at least two stages");
   static_assert(QB % 1024 == 0 && KV % 1024 == 0, "swizzled tiles are 1024-byte aligned");
 };
@@ -229,16 +235,16 @@ struct AttnWalk {
   }
 };
 
-// Range starts of `groups` CTAs over `units` (units >= groups), and the CTA that holds unit x.
-__host__ __device__ __forceinline__ int range_start(int c, int units, int groups) {
-  return static_cast<int>(static_cast<int64_t>(units) * c / groups);
-}
-__host__ __device__ __forceinline__ int range_owner(int x, int units, int groups) {
-  int c = static_cast<int>(static_cast<int64_t>(x) * groups / units);
-  while (c + 1 < groups && range_start(c + 1, units, groups) <= x) ++c;
-  while (c > 0 && range_start(c, units, groups) > x) --c;
-  return c;
-}
+// `units` units over `groups` CTAs (units >= groups): the first `rem` have one more than the others.
+struct AttnSplit {
+  int each, rem;
+  __device__ __forceinline__ AttnSplit(int units, int groups) : each(units / groups), rem(units - each * groups) {}
+  __device__ __forceinline__ int start(int c) const { return c * each + min(c, rem); }
+  __device__ __forceinline__ int owner(int x) const {  // the CTA that holds unit x
+    const int wide = rem * (each + 1);
+    return x < wide ? x / (each + 1) : rem + (x - wide) / each;
+  }
+};
 
 __device__ __forceinline__ int seq_nodes(const AttnArgs& a, int64_t b) {
   const int n = a.counts != nullptr ? a.counts[b] : a.t;
@@ -257,6 +263,9 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+// 1 / sum of a row's weights; 0 where it saw nothing.
+__device__ __forceinline__ float inverse(float sum) { return sum == 0.f ? 0.f : __frcp_rn(sum); }
 
 // 16 bytes global -> shared without registers; zeros, and nothing read, if !have.
 __device__ __forceinline__ void cp_async16_zfill(void* dst, const void* src, bool have) {
@@ -311,6 +320,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   using C = ACfg<D, R>;
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr int RC = C::RC;
+  constexpr int RH = C::RH;
   constexpr int ST = C::ST;
   const AttnArgs& a = ta.a;
   extern __shared__ uint8_t smem_raw[];
@@ -337,16 +347,19 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   uint64_t* scfull = qempty + 2;      // scales of a tile
   uint64_t* scempty = scfull + kScaleStages;
   uint64_t* final_bar = scempty + kScaleStages;  // 2
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(final_bar + 2);
-  WaitControl* ctl = reinterpret_cast<WaitControl*>(tmem_slot + 2);
+  uint64_t* done = final_bar + 2;                // the softmax warps have no more to do
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  WaitControl* ctl = reinterpret_cast<WaitControl*>(done + 2);
   float* sScale = reinterpret_cast<float*>(smem + C::OFF_CTRL + 640);  // [stages][2][128]: ks, vs
   uint32_t* sPages = reinterpret_cast<uint32_t*>(sScale + kScaleStages * 2 * kTile);  // [stages]: pages that exist
   float* wred = reinterpret_cast<float*>(smem + C::OFF_CTRL + 640 + C::SCALES);  // [2 groups][2][4 warps][32]
-  float* refs = wred + 2 * 2 * 4 * 32;                               // [2 groups][2][32]: m, its factor
-  float* ftab = refs + 2 * 2 * 32;                                   // [2 groups][128], 32 zeros
+  float* refs = wred + 2 * 2 * 4 * 32;                               // [2 groups][3][32]: m, its factor, sums
+  float* fin = refs + 2 * 3 * 32;                                    // [4][64]: m, sum, factors of the two streams
+  float* ftab = fin + 4 * 64;                                        // [2 groups][128], 32 zeros
   unsigned long long* rmask = reinterpret_cast<unsigned long long*>(ftab + 2 * 128 + 32);  // [2][64]
-  int* pre = reinterpret_cast<int*>(rmask + 2 * 64);                 // [nb + 1] first unit of a sequence
-  static_assert((4 * 6 + 22 + 2 * kScaleStages) * 8 + 8 + sizeof(WaitControl) <= 640, "barriers");
+  int* rows = reinterpret_cast<int*>(rmask + 2 * 64);                // [64] node | query head of the group << 16
+  int* pre = rows + 64;                                              // [nb + 1] first unit of a sequence
+  static_assert((4 * 6 + 24 + 2 * kScaleStages) * 8 + 8 + sizeof(WaitControl) <= 640, "barriers");
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -366,16 +379,17 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       mbar_init(&vbfull[i], 4);
       mbar_init(&vbempty[i], 1);
       mbar_init(&sfull[i], 1);
-      mbar_init(&sempty[i], 8);
-      mbar_init(&pfull[i], 8);
+      mbar_init(&sempty[i], C::GW);
+      mbar_init(&pfull[i], C::GW);
       mbar_init(&pempty[i], 1);
-      mbar_init(&qfull[i], 4);
+      mbar_init(&qfull[i], 1);
       mbar_init(&qempty[i], 9);  // the last K.Q of the segment, and the softmax warps
       mbar_init(&final_bar[i], 1);
     }
+    mbar_init(done, 8);
     for (int i = 0; i < kScaleStages; ++i) {
       mbar_init(&scfull[i], 33);  // each lane's copies, and the page word
-      mbar_init(&scempty[i], 8);
+      mbar_init(&scempty[i], C::GW);
     }
     ctl->abort = 0;
     for (int i = 0; i < 32; ++i) ftab[2 * 128 + i] = 0.f;
@@ -393,6 +407,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     for (int i = threadIdx.x; i < C::ZB / 16; i += kAttnThreads)
       reinterpret_cast<uint4*>(smem + C::OFF_Z)[i] = make_uint4(0u, 0u, 0u, 0u);
     fence_proxy_async_smem();
+  }
+  const int gi = blockIdx.x / ta.rts, rt = blockIdx.x - gi * ta.rts;
+  if (threadIdx.x >= 64 && threadIdx.x < 64 + R) {
+    const int r = threadIdx.x - 64;
+    const int n = (rt * R + r) / grp;
+    rows[r] = min(n, 0x7fff) | ((rt * R + r - n * grp) << 16);
   }
   pdl_wait();  // lengths, tables, masks, q and the cache may come from the preceding kernel
   // units before each sequence; one at least, so that every output row is written
@@ -423,13 +443,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   const uint32_t tmem = *tmem_slot;
   const int units = pre[ta.nb];
   const int groups = min(ta.groups, units);
-  const int gi = blockIdx.x / ta.rts, rt = blockIdx.x - gi * ta.rts;
-  const int x0 = gi < groups ? range_start(gi, units, groups) : 0;
-  const int x1 = gi < groups ? range_start(gi + 1, units, groups) : 0;  // an empty range: nothing to do
+  const AttnSplit range(units, groups);
+  const int x0 = gi < groups ? range.start(gi) : 0;
+  const int x1 = gi < groups ? range.start(gi + 1) : 0;  // an empty range: nothing to do
 
   if (warp < 4) setmaxnreg_dec<kRegsIssue>();
   if (warp == 0 || warp == 3) {
-    // ---------------- warp 0: K and V by TMA, one box per page of the tile; warp 3: the scales ----------------
+    // ------- warp 0: K and V by TMA, one box per page of the tile; warp 3: scales, and each segment's Q and row masks -------
     const int box = min(a.c.page, kTile);           // rows of a box
     const int per = kTile / box;                    // boxes of a tile
     const int tiles_pp = max(a.c.page / kTile, 1);  // tiles of a page
@@ -442,12 +462,16 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     int i_seg = 0;
     int64_t keys = 0;
     const int* table = nullptr;
+    int seg = -1;
+    bool fresh = false;  // the looked-up tile is its segment's first
     int pg = -1;       // the looked-up page, not yet checked against the cache
     int pg_row = 0;    // first row of the box (or four slots) in its (page, head)
     auto look_up = [&]() {
-      if (i_seg == sg.n_kt) {
+      fresh = i_seg == sg.n_kt;
+      if (fresh) {
         if (!wk.next(pre, heads, sg)) return;
         i_seg = 0;
+        ++seg;
         const int64_t room = static_cast<int64_t>(a.c.table_cols) * a.c.page;
         keys = seq_ctx(a, ta.b0 + sg.b) + seq_nodes(a, ta.b0 + sg.b);
         keys = keys < room ? keys : room;
@@ -459,15 +483,68 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       pg = -1;
       if (my_box < per && static_cast<int64_t>(kt) * kTile + my_box * box < keys) pg = table[pi];
     };
+    // Q of a segment (row r = node r / grp, query head r % grp of the group) into its swizzled K-major panels
+    auto load_q = [&](int sq, const AttnSeg& q_sg) -> bool {
+      const int qb = sq % C::NQ;
+      const int64_t b = ta.b0 + q_sg.b;
+      if (!mbar_wait_or_abort(&qempty[qb], ((sq / C::NQ) & 1) ^ 1, ctl)) return false;
+      const int nodes = seq_nodes(a, b);
+#pragma unroll 1
+      for (int e0 = 0; e0 < R * (D / 8); e0 += 32 * 4) {
+        uint4 v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int e = e0 + k * 32 + lane;
+          const int r = e / (D / 8), c = e - r * (D / 8);
+          const int ng = r < R ? rows[r] : 0x7fff;
+          const int n = ng & 0xffff, g = ng >> 16;
+          v[k] = make_uint4(0u, 0u, 0u, 0u);
+          if (n < a.t) {
+            const T* x = static_cast<const T*>(a.q) + b * a.q_sb + n * a.q_st + (q_sg.h * grp + g) * a.q_sh + c * 8;
+            if (ta.qvec) {
+              v[k] = *reinterpret_cast<const uint4*>(x);
+            } else {
+              const unsigned short* y = reinterpret_cast<const unsigned short*>(x);
+              v[k] = make_uint4(y[0] | (static_cast<uint32_t>(y[1]) << 16), y[2] | (static_cast<uint32_t>(y[3]) << 16),
+                                y[4] | (static_cast<uint32_t>(y[5]) << 16), y[6] | (static_cast<uint32_t>(y[7]) << 16));
+            }
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int e = e0 + k * 32 + lane;
+          const int r = e / (D / 8), c = e - r * (D / 8);
+          if (r < R)
+            *reinterpret_cast<uint4*>(sQ + qb * C::QB + (c >> 3) * R * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[k];
+        }
+      }
+      for (int r = lane; r < R; r += 32) {
+        const int n = rows[r] & 0xffff;
+        rmask[qb * 64 + r] = n < a.t ? node_mask(a, b, n, nodes) : 0ull;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&qfull[qb]);
+      return true;
+    };
     const int total = x1 - x0;
-    if (total > 0) look_up();
-    const int page_rows = heads * a.c.page;
     bool ok = true;
-    int it = 0;
+    const int page_rows = heads * a.c.page;
+    int it = -1;  // the tile being loaded; its pages were looked up a step ago
+#pragma unroll 1
     for (; it < total; ++it) {
-      const bool have = pg >= 0 && pg < a.c.pages;
-      const int row = have ? pg * page_rows + pg_row : 0;
+      bool have = false;
+      int row = 0;
+      if (it >= 0) {
+        if (warp == 3 && fresh) {
+          ok = load_q(seg, sg);
+          if (!__all_sync(0xffffffffu, ok)) break;
+        }
+        have = pg >= 0 && pg < a.c.pages;
+        row = have ? pg * page_rows + pg_row : 0;
+      }
       if (it + 1 < total) look_up();
+      if (it < 0) continue;
       const uint32_t boxes = __ballot_sync(0xffffffffu, have);
       if (warp == 0) {
         const uint32_t bytes = __popc(boxes) * box * D;
@@ -491,7 +568,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         if (have) tma_load_2d(sV + s * C::KV + lane * box * D, &tm_v, &vfull[s], 0, row, pol);
       } else {
         const int sc = it % kScaleStages;
-        if (it >= kScaleStages) ok = mbar_wait_at(&scempty[sc], ((it / kScaleStages) & 1) ^ 1, ctl, kSiteAtTma);
+        if (it >= kScaleStages) ok = mbar_wait_or_abort(&scempty[sc], ((it / kScaleStages) & 1) ^ 1, ctl);
         if (!__all_sync(0xffffffffu, ok)) break;
         float* dst = sScale + sc * 2 * kTile + lane * 4;
         cp_async16_zfill(dst, a.c.ks + row, have);
@@ -509,6 +586,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         mbar_wait_at(&vfull[j % ST], (j / ST) & 1, ctl, kSiteAtDrain, false);
       }
     if (warp == 3) cp_async_wait_all();
+    // Warp 0 watches the time for all roles: its own waits run out here, the others' while it waits for the
+    // softmax warps to be done.
+    if (warp == 0 && ok) mbar_wait_at(done, 0, ctl, kSiteAtDone);
   } else if (warp == 1) {
     // ---------------- K . Q ----------------
     if (lane == 0) {
@@ -520,19 +600,22 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       for (; ok && wk.next(pre, heads, sg); ++seg) {
         const int qb = seg % C::NQ;
         const uint32_t q_base = smem_u32(sQ + qb * C::QB);
-        if (!mbar_wait_at(&qfull[qb], (seg / C::NQ) & 1, ctl, kSiteAtQk)) break;
+        if (!mbar_wait_or_abort(&qfull[qb], (seg / C::NQ) & 1, ctl)) break;
         for (int i = 0; i < sg.n_kt; ++i, ++it) {
           const int t = it & 1;
           const uint32_t ph = (it >> 1) & 1;
-          if (!mbar_wait_at(&afull[t], ph, ctl, kSiteAtQk) || !mbar_wait_at(&sempty[t], ph ^ 1, ctl, kSiteAtQk)) {
+          if (!mbar_wait_or_abort(&afull[t], ph, ctl) || !mbar_wait_or_abort(&sempty[t], ph ^ 1, ctl)) {
             ok = false;
             break;
           }
           tc_fence_after();
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint64_t bd = make_sdesc(q_base + (kk >> 2) * R * 128 + (kk & 3) * 32, 16, 1024, kLayoutSW128);
-            umma_f16_ts(tmem + C::S_COL + t * R, tmem + t * C::A_COLS + kk * 8, bd, idesc, kk > 0);
+          uint32_t a_col = tmem + t * C::A_COLS;
+#pragma unroll 1
+          for (int p = 0; p < D / 64; ++p) {  // panels of 64 elements of the head dimension
+            uint64_t bd = make_sdesc(q_base + p * R * 128, 16, 1024, kLayoutSW128);
+#pragma unroll 1
+            for (int kk = 0; kk < 4; ++kk, a_col += 8, bd += 32 >> 4)
+              umma_f16_ts(tmem + C::S_COL + t * R, a_col, bd, idesc, p + kk);
           }
           umma_commit(&sfull[t]);
           umma_commit(&aempty[t]);
@@ -554,21 +637,22 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         for (int i = 0; i < sg.n_kt; ++i, ++it) {
           const int t = it & 1;
           const uint32_t ph = (it >> 1) & 1;
-          if (!mbar_wait_at(&vbfull[t], ph, ctl, kSiteAtPv) || !mbar_wait_at(&pfull[t], ph, ctl, kSiteAtPv)) {
+          if (!mbar_wait_or_abort(&vbfull[t], ph, ctl) || !mbar_wait_or_abort(&pfull[t], ph, ctl)) {
             ok = false;
             break;
           }
           tc_fence_after();
+          const uint32_t o_tmem = tmem + C::O_COL + (C::ALT ? t * 2 * R : 0);
+          constexpr int first = C::ALT ? 1 : 0;  // the last tile of a segment that starts an accumulator
           const uint32_t v_base = smem_u32(sVB + t * C::VB);
           const uint32_t p_base = smem_u32(sP + t * C::PB);
           // the second 64 rows of V^T: the next panel, or zeros
           const uint32_t lbo = D == 128 ? kTile * 128 : smem_u32(smem + C::OFF_Z) - v_base;
-#pragma unroll
-          for (int kk = 0; kk < kTile / 16; ++kk) {
-            const uint64_t ad = make_sdesc(v_base + kk * 2048, lbo, 1024, kLayoutSW128);
-            const uint64_t bd = make_sdesc(p_base + kk * 2048, kTile * 128, 1024, kLayoutSW128);
-            umma_f16(tmem + C::O_COL, ad, bd, idesc, i > 0 || kk > 0);
-          }
+          uint64_t ad = make_sdesc(v_base, lbo, 1024, kLayoutSW128);
+          uint64_t bd = make_sdesc(p_base, kTile * 128, 1024, kLayoutSW128);
+#pragma unroll 1
+          for (int kk = 0; kk < kTile / 16; ++kk, ad += 2048 >> 4, bd += 2048 >> 4)
+            umma_f16(o_tmem, ad, bd, idesc, i > first || kk > 0);
           umma_commit(&pempty[t]);
           umma_commit(&vbempty[t]);
         }
@@ -585,12 +669,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     const int total = x1 - x0;
     for (int it = 0; it < total; ++it) {
       const int s = it % ST, t = it & 1;
-      if (!mbar_wait_at(&kfull[s], (it / ST) & 1, ctl, kSiteAtK)) break;
+      if (!mbar_wait_or_abort(&kfull[s], (it / ST) & 1, ctl)) break;
       // D = 128: 128-byte rows, 128-byte swizzle; D = 64: 64-byte rows, 64-byte swizzle (16-byte
       // chunk index exclusive-or bits 7, 8 of the address)
       const uint8_t* src = sK + s * C::KV + row * D;
       const int sw = D == 128 ? (row & 7) : ((row >> 1) & 3);
-      if (!mbar_wait_at(&aempty[t], ((it >> 1) & 1) ^ 1, ctl, kSiteAtK)) break;
+      if (!mbar_wait_or_abort(&aempty[t], ((it >> 1) & 1) ^ 1, ctl)) break;
       tc_fence_after();
       uint32_t dep = 0;
 #pragma unroll 1
@@ -613,53 +697,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     }
   } else if (warp < 12) {
     setmaxnreg_dec<kRegsV>();
-    // ---------------- V codes -> shared memory; Q and the row masks of each segment ----------------
+    // ---------------- V codes -> shared memory ----------------
     const int w = warp - 8;
-    int it = 0, seg = 0;
-    bool ok = true;
-    AttnWalk wk(pre, ta.nb, x0, x1);
-    AttnSeg sg;
-    for (; ok && wk.next(pre, heads, sg); ++seg) {
-      const int64_t b = ta.b0 + sg.b;
-      {
-        const int qb = seg % C::NQ;
-        if (!mbar_wait_at(&qempty[qb], ((seg / C::NQ) & 1) ^ 1, ctl, kSiteAtV)) break;
-        const int nodes = seq_nodes(a, b);
-        const int tid = w * 32 + lane;
-        for (int e = tid; e < R * (D / 8); e += 128) {
-          const int r = e / (D / 8), c = e - r * (D / 8);
-          const int n = (rt * R + r) / grp, g = (rt * R + r) - n * grp;
-          uint4 v = make_uint4(0u, 0u, 0u, 0u);
-          if (n < a.t) {
-            const T* x = static_cast<const T*>(a.q) + b * a.q_sb + n * a.q_st + (sg.h * grp + g) * a.q_sh + c * 8;
-            if (ta.qvec) {
-              v = *reinterpret_cast<const uint4*>(x);
-            } else {
-              const unsigned short* y = reinterpret_cast<const unsigned short*>(x);
-              v = make_uint4(y[0] | (static_cast<uint32_t>(y[1]) << 16), y[2] | (static_cast<uint32_t>(y[3]) << 16),
-                             y[4] | (static_cast<uint32_t>(y[5]) << 16), y[6] | (static_cast<uint32_t>(y[7]) << 16));
-            }
-          }
-          *reinterpret_cast<uint4*>(sQ + qb * C::QB + (c >> 3) * R * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
-        }
-        for (int r = tid; r < R; r += 128) {
-          const int n = (rt * R + r) / grp;
-          rmask[qb * 64 + r] = n < a.t ? node_mask(a, b, n, nodes) : 0ull;
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&qfull[qb]);
-      }
-      for (int i = 0; i < sg.n_kt; ++i, ++it) {
+    const int total = x1 - x0;
+    {
+      for (int it = 0; it < total; ++it) {
         const int s = it % ST, t = it & 1;
-        if (!mbar_wait_at(&vfull[s], (it / ST) & 1, ctl, kSiteAtV)) {
-          ok = false;
-          break;
-        }
-        if (!mbar_wait_at(&vbempty[t], ((it >> 1) & 1) ^ 1, ctl, kSiteAtV)) {
-          ok = false;
-          break;
-        }
+        if (!mbar_wait_or_abort(&vfull[s], (it / ST) & 1, ctl)) break;
+        if (!mbar_wait_or_abort(&vbempty[t], ((it >> 1) & 1) ^ 1, ctl)) break;
         const uint8_t* src = sV + s * C::KV;
         uint8_t* dst = sVB + t * C::VB;
         uint32_t dep = 0;
@@ -709,7 +754,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   } else {
     // ---------------- softmax: thread = slot for the scores, = head dimension for the output ----------------
     setmaxnreg_inc<kRegsSoft>();
-    const int g = (warp - 12) >> 2;    // rows [g RC, (g + 1) RC) of the block
+    const int g = (warp - 12) >> 2;    // group: tiles it % 2 == g, or rows [g RC, (g + 1) RC) of every tile
+    constexpr int STEP = C::ALT ? 2 : 1;
+    const int cb = C::ALT ? 0 : g * RC;            // first row of the group's tiles
+    const int o_col = C::O_COL + (C::ALT ? g * 2 * R : cb);  // its accumulator: hi columns; lo: R further
     const int w = warp & 3;
     const int q = w;                   // TMEM lanes of this warp
     const int row = q * 32 + lane;
@@ -718,52 +766,61 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     const uint32_t lanes = tmem + (static_cast<uint32_t>(q * 32) << 16);
     float* gmax = wred + g * 2 * 4 * 32;
     float* gsum = gmax + 4 * 32;
-    float* mref = refs + g * 2 * 32;
+    float* mref = refs + g * 3 * 32;
     float* fac = mref + 32;
     float* tab = ftab + g * 128;
     const float* zeros = ftab + 2 * 128;
-    int it = 0, seg = 0;
+    int it0 = 0, seg = 0;  // it0: the segment's first tile
     bool ok = true;
     AttnWalk wk(pre, ta.nb, x0, x1);
     AttnSeg sg;
-    for (; ok && wk.next(pre, heads, sg); ++seg) {
+    for (; ok && wk.next(pre, heads, sg); it0 += sg.n_kt, ++seg) {
       const int64_t b = ta.b0 + sg.b;
       const int64_t ctx = seq_ctx(a, b);
       const int nodes = seq_nodes(a, b);
       const int64_t keys = ctx + nodes;
       const int qb = seg % C::NQ;
-      const bool got_q = mbar_wait_at(&qfull[qb], (seg / C::NQ) & 1, ctl, kSiteAtSoft);
+      const bool got_q = mbar_wait_or_abort(&qfull[qb], (seg / C::NQ) & 1, ctl);
       if (tid < RC) mref[tid] = kLowest;
-      if (named_bar_any(bar, 128, !got_q)) break;
-      const unsigned long long* masks = rmask + qb * 64 + g * RC;
+      // A group that gives up still meets the other at the segment's end (barrier 3), where both leave.
+      if (named_bar_any(bar, 128, !got_q)) ok = false;
+      const unsigned long long* masks = rmask + qb * 64 + cb;
       float l[RC];
 #pragma unroll
       for (int c = 0; c < RC; ++c) l[c] = 0.f;
-      for (int i = 0; i < sg.n_kt; ++i, ++it) {
+      const int i0 = C::ALT ? (it0 ^ g) & 1 : 0;  // the group's first tile of the segment
+      for (int i = i0; ok && i < sg.n_kt; i += STEP) {
+        const int it = it0 + i;
         const int t = it & 1;
         const uint32_t ph = (it >> 1) & 1;
-        const int64_t j = static_cast<int64_t>(sg.kt0 + i) * kTile + row;
+        const int64_t j0 = static_cast<int64_t>(sg.kt0 + i) * kTile;
+        const int left = static_cast<int>(min(keys - j0, static_cast<int64_t>(kTile)));  // slots of the tile
         const int sc = it % kScaleStages;
-        bool fine = mbar_wait_at(&scfull[sc], (it / kScaleStages) & 1, ctl, kSiteAtSoft);
+        bool fine = mbar_wait_or_abort(&scfull[sc], (it / kScaleStages) & 1, ctl);
         const float ks = sScale[sc * 2 * kTile + row] * a.scale_log2;
         const float vs = sScale[sc * 2 * kTile + kTile + row];
-        const bool there = j < keys && ((sPages[sc] >> (row >> 2)) & 1);
+        const bool there = row < left && ((sPages[sc] >> (row >> 2)) & 1);
         // a node's slot is seen by the rows whose mask names it, a context slot by all
-        const int node = j >= ctx ? static_cast<int>(j - ctx) : -1;
+        const int node = row + static_cast<int>(max(j0 - ctx, static_cast<int64_t>(-kTile)));
         const bool masked = !there || node >= 0;
-        fine = mbar_wait_at(&sfull[t], ph, ctl, kSiteAtSoft) && fine;
+        fine = mbar_wait_or_abort(&sfull[t], ph, ctl) && fine;
         tc_fence_after();
         // x = score - reference, in powers of two; -inf where the row does not see the slot.  A vote
         // over the group: does any score exceed its row's reference by more than 8?  Then once more
         // from 0 for the rows' maxima, and again from the new references.
         float x[RC];
+        uint32_t see = 0;  // rows that see a slot that not all see
+        if (masked && there) {
+#pragma unroll 1
+          for (int c = 0; c < RC; ++c) see |= static_cast<uint32_t>((masks[c] >> node) & 1) << c;
+        }
         int pass = 0;
 #pragma unroll 1
         for (;; ++pass) {
           const float* m = pass == 1 ? zeros : mref;
 #pragma unroll
           for (int c = 0; c < RC; c += 8)
-            tmem_ld8(lanes + C::S_COL + t * R + g * RC + c, reinterpret_cast<uint32_t*>(x) + c);
+            tmem_ld8(lanes + C::S_COL + t * R + cb + c, reinterpret_cast<uint32_t*>(x) + c);
           tmem_ld_wait();
           const float2 k2 = make_float2(ks, ks);
 #pragma unroll
@@ -779,7 +836,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           if (masked) {
 #pragma unroll
             for (int c = 0; c < RC; ++c)
-              if (!there || !((masks[c] >> node) & 1)) x[c] = -INFINITY;
+              if (!((see >> c) & 1)) x[c] = -INFINITY;
           }
           if (pass == 2) break;
           if (pass == 0) {
@@ -802,8 +859,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             mref[tid] = best;
             fac[tid] = exp2_approx(old - best);
           }
-          // the accumulator is still: the last tile's V . P is complete, the next waits for this one's weights
-          if (i > 0) fine = mbar_wait_at(&pempty[t ^ 1], ((it - 1) >> 1) & 1, ctl, kSiteAtSoft);
+          // the accumulator is still: its last V . P is complete, the next waits for this tile's weights
+          if (i > i0) fine = mbar_wait_or_abort(&pempty[(it - STEP) & 1], ((it - STEP) >> 1) & 1, ctl);
           if (named_bar_any(bar, 128, !fine)) {
             ok = false;
             break;
@@ -811,10 +868,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           tc_fence_after();
 #pragma unroll
           for (int c = 0; c < RC; ++c) l[c] *= fac[c];
-          if (i > 0) {
+          if (i > i0) {
 #pragma unroll 1
             for (int c = 0; c < 2 * RC; c += 8) {  // hi, then lo
-              const uint32_t at = lanes + C::O_COL + (c < RC ? g * RC + c : R + g * RC + c - RC);
+              const uint32_t at = lanes + o_col + (c < RC ? c : R + c - RC);
               const float* f = fac + c % RC;
               uint32_t o[8];
               tmem_ld8(at, o);
@@ -834,7 +891,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           mbar_arrive(&scempty[sc]);
         }
         // weights
-        if (!mbar_wait_at(&pempty[t], ph ^ 1, ctl, kSiteAtSoft)) ctl->abort = 1;
+        if (!mbar_wait_or_abort(&pempty[t], ph ^ 1, ctl)) ctl->abort = 1;
         uint8_t* prow = sP + t * C::PB + row * 128;
 #pragma unroll
         for (int c0 = 0; c0 < RC; c0 += 8) {
@@ -854,7 +911,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             const __nv_bfloat162 r = __float22bfloat162_rn(left);
             lo[e] = *reinterpret_cast<const uint32_t*>(&r);
           }
-          const int nh = g * RC + c0, nl = R + nh;  // columns of P
+          const int nh = cb + c0, nl = R + nh;  // columns of P
           *reinterpret_cast<uint4*>(prow + (nh >> 6) * kTile * 128 + ((((nh & 63) >> 3) ^ (row & 7)) << 4)) =
               make_uint4(hi[0], hi[1], hi[2], hi[3]);
           *reinterpret_cast<uint4*>(prow + (nl >> 6) * kTile * 128 + ((((nl & 63) >> 3) ^ (row & 7)) << 4)) =
@@ -864,8 +921,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         if (masked && !(fabsf(vs) <= 3.402823466e38f)) {
 #pragma unroll 1
           for (int c = 0; c < RC; ++c) {
-            if (there && ((masks[c] >> node) & 1)) continue;
-            const int nh = g * RC + c, nl = R + nh;
+            if ((see >> c) & 1) continue;
+            const int nh = cb + c, nl = R + nh;
             *reinterpret_cast<unsigned short*>(prow + (nh >> 6) * kTile * 128 + ((((nh & 63) >> 3) ^ (row & 7)) << 4) + (nh & 7) * 2) = 0;
             *reinterpret_cast<unsigned short*>(prow + (nl >> 6) * kTile * 128 + ((((nl & 63) >> 3) ^ (row & 7)) << 4) + (nl & 7) * 2) = 0;
           }
@@ -874,124 +931,163 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&pfull[t]);
       }
-      if (!ok) break;
       // ---- the segment's end: sums of the weights, output or piece ----
-      bool fine = mbar_wait_at(&pempty[(it - 1) & 1], ((it - 1) >> 1) & 1, ctl, kSiteAtSoft);
+      const int last = it0 + i0 + (sg.n_kt - 1 - i0) / STEP * STEP;  // the group's last tile
+      const bool any = i0 < sg.n_kt;
+      const bool fine = ok && (!any || mbar_wait_or_abort(&pempty[last & 1], (last >> 1) & 1, ctl));
       {
         const float sum = warp_columns<RC, false>(l, lane);
         if (lane % (32 / RC) == 0) gsum[w * 32 + lane / (32 / RC)] = sum;
       }
-      if (named_bar_any(bar, 128, !fine || ctl->abort)) break;
+      named_bar_sync(bar, 128);
+      if (tid < RC) mref[64 + tid] = ((gsum[tid] + gsum[32 + tid]) + gsum[64 + tid]) + gsum[96 + tid];
+      if (named_bar_any(3, 256, !fine || ctl->abort)) break;
       tc_fence_after();
       if (lane == 0) mbar_arrive(&qempty[qb]);  // the masks are read no more
       const bool mine = row < D;                 // this thread's head dimension
-      if (tid < RC) fac[tid] = ((gsum[tid] + gsum[32 + tid]) + gsum[64 + tid]) + gsum[96 + tid];  // sum of the weights
-      named_bar_sync(bar, 128);
-      // eight rows' values of this thread's head dimension, divided by their sums, to the output
-      auto emit = [&](int c0, const float (&o)[8]) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int r = rt * R + g * RC + c0 + e;
-          const int n = r / grp, gh = r - n * grp;
-          if (mine && n < a.t) {
-            const float den = fac[c0 + e];
-            const float y = den == 0.f || n >= nodes ? 0.f : o[e] / den;
-            static_cast<T*>(a.o)[((b * a.t + n) * a.hq + sg.h * grp + gh) * static_cast<int64_t>(D) + row] = from_f32<T>(y);
-          }
-        }
-      };
-      constexpr int PIECE = R * D + 2 * R;
-      const int c_first = range_owner(sg.u0, units, groups);
-      const int c_last = range_owner(sg.u0 + sg.tiles - 1, units, groups);
-      const bool split = c_last > c_first;
-      float* piece = ta.pieces + (static_cast<int64_t>(blockIdx.x) * 2 + sg.slot) * PIECE;
-#pragma unroll 1
-      for (int c0 = 0; c0 < RC; c0 += 8) {
-        uint32_t hi[8], lo[8];
-        float o[8];
-        tmem_ld8(lanes + C::O_COL + g * RC + c0, hi);
-        tmem_ld8(lanes + C::O_COL + R + g * RC + c0, lo);
-        tmem_ld_wait();
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = __uint_as_float(hi[e]) + __uint_as_float(lo[e]);
-        if (!split) {
-          emit(c0, o);
-        } else if (mine) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) piece[(g * RC + c0 + e) * D + row] = o[e];
+      // From here on a group has the rows [rb, rb + RH): their references and sums, of both streams' where
+      // there are two.
+      const int rb = g * RH;
+      if (tid < RH) {
+        const int c = rb + tid;
+        if constexpr (C::ALT) {
+          const float m0 = refs[c], m1 = refs[96 + c], top = fmaxf(m0, m1);
+          const float f0 = exp2_approx(m0 - top), f1 = exp2_approx(m1 - top);
+          fin[c] = top;
+          fin[64 + c] = f0 * refs[64 + c] + f1 * refs[160 + c];
+          fin[128 + c] = f0;
+          fin[192 + c] = f1;
+        } else {
+          fin[c] = mref[tid];
+          fin[64 + c] = mref[64 + tid];
+          fin[128 + c] = 1.f;
         }
       }
-      tc_fence_before();
-      if (split) {
-        if (tid < RC) piece[R * D + g * RC + tid] = mref[tid];
-        if (tid < RC) piece[R * D + R + g * RC + tid] = fac[tid];
-        __threadfence();
-        named_bar_sync(bar, 128);
-        if (tid == 0) {
-          int* cnt = ta.counters + (c_first * ta.rts + rt) * 2 + g;
-          const bool last = atomicAdd(cnt, 1) == c_last - c_first;
-          if (last) *cnt = 0;
-          gmax[0] = last ? 1.f : 0.f;
-        }
-        named_bar_sync(bar, 128);
-        if (gmax[0] != 0.f) {
-          __threadfence();
-          // piece p of the (sequence, head): CTA c_first + p's first segment, unless it started before
-          auto piece_of = [&](int p) {
-            const int c = c_first + p;
-            const int slot = range_start(c, units, groups) >= sg.u0 ? 0 : 1;
-            return ta.pieces + (static_cast<int64_t>(c * ta.rts + rt) * 2 + slot) * PIECE;
-          };
-          const int n = c_last - c_first + 1;
-          constexpr int SUB = 128 / RC;  // threads of one row
-          const int c = tid % RC, sub = tid / RC;
+      named_bar_sync(bar, 128);
+      T* out = static_cast<T*>(a.o) + (b * a.t * a.hq + sg.h * grp) * static_cast<int64_t>(D) + row;
+      constexpr int PIECE = R * D + 2 * R;
+      const int c_first = range.owner(sg.u0);
+      const int c_last = range.owner(sg.u0 + sg.tiles - 1);
+      const bool split = c_last > c_first;
+      float* piece = ta.pieces + (static_cast<int64_t>(blockIdx.x) * 2 + sg.slot) * PIECE;
+      // piece p of the (sequence, head): CTA c_first + p's first segment, unless it started before
+      auto piece_of = [&](int p) {
+        const int c = c_first + p;
+        const int slot = range.start(c) >= sg.u0 ? 0 : 1;
+        return ta.pieces + (static_cast<int64_t>(c * ta.rts + rt) * 2 + slot) * PIECE;
+      };
+      const int n_p = c_last - c_first + 1;
+      // Stage 0, of a (sequence, head) that several CTAs share: accumulator -> piece, and the last of them
+      // goes on.  Stage 1: accumulator, or the joined pieces -> output.
+#pragma unroll 1
+      for (int stage = split ? 0 : 1; stage < 2; ++stage) {
+        const bool join = split && stage == 1;
+        if (join) {
+          constexpr int SUB = 128 / RH;  // threads of one row
+          const int c = tid % RH, sub = tid / RH;
           float m = kLowest;
-          for (int p = sub; p < n; p += SUB) m = fmaxf(m, __ldcg(piece_of(p) + R * D + g * RC + c));
+#pragma unroll 1
+          for (int p = sub; p < n_p; p += SUB) m = fmaxf(m, __ldcg(piece_of(p) + R * D + rb + c));
           tab[tid] = m;
           named_bar_sync(bar, 128);
-          m = tab[c];
-          for (int k = 1; k < SUB; ++k) m = fmaxf(m, tab[c + k * RC]);
+#pragma unroll 1
+          for (int k = 0; k < SUB; ++k) m = fmaxf(m, tab[c + k * RH]);
           named_bar_sync(bar, 128);
           float sum = 0.f;
-          for (int p = sub; p < n; p += SUB) {
-            const float* pp = piece_of(p) + R * D + g * RC + c;
+#pragma unroll 1
+          for (int p = sub; p < n_p; p += SUB) {
+            const float* pp = piece_of(p) + R * D + rb + c;
             sum += __ldcg(pp + R) * exp2_approx(__ldcg(pp) - m);
           }
           tab[tid] = sum;
-          if (tid < RC) mref[tid] = m;
+          if (tid < RH) fin[rb + tid] = m;
           named_bar_sync(bar, 128);
-          if (tid < RC) {
-            for (int k = 1; k < SUB; ++k) sum += tab[tid + k * RC];
-            fac[tid] = sum;
-          }
+          if (tid < RH) {
 #pragma unroll 1
-          for (int c0 = 0; c0 < RC; c0 += 8) {
-            float o[8];
+            for (int k = 1; k < SUB; ++k) sum += tab[tid + k * RH];
+            fin[64 + rb + tid] = sum;
+          }
+        }
+        if (stage == 1) {
+          if (tid < RH) fin[64 + rb + tid] = inverse(fin[64 + rb + tid]);
+          named_bar_sync(bar, 128);
+        }
+#pragma unroll 1
+        for (int c0 = 0; c0 < RH; c0 += 8) {
+          float o[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) o[e] = 0.f;
-            for (int p0 = 0; p0 < n; p0 += 16) {
+          for (int e = 0; e < 8; ++e) o[e] = 0.f;
+          if (!join) {
+#pragma unroll 1
+            for (int k = 0; k < (C::ALT ? 2 : 1); ++k) {
+              // (a stream without a tile has no accumulator)
+              if (C::ALT && sg.n_kt == 1 && k != (it0 & 1)) continue;
+              uint32_t hi[8], lo[8];
+              tmem_ld8(lanes + C::O_COL + k * 2 * R + rb + c0, hi);
+              tmem_ld8(lanes + C::O_COL + k * 2 * R + R + rb + c0, lo);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                o[e] += (__uint_as_float(hi[e]) + __uint_as_float(lo[e])) * fin[128 + 64 * k + rb + c0 + e];
+            }
+          } else {
+#pragma unroll 1
+            for (int p0 = 0; p0 < n_p; p0 += 16) {
               named_bar_sync(bar, 128);
               // the factors of 16 pieces and 8 rows, one a thread
-              const int p = p0 + (tid >> 3), e = c0 + (tid & 7);
-              tab[tid] = p < n ? exp2_approx(__ldcg(piece_of(p) + R * D + g * RC + e) - mref[e]) : 0.f;
+              const int p = p0 + (tid >> 3), e = rb + c0 + (tid & 7);
+              tab[tid] = p < n_p ? exp2_approx(__ldcg(piece_of(p) + R * D + e) - fin[e]) : 0.f;
               named_bar_sync(bar, 128);
               if (mine) {
-                const int n2 = min(16, n - p0);
-#pragma unroll 4
+                const int n2 = min(16, n_p - p0);
+#pragma unroll 2
                 for (int k = 0; k < n2; ++k) {
-                  const float* pp = piece_of(p0 + k) + (g * RC + c0) * D + row;
+                  const float* pp = piece_of(p0 + k) + (rb + c0) * D + row;
 #pragma unroll
                   for (int q8 = 0; q8 < 8; ++q8) o[q8] += tab[k * 8 + q8] * __ldcg(pp + q8 * D);
                 }
               }
             }
-            emit(c0, o);
           }
+          if (mine) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              if (stage == 0) {
+                piece[(rb + c0 + e) * D + row] = o[e];
+              } else {
+                const int ng = rows[rb + c0 + e];
+                const int n = ng & 0xffff;
+                if (n < a.t)
+                  out[(n * a.hq + (ng >> 16)) * static_cast<int64_t>(D)] =
+                      from_f32<T>(n >= nodes ? 0.f : o[e] * fin[64 + rb + c0 + e]);
+              }
+            }
+          }
+        }
+        if (!join) {
+          tc_fence_before();
+          if (C::ALT) named_bar_sync(3, 256);  // both groups have read both accumulators
+        }
+        if (stage == 0) {
+          if (tid < RH) piece[R * D + rb + tid] = fin[rb + tid];
+          if (tid < RH) piece[R * D + R + rb + tid] = fin[64 + rb + tid];
+          __threadfence();
+          named_bar_sync(bar, 128);
+          if (tid == 0) {
+            int* cnt = ta.counters + (c_first * ta.rts + rt) * 2 + g;
+            const bool final_one = atomicAdd(cnt, 1) == c_last - c_first;
+            if (final_one) *cnt = 0;
+            gmax[0] = final_one ? 1.f : 0.f;
+          }
+          named_bar_sync(bar, 128);
+          if (gmax[0] == 0.f) break;
+          __threadfence();
         }
       }
       // mref, fac and gsum are free for the next segment once everyone is here
       named_bar_sync(bar, 128);
     }
+    if (lane == 0) mbar_arrive(done);
   }
   tc_fence_before();
   __syncthreads();
