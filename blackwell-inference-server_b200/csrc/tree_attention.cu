@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) attn_rows_kernel(const __grid_
 // is joined by its last CTA (a ticket) from the pieces in the workspace, in range order, so results
 // do not depend on timing.
 //
-// One CTA per SM, five warpgroups: 0 TMA (one box per page) and scales, 1 issues K.Q, 2 issues V.P;
+// One CTA per SM, five warpgroups: 0 and 3 TMA (one box per page), scales and Q, 1 issues K.Q, 2 issues V.P;
 // 4-7 dequantise K into TMEM (thread = slot); 8-11 dequantise V into shared memory and load Q; 12-15
 // and 16-19 are two softmax groups of half the rows each.
 // ---------------------------------------------------------------------------
@@ -449,40 +449,16 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 
   if (warp < 4) setmaxnreg_dec<kRegsIssue>();
   if (warp == 0 || warp == 3) {
-    // ------- warp 0: K and V by TMA, one box per page of the tile; warp 3: scales, and each segment's Q and row masks -------
+    // ------- TMA, one box per page of a tile.  Warp 0: K.  Warp 3: V, the scales, each segment's Q and row masks -------
     const int box = min(a.c.page, kTile);           // rows of a box
     const int per = kTile / box;                    // boxes of a tile
     const int tiles_pp = max(a.c.page / kTile, 1);  // tiles of a page
+    const int page_rows = heads * a.c.page;
     const uint64_t pol = ta.rts > 1 ? l2_policy_evict_normal() : l2_policy_evict_first();
-    // lane i looks up the page of box i (of the box its four slots' scales lie in) one tile ahead
-    const int my_box = warp == 0 ? lane : lane * 4 / box;
-    AttnWalk wk(pre, ta.nb, x0, x1);
-    AttnSeg sg;
-    sg.n_kt = 0;
-    int i_seg = 0;
-    int64_t keys = 0;
-    const int* table = nullptr;
-    int seg = -1;
-    bool fresh = false;  // the looked-up tile is its segment's first
-    int pg = -1;       // the looked-up page, not yet checked against the cache
-    int pg_row = 0;    // first row of the box (or four slots) in its (page, head)
-    auto look_up = [&]() {
-      fresh = i_seg == sg.n_kt;
-      if (fresh) {
-        if (!wk.next(pre, heads, sg)) return;
-        i_seg = 0;
-        ++seg;
-        const int64_t room = static_cast<int64_t>(a.c.table_cols) * a.c.page;
-        keys = seq_ctx(a, ta.b0 + sg.b) + seq_nodes(a, ta.b0 + sg.b);
-        keys = keys < room ? keys : room;
-        table = a.c.table + (ta.b0 + sg.b) * a.c.table_ld;
-      }
-      const int kt = sg.kt0 + i_seg++;
-      const int pi = tiles_pp > 1 ? kt / tiles_pp : kt * per + my_box;
-      pg_row = sg.h * a.c.page + (tiles_pp > 1 ? (kt - pi * tiles_pp) * kTile : 0) + (warp == 3 ? lane * 4 % box : 0);
-      pg = -1;
-      if (my_box < per && static_cast<int64_t>(kt) * kTile + my_box * box < keys) pg = table[pi];
-    };
+    uint8_t* ring = warp == 0 ? sK : sV;
+    const CUtensorMap* tm = warp == 0 ? &tm_k : &tm_v;
+    uint64_t* full = warp == 0 ? kfull : vfull;
+    uint64_t* empty = warp == 0 ? kempty : vempty;
     // Q of a segment (row r = node r / grp, query head r % grp of the group) into its swizzled K-major panels
     auto load_q = [&](int sq, const AttnSeg& q_sg) -> bool {
       const int qb = sq % C::NQ;
@@ -527,67 +503,78 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       if (lane == 0) mbar_arrive(&qfull[qb]);
       return true;
     };
-    const int total = x1 - x0;
     bool ok = true;
-    const int page_rows = heads * a.c.page;
-    int it = -1;  // the tile being loaded; its pages were looked up a step ago
+    int it = 0, seg = 0;
+    AttnWalk wk(pre, ta.nb, x0, x1);
+    AttnSeg sg;
 #pragma unroll 1
-    for (; it < total; ++it) {
-      bool have = false;
-      int row = 0;
-      if (it >= 0) {
-        if (warp == 3 && fresh) {
-          ok = load_q(seg, sg);
-          if (!__all_sync(0xffffffffu, ok)) break;
-        }
-        have = pg >= 0 && pg < a.c.pages;
-        row = have ? pg * page_rows + pg_row : 0;
+    for (; ok && wk.next(pre, heads, sg); ++seg) {
+      const int64_t room = static_cast<int64_t>(a.c.table_cols) * a.c.page;
+      const int64_t keys = min(seq_ctx(a, ta.b0 + sg.b) + seq_nodes(a, ta.b0 + sg.b), room);
+      const int* table = a.c.table + (ta.b0 + sg.b) * a.c.table_ld;
+      // 32 boxes' pages at a time, one a lane, fetched while the boxes before them are loaded
+      const int batch = 32 / per;  // tiles
+      auto fetch = [&](int i) -> int {
+        const int64_t slot = static_cast<int64_t>(sg.kt0 + i) * kTile + lane * box;
+        const int pi = tiles_pp > 1 ? (sg.kt0 + i + lane) / tiles_pp : (sg.kt0 + i) * per + lane;
+        return slot < keys ? table[pi] : -1;
+      };
+      int raw = fetch(0), base = -1;
+      if (warp == 3 && !load_q(seg, sg)) {
+        ok = false;
+        break;
       }
-      if (it + 1 < total) look_up();
-      if (it < 0) continue;
-      const uint32_t boxes = __ballot_sync(0xffffffffu, have);
-      if (warp == 0) {
-        const uint32_t bytes = __popc(boxes) * box * D;
+#pragma unroll 1
+      for (int i = 0; i < sg.n_kt; ++i, ++it) {
+        if ((i & (batch - 1)) == 0) {
+          base = raw >= 0 && raw < a.c.pages ? raw * page_rows + sg.h * a.c.page : -1;
+          if (i + batch < sg.n_kt) raw = fetch(i + batch);
+        }
+        const int first = (i & (batch - 1)) * per;  // lane of the tile's first box
+        const int off = tiles_pp > 1 ? (sg.kt0 + i) % tiles_pp * kTile : 0;
+        const int mine = __shfl_sync(0xffffffffu, base, first + (lane & (per - 1)));
+        const bool have = lane < per && mine >= 0;
+        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, have)) * box * D;
         const int s = it % ST;
-        if (it >= ST) ok = mbar_wait_at(&kempty[s], ((it / ST) & 1) ^ 1, ctl, kSiteAtTma);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
+        if (it >= ST) {
+          // warp 0 watches the time for all roles
+          const uint32_t ph = ((it / ST) & 1) ^ 1;
+          ok = warp == 0 ? mbar_wait_at(&empty[s], ph, ctl, kSiteAtTma) : mbar_wait_or_abort(&empty[s], ph, ctl);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
         }
-        if (lane == 0) mbar_arrive_expect_tx(&kfull[s], bytes);
+        if (lane == 0) mbar_arrive_expect_tx(&full[s], bytes);
         __syncwarp();
-        if (have) tma_load_2d(sK + s * C::KV + lane * box * D, &tm_k, &kfull[s], 0, row, pol);
-        if (it >= ST) ok = mbar_wait_at(&vempty[s], ((it / ST) & 1) ^ 1, ctl, kSiteAtTma);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          mbar_wait_at(&kfull[s], (it / ST) & 1, ctl, kSiteAtDrain, false);  // this tile's K has no V behind it
-          break;
-        }
-        if (lane == 0) mbar_arrive_expect_tx(&vfull[s], bytes);
-        __syncwarp();
-        if (have) tma_load_2d(sV + s * C::KV + lane * box * D, &tm_v, &vfull[s], 0, row, pol);
-      } else {
-        const int sc = it % kScaleStages;
-        if (it >= kScaleStages) ok = mbar_wait_or_abort(&scempty[sc], ((it / kScaleStages) & 1) ^ 1, ctl);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        float* dst = sScale + sc * 2 * kTile + lane * 4;
-        cp_async16_zfill(dst, a.c.ks + row, have);
-        cp_async16_zfill(dst + kTile, a.c.vs + row, have);
-        cp_async_arrive_noinc(&scfull[sc]);
-        if (lane == 0) {
-          sPages[sc] = boxes;  // bit l: slots 4 l .. 4 l + 3 exist
-          mbar_arrive(&scfull[sc]);
+        if (have) tma_load_2d(ring + s * C::KV + lane * box * D, tm, &full[s], 0, mine + off, pol);
+        if (warp == 3) {  // scales, four slots a lane
+          const int sc = it % kScaleStages;
+          const int at = __shfl_sync(0xffffffffu, base, first + lane * 4 / box);
+          const uint32_t there = __ballot_sync(0xffffffffu, at >= 0);
+          if (it >= kScaleStages) {
+            ok = mbar_wait_or_abort(&scempty[sc], ((it / kScaleStages) & 1) ^ 1, ctl);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) {
+              ++it;  // (this tile's V is on its way)
+              break;
+            }
+          }
+          const int64_t row = at >= 0 ? at + off + lane * 4 % box : 0;
+          float* dst = sScale + sc * 2 * kTile + lane * 4;
+          cp_async16_zfill(dst, a.c.ks + row, at >= 0);
+          cp_async16_zfill(dst + kTile, a.c.vs + row, at >= 0);
+          cp_async_arrive_noinc(&scfull[sc]);
+          if (lane == 0) {
+            sPages[sc] = there;  // bit l: slots 4 l .. 4 l + 3 exist
+            mbar_arrive(&scfull[sc]);
+          }
         }
       }
     }
-    if (warp == 0 && !ok)  // wait (bounded) for the copies still in flight into this CTA's shared memory
-      for (int j = (it > ST ? it - ST : 0); j < it; ++j) {
-        mbar_wait_at(&kfull[j % ST], (j / ST) & 1, ctl, kSiteAtDrain, false);
-        mbar_wait_at(&vfull[j % ST], (j / ST) & 1, ctl, kSiteAtDrain, false);
-      }
+    if (!ok)  // wait (bounded) for the copies still in flight into this CTA's shared memory
+      for (int j = (it > ST ? it - ST : 0); j < it; ++j)
+        mbar_wait_at(&full[j % ST], (j / ST) & 1, ctl, kSiteAtDrain, false);
     if (warp == 3) cp_async_wait_all();
-    // Warp 0 watches the time for all roles: its own waits run out here, the others' while it waits for the
-    // softmax warps to be done.
+    // (the other roles' waits run out while warp 0 waits for the softmax warps to be done)
     if (warp == 0 && ok) mbar_wait_at(done, 0, ctl, kSiteAtDone);
   } else if (warp == 1) {
     // ---------------- K . Q ----------------
