@@ -146,7 +146,7 @@ constexpr int kRegsIssue = 72, kRegsK = 80, kRegsV = 72, kRegsSoft = 128;
 static_assert(kRegsIssue + kRegsK + kRegsV + 2 * kRegsSoft == 5 * 96, "register split");
 constexpr int kScaleStages = 4;   // tiles whose scales are on their way or in use
 constexpr float kLowest = -3.0e38f;  // a row's reference before any score: finite, so differences are
-constexpr int kAttnMaxBatch = 1024;  // sequences of one launch (their unit ranges lie in shared memory)
+constexpr int kAttnMaxBatch = 512;  // sequences of one launch (their unit ranges lie in shared memory)
 constexpr size_t kAttnCounterBytes = 4096;
 enum AttnSite : int { kSiteAtTma = 401, kSiteAtDrain = 402, kSiteAtDone = 403, kSiteAtFinal = 404 };
 
@@ -171,7 +171,7 @@ struct ACfg {
   static constexpr int OFF_Q = OFF_P + 2 * PB;
   static constexpr int OFF_RING = OFF_Q + NQ * QB;
   static constexpr int SCALES = kScaleStages * (2 * kTile * 4 + 16);
-  static constexpr int CTRL = 640 + SCALES + 2 * 4 * 32 * 4 * 2 + 2 * 3 * 32 * 4 + 4 * 64 * 4 + (2 * 128 + 32) * 4 + 2 * 64 * 8 + 64 * 4 +
+  static constexpr int CTRL = 640 + SCALES + 2 * 4 * 32 * 4 * 2 + 2 * 3 * 32 * 4 + 4 * 64 * 4 + (2 * 256 + 32) * 4 + 2 * 64 * 8 + 64 * 4 +
                               (kAttnMaxBatch + 1) * 4 + 64;
   static constexpr int ROOM = 227 * 1024 - 1024 - OFF_RING - CTRL;
   static constexpr int ST = ROOM / (2 * KV) < 6 ? ROOM / (2 * KV) : 6;  // stages of a K and a V tile
@@ -323,8 +323,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   constexpr int RH = C::RH;
   constexpr int ST = C::ST;
   const AttnArgs& a = ta.a;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* sVB = smem + C::OFF_VB;
   uint8_t* sP = smem + C::OFF_P;
   uint8_t* sQ = smem + C::OFF_Q;
@@ -335,13 +334,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   uint64_t* vfull = kempty + ST;
   uint64_t* vempty = vfull + ST;
   uint64_t* afull = vempty + ST;      // 2: K dequantised in TMEM
-  uint64_t* aempty = afull + 2;
-  uint64_t* vbfull = aempty + 2;      // 2: V dequantised
-  uint64_t* vbempty = vbfull + 2;
-  uint64_t* sfull = vbempty + 2;      // 2: scores
+  uint64_t* vbfull = afull + 2;       // 2: V dequantised
+  uint64_t* sfull = vbfull + 2;       // 2: scores (and the K tile is read)
   uint64_t* sempty = sfull + 2;
   uint64_t* pfull = sempty + 2;       // 2: weights
-  uint64_t* pempty = pfull + 2;       //    (and the accumulator holds the tile's contribution)
+  uint64_t* pempty = pfull + 2;       //    read, as is the V tile, and added to the accumulator
   uint64_t* qfull = pempty + 2;       // 2: Q and the row masks of a segment
   uint64_t* qempty = qfull + 2;
   uint64_t* scfull = qempty + 2;      // scales of a tile
@@ -355,8 +352,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   float* wred = reinterpret_cast<float*>(smem + C::OFF_CTRL + 640 + C::SCALES);  // [2 groups][2][4 warps][32]
   float* refs = wred + 2 * 2 * 4 * 32;                               // [2 groups][3][32]: m, its factor, sums
   float* fin = refs + 2 * 3 * 32;                                    // [4][64]: m, sum, factors of the two streams
-  float* ftab = fin + 4 * 64;                                        // [2 groups][128], 32 zeros
-  unsigned long long* rmask = reinterpret_cast<unsigned long long*>(ftab + 2 * 128 + 32);  // [2][64]
+  float* ftab = fin + 4 * 64;                                        // [2 groups][2][128], 32 zeros
+  unsigned long long* rmask = reinterpret_cast<unsigned long long*>(ftab + 2 * 256 + 32);  // [2][64]
   int* rows = reinterpret_cast<int*>(rmask + 2 * 64);                // [64] node | query head of the group << 16
   int* pre = rows + 64;                                              // [nb + 1] first unit of a sequence
   static_assert((4 * 6 + 24 + 2 * kScaleStages) * 8 + 8 + sizeof(WaitControl) <= 640, "barriers");
@@ -375,9 +372,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&afull[i], 4);
-      mbar_init(&aempty[i], 1);
       mbar_init(&vbfull[i], 4);
-      mbar_init(&vbempty[i], 1);
       mbar_init(&sfull[i], 1);
       mbar_init(&sempty[i], C::GW);
       mbar_init(&pfull[i], C::GW);
@@ -392,7 +387,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       mbar_init(&scempty[i], C::GW);
     }
     ctl->abort = 0;
-    for (int i = 0; i < 32; ++i) ftab[2 * 128 + i] = 0.f;
+    for (int i = 0; i < 32; ++i) ftab[2 * 256 + i] = 0.f;
     ctl->status = ta.status;
     ctl->limit = ta.limit;
     fence_mbar_init();
@@ -605,7 +600,6 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
               umma_f16_ts(tmem + C::S_COL + t * R, a_col, bd, idesc, p + kk);
           }
           umma_commit(&sfull[t]);
-          umma_commit(&aempty[t]);
         }
         if (ok) umma_commit(&qempty[qb]);
       }
@@ -641,7 +635,6 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           for (int kk = 0; kk < kTile / 16; ++kk, ad += 2048 >> 4, bd += 2048 >> 4)
             umma_f16(o_tmem, ad, bd, idesc, i > first || kk > 0);
           umma_commit(&pempty[t]);
-          umma_commit(&vbempty[t]);
         }
       }
       umma_commit(&final_bar[1]);
@@ -661,7 +654,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       // chunk index exclusive-or bits 7, 8 of the address)
       const uint8_t* src = sK + s * C::KV + row * D;
       const int sw = D == 128 ? (row & 7) : ((row >> 1) & 3);
-      if (!mbar_wait_or_abort(&aempty[t], ((it >> 1) & 1) ^ 1, ctl)) break;
+      if (!mbar_wait_or_abort(&sfull[t], ((it >> 1) & 1) ^ 1, ctl)) break;
       tc_fence_after();
       uint32_t dep = 0;
 #pragma unroll 1
@@ -691,7 +684,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       for (int it = 0; it < total; ++it) {
         const int s = it % ST, t = it & 1;
         if (!mbar_wait_or_abort(&vfull[s], (it / ST) & 1, ctl)) break;
-        if (!mbar_wait_or_abort(&vbempty[t], ((it >> 1) & 1) ^ 1, ctl)) break;
+        if (!mbar_wait_or_abort(&pempty[t], ((it >> 1) & 1) ^ 1, ctl)) break;
         const uint8_t* src = sV + s * C::KV;
         uint8_t* dst = sVB + t * C::VB;
         uint32_t dep = 0;
@@ -755,8 +748,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     float* gsum = gmax + 4 * 32;
     float* mref = refs + g * 3 * 32;
     float* fac = mref + 32;
-    float* tab = ftab + g * 128;
-    const float* zeros = ftab + 2 * 128;
+    float* tab = ftab + g * 256;
+    const float* zeros = ftab + 2 * 256;
     int it0 = 0, seg = 0;  // it0: the segment's first tile
     bool ok = true;
     AttnWalk wk(pre, ta.nb, x0, x1);
@@ -971,29 +964,29 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         const bool join = split && stage == 1;
         if (join) {
           constexpr int SUB = 128 / RH;  // threads of one row
-          const int c = tid % RH, sub = tid / RH;
-          float m = kLowest;
+          float m = kLowest, sum = 0.f;
 #pragma unroll 1
-          for (int p = sub; p < n_p; p += SUB) m = fmaxf(m, __ldcg(piece_of(p) + R * D + rb + c));
-          tab[tid] = m;
-          named_bar_sync(bar, 128);
-#pragma unroll 1
-          for (int k = 0; k < SUB; ++k) m = fmaxf(m, tab[c + k * RH]);
-          named_bar_sync(bar, 128);
-          float sum = 0.f;
-#pragma unroll 1
-          for (int p = sub; p < n_p; p += SUB) {
-            const float* pp = piece_of(p) + R * D + rb + c;
-            sum += __ldcg(pp + R) * exp2_approx(__ldcg(pp) - m);
+          for (int p = tid / RH; p < n_p; p += SUB) {
+            const float* pp = piece_of(p) + R * D + rb + tid % RH;
+            const float pm = __ldcg(pp), ps = __ldcg(pp + R);
+            const float top = fmaxf(m, pm);
+            sum = sum * exp2_approx(m - top) + ps * exp2_approx(pm - top);
+            m = top;
           }
-          tab[tid] = sum;
-          if (tid < RH) fin[rb + tid] = m;
+          tab[tid] = m;
+          tab[128 + tid] = sum;
           named_bar_sync(bar, 128);
           if (tid < RH) {
 #pragma unroll 1
-            for (int k = 1; k < SUB; ++k) sum += tab[tid + k * RH];
+            for (int k = 1; k < SUB; ++k) {
+              const float pm = tab[tid + k * RH], top = fmaxf(m, pm);
+              sum = sum * exp2_approx(m - top) + tab[128 + tid + k * RH] * exp2_approx(pm - top);
+              m = top;
+            }
+            fin[rb + tid] = m;
             fin[64 + rb + tid] = sum;
           }
+          named_bar_sync(bar, 128);
         }
         if (stage == 1) {
           if (tid < RH) fin[64 + rb + tid] = inverse(fin[64 + rb + tid]);
@@ -1018,22 +1011,26 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                 o[e] += (__uint_as_float(hi[e]) + __uint_as_float(lo[e])) * fin[128 + 64 * k + rb + c0 + e];
             }
           } else {
+            // four pieces at a time: every thread's values and, by one warp, their factors on the way together
 #pragma unroll 1
-            for (int p0 = 0; p0 < n_p; p0 += 16) {
-              named_bar_sync(bar, 128);
-              // the factors of 16 pieces and 8 rows, one a thread
-              const int p = p0 + (tid >> 3), e = rb + c0 + (tid & 7);
-              tab[tid] = p < n_p ? exp2_approx(__ldcg(piece_of(p) + R * D + e) - fin[e]) : 0.f;
-              named_bar_sync(bar, 128);
-              if (mine) {
-                const int n2 = min(16, n_p - p0);
-#pragma unroll 2
-                for (int k = 0; k < n2; ++k) {
-                  const float* pp = piece_of(p0 + k) + (rb + c0) * D + row;
+            for (int p0 = 0; p0 < n_p; p0 += 4) {
+              float v[4][8];
 #pragma unroll
-                  for (int q8 = 0; q8 < 8; ++q8) o[q8] += tab[k * 8 + q8] * __ldcg(pp + q8 * D);
-                }
+              for (int k = 0; k < 4; ++k) {
+                const float* pp = piece_of(min(p0 + k, n_p - 1)) + (rb + c0) * D + (mine ? row : 0);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[k][e] = __ldcg(pp + e * D);
               }
+              if (tid < 32) {
+                const int p = p0 + (tid >> 3), e = rb + c0 + (tid & 7);
+                tab[tid] = p < n_p ? exp2_approx(__ldcg(piece_of(p) + R * D + e) - fin[e]) : 0.f;
+              }
+              named_bar_sync(bar, 128);
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] += v[k][e] * tab[k * 8 + e];
+              named_bar_sync(bar, 128);
             }
           }
           if (mine) {
@@ -1058,17 +1055,17 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         if (stage == 0) {
           if (tid < RH) piece[R * D + rb + tid] = fin[rb + tid];
           if (tid < RH) piece[R * D + R + rb + tid] = fin[64 + rb + tid];
-          __threadfence();
           named_bar_sync(bar, 128);
           if (tid == 0) {
             int* cnt = ta.counters + (c_first * ta.rts + rt) * 2 + g;
+            __threadfence();  // the group's stores, seen through the barrier, come before the ticket
             const bool final_one = atomicAdd(cnt, 1) == c_last - c_first;
+            __threadfence();
             if (final_one) *cnt = 0;
             gmax[0] = final_one ? 1.f : 0.f;
           }
           named_bar_sync(bar, 128);
           if (gmax[0] == 0.f) break;
-          __threadfence();
         }
       }
       // mref, fac and gsum are free for the next segment once everyone is here
