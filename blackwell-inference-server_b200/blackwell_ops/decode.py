@@ -26,7 +26,7 @@ import threading
 
 import torch
 
-from ._lib import DTYPE_CODE, check, lib, stream_ptr
+from ._lib import DTYPE_CODE, check, lib
 
 MAX_NODES = 64      # nodes of a draft tree: one bit each
 MAX_HEAD_DIM = 256
@@ -36,13 +36,22 @@ _ws_lock = threading.Lock()
 _workspaces: dict[tuple[int, int], torch.Tensor] = {}
 
 
+# These operators are called once a layer and step, so what a call costs on the host counts: the current
+# stream's handle and device come without the objects around them.
+_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+
+
 def _call(op: str, dev: torch.device, fn, *args) -> None:
     """fn(*args, stream) on dev's current stream."""
-    if dev.index == torch.cuda.current_device():
-        check(fn(*args, stream_ptr(dev)), op)
+    index = dev.index
+    if index == _current_device():
+        status = fn(*args, _stream(index))
     else:
         with torch.cuda.device(dev):
-            check(fn(*args, stream_ptr(dev)), op)
+            status = fn(*args, _stream(index))
+    if status:
+        check(status, op)
 
 
 def reset_workspaces() -> None:
@@ -53,12 +62,12 @@ def reset_workspaces() -> None:
 
 
 def _workspace(dev: torch.device, nbytes: int) -> torch.Tensor:
-    key = (dev.index, stream_ptr(dev))
+    """Scratch of the current stream; its counters start, and stay, zero."""
+    key = (dev.index, _stream(dev.index))
     ws = _workspaces.get(key)
     if ws is None or ws.numel() < nbytes:
         with _ws_lock:
-            ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=dev)
-            _workspaces[key] = ws
+            ws = _workspaces[key] = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=dev)
     return ws
 
 
@@ -151,31 +160,38 @@ def rotary_plan(rot_dim: int, base: float = 10000.0, scaling: dict | None = None
     return RotaryPlan(f, mag, interleaved, device)
 
 
-def _rows(x: torch.Tensor, name: str, lead: tuple | None) -> tuple[torch.Tensor, int, int, int, int, int]:
-    """x [.., heads, d] as (x, b, t, stride b, stride t, stride of heads); leading dims must merge into two."""
+def _rows(x: torch.Tensor, name: str, lead: tuple) -> tuple[torch.Tensor, tuple, int, int, int, int, int]:
+    """x [.., heads, d] as (x, shape, b, t, stride b, stride t, stride of heads); its leading dimensions are
+    merged into two."""
     if not x.is_cuda:
         raise RuntimeError(f"{name} must be CUDA")
     if x.dtype not in _HALF:
         raise RuntimeError(f"{name} must be fp16 or bf16")
-    if x.dim() < 3:
+    shape = x.shape
+    n = len(shape)
+    if n < 3:
         raise RuntimeError(f"{name} must be [.., heads, d]")
-    if lead is not None and tuple(x.shape[:-2]) != lead:
+    if shape[:-2] != lead:
         raise RuntimeError(f"{name} must have leading dimensions {list(lead)}")
-    if x.shape[-1] > 1 and x.stride(-1) != 1:
+    stride = x.stride()
+    if stride[-1] != 1 and shape[-1] > 1:
         x = x.contiguous()
-    if x.dim() == 3:
-        return x, 1, x.shape[0], 0, x.stride(0), x.stride(1)
-    if x.dim() > 4:
-        x = x.reshape(-1, *x.shape[-3:])
-    return x, x.shape[0], x.shape[1], x.stride(0), x.stride(1), x.stride(2)
+        stride = x.stride()
+    if n == 4:
+        return x, shape, shape[0], shape[1], stride[0], stride[1], stride[2]
+    if n == 3:
+        return x, shape, 1, shape[0], 0, stride[0], stride[1]
+    x = x.reshape(-1, *shape[-3:])
+    stride = x.stride()
+    return x, shape, x.shape[0], x.shape[1], stride[0], stride[1], stride[2]
 
 
 def _positions(positions: torch.Tensor, lead: tuple, dev: torch.device) -> torch.Tensor:
     if positions.device != dev:
         raise RuntimeError("positions must be on the inputs' device")
-    if positions.dtype not in (torch.int32, torch.int64):
+    if positions.dtype is not torch.int32 and positions.dtype is not torch.int64:
         raise RuntimeError("positions must be int32 or int64")
-    if tuple(positions.shape) != lead:
+    if positions.shape != lead:
         raise RuntimeError(f"positions must be {list(lead)}")
     return positions if positions.is_contiguous() else positions.contiguous()
 
@@ -186,26 +202,26 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
 
     Pair i of the first ``plan.rot_dim`` elements of a head turns by ``position * f_i``; the other
     elements are copied.  32-bit arithmetic, rounded once.  Returns new contiguous tensors."""
-    lead = tuple(q.shape[:-2])
-    q, b, t, qb, qt, qh = _rows(q, "q", lead)
-    dev, d, hq = q.device, q.shape[-1], q.shape[-2]
+    lead = q.shape[:-2]
+    q, shape, b, t, qb, qt, qh = _rows(q, "q", lead)
+    dev, dt, hq, d = q.device, q.dtype, shape[-2], shape[-1]
     if plan.rot_dim > d or d > MAX_HEAD_DIM:
         raise RuntimeError(f"rotary: need rot_dim <= D <= {MAX_HEAD_DIM}")
     if plan.device != dev:
         raise RuntimeError("rotary: the plan is on another device")
     positions = _positions(positions, lead, dev)
-    q_out = torch.empty((*lead, hq, d), dtype=q.dtype, device=dev)
+    q_out = torch.empty(shape, dtype=dt, device=dev)
     k_out, hk, kb, kt, kh, kp, kop = None, 0, 0, 0, 0, None, None
     if k is not None:
-        k, _, _, kb, kt, kh = _rows(k, "k", lead)
-        if k.dtype != q.dtype or k.device != dev or k.shape[-1] != d:
+        k, kshape, _, _, kb, kt, kh = _rows(k, "k", lead)
+        if k.dtype is not dt or k.device != dev or kshape[-1] != d:
             raise RuntimeError("k must have q's dtype, device and head dimension")
-        hk = k.shape[-2]
-        k_out = torch.empty((*lead, hk, d), dtype=k.dtype, device=dev)
+        hk = kshape[-2]
+        k_out = torch.empty(kshape, dtype=dt, device=dev)
         kp, kop = k.data_ptr(), k_out.data_ptr()
     if d:
         _call("rotary", dev, lib.bw_rotary, q.data_ptr(), qb, qt, qh, hq, kp, kb, kt, kh, hk, q_out.data_ptr(), kop,
-              DTYPE_CODE[q.dtype], b, t, d, positions.data_ptr(), positions.dtype == torch.int64, plan._ptr,
+              DTYPE_CODE[dt], b, t, d, positions.data_ptr(), positions.dtype is torch.int64, plan._ptr,
               plan.magnitude, plan.rot_dim, plan.interleaved)
     return q_out, k_out
 
@@ -264,67 +280,68 @@ class KVCacheInt8:
             raise RuntimeError(f"{op}: takes one layer of the cache; pass cache.layer(i)")
 
 
-def _ints(x: torch.Tensor | None, name: str, shape: tuple, dev: torch.device) -> torch.Tensor | None:
+def _ints(x: torch.Tensor, name: str, shape: tuple, dev: torch.device) -> torch.Tensor:
     """A contiguous int32 tensor of that shape."""
     if x is None:
-        return None
-    if x.dtype != torch.int32 or x.device != dev:
+        raise RuntimeError(f"{name} must be {list(shape)}")
+    if x.dtype is not torch.int32 or x.device != dev:
         raise RuntimeError(f"{name} must be int32 on the cache's device")
-    if tuple(x.shape) != shape:
+    if x.shape != shape:
         raise RuntimeError(f"{name} must be {list(shape)}")
     return x if x.is_contiguous() else x.contiguous()
 
 
-def _table(table: torch.Tensor, dev: torch.device) -> torch.Tensor:
-    if table.dtype != torch.int32 or table.device != dev:
+def _table(table: torch.Tensor, dev: torch.device) -> tuple[torch.Tensor, int, int, int]:
+    """(table, its sequences, row stride, columns)"""
+    if table.dtype is not torch.int32 or table.device != dev:
         raise RuntimeError("table must be int32 on the cache's device")
     if table.dim() != 2:
         raise RuntimeError("table must be [B, pages of a sequence]")
-    if table.stride(1) != 1 or table.stride(0) < table.shape[1]:
+    b, cols = table.shape
+    ld, unit = table.stride()
+    if unit != 1 or ld < cols:
         table = table.contiguous()
-    return table
-
-
-def _ptr(x: torch.Tensor | None) -> int | None:
-    return None if x is None else x.data_ptr()
+        ld = cols
+    return table, b, ld, cols
 
 
 def _write(q, k, v, positions, plan, cache, table, start, counts, op):
-    cache._one_layer(op)
+    if cache.layers is not None:
+        cache._one_layer(op)
     dev = cache.device
     if k.dim() != 4:
         raise RuntimeError(f"{op}: k must be [B, T, heads, D]")
-    lead = tuple(k.shape[:2])
-    k, b, t, kb, kt, kh = _rows(k, "k", lead)
-    v, _, _, vb, vt, vh = _rows(v, "v", lead)
-    if k.shape[2:] != (cache.heads, cache.head_dim) or v.shape[2:] != k.shape[2:]:
-        raise RuntimeError(f"{op}: k and v must be [B, T, {cache.heads}, {cache.head_dim}] like the cache")
-    if k.dtype != v.dtype or k.device != dev or v.device != dev:
+    lead = k.shape[:2]
+    k, kshape, b, t, kb, kt, kh = _rows(k, "k", lead)
+    v, vshape, _, _, vb, vt, vh = _rows(v, "v", lead)
+    d, dt = cache.head_dim, k.dtype
+    if kshape[2] != cache.heads or kshape[3] != d or vshape != kshape:
+        raise RuntimeError(f"{op}: k and v must be [B, T, {cache.heads}, {d}] like the cache")
+    if v.dtype is not dt or k.device != dev or v.device != dev:
         raise RuntimeError(f"{op}: k and v must share one dtype and be on the cache's device")
-    table = _table(table, dev)
-    if table.shape[0] != b:
+    table, rows, ld, cols = _table(table, dev)
+    if rows != b:
         raise RuntimeError(f"{op}: table must have a row for each of {b} sequences")
     start = _ints(start, "start", (b,), dev)
-    if start is None:
-        raise RuntimeError(f"{op}: start must be [B]")
-    counts = _ints(counts, "counts", (b,), dev)
+    if counts is not None:
+        counts = _ints(counts, "counts", (b,), dev)
     q_out, qp, qb, qt, qh, hq, qop = None, None, 0, 0, 0, 0, None
     pp, p64, sp, mag, rot, inter = None, 0, None, 1.0, 0, 0
     if plan is not None:
-        q, _, _, qb, qt, qh = _rows(q, "q", lead)
-        if q.dtype != k.dtype or q.device != dev or q.shape[3] != cache.head_dim:
+        q, qshape, _, _, qb, qt, qh = _rows(q, "q", lead)
+        if q.dtype is not dt or q.device != dev or qshape[3] != d:
             raise RuntimeError(f"{op}: q must have k's dtype, device and head dimension")
-        if plan.device != dev or plan.rot_dim > cache.head_dim:
+        if plan.device != dev or plan.rot_dim > d:
             raise RuntimeError(f"{op}: the plan must be on the cache's device with rot_dim <= D")
         positions = _positions(positions, lead, dev)
-        hq = q.shape[2]
-        q_out = torch.empty((b, t, hq, cache.head_dim), dtype=q.dtype, device=dev)
+        hq = qshape[2]
+        q_out = torch.empty(qshape, dtype=dt, device=dev)
         qp, qop = q.data_ptr(), q_out.data_ptr()
-        pp, p64, sp = positions.data_ptr(), positions.dtype == torch.int64, plan._ptr
+        pp, p64, sp = positions.data_ptr(), positions.dtype is torch.int64, plan._ptr
         mag, rot, inter = plan.magnitude, plan.rot_dim, plan.interleaved
     _call(op, dev, lib.bw_rotary_kv_write_int8, qp, qb, qt, qh, hq, k.data_ptr(), kb, kt, kh, v.data_ptr(), vb, vt, vh,
-          qop, DTYPE_CODE[k.dtype], b, t, pp, p64, sp, mag, rot, inter, *cache._ptrs, *cache._dims, table.data_ptr(),
-          table.stride(0), table.shape[1], start.data_ptr(), _ptr(counts))
+          qop, DTYPE_CODE[dt], b, t, pp, p64, sp, mag, rot, inter, *cache._ptrs, *cache._dims, table.data_ptr(), ld, cols,
+          start.data_ptr(), None if counts is None else counts.data_ptr())
     return q_out
 
 
@@ -355,15 +372,15 @@ def kv_read_int8(cache: KVCacheInt8, table: torch.Tensor, start: torch.Tensor | 
         raise RuntimeError("kv_read_int8: dtype must be fp16 or bf16")
     if n < 0:
         raise RuntimeError("kv_read_int8: n must not be negative")
-    table = _table(table, dev)
-    b = table.shape[0]
-    start, lens = _ints(start, "start", (b,), dev), _ints(lens, "lens", (b,), dev)
-    shape = (b, n, cache.heads, cache.head_dim) if cache.layers is None else (cache.layers, b, n, cache.heads,
-                                                                               cache.head_dim)
+    table, b, ld, cols = _table(table, dev)
+    sp = None if start is None else _ints(start, "start", (b,), dev)
+    lp = None if lens is None else _ints(lens, "lens", (b,), dev)
+    layers = cache.layers
+    shape = (b, n, cache.heads, cache.head_dim) if layers is None else (layers, b, n, cache.heads, cache.head_dim)
     k = torch.empty(shape, dtype=dtype, device=dev)
     v = torch.empty(shape, dtype=dtype, device=dev)
-    _call("kv_read_int8", dev, lib.bw_kv_read_int8, *cache._ptrs, 1 if cache.layers is None else cache.layers,
-          *cache._dims, table.data_ptr(), table.stride(0), table.shape[1], _ptr(start), _ptr(lens), b, n,
+    _call("kv_read_int8", dev, lib.bw_kv_read_int8, *cache._ptrs, 1 if layers is None else layers, *cache._dims,
+          table.data_ptr(), ld, cols, None if sp is None else sp.data_ptr(), None if lp is None else lp.data_ptr(), b, n,
           k.data_ptr(), v.data_ptr(), DTYPE_CODE[dtype])
     return k, v
 
@@ -375,17 +392,14 @@ def kv_move_int8(cache: KVCacheInt8, table: torch.Tensor, start: torch.Tensor, p
     The tree of sequence b lies at slots ``start[b] + node``; nodes ``path[b, :taken[b]]`` (as
     ``verify_tree`` gives them) go to slots ``start[b] + 1, start[b] + 2, ..``."""
     dev = cache.device
-    table = _table(table, dev)
-    b = table.shape[0]
+    table, b, ld, cols = _table(table, dev)
     if path.dim() != 2 or path.shape[1] > MAX_NODES:
         raise RuntimeError(f"path must be [B, T] with T <= {MAX_NODES}")
-    path = _ints(path, "path", (b, path.shape[1]), dev)
+    t = path.shape[1]
+    path = _ints(path, "path", (b, t), dev)
     start, taken = _ints(start, "start", (b,), dev), _ints(taken, "taken", (b,), dev)
-    if start is None or taken is None:
-        raise RuntimeError("kv_move_int8: start and taken must be [B]")
     _call("kv_move_int8", dev, lib.bw_kv_move_int8, *cache._ptrs, 1 if cache.layers is None else cache.layers,
-          *cache._dims, table.data_ptr(), table.stride(0), table.shape[1], start.data_ptr(), path.data_ptr(),
-          path.shape[1], taken.data_ptr(), b, path.shape[1])
+          *cache._dims, table.data_ptr(), ld, cols, start.data_ptr(), path.data_ptr(), t, taken.data_ptr(), b, t)
 
 
 # ---------------------------------------------------------------- trees
@@ -402,11 +416,12 @@ def tree_positions(parents: torch.Tensor, ctx_lens: torch.Tensor | None = None) 
     dev = parents.device
     parents = parents.contiguous()
     b, t = parents.shape
-    ctx_lens = _ints(ctx_lens, "ctx_lens", (b,), dev)
+    if ctx_lens is not None:
+        ctx_lens = _ints(ctx_lens, "ctx_lens", (b,), dev)
     mask = torch.empty((b, t), dtype=torch.int64, device=dev)
     pos = torch.empty((b, t), dtype=torch.int32, device=dev)
-    _call("tree_positions", dev, lib.bw_tree_positions, parents.data_ptr(), t, _ptr(ctx_lens), b, t, mask.data_ptr(),
-          pos.data_ptr())
+    _call("tree_positions", dev, lib.bw_tree_positions, parents.data_ptr(), t,
+          None if ctx_lens is None else ctx_lens.data_ptr(), b, t, mask.data_ptr(), pos.data_ptr())
     return mask, pos
 
 
@@ -420,40 +435,47 @@ def tree_attention_int8(q: torch.Tensor, cache: KVCacheInt8, table: torch.Tensor
     limits a sequence's nodes: later ones are not seen and give zeros, and so does a node that sees
     nothing.  Query head h reads key head ``h // (Hq / heads)``.  T <= 64; T = 1 is ordinary decoding.
     ``softmax_scale`` defaults to ``D ** -0.5``."""
-    cache._one_layer("tree_attention_int8")
-    dev = cache.device
-    if not q.is_cuda or q.dtype not in _HALF:
+    if cache.layers is not None:
+        cache._one_layer("tree_attention_int8")
+    dev, dt = cache.device, q.dtype
+    if not q.is_cuda or dt not in _HALF:
         raise RuntimeError("q must be CUDA fp16 or bf16")
     if q.dim() != 4 or q.device != dev:
         raise RuntimeError("q must be [B, T, heads, D] on the cache's device")
-    b, t, hq, d = q.shape
+    shape = q.shape
+    b, t, hq, d = shape
+    heads = cache.heads
     if d != cache.head_dim:
         raise RuntimeError(f"q must have the cache's head dimension {cache.head_dim}")
-    if hq == 0 or hq % cache.heads:
-        raise RuntimeError(f"q's heads must be a multiple of the cache's {cache.heads}")
+    if hq == 0 or hq % heads:
+        raise RuntimeError(f"q's heads must be a multiple of the cache's {heads}")
     if t > MAX_NODES:
         raise RuntimeError(f"at most {MAX_NODES} nodes a sequence")
-    if d > 1 and q.stride(3) != 1:
+    stride = q.stride()
+    if stride[3] != 1 and d > 1:
         q = q.contiguous()
-    table = _table(table, dev)
-    if table.shape[0] != b:
+        stride = q.stride()
+    table, rows, ld, cols = _table(table, dev)
+    if rows != b:
         raise RuntimeError(f"table must have a row for each of {b} sequences")
-    ctx_lens, counts = _ints(ctx_lens, "ctx_lens", (b,), dev), _ints(counts, "counts", (b,), dev)
-    if ctx_lens is None:
-        raise RuntimeError("ctx_lens must be [B]")
+    ctx_lens = _ints(ctx_lens, "ctx_lens", (b,), dev)
+    if counts is not None:
+        counts = _ints(counts, "counts", (b,), dev)
     if mask is not None:
-        if mask.dtype != torch.int64 or mask.device != dev or tuple(mask.shape) != (b, t):
+        if mask.dtype is not torch.int64 or mask.device != dev or mask.shape != (b, t):
             raise RuntimeError(f"mask must be int64 [{b}, {t}] on the cache's device")
-        mask = mask.contiguous()
-    out = torch.empty((b, t, hq, d), dtype=q.dtype, device=dev)
+        if not mask.is_contiguous():
+            mask = mask.contiguous()
+    out = torch.empty(shape, dtype=dt, device=dev)
     if b == 0 or t == 0:
         return out
-    nbytes = lib.bw_tree_attention_int8_workspace_size(b, t, hq, cache.heads, d)
+    nbytes = lib.bw_tree_attention_int8_workspace_size(b, t, hq, heads, d)
     ws = _workspace(dev, nbytes) if nbytes else None
-    _call("tree_attention_int8", dev, lib.bw_tree_attention_int8, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2),
-          DTYPE_CODE[q.dtype], out.data_ptr(), *cache._ptrs, *cache._dims, table.data_ptr(), table.stride(0),
-          table.shape[1], ctx_lens.data_ptr(), _ptr(mask), _ptr(counts), b, t, hq,
-          d ** -0.5 if softmax_scale is None else float(softmax_scale), _ptr(ws), 0 if ws is None else ws.numel())
+    _call("tree_attention_int8", dev, lib.bw_tree_attention_int8, q.data_ptr(), stride[0], stride[1], stride[2],
+          DTYPE_CODE[dt], out.data_ptr(), *cache._ptrs, *cache._dims, table.data_ptr(), ld, cols, ctx_lens.data_ptr(),
+          None if mask is None else mask.data_ptr(), None if counts is None else counts.data_ptr(), b, t, hq,
+          d ** -0.5 if softmax_scale is None else float(softmax_scale), None if ws is None else ws.data_ptr(),
+          0 if ws is None else nbytes)
     return out
 
 
@@ -482,13 +504,14 @@ def verify_tree(target_probs: torch.Tensor, tokens: torch.Tensor, parents: torch
     b, t, v = target_probs.shape
     if t > MAX_NODES:
         raise RuntimeError(f"at most {MAX_NODES} nodes a sequence")
-    if tokens.dtype != torch.int64 or tokens.device != dev or tuple(tokens.shape) != (b, t):
+    nodes, row = (b, t), (b, v)
+    if tokens.dtype is not torch.int64 or tokens.device != dev or tokens.shape != nodes:
         raise RuntimeError(f"tokens must be int64 [{b}, {t}] on the probabilities' device")
-    if parents.dtype != torch.int32 or parents.device != dev or tuple(parents.shape) != (b, t):
+    if parents.dtype is not torch.int32 or parents.device != dev or parents.shape != nodes:
         raise RuntimeError(f"parents must be int32 [{b}, {t}] on the probabilities' device")
-    if accept_u.dtype != torch.float32 or accept_u.device != dev or tuple(accept_u.shape) != (b, t):
+    if accept_u.dtype is not torch.float32 or accept_u.device != dev or accept_u.shape != nodes:
         raise RuntimeError(f"accept_u must be fp32 [{b}, {t}] on the probabilities' device")
-    if sample_e.dtype != torch.float32 or sample_e.device != dev or tuple(sample_e.shape) != (b, v):
+    if sample_e.dtype is not torch.float32 or sample_e.device != dev or sample_e.shape != row:
         raise RuntimeError(f"sample_e must be fp32 [{b}, {v}] on the probabilities' device")
     if draft_probs is not None:
         if draft_probs.dtype != torch.float32 or draft_probs.device != dev or draft_probs.shape != target_probs.shape:
@@ -501,7 +524,8 @@ def verify_tree(target_probs: torch.Tensor, tokens: torch.Tensor, parents: torch
     out = torch.empty((b, t), dtype=torch.int64, device=dev)
     if b and not t:
         n.zero_()
-    _call("verify_tree", dev, lib.bw_verify_tree, target_probs.data_ptr(), _ptr(draft_probs), tokens.data_ptr(),
+    _call("verify_tree", dev, lib.bw_verify_tree, target_probs.data_ptr(),
+          None if draft_probs is None else draft_probs.data_ptr(), tokens.data_ptr(),
           parents.data_ptr(), accept_u.data_ptr(), sample_e.data_ptr(), b, t, v, n.data_ptr(), path.data_ptr(),
           out.data_ptr())
     return n, path, out

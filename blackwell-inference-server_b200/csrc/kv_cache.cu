@@ -14,6 +14,8 @@
 // order of a bf16 ulp to codes of 1/127 of the row's maximum.
 #include <stdio.h>
 
+#include <type_traits>
+
 #include "kv_cache.cuh"
 #include "quant_math.cuh"
 
@@ -128,10 +130,161 @@ __global__ void __launch_bounds__(256) rotary_rows_kernel(const __grid_constant_
   }
 }
 
+// Eight 16-bit values of a 16-byte chunk <-> fp32.
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& v, float* f) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (std::is_same<T, __half>::value) {
+      const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      f[2 * i] = p.x;
+      f[2 * i + 1] = p.y;
+    } else {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float* f) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (std::is_same<T, __half>::value) {
+      const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint2 codes8(const float* f, float sc, float rcp) {
+  uint32_t w[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    w[h] = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[h] |= static_cast<uint32_t>(static_cast<uint8_t>(quant_fast<BW_DTYPE_F32>(f[4 * h + i], sc, rcp))) << (8 * i);
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+// Aligned rows of D = 16 L elements, rot a multiple of 16.  L lanes hold a row, 16 elements each in two
+// 16-byte chunks, so every pair lies in one lane: half layout, rotated lane j: elements 8 j .. and
+// rot/2 + 8 j ..; interleaved, and where nothing turns: 16 consecutive elements.  The sines of a lane's
+// eight pairs are computed once a token and serve the rows that the lane takes in turn (every `gpt`-th
+// row of the token): bound by the bytes where tokens are many, by latency where they are few, for which
+// the host spreads a token over more lanes.
+template <typename T, int L, bool WRITE>
+__global__ void __launch_bounds__(256) rotary_vec_kernel(const __grid_constant__ RotArgs a, int gpt) {
+  constexpr int D = 16 * L;
+  const int j = threadIdx.x % L;
+  const int64_t group = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / L;
+  const int64_t tok = group / gpt;
+  const int g = static_cast<int>(group - tok * gpt);
+  if (tok >= a.b * a.t) return;  // (a whole group at once: the shuffles below stay inside one)
+  const int64_t b = tok / a.t, t = tok - b * a.t;
+  const bool turns = j < a.rot / 16;
+  const int e0 = !turns || a.interleaved ? 16 * j : 8 * j;
+  const int e1 = !turns || a.interleaved ? 16 * j + 8 : a.rot / 2 + 8 * j;
+  const int hq = a.q.heads, hqk = hq + a.k.heads, rows = hqk + a.v.heads;
+  int64_t krow = -1;
+  if (WRITE && (a.counts == nullptr || t < a.counts[b])) krow = kv_row(a.cache, b, static_cast<int64_t>(a.start[b]) + t);
+  float co[8], si[8];
+  if (turns) {
+    const int64_t pos = position_of(a, tok);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) turn(pos, a.step[8 * j + i], a.mag, co[i], si[i]);
+  }
+  const unsigned lanes = L == 32 ? 0xffffffffu : ((1u << L) - 1u) << ((threadIdx.x & 31) / L * L);
+#pragma unroll 2
+  for (int h = g; h < rows; h += gpt) {
+    const int which = h < hq ? 0 : (h < hqk ? 1 : 2);
+    const int hh = which == 0 ? h : (which == 1 ? h - hq : h - hqk);
+    const RowSet& s = which == 0 ? a.q : (which == 1 ? a.k : a.v);
+    const T* x = static_cast<const T*>(s.p) + b * s.sb + t * s.st + hh * s.sh;
+    const bool plain = which == 2;  // values do not turn: 16 consecutive elements a lane
+    const int f0 = plain ? 16 * j : e0, f1 = plain ? 16 * j + 8 : e1;
+    float v[16];
+    unpack8<T>(*reinterpret_cast<const uint4*>(x + f0), v);
+    unpack8<T>(*reinterpret_cast<const uint4*>(x + f1), v + 8);
+    if (turns && !plain) {
+      if (a.interleaved) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float x0 = v[2 * i], x1 = v[2 * i + 1];
+          v[2 * i] = x0 * co[i] - x1 * si[i];
+          v[2 * i + 1] = x0 * si[i] + x1 * co[i];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float x0 = v[i], x1 = v[8 + i];
+          v[i] = x0 * co[i] - x1 * si[i];
+          v[8 + i] = x0 * si[i] + x1 * co[i];
+        }
+      }
+    }
+    if (!WRITE || which == 0) {
+      T* y = static_cast<T*>(which == 0 ? a.q_out : a.k_out) + (tok * s.heads + hh) * D;
+      *reinterpret_cast<uint4*>(y + f0) = pack8<T>(v);
+      *reinterpret_cast<uint4*>(y + f1) = pack8<T>(v + 8);
+      continue;
+    }
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(v[i]));
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(lanes, m, o));
+    if (krow < 0) continue;
+    const int64_t row = krow + static_cast<int64_t>(hh) * a.cache.page;
+    const float sc = __fdiv_rn(m, 127.0f);
+    const float rcp = __frcp_rn(sc);
+    int8_t* q = (which == 1 ? a.cache.k : a.cache.v) + row * D;
+    *reinterpret_cast<uint2*>(q + f0) = codes8(v, sc, rcp);
+    *reinterpret_cast<uint2*>(q + f1) = codes8(v + 8, sc, rcp);
+    if (j == 0) (which == 1 ? a.cache.ks : a.cache.vs)[row] = sc;
+  }
+}
+
+static bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+static bool rows_aligned(const RowSet& s) {
+  return s.heads == 0 || (aligned16(s.p) && s.sb % 8 == 0 && s.st % 8 == 0 && s.sh % 8 == 0);
+}
+
+template <typename T, int L>
+static int launch_rotary_vec(const RotArgs& a, bool write, cudaStream_t st) {
+  // Row groups of a token: eight (a lane's sines then serve many rows), more where the tokens alone do not
+  // fill the SMs, up to one for each row.
+  const int rows = a.q.heads + a.k.heads + a.v.heads;
+  const int64_t tokens = a.b * a.t;
+  int gpt = 8;
+  while (gpt < rows && tokens * gpt * L < 1024L * num_sms()) gpt *= 2;
+  const int64_t blocks = (tokens * gpt * L + 255) / 256;
+  if (blocks > INT32_MAX) return fail(BW_ERR_INVALID_ARGUMENT, "rotary: too many tokens");
+  if (write) rotary_vec_kernel<T, L, true><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a, gpt);
+  else rotary_vec_kernel<T, L, false><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a, gpt);
+  return check_launch("rotary_vec_kernel");
+}
+
 template <typename T>
 static int launch_rotary(const RotArgs& a, bool write, cudaStream_t st) {
   const int64_t rows = a.b * a.t * (a.q.heads + a.k.heads + a.v.heads);
   if (rows == 0) return BW_OK;
+  if (a.rot % 16 == 0 && rows_aligned(a.q) && rows_aligned(a.k) && rows_aligned(a.v) && aligned16(a.q_out) &&
+      aligned16(a.k_out) && aligned16(a.cache.k) && aligned16(a.cache.v)) {
+    switch (a.d) {
+      case 32: return launch_rotary_vec<T, 2>(a, write, st);
+      case 64: return launch_rotary_vec<T, 4>(a, write, st);
+      case 128: return launch_rotary_vec<T, 8>(a, write, st);
+      case 256: return launch_rotary_vec<T, 16>(a, write, st);
+      default: break;
+    }
+  }
   const int64_t blocks = (rows + 7) / 8;
   const int grid = static_cast<int>(blocks < 16L * num_sms() ? blocks : 16L * num_sms());
   if (write) rotary_rows_kernel<T, true><<<grid, 256, 0, st>>>(a);
@@ -197,6 +350,77 @@ __global__ void __launch_bounds__(256) kv_read_rows_kernel(const __grid_constant
   }
 }
 
+// 16 codes -> 16 values, 32 bytes.
+template <typename T>
+__device__ __forceinline__ void values16(const uint4& c, float s, uint4* out) {
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+  float f[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) f[i] = static_cast<float>(static_cast<int8_t>(w[i >> 2] >> (8 * (i & 3)))) * s;
+  out[0] = pack8<T>(f);
+  out[1] = pack8<T>(f + 8);
+}
+
+// Aligned rows of a multiple of 16 elements: 16 codes of k and of v a thread, UNROLL of them on their way.
+// blockIdx.y: layer and sequence.  Bound by the bytes: one page lookup and one scale serve a row's chunks.
+template <typename T>
+__global__ void __launch_bounds__(256) kv_read_vec_kernel(const __grid_constant__ ReadArgs a, int chunks) {
+  constexpr int UNROLL = 2;
+  const unsigned per_slot = a.c.heads * chunks;
+  const unsigned total = static_cast<unsigned>(a.n) * per_slot;
+  const unsigned layer = blockIdx.y / static_cast<unsigned>(a.b);
+  const int64_t b = blockIdx.y - layer * static_cast<unsigned>(a.b);
+  const int64_t start = a.start != nullptr ? a.start[b] : 0;
+  const int64_t len = a.lens != nullptr ? a.lens[b] : a.n;
+  const unsigned e0 = blockIdx.x * (256 * UNROLL) + threadIdx.x;
+  uint4 k[UNROLL], v[UNROLL];
+  float ks[UNROLL], vs[UNROLL];
+#pragma unroll
+  for (int u = 0; u < UNROLL; ++u) {
+    const unsigned e = e0 + u * 256;
+    k[u] = v[u] = make_uint4(0u, 0u, 0u, 0u);
+    ks[u] = vs[u] = 0.f;
+    if (e >= total) continue;
+    const unsigned i = e / per_slot, hc = e - i * per_slot;
+    const unsigned h = hc / static_cast<unsigned>(chunks), c = hc - h * chunks;
+    int64_t row = i < len ? kv_row(a.c, b, start + i) : -1;
+    if (row < 0) continue;
+    row += layer * a.layer_rows + static_cast<int64_t>(h) * a.c.page;
+    k[u] = __ldg(reinterpret_cast<const uint4*>(a.c.k + row * a.c.d) + c);
+    v[u] = __ldg(reinterpret_cast<const uint4*>(a.c.v + row * a.c.d) + c);
+    ks[u] = __ldg(a.c.ks + row);
+    vs[u] = __ldg(a.c.vs + row);
+  }
+#pragma unroll
+  for (int u = 0; u < UNROLL; ++u) {
+    const unsigned e = e0 + u * 256;
+    if (e >= total) continue;
+    const int64_t at = (static_cast<int64_t>(blockIdx.y) * total + e) * 2;
+    uint4 o[2];
+    values16<T>(k[u], ks[u], o);
+    __stcs(static_cast<uint4*>(a.k_out) + at, o[0]);
+    __stcs(static_cast<uint4*>(a.k_out) + at + 1, o[1]);
+    values16<T>(v[u], vs[u], o);
+    __stcs(static_cast<uint4*>(a.v_out) + at, o[0]);
+    __stcs(static_cast<uint4*>(a.v_out) + at + 1, o[1]);
+  }
+}
+
+template <typename T>
+static int launch_read(const ReadArgs& a, cudaStream_t st) {
+  const int64_t total = a.n * a.c.heads * (a.c.d / 16);
+  if (a.c.d % 16 == 0 && a.layers * a.b <= 65535 && total < INT32_MAX && aligned16(a.c.k) && aligned16(a.c.v) &&
+      aligned16(a.k_out) && aligned16(a.v_out)) {
+    const dim3 grid(static_cast<unsigned>((total + 511) / 512), static_cast<unsigned>(a.layers * a.b));
+    kv_read_vec_kernel<T><<<grid, 256, 0, st>>>(a, a.c.d / 16);
+    return check_launch("kv_read_vec_kernel");
+  }
+  const int64_t blocks = (a.layers * a.b * a.n * a.c.heads + 7) / 8;
+  const int grid = static_cast<int>(blocks < 16L * num_sms() ? blocks : 16L * num_sms());
+  kv_read_rows_kernel<T><<<grid, 256, 0, st>>>(a);
+  return check_launch("kv_read_rows_kernel");
+}
+
 // ---------------------------------------------------------------------------
 // move accepted nodes
 // ---------------------------------------------------------------------------
@@ -243,6 +467,71 @@ __global__ void __launch_bounds__(256) kv_move_kernel(const __grid_constant__ Kv
     if (j == 0) {
       c.ks[dst[i]] = sc[0][i];
       c.vs[dst[i]] = sc[1][i];
+    }
+  }
+}
+
+// Aligned rows of a multiple of 16 bytes: one CTA per (sequence, layer), so the slots are looked up once for
+// all heads; four heads' rows at a time are read into registers (16-byte chunks), then written.
+template <int PER>  // chunks of a head's k and v rows a thread holds
+__global__ void __launch_bounds__(128) kv_move_vec_kernel(const __grid_constant__ KvCache c, int64_t layer_rows, int t,
+                                                          const int* __restrict__ start, const int* __restrict__ path,
+                                                          int64_t path_ld, const int* __restrict__ taken) {
+  constexpr int HEADS = 4;
+  __shared__ int64_t src[kTreeMaxNodes], dst[kTreeMaxNodes];
+  const int64_t b = blockIdx.x, layer = blockIdx.y;
+  int n = taken[b];
+  n = n < t - 1 ? n : t - 1;
+  if (n <= 0) return;
+  if (threadIdx.x < n) {
+    const int node = path[b * path_ld + threadIdx.x];
+    int64_t s = -1, d = -1;
+    if (node >= 0 && node < t) {
+      s = kv_row(c, b, static_cast<int64_t>(start[b]) + node);
+      d = kv_row(c, b, static_cast<int64_t>(start[b]) + 1 + threadIdx.x);
+    }
+    const bool ok = s >= 0 && d >= 0 && s != d;
+    src[threadIdx.x] = ok ? layer * layer_rows + s : -1;
+    dst[threadIdx.x] = ok ? layer * layer_rows + d : -1;
+  }
+  __syncthreads();
+  const int chunks = c.d / 16;           // of a row
+  const int per_head = n * chunks;       // of k, and as many of v
+  for (int h0 = 0; h0 < c.heads; h0 += HEADS) {
+    uint4 buf[HEADS][PER];
+    float sc[HEADS];
+#pragma unroll
+    for (int hh = 0; hh < HEADS; ++hh) {
+      const int64_t hrow = static_cast<int64_t>(h0 + hh) * c.page;
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        const int e = threadIdx.x + 128 * k;
+        if (h0 + hh >= c.heads || e >= 2 * per_head) continue;
+        const int r = (e < per_head ? e : e - per_head) / chunks, ch = (e < per_head ? e : e - per_head) - r * chunks;
+        if (src[r] >= 0)
+          buf[hh][k] = *(reinterpret_cast<const uint4*>((e < per_head ? c.k : c.v) + (src[r] + hrow) * c.d) + ch);
+      }
+      if (h0 + hh < c.heads && threadIdx.x < 2 * n) {
+        const int r = threadIdx.x < n ? threadIdx.x : threadIdx.x - n;
+        if (src[r] >= 0) sc[hh] = (threadIdx.x < n ? c.ks : c.vs)[src[r] + hrow];
+      }
+    }
+    __syncthreads();  // these heads' rows are all read
+#pragma unroll
+    for (int hh = 0; hh < HEADS; ++hh) {
+      const int64_t hrow = static_cast<int64_t>(h0 + hh) * c.page;
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        const int e = threadIdx.x + 128 * k;
+        if (h0 + hh >= c.heads || e >= 2 * per_head) continue;
+        const int r = (e < per_head ? e : e - per_head) / chunks, ch = (e < per_head ? e : e - per_head) - r * chunks;
+        if (src[r] >= 0)
+          *(reinterpret_cast<uint4*>((e < per_head ? c.k : c.v) + (dst[r] + hrow) * c.d) + ch) = buf[hh][k];
+      }
+      if (h0 + hh < c.heads && threadIdx.x < 2 * n) {
+        const int r = threadIdx.x < n ? threadIdx.x : threadIdx.x - n;
+        if (src[r] >= 0) (threadIdx.x < n ? c.ks : c.vs)[dst[r] + hrow] = sc[hh];
+      }
     }
   }
 }
@@ -381,11 +670,7 @@ extern "C" int bw_kv_read_int8(const int8_t* cache_k, const int8_t* cache_v, con
   a.v_out = v_out;
   if (int s = require_sm100()) return s;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int64_t blocks = (layers * b * n * heads + 7) / 8;
-  const int grid = static_cast<int>(blocks < 16L * num_sms() ? blocks : 16L * num_sms());
-  if (dtype == BW_DTYPE_BF16) kv_read_rows_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a);
-  else kv_read_rows_kernel<__half><<<grid, 256, 0, st>>>(a);
-  return check_launch("kv_read_rows_kernel");
+  return dtype == BW_DTYPE_BF16 ? launch_read<__nv_bfloat16>(a, st) : launch_read<__half>(a, st);
 }
 
 extern "C" int bw_kv_move_int8(int8_t* cache_k, int8_t* cache_v, float* k_scale, float* v_scale, int64_t layers,
@@ -402,6 +687,18 @@ extern "C" int bw_kv_move_int8(int8_t* cache_k, int8_t* cache_v, float* k_scale,
   if (layers == 0 || b == 0 || t <= 1) return BW_OK;
   if (!start || !path || !taken) return fail(BW_ERR_INVALID_ARGUMENT, "kv_move_int8: null pointer");
   if (int s = require_sm100()) return s;
+  // chunks of 16 bytes that a thread of 128 holds for a head: at most (t - 1) rows of k and v; beyond four
+  // (trees of 33 nodes and more at d = 128) the registers run out, and the rows go through shared memory
+  const int64_t held = (2 * (t - 1) * (d / 16) + 127) / 128;
+  if (d % 16 == 0 && held <= 4 && aligned16(cache_k) && aligned16(cache_v)) {
+    const dim3 vgrid(static_cast<unsigned>(b), static_cast<unsigned>(layers));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (held <= 2)
+      kv_move_vec_kernel<2><<<vgrid, 128, 0, st>>>(c, pages * heads * page, static_cast<int>(t), start, path, path_ld, taken);
+    else
+      kv_move_vec_kernel<4><<<vgrid, 128, 0, st>>>(c, pages * heads * page, static_cast<int>(t), start, path, path_ld, taken);
+    return check_launch("kv_move_vec_kernel");
+  }
   const dim3 grid(static_cast<unsigned>(b), static_cast<unsigned>(heads), static_cast<unsigned>(layers));
   kv_move_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(c, pages * heads * page, static_cast<int>(t),
                                                                       start, path, path_ld, taken);

@@ -31,7 +31,9 @@ struct KvCache {
 // Row index (into [pages][heads][page]) of head 0 of a slot, -1 if the slot does not exist.
 __device__ __forceinline__ int64_t kv_row(const KvCache& c, int64_t b, int64_t slot) {
   if (slot < 0) return -1;
-  const int64_t pi = slot / c.page;
+  // (64-bit division is many times a 32-bit one)
+  const int64_t pi = slot <= UINT32_MAX ? static_cast<int64_t>(static_cast<uint32_t>(slot) / static_cast<uint32_t>(c.page))
+                                        : slot / c.page;
   if (pi >= c.table_cols) return -1;
   const int64_t pg = c.table[b * c.table_ld + pi];
   if (pg < 0 || pg >= c.pages) return -1;

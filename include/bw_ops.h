@@ -313,7 +313,7 @@ int bw_dequantize_kv_int8(const int8_t* q, int64_t ldq, const float* scale, int6
  *   dtype      F16 | BF16 (32-bit arithmetic, rounded once)
  *   positions  [b, t] int32, or int64 if positions64
  *   steps      [rot/2] turns per position in units of 2^-64: round(f_i / 2pi * 2^64) mod 2^64
- *   hk == 0: no keys.  An output may be its own input where that is contiguous.
+ *   hk == 0: no keys.  Outputs do not overlap inputs.
  */
 int bw_rotary(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int hq, const void* k, int64_t k_sb,
               int64_t k_st, int64_t k_sh, int hk, void* q_out, void* k_out, int dtype, int64_t b, int64_t t,
