@@ -161,22 +161,41 @@ __device__ __forceinline__ uint4 pack8(const float* f) {
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
-__device__ __forceinline__ uint2 codes8(const float* f, float sc, float rcp) {
-  uint32_t w[2];
+// Codes of 16 values of a row with scale sc, rcp = RN(1 / sc): clamp(rne(RN(x / sc)), +-127), NaN -> 0.
+// x * rcp lies within 2.5 fp32 ulps of RN(x / sc), so the two round to the same integer unless x * rcp is
+// within 4e-5 of a half; adding 1.5 * 2^23 rounds to the nearest even integer and leaves the code in the low
+// byte.  |x| <= 127 sc keeps it in range.  A row with a value near a half (one in 800 of 16), a NaN, or a
+// scale that is zero, subnormal or not finite, takes the IEEE divisions.  The test is made once for all 16:
+// sixteen branches, one a value, cost the write three quarters of its time.
+__device__ __forceinline__ void codes16(const float* x, float sc, float rcp, uint2& lo, uint2& hi) {
+  constexpr float kMagic = 12582912.0f;
+  float y[16];
+  bool slow = !(rcp <= 3.402823466e38f) || !(sc > 0.f);
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    w[h] = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      w[h] |= static_cast<uint32_t>(static_cast<uint8_t>(quant_fast<BW_DTYPE_F32>(f[4 * h + i], sc, rcp))) << (8 * i);
+  for (int i = 0; i < 16; ++i) {
+    const float q = __fmul_rn(x[i], rcp);
+    y[i] = __fadd_rn(q, kMagic);
+    slow |= !(fabsf(__fsub_rn(q, __fsub_rn(y[i], kMagic))) < 0.49996f);  // (NaN: true)
   }
-  return make_uint2(w[0], w[1]);
+  if (slow) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) y[i] = kMagic + static_cast<float>(quant_one<BW_DTYPE_F32>(x[i], sc));
+  }
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t a = __byte_perm(__float_as_uint(y[4 * i]), __float_as_uint(y[4 * i + 1]), 0x0040);
+    const uint32_t b = __byte_perm(__float_as_uint(y[4 * i + 2]), __float_as_uint(y[4 * i + 3]), 0x0040);
+    w[i] = __byte_perm(a, b, 0x5410);
+  }
+  lo = make_uint2(w[0], w[1]);
+  hi = make_uint2(w[2], w[3]);
 }
 
 // Aligned rows of D = 16 L elements, rot a multiple of 16.  L lanes hold a row, 16 elements each in two
-// 16-byte chunks, so every pair lies in one lane: half layout, rotated lane j: elements 8 j .. and
-// rot/2 + 8 j ..; interleaved, and where nothing turns: 16 consecutive elements.  The sines of a lane's
-// eight pairs are computed once a token and serve the rows that the lane takes in turn (every `gpt`-th
+// 16-byte chunks: of the part that turns, lane j elements 8 j .. and rot/2 + 8 j .., so every pair of either
+// layout lies in one lane; the rest, and rows that do not turn, in the same way.  The sines of a lane's eight
+// pairs are computed once a token and serve the rows that the lane takes in turn (every `gpt`-th
 // row of the token): bound by the bytes where tokens are many, by latency where they are few, for which
 // the host spreads a token over more lanes.
 template <typename T, int L, bool WRITE>
@@ -189,8 +208,8 @@ __global__ void __launch_bounds__(256) rotary_vec_kernel(const __grid_constant__
   if (tok >= a.b * a.t) return;  // (a whole group at once: the shuffles below stay inside one)
   const int64_t b = tok / a.t, t = tok - b * a.t;
   const bool turns = j < a.rot / 16;
-  const int e0 = !turns || a.interleaved ? 16 * j : 8 * j;
-  const int e1 = !turns || a.interleaved ? 16 * j + 8 : a.rot / 2 + 8 * j;
+  const int e0 = turns ? 8 * j : a.rot / 2 + 8 * j;  // (the rest starts at rot, at lane rot / 16)
+  const int e1 = turns ? a.rot / 2 + 8 * j : D / 2 + 8 * j;
   const int hq = a.q.heads, hqk = hq + a.k.heads, rows = hqk + a.v.heads;
   int64_t krow = -1;
   if (WRITE && (a.counts == nullptr || t < a.counts[b])) krow = kv_row(a.cache, b, static_cast<int64_t>(a.start[b]) + t);
@@ -198,7 +217,10 @@ __global__ void __launch_bounds__(256) rotary_vec_kernel(const __grid_constant__
   if (turns) {
     const int64_t pos = position_of(a, tok);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) turn(pos, a.step[8 * j + i], a.mag, co[i], si[i]);
+    for (int i = 0; i < 8; ++i) {
+      const int pair = !a.interleaved ? 8 * j + i : (i < 4 ? e0 / 2 + i : e1 / 2 + i - 4);
+      turn(pos, a.step[pair], a.mag, co[i], si[i]);
+    }
   }
   const unsigned lanes = L == 32 ? 0xffffffffu : ((1u << L) - 1u) << ((threadIdx.x & 31) / L * L);
 #pragma unroll 2
@@ -207,8 +229,8 @@ __global__ void __launch_bounds__(256) rotary_vec_kernel(const __grid_constant__
     const int hh = which == 0 ? h : (which == 1 ? h - hq : h - hqk);
     const RowSet& s = which == 0 ? a.q : (which == 1 ? a.k : a.v);
     const T* x = static_cast<const T*>(s.p) + b * s.sb + t * s.st + hh * s.sh;
-    const bool plain = which == 2;  // values do not turn: 16 consecutive elements a lane
-    const int f0 = plain ? 16 * j : e0, f1 = plain ? 16 * j + 8 : e1;
+    const bool plain = which == 2;  // values do not turn
+    const int f0 = plain ? 8 * j : e0, f1 = plain ? D / 2 + 8 * j : e1;
     float v[16];
     unpack8<T>(*reinterpret_cast<const uint4*>(x + f0), v);
     unpack8<T>(*reinterpret_cast<const uint4*>(x + f1), v + 8);
@@ -245,8 +267,10 @@ __global__ void __launch_bounds__(256) rotary_vec_kernel(const __grid_constant__
     const float sc = __fdiv_rn(m, 127.0f);
     const float rcp = __frcp_rn(sc);
     int8_t* q = (which == 1 ? a.cache.k : a.cache.v) + row * D;
-    *reinterpret_cast<uint2*>(q + f0) = codes8(v, sc, rcp);
-    *reinterpret_cast<uint2*>(q + f1) = codes8(v + 8, sc, rcp);
+    uint2 lo, hi;
+    codes16(v, sc, rcp, lo, hi);
+    *reinterpret_cast<uint2*>(q + f0) = lo;
+    *reinterpret_cast<uint2*>(q + f1) = hi;
     if (j == 0) (which == 1 ? a.cache.ks : a.cache.vs)[row] = sc;
   }
 }
@@ -350,22 +374,21 @@ __global__ void __launch_bounds__(256) kv_read_rows_kernel(const __grid_constant
   }
 }
 
-// 16 codes -> 16 values, 32 bytes.
+// 8 codes -> 8 values, 16 bytes.
 template <typename T>
-__device__ __forceinline__ void values16(const uint4& c, float s, uint4* out) {
-  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-  float f[16];
+__device__ __forceinline__ uint4 values8(const uint2& c, float s) {
+  float f[8];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) f[i] = static_cast<float>(static_cast<int8_t>(w[i >> 2] >> (8 * (i & 3)))) * s;
-  out[0] = pack8<T>(f);
-  out[1] = pack8<T>(f + 8);
+  for (int i = 0; i < 8; ++i) f[i] = static_cast<float>(static_cast<int8_t>((i < 4 ? c.x : c.y) >> (8 * (i & 3)))) * s;
+  return pack8<T>(f);
 }
 
-// Aligned rows of a multiple of 16 elements: 16 codes of k and of v a thread, UNROLL of them on their way.
-// blockIdx.y: layer and sequence.  Bound by the bytes: one page lookup and one scale serve a row's chunks.
+// Aligned rows of a multiple of 8 elements: 8 codes of k and of v -> 16 bytes each, so that a warp's stores
+// are 512 consecutive bytes (with 16 codes a thread two stores each filled half of every sector).  UNROLL
+// chunks are on their way at once.  blockIdx.y: layer and sequence.
 template <typename T>
 __global__ void __launch_bounds__(256) kv_read_vec_kernel(const __grid_constant__ ReadArgs a, int chunks) {
-  constexpr int UNROLL = 2;
+  constexpr int UNROLL = 4;
   const unsigned per_slot = a.c.heads * chunks;
   const unsigned total = static_cast<unsigned>(a.n) * per_slot;
   const unsigned layer = blockIdx.y / static_cast<unsigned>(a.b);
@@ -373,12 +396,12 @@ __global__ void __launch_bounds__(256) kv_read_vec_kernel(const __grid_constant_
   const int64_t start = a.start != nullptr ? a.start[b] : 0;
   const int64_t len = a.lens != nullptr ? a.lens[b] : a.n;
   const unsigned e0 = blockIdx.x * (256 * UNROLL) + threadIdx.x;
-  uint4 k[UNROLL], v[UNROLL];
+  uint2 k[UNROLL], v[UNROLL];
   float ks[UNROLL], vs[UNROLL];
 #pragma unroll
   for (int u = 0; u < UNROLL; ++u) {
     const unsigned e = e0 + u * 256;
-    k[u] = v[u] = make_uint4(0u, 0u, 0u, 0u);
+    k[u] = v[u] = make_uint2(0u, 0u);
     ks[u] = vs[u] = 0.f;
     if (e >= total) continue;
     const unsigned i = e / per_slot, hc = e - i * per_slot;
@@ -386,8 +409,8 @@ __global__ void __launch_bounds__(256) kv_read_vec_kernel(const __grid_constant_
     int64_t row = i < len ? kv_row(a.c, b, start + i) : -1;
     if (row < 0) continue;
     row += layer * a.layer_rows + static_cast<int64_t>(h) * a.c.page;
-    k[u] = __ldg(reinterpret_cast<const uint4*>(a.c.k + row * a.c.d) + c);
-    v[u] = __ldg(reinterpret_cast<const uint4*>(a.c.v + row * a.c.d) + c);
+    k[u] = __ldg(reinterpret_cast<const uint2*>(a.c.k + row * a.c.d) + c);
+    v[u] = __ldg(reinterpret_cast<const uint2*>(a.c.v + row * a.c.d) + c);
     ks[u] = __ldg(a.c.ks + row);
     vs[u] = __ldg(a.c.vs + row);
   }
@@ -395,24 +418,19 @@ __global__ void __launch_bounds__(256) kv_read_vec_kernel(const __grid_constant_
   for (int u = 0; u < UNROLL; ++u) {
     const unsigned e = e0 + u * 256;
     if (e >= total) continue;
-    const int64_t at = (static_cast<int64_t>(blockIdx.y) * total + e) * 2;
-    uint4 o[2];
-    values16<T>(k[u], ks[u], o);
-    __stcs(static_cast<uint4*>(a.k_out) + at, o[0]);
-    __stcs(static_cast<uint4*>(a.k_out) + at + 1, o[1]);
-    values16<T>(v[u], vs[u], o);
-    __stcs(static_cast<uint4*>(a.v_out) + at, o[0]);
-    __stcs(static_cast<uint4*>(a.v_out) + at + 1, o[1]);
+    const int64_t at = static_cast<int64_t>(blockIdx.y) * total + e;
+    __stcs(static_cast<uint4*>(a.k_out) + at, values8<T>(k[u], ks[u]));
+    __stcs(static_cast<uint4*>(a.v_out) + at, values8<T>(v[u], vs[u]));
   }
 }
 
 template <typename T>
 static int launch_read(const ReadArgs& a, cudaStream_t st) {
-  const int64_t total = a.n * a.c.heads * (a.c.d / 16);
-  if (a.c.d % 16 == 0 && a.layers * a.b <= 65535 && total < INT32_MAX && aligned16(a.c.k) && aligned16(a.c.v) &&
+  const int64_t total = a.n * a.c.heads * (a.c.d / 8);
+  if (a.c.d % 8 == 0 && a.layers * a.b <= 65535 && total < INT32_MAX && aligned16(a.c.k) && aligned16(a.c.v) &&
       aligned16(a.k_out) && aligned16(a.v_out)) {
-    const dim3 grid(static_cast<unsigned>((total + 511) / 512), static_cast<unsigned>(a.layers * a.b));
-    kv_read_vec_kernel<T><<<grid, 256, 0, st>>>(a, a.c.d / 16);
+    const dim3 grid(static_cast<unsigned>((total + 1023) / 1024), static_cast<unsigned>(a.layers * a.b));
+    kv_read_vec_kernel<T><<<grid, 256, 0, st>>>(a, a.c.d / 8);
     return check_launch("kv_read_vec_kernel");
   }
   const int64_t blocks = (a.layers * a.b * a.n * a.c.heads + 7) / 8;

@@ -16,7 +16,7 @@
 
 namespace bw {
 
-constexpr int kVerifyThreads = 512;
+constexpr int kVerifyThreads = 1024;
 constexpr int kVerifyCluster = 8;
 
 struct VerifyArgs {
@@ -77,6 +77,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_tree_kernel(const Verif
   const int rank = static_cast<int>(cluster_ctarank());
   const int64_t b = blockIdx.x / kVerifyCluster;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int threads = blockDim.x;
   if (tid < a.t) {
     const int p = a.parents[b * a.t + tid];
     const int64_t x = a.tok[b * a.t + tid];
@@ -95,6 +96,21 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_tree_kernel(const Verif
   const int64_t per = ((a.v + kVerifyCluster - 1) / kVerifyCluster + 3) / 4 * 4;
   const int64_t v0 = min(per * rank, a.v), v1 = min(v0 + per, a.v);
   __syncthreads();
+  // What is left of four consecutive tokens' weights after the first r rejections.
+  auto rest = [&](float4& w, const float4& qw, int64_t v, int r) {
+    if (DRAFT) {
+      w = make_float4(residual(w.x, qw.x, z, r), residual(w.y, qw.y, z, r), residual(w.z, qw.z, z, r),
+                      residual(w.w, qw.w, z, r));
+    } else {
+      for (int j = 0; j < r; ++j) {
+        const int64_t off = dropped[j] - v;
+        if (off == 0) w.x = 0.f;
+        if (VEC && off == 1) w.y = 0.f;
+        if (VEC && off == 2) w.z = 0.f;
+        if (VEC && off == 3) w.w = 0.f;
+      }
+    }
+  };
   int phase = 0;
 #pragma unroll 1
   for (;;) {
@@ -136,21 +152,27 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_tree_kernel(const Verif
     const float* p = a.p + (b * a.t + cur) * a.v;
     const float* q = DRAFT ? a.q + (b * a.t + cur) * a.v : nullptr;
     float sum = 0.f;
-    for (int64_t v = v0 + tid; v < v1; v += kVerifyThreads) {
-      float w = p[v];
-      if (DRAFT) {
-        w = residual(w, q[v], z, r);
-      } else {
-        for (int j = 0; j < r; ++j)
-          if (dropped[j] == v) w = 0.f;
+    if constexpr (VEC) {
+#pragma unroll 4
+      for (int64_t v = v0 + tid * 4; v < v1; v += threads * 4) {
+        float4 w = __ldg(reinterpret_cast<const float4*>(p + v));
+        const float4 qw = DRAFT ? __ldg(reinterpret_cast<const float4*>(q + v)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        rest(w, qw, v, r);
+        sum += (w.x + w.y) + (w.z + w.w);
       }
-      sum += w;
+    } else {
+#pragma unroll 4
+      for (int64_t v = v0 + tid; v < v1; v += threads) {
+        float4 w = make_float4(__ldg(p + v), 0.f, 0.f, 0.f);
+        rest(w, make_float4(DRAFT ? __ldg(q + v) : 0.f, 0.f, 0.f, 0.f), v, r);
+        sum += w.x;
+      }
     }
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) red[warp] = sum;
     __syncthreads();
     sum = 0.f;
-    for (int k = 0; k < kVerifyThreads / 32; ++k) sum += red[k];
+    for (int k = 0; k < threads / 32; ++k) sum += red[k];
     cluster_share(&sums[phase & 1], sum, rank);
     if (tid == 0) {
       float s = 0.f;
@@ -167,15 +189,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_tree_kernel(const Verif
 #pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {  // second pass: the residual was empty
     unsigned long long best = 0;  // no candidate
-    auto score = [&](float w, float qw, float ew, int64_t v) {
-      if (pass == 0) {
-        if (DRAFT) {
-          w = residual(w, qw, z, r);
-        } else {
-          for (int j = 0; j < r; ++j)
-            if (dropped[j] == v) w = 0.f;
-        }
-      }
+    auto score = [&](float w, float ew, int64_t v) {
       if (w > 0.f) {
         const float s = __fdiv_rn(w, ew);
         const unsigned long long key =
@@ -183,19 +197,27 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_tree_kernel(const Verif
         if (s >= 0.f && key > best) best = key;
       }
     };
+    const int rr = pass == 0 ? r : 0;
     if constexpr (VEC) {
-#pragma unroll 2
-      for (int64_t v = v0 + tid * 4; v < v1; v += kVerifyThreads * 4) {
-        const float4 pw = __ldg(reinterpret_cast<const float4*>(p + v)), ew = __ldg(reinterpret_cast<const float4*>(e + v));
-        const float4 qw = DRAFT ? __ldg(reinterpret_cast<const float4*>(q + v)) : make_float4(0.f, 0.f, 0.f, 0.f);
-        score(pw.x, qw.x, ew.x, v);
-        score(pw.y, qw.y, ew.y, v + 1);
-        score(pw.z, qw.z, ew.z, v + 2);
-        score(pw.w, qw.w, ew.w, v + 3);
+#pragma unroll 4
+      for (int64_t v = v0 + tid * 4; v < v1; v += threads * 4) {
+        float4 w = __ldg(reinterpret_cast<const float4*>(p + v));
+        const float4 ew = __ldg(reinterpret_cast<const float4*>(e + v));
+        const float4 qw = DRAFT && rr > 0 ? __ldg(reinterpret_cast<const float4*>(q + v)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        rest(w, qw, v, rr);
+        score(w.x, ew.x, v);
+        score(w.y, ew.y, v + 1);
+        score(w.z, ew.z, v + 2);
+        score(w.w, ew.w, v + 3);
       }
     } else {
 #pragma unroll 4
-      for (int64_t v = v0 + tid; v < v1; v += kVerifyThreads) score(__ldg(p + v), DRAFT ? __ldg(q + v) : 0.f, __ldg(e + v), v);
+      for (int64_t v = v0 + tid; v < v1; v += threads) {
+        float4 w = make_float4(__ldg(p + v), 0.f, 0.f, 0.f);
+        const float ew = __ldg(e + v);
+        rest(w, make_float4(DRAFT && rr > 0 ? __ldg(q + v) : 0.f, 0.f, 0.f, 0.f), v, rr);
+        score(w.x, ew, v);
+      }
     }
     for (int o = 16; o > 0; o >>= 1) {
       const unsigned long long k = __shfl_xor_sync(0xffffffffu, best, o);
@@ -204,7 +226,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_tree_kernel(const Verif
     if (lane == 0) redk[warp] = best;
     __syncthreads();
     best = 0;
-    for (int k = 0; k < kVerifyThreads / 32; ++k) best = redk[k] > best ? redk[k] : best;
+    for (int k = 0; k < threads / 32; ++k) best = redk[k] > best ? redk[k] : best;
     cluster_share(&keys[pass], best, rank);
     best = 0;
     for (int k = 0; k < kVerifyCluster; ++k) best = keys[pass][k] > best ? keys[pass][k] : best;
@@ -215,7 +237,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_tree_kernel(const Verif
         a.out[b * a.t + taken] = best == 0 ? 0 : static_cast<int64_t>(0xffffffffu - static_cast<uint32_t>(best));
         a.path[b * a.t + taken] = -1;
       }
-      for (int i = taken + 1 + tid; i < a.t; i += kVerifyThreads) {
+      for (int i = taken + 1 + tid; i < a.t; i += threads) {
         a.path[b * a.t + i] = -1;
         a.out[b * a.t + i] = -1;
       }
@@ -229,7 +251,8 @@ template <bool DRAFT, bool VEC>
 static int launch_verify(const VerifyArgs& a, int64_t b, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(b * kVerifyCluster));
-  cfg.blockDim = dim3(kVerifyThreads);
+  // one CTA an SM while there is an SM for each, two smaller ones where there are more
+  cfg.blockDim = dim3(b * kVerifyCluster <= num_sms() ? kVerifyThreads : kVerifyThreads / 2);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
