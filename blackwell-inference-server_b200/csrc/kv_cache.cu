@@ -194,34 +194,44 @@ __device__ __forceinline__ void codes16(const float* x, float sc, float rcp, uin
 
 // Aligned rows of D = 16 L elements, rot a multiple of 16.  L lanes hold a row, 16 elements each in two
 // 16-byte chunks: of the part that turns, lane j elements 8 j .. and rot/2 + 8 j .., so every pair of either
-// layout lies in one lane; the rest, and rows that do not turn, in the same way.  The sines of a lane's eight
-// pairs are computed once a token and serve the rows that the lane takes in turn (every `gpt`-th
-// row of the token): bound by the bytes where tokens are many, by latency where they are few, for which
-// the host spreads a token over more lanes.
-template <typename T, int L, bool WRITE>
-__global__ void __launch_bounds__(256) rotary_vec_kernel(const __grid_constant__ RotArgs a, int gpt) {
+// layout lies in one lane; the rest, and rows that do not turn, in the same way.  A CTA's 256 threads hold
+// the row groups of one to sixteen tokens and compute each of their sines once, one a thread, into shared
+// memory; a group takes every `gpt`-th row of its token.  Bound by the bytes where tokens are many (which
+// wants many warps: with each lane's sines in its registers four warps a scheduler did not cover the
+// latency), by latency where they are few, for which the host spreads a token over more groups.
+template <typename T, int L, bool WRITE, bool INTER>
+__global__ void __launch_bounds__(256, WRITE ? 3 : 4) rotary_vec_kernel(const __grid_constant__ RotArgs a, int gpt) {
   constexpr int D = 16 * L;
+  __shared__ __align__(16) float2 turns_of[256];  // (cos, sin) of the CTA's tokens' pairs
   const int j = threadIdx.x % L;
   const int64_t group = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / L;
   const int64_t tok = group / gpt;
   const int g = static_cast<int>(group - tok * gpt);
+  const int half = a.rot / 2;
+  // gpt * L is a power of two: whole tokens in a CTA, or a part of one
+  const int in_cta = max(1, 256 / (gpt * L));
+  const int64_t tok0 = static_cast<int64_t>(blockIdx.x) * 256 / (gpt * L);
+  for (int e = threadIdx.x; e < in_cta * half; e += 256) {
+    const int k = e / half;
+    if (tok0 + k < a.b * a.t) {
+      float co, si;
+      turn(position_of(a, tok0 + k), a.step[e - k * half], a.mag, co, si);
+      turns_of[e] = make_float2(co, si);
+    }
+  }
+  __syncthreads();
   if (tok >= a.b * a.t) return;  // (a whole group at once: the shuffles below stay inside one)
   const int64_t b = tok / a.t, t = tok - b * a.t;
   const bool turns = j < a.rot / 16;
   const int e0 = turns ? 8 * j : a.rot / 2 + 8 * j;  // (the rest starts at rot, at lane rot / 16)
   const int e1 = turns ? a.rot / 2 + 8 * j : D / 2 + 8 * j;
   const int hq = a.q.heads, hqk = hq + a.k.heads, rows = hqk + a.v.heads;
+  // pairs of the lane: eight of the half layout, four of each chunk of the interleaved one
+  const float4* cs0 = reinterpret_cast<const float4*>(turns_of + static_cast<int>(tok - tok0) * half) +
+                      (INTER ? e0 / 4 : 4 * j);
+  const float4* cs1 = INTER ? cs0 - e0 / 4 + e1 / 4 : cs0 + 2;
   int64_t krow = -1;
   if (WRITE && (a.counts == nullptr || t < a.counts[b])) krow = kv_row(a.cache, b, static_cast<int64_t>(a.start[b]) + t);
-  float co[8], si[8];
-  if (turns) {
-    const int64_t pos = position_of(a, tok);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int pair = !a.interleaved ? 8 * j + i : (i < 4 ? e0 / 2 + i : e1 / 2 + i - 4);
-      turn(pos, a.step[pair], a.mag, co[i], si[i]);
-    }
-  }
   const unsigned lanes = L == 32 ? 0xffffffffu : ((1u << L) - 1u) << ((threadIdx.x & 31) / L * L);
 #pragma unroll 2
   for (int h = g; h < rows; h += gpt) {
@@ -235,20 +245,19 @@ __global__ void __launch_bounds__(256) rotary_vec_kernel(const __grid_constant__
     unpack8<T>(*reinterpret_cast<const uint4*>(x + f0), v);
     unpack8<T>(*reinterpret_cast<const uint4*>(x + f1), v + 8);
     if (turns && !plain) {
-      if (a.interleaved) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float x0 = v[2 * i], x1 = v[2 * i + 1];
-          v[2 * i] = x0 * co[i] - x1 * si[i];
-          v[2 * i + 1] = x0 * si[i] + x1 * co[i];
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float x0 = v[i], x1 = v[8 + i];
-          v[i] = x0 * co[i] - x1 * si[i];
-          v[8 + i] = x0 * si[i] + x1 * co[i];
-        }
+      for (int p = 0; p < 4; ++p) {  // two pairs
+        const float4 cs = p < 2 ? cs0[p] : cs1[p - 2];
+        // half layout: elements 2 p, 2 p + 1 with their partners 8 on; interleaved: four neighbours
+        float& x0 = v[INTER ? 4 * p : 2 * p];
+        float& x1 = v[INTER ? 4 * p + 1 : 2 * p + 8];
+        float& y0 = v[INTER ? 4 * p + 2 : 2 * p + 1];
+        float& y1 = v[INTER ? 4 * p + 3 : 2 * p + 9];
+        const float u0 = x0, u1 = x1, w0 = y0, w1 = y1;
+        x0 = u0 * cs.x - u1 * cs.y;
+        x1 = u0 * cs.y + u1 * cs.x;
+        y0 = w0 * cs.z - w1 * cs.w;
+        y1 = w0 * cs.w + w1 * cs.z;
       }
     }
     if (!WRITE || which == 0) {
@@ -290,8 +299,14 @@ static int launch_rotary_vec(const RotArgs& a, bool write, cudaStream_t st) {
   while (gpt < rows && tokens * gpt * L < 1024L * num_sms()) gpt *= 2;
   const int64_t blocks = (tokens * gpt * L + 255) / 256;
   if (blocks > INT32_MAX) return fail(BW_ERR_INVALID_ARGUMENT, "rotary: too many tokens");
-  if (write) rotary_vec_kernel<T, L, true><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a, gpt);
-  else rotary_vec_kernel<T, L, false><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a, gpt);
+  const unsigned grid = static_cast<unsigned>(blocks);
+  if (write) {
+    if (a.interleaved) rotary_vec_kernel<T, L, true, true><<<grid, 256, 0, st>>>(a, gpt);
+    else rotary_vec_kernel<T, L, true, false><<<grid, 256, 0, st>>>(a, gpt);
+  } else {
+    if (a.interleaved) rotary_vec_kernel<T, L, false, true><<<grid, 256, 0, st>>>(a, gpt);
+    else rotary_vec_kernel<T, L, false, false><<<grid, 256, 0, st>>>(a, gpt);
+  }
   return check_launch("rotary_vec_kernel");
 }
 
@@ -377,61 +392,87 @@ __global__ void __launch_bounds__(256) kv_read_rows_kernel(const __grid_constant
 // 8 codes -> 8 values, 16 bytes.
 template <typename T>
 __device__ __forceinline__ uint4 values8(const uint2& c, float s) {
+  // code + 128 in the low byte of 2^23, less 2^23 + 128: an addition where an int-to-float conversion runs at
+  // a quarter of the rate (and bound the whole read)
+  const uint32_t w[2] = {c.x ^ 0x80808080u, c.y ^ 0x80808080u};
   float f[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = static_cast<float>(static_cast<int8_t>((i < 4 ? c.x : c.y) >> (8 * (i & 3)))) * s;
+  for (int i = 0; i < 8; ++i)
+    f[i] = (__uint_as_float(__byte_perm(w[i >> 2], 0x4B000000u, 0x7440 | (i & 3))) - 8388736.0f) * s;
   return pack8<T>(f);
 }
 
-// Aligned rows of a multiple of 8 elements: 8 codes of k and of v -> 16 bytes each, so that a warp's stores
-// are 512 consecutive bytes (with 16 codes a thread two stores each filled half of every sector).  UNROLL
-// chunks are on their way at once.  blockIdx.y: layer and sequence.
-template <typename T>
-__global__ void __launch_bounds__(256) kv_read_vec_kernel(const __grid_constant__ ReadArgs a, int chunks) {
-  constexpr int UNROLL = 4;
-  const unsigned per_slot = a.c.heads * chunks;
-  const unsigned total = static_cast<unsigned>(a.n) * per_slot;
+// 32 bytes in one store (a whole sector), first to leave L2.
+__device__ __forceinline__ void st_global_32(void* p, const uint4& a, const uint4& b) {
+  asm volatile("st.global.cs.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w),
+               "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+               : "memory");
+}
+
+// Aligned rows of D = 16 C elements, C a power of two: 16 codes of k and of v -> one 32-byte store each.  A
+// warp has one head and reads consecutive slots, which lie side by side in a page; the CTA's eight warps have
+// eight heads, which lie side by side in the output.  UNROLL slots a lane are on their way at once.
+// blockIdx.x: slots; y: layer and sequence.
+template <typename T, int C>
+__global__ void __launch_bounds__(256) kv_read_vec_kernel(const __grid_constant__ ReadArgs a) {
+  constexpr int UNROLL = 2, ACROSS = 32 / C, SLOTS = ACROSS * UNROLL;
+  const int lane = threadIdx.x & 31;
+  const int ch = lane % C;
   const unsigned layer = blockIdx.y / static_cast<unsigned>(a.b);
   const int64_t b = blockIdx.y - layer * static_cast<unsigned>(a.b);
   const int64_t start = a.start != nullptr ? a.start[b] : 0;
-  const int64_t len = a.lens != nullptr ? a.lens[b] : a.n;
-  const unsigned e0 = blockIdx.x * (256 * UNROLL) + threadIdx.x;
-  uint2 k[UNROLL], v[UNROLL];
-  float ks[UNROLL], vs[UNROLL];
+  const int64_t len = min(a.lens != nullptr ? static_cast<int64_t>(a.lens[b]) : a.n, a.n);
+  const int64_t i0 = static_cast<int64_t>(blockIdx.x) * SLOTS + lane / C;
+  int64_t row[UNROLL];
 #pragma unroll
   for (int u = 0; u < UNROLL; ++u) {
-    const unsigned e = e0 + u * 256;
-    k[u] = v[u] = make_uint2(0u, 0u);
-    ks[u] = vs[u] = 0.f;
-    if (e >= total) continue;
-    const unsigned i = e / per_slot, hc = e - i * per_slot;
-    const unsigned h = hc / static_cast<unsigned>(chunks), c = hc - h * chunks;
-    int64_t row = i < len ? kv_row(a.c, b, start + i) : -1;
-    if (row < 0) continue;
-    row += layer * a.layer_rows + static_cast<int64_t>(h) * a.c.page;
-    k[u] = __ldg(reinterpret_cast<const uint2*>(a.c.k + row * a.c.d) + c);
-    v[u] = __ldg(reinterpret_cast<const uint2*>(a.c.v + row * a.c.d) + c);
-    ks[u] = __ldg(a.c.ks + row);
-    vs[u] = __ldg(a.c.vs + row);
+    row[u] = i0 + u * ACROSS < len ? kv_row(a.c, b, start + i0 + u * ACROSS) : -1;
+    if (row[u] >= 0) row[u] += layer * a.layer_rows;
   }
+  const int8_t* codes = blockIdx.z ? a.c.v : a.c.k;
+  const float* scales = blockIdx.z ? a.c.vs : a.c.ks;
+  uint4* out = static_cast<uint4*>(blockIdx.z ? a.v_out : a.k_out);
+  for (int h = threadIdx.x >> 5; h < a.c.heads; h += 8) {
+    uint4 x[UNROLL];
+    float sc[UNROLL];
 #pragma unroll
-  for (int u = 0; u < UNROLL; ++u) {
-    const unsigned e = e0 + u * 256;
-    if (e >= total) continue;
-    const int64_t at = static_cast<int64_t>(blockIdx.y) * total + e;
-    __stcs(static_cast<uint4*>(a.k_out) + at, values8<T>(k[u], ks[u]));
-    __stcs(static_cast<uint4*>(a.v_out) + at, values8<T>(v[u], vs[u]));
+    for (int u = 0; u < UNROLL; ++u) {
+      x[u] = make_uint4(0u, 0u, 0u, 0u);
+      sc[u] = 0.f;
+      if (row[u] < 0) continue;
+      const int64_t r = row[u] + static_cast<int64_t>(h) * a.c.page;
+      x[u] = __ldg(reinterpret_cast<const uint4*>(codes + r * (16 * C)) + ch);
+      sc[u] = __ldg(scales + r);
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int64_t i = i0 + u * ACROSS;
+      if (i >= a.n) continue;
+      st_global_32(out + (((blockIdx.y * a.n + i) * a.c.heads + h) * C + ch) * 2,
+                   values8<T>(make_uint2(x[u].x, x[u].y), sc[u]), values8<T>(make_uint2(x[u].z, x[u].w), sc[u]));
+    }
   }
+}
+
+template <typename T, int C>
+static int launch_read_vec(const ReadArgs& a, cudaStream_t st) {
+  constexpr int SLOTS = 32 / C * 2;
+  const dim3 grid(static_cast<unsigned>((a.n + SLOTS - 1) / SLOTS), static_cast<unsigned>(a.layers * a.b), 2);
+  kv_read_vec_kernel<T, C><<<grid, 256, 0, st>>>(a);
+  return check_launch("kv_read_vec_kernel");
 }
 
 template <typename T>
 static int launch_read(const ReadArgs& a, cudaStream_t st) {
-  const int64_t total = a.n * a.c.heads * (a.c.d / 8);
-  if (a.c.d % 8 == 0 && a.layers * a.b <= 65535 && total < INT32_MAX && aligned16(a.c.k) && aligned16(a.c.v) &&
-      aligned16(a.k_out) && aligned16(a.v_out)) {
-    const dim3 grid(static_cast<unsigned>((total + 1023) / 1024), static_cast<unsigned>(a.layers * a.b));
-    kv_read_vec_kernel<T><<<grid, 256, 0, st>>>(a, a.c.d / 8);
-    return check_launch("kv_read_vec_kernel");
+  if (a.layers * a.b <= 65535 && aligned16(a.c.k) && aligned16(a.c.v) &&
+      (reinterpret_cast<uintptr_t>(a.k_out) | reinterpret_cast<uintptr_t>(a.v_out)) % 32 == 0) {
+    switch (a.c.d) {
+      case 32: return launch_read_vec<T, 2>(a, st);
+      case 64: return launch_read_vec<T, 4>(a, st);
+      case 128: return launch_read_vec<T, 8>(a, st);
+      case 256: return launch_read_vec<T, 16>(a, st);
+      default: break;
+    }
   }
   const int64_t blocks = (a.layers * a.b * a.n * a.c.heads + 7) / 8;
   const int grid = static_cast<int>(blocks < 16L * num_sms() ? blocks : 16L * num_sms());
@@ -591,6 +632,7 @@ static KvCache make_cache(void* k, void* v, float* ks, float* vs, int64_t pages,
   // out of int range: 0, which check_kv_cache refuses
   c.heads = heads > 0 && heads <= 65535 ? static_cast<int>(heads) : 0;
   c.page = page > 0 && page <= (1 << 24) ? static_cast<int>(page) : 0;
+  c.shift = page_shift(c.page);
   c.d = d > 0 && d <= kKvMaxDim ? static_cast<int>(d) : 0;
   c.table = table;
   c.table_ld = table_ld;

@@ -23,6 +23,7 @@ struct KvCache {
   float* vs;
   int64_t pages;
   int heads, page, d;
+  int shift;  // page = 1 << shift, or -1
   const int* table;
   int64_t table_ld;
   int table_cols;
@@ -31,9 +32,7 @@ struct KvCache {
 // Row index (into [pages][heads][page]) of head 0 of a slot, -1 if the slot does not exist.
 __device__ __forceinline__ int64_t kv_row(const KvCache& c, int64_t b, int64_t slot) {
   if (slot < 0) return -1;
-  // (64-bit division is many times a 32-bit one)
-  const int64_t pi = slot <= UINT32_MAX ? static_cast<int64_t>(static_cast<uint32_t>(slot) / static_cast<uint32_t>(c.page))
-                                        : slot / c.page;
+  const int64_t pi = c.shift >= 0 ? slot >> c.shift : slot / c.page;
   if (pi >= c.table_cols) return -1;
   const int64_t pg = c.table[b * c.table_ld + pi];
   if (pg < 0 || pg >= c.pages) return -1;
@@ -48,6 +47,12 @@ template <>
 __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+inline int page_shift(int page) {
+  for (int s = 0; s < 31; ++s)
+    if (page == 1 << s) return s;
+  return -1;
+}
 
 // Argument check shared by the entry points that take a cache.
 int check_kv_cache(const KvCache& c, int64_t b, const char* op);

@@ -1194,6 +1194,7 @@ extern "C" int bw_tree_attention_int8(const void* q, int64_t q_sb, int64_t q_st,
   a.c.pages = pages;
   a.c.heads = heads > 0 && heads <= 65535 ? static_cast<int>(heads) : 0;
   a.c.page = page > 0 && page <= (1 << 24) ? static_cast<int>(page) : 0;
+  a.c.shift = page_shift(a.c.page);
   a.c.d = d > 0 && d <= kKvMaxDim ? static_cast<int>(d) : 0;
   a.c.table = table;
   a.c.table_ld = table_ld;
