@@ -162,22 +162,29 @@ __device__ __forceinline__ uint4 pack8(const float* f) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 // Codes of 16 values of a row with scale sc, rcp = RN(1 / sc): clamp(rne(RN(x / sc)), +-127), NaN -> 0.
-// x * rcp lies within 2.5 fp32 ulps of RN(x / sc), so the two round to the same integer unless x * rcp is
-// within 4e-5 of a half; adding 1.5 * 2^23 rounds to the nearest even integer and leaves the code in the low
-// byte.  |x| <= 127 sc keeps it in range.  A row with a value near a half (one in 800 of 16), a NaN, or a
-// scale that is zero, subnormal or not finite, takes the IEEE divisions.  The test is made once for all 16:
-// sixteen branches, one a value, cost the write three quarters of its time.
+// The IEEE quotient without a division (Markstein 1990): q = RN(x rcp), and twice q = RN(q + (x - q sc) rcp)
+// with the remainder exact in an FMA; the first step leaves q within an ulp of x / sc, the second rounds it
+// correctly.  Adding 1.5 * 2^23 rounds to the nearest even integer and leaves the code in the low byte;
+// |x| <= 127 sc keeps it in range.  Rows whose remainders could be subnormal, or with a NaN or an infinity,
+// take the divisions.  (Multiplying once and dividing only near a half, as the weight quantisers do, does not
+// pay here: bf16 values over a bf16 maximum meet exact halves in almost every warp.)
 __device__ __forceinline__ void codes16(const float* x, float sc, float rcp, uint2& lo, uint2& hi) {
   constexpr float kMagic = 12582912.0f;
   float y[16];
-  bool slow = !(rcp <= 3.402823466e38f) || !(sc > 0.f);
+  const float2 s2 = make_float2(-sc, -sc), r2 = make_float2(rcp, rcp);
+  float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const float q = __fmul_rn(x[i], rcp);
-    y[i] = __fadd_rn(q, kMagic);
-    slow |= !(fabsf(__fsub_rn(q, __fsub_rn(y[i], kMagic))) < 0.49996f);  // (NaN: true)
+  for (int i = 0; i < 16; i += 2) {
+    const float2 v = make_float2(x[i], x[i + 1]);
+    sum = __fadd2_rn(sum, make_float2(fabsf(v.x), fabsf(v.y)));
+    float2 q = __fmul2_rn(v, r2);
+    q = __ffma2_rn(__ffma2_rn(q, s2, v), r2, q);
+    q = __ffma2_rn(__ffma2_rn(q, s2, v), r2, q);
+    const float2 z = __fadd2_rn(q, make_float2(kMagic, kMagic));
+    y[i] = z.x;
+    y[i + 1] = z.y;
   }
-  if (slow) {
+  if (!(sum.x + sum.y <= 3.402823466e38f) || !(sc > 0x1p-100f && sc <= 3.402823466e38f)) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) y[i] = kMagic + static_cast<float>(quant_one<BW_DTYPE_F32>(x[i], sc));
   }
@@ -233,54 +240,71 @@ __global__ void __launch_bounds__(256, WRITE ? 3 : 4) rotary_vec_kernel(const __
   int64_t krow = -1;
   if (WRITE && (a.counts == nullptr || t < a.counts[b])) krow = kv_row(a.cache, b, static_cast<int64_t>(a.start[b]) + t);
   const unsigned lanes = L == 32 ? 0xffffffffu : ((1u << L) - 1u) << ((threadIdx.x & 31) / L * L);
-#pragma unroll 2
-  for (int h = g; h < rows; h += gpt) {
-    const int which = h < hq ? 0 : (h < hqk ? 1 : 2);
-    const int hh = which == 0 ? h : (which == 1 ? h - hq : h - hqk);
-    const RowSet& s = which == 0 ? a.q : (which == 1 ? a.k : a.v);
-    const T* x = static_cast<const T*>(s.p) + b * s.sb + t * s.st + hh * s.sh;
-    const bool plain = which == 2;  // values do not turn
-    const int f0 = plain ? 8 * j : e0, f1 = plain ? D / 2 + 8 * j : e1;
-    float v[16];
-    unpack8<T>(*reinterpret_cast<const uint4*>(x + f0), v);
-    unpack8<T>(*reinterpret_cast<const uint4*>(x + f1), v + 8);
-    if (turns && !plain) {
+  // rows on their way at once (8191 tokens of 72 rows: 59 us with two, 62 with one; the write, with its
+  // codes' registers, 27 us with one, 29 with two)
+  constexpr int UNROLL = WRITE ? 1 : 2;
+  for (int h0 = g; h0 < rows; h0 += gpt * UNROLL) {
+    uint4 raw[UNROLL][2];
 #pragma unroll
-      for (int p = 0; p < 4; ++p) {  // two pairs
-        const float4 cs = p < 2 ? cs0[p] : cs1[p - 2];
-        // half layout: elements 2 p, 2 p + 1 with their partners 8 on; interleaved: four neighbours
-        float& x0 = v[INTER ? 4 * p : 2 * p];
-        float& x1 = v[INTER ? 4 * p + 1 : 2 * p + 8];
-        float& y0 = v[INTER ? 4 * p + 2 : 2 * p + 1];
-        float& y1 = v[INTER ? 4 * p + 3 : 2 * p + 9];
-        const float u0 = x0, u1 = x1, w0 = y0, w1 = y1;
-        x0 = u0 * cs.x - u1 * cs.y;
-        x1 = u0 * cs.y + u1 * cs.x;
-        y0 = w0 * cs.z - w1 * cs.w;
-        y1 = w0 * cs.w + w1 * cs.z;
+    for (int u = 0; u < UNROLL; ++u) {
+      const int h = h0 + u * gpt;
+      if (h >= rows) continue;
+      const int which = h < hq ? 0 : (h < hqk ? 1 : 2);
+      const int hh = which == 0 ? h : (which == 1 ? h - hq : h - hqk);
+      const RowSet& s = which == 0 ? a.q : (which == 1 ? a.k : a.v);
+      const T* x = static_cast<const T*>(s.p) + b * s.sb + t * s.st + hh * s.sh;
+      raw[u][0] = *reinterpret_cast<const uint4*>(x + (which == 2 ? 8 * j : e0));
+      raw[u][1] = *reinterpret_cast<const uint4*>(x + (which == 2 ? D / 2 + 8 * j : e1));
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int h = h0 + u * gpt;
+      if (h >= rows) continue;
+      const int which = h < hq ? 0 : (h < hqk ? 1 : 2);
+      const int hh = which == 0 ? h : (which == 1 ? h - hq : h - hqk);
+      const bool plain = which == 2;  // values do not turn
+      const int f0 = plain ? 8 * j : e0, f1 = plain ? D / 2 + 8 * j : e1;
+      float v[16];
+      unpack8<T>(raw[u][0], v);
+      unpack8<T>(raw[u][1], v + 8);
+      if (turns && !plain) {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {  // two pairs
+          const float4 cs = p < 2 ? cs0[p] : cs1[p - 2];
+          // half layout: elements 2 p, 2 p + 1 with their partners 8 on; interleaved: four neighbours
+          float& x0 = v[INTER ? 4 * p : 2 * p];
+          float& x1 = v[INTER ? 4 * p + 1 : 2 * p + 8];
+          float& y0 = v[INTER ? 4 * p + 2 : 2 * p + 1];
+          float& y1 = v[INTER ? 4 * p + 3 : 2 * p + 9];
+          const float u0 = x0, u1 = x1, w0 = y0, w1 = y1;
+          x0 = u0 * cs.x - u1 * cs.y;
+          x1 = u0 * cs.y + u1 * cs.x;
+          y0 = w0 * cs.z - w1 * cs.w;
+          y1 = w0 * cs.w + w1 * cs.z;
+        }
       }
-    }
-    if (!WRITE || which == 0) {
-      T* y = static_cast<T*>(which == 0 ? a.q_out : a.k_out) + (tok * s.heads + hh) * D;
-      *reinterpret_cast<uint4*>(y + f0) = pack8<T>(v);
-      *reinterpret_cast<uint4*>(y + f1) = pack8<T>(v + 8);
-      continue;
-    }
-    float m = 0.f;
+      if (!WRITE || which == 0) {
+        T* y = static_cast<T*>(which == 0 ? a.q_out : a.k_out) + (tok * (which == 0 ? hq : a.k.heads) + hh) * D;
+        *reinterpret_cast<uint4*>(y + f0) = pack8<T>(v);
+        *reinterpret_cast<uint4*>(y + f1) = pack8<T>(v + 8);
+        continue;
+      }
+      float m = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(v[i]));
+      for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(v[i]));
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(lanes, m, o));
-    if (krow < 0) continue;
-    const int64_t row = krow + static_cast<int64_t>(hh) * a.cache.page;
-    const float sc = __fdiv_rn(m, 127.0f);
-    const float rcp = __frcp_rn(sc);
-    int8_t* q = (which == 1 ? a.cache.k : a.cache.v) + row * D;
-    uint2 lo, hi;
-    codes16(v, sc, rcp, lo, hi);
-    *reinterpret_cast<uint2*>(q + f0) = lo;
-    *reinterpret_cast<uint2*>(q + f1) = hi;
-    if (j == 0) (which == 1 ? a.cache.ks : a.cache.vs)[row] = sc;
+      for (int o = L / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(lanes, m, o));
+      if (krow < 0) continue;
+      const int64_t row = krow + static_cast<int64_t>(hh) * a.cache.page;
+      const float sc = __fdiv_rn(m, 127.0f);
+      const float rcp = __frcp_rn(sc);
+      int8_t* q = (which == 1 ? a.cache.k : a.cache.v) + row * D;
+      uint2 lo, hi;
+      codes16(v, sc, rcp, lo, hi);
+      *reinterpret_cast<uint2*>(q + f0) = lo;
+      *reinterpret_cast<uint2*>(q + f1) = hi;
+      if (j == 0) (which == 1 ? a.cache.ks : a.cache.vs)[row] = sc;
+    }
   }
 }
 
