@@ -104,3 +104,16 @@ def test_c_refusals():
     assert att(hq=3) == bad and att(dt=2) == bad and att(t=65) == bad
     assert lib.bw_verify_tree(None, None, None, None, None, None, 1, 1, 0, None, None, None, None) == bad
     assert lib.bw_verify_tree(None, None, None, None, None, None, 0, 1, 8, None, None, None, None) == 0
+
+
+def test_lookup_tree():
+    from blackwell_inference.spec_decode import lookup_tree
+
+    # 1 2 3 4 | 1 2 3 5 | 1 2 3: continuations of (1 2 3), the later first
+    tok, par = lookup_tree([1, 2, 3, 4, 1, 2, 3, 5, 1, 2, 3], 8, branches=2)
+    assert tok[0] == 3 and par[0] == -1
+    assert (tok[1], par[1]) == (5, 0) and 4 in tok and par[tok.index(4)] == 0
+    assert all(0 <= p < i for i, p in enumerate(par) if i)
+    assert lookup_tree([7], 8) == ([7], [-1]) and lookup_tree([1, 2, 1], 1) == ([1], [-1])
+    tok, par = lookup_tree([9] * 40, 16)
+    assert len(tok) <= 16 and set(tok) == {9}
