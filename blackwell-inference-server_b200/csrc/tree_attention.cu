@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   int* pre = rows + 64;                                              // [nb + 1] first unit of a sequence
   static_assert((4 * 6 + 24 + 2 * kScaleStages) * 8 + 8 + sizeof(WaitControl) <= 640, "barriers");
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = warp_uniform(threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   const int grp = a.hq / a.c.heads;  // query heads of a key head
   const int heads = a.c.heads;
@@ -573,73 +573,79 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     if (warp == 0 && ok) mbar_wait_at(done, 0, ctl, kSiteAtDone);
   } else if (warp == 1) {
     // ---------------- K . Q ----------------
-    if (lane == 0) {
-      constexpr uint32_t idesc = make_idesc_f16(128, R, BF16, false);
-      int it = 0, seg = 0;
-      bool ok = true;
-      AttnWalk wk(pre, ta.nb, x0, x1);
-      AttnSeg sg;
-      for (; ok && wk.next(pre, heads, sg); ++seg) {
-        const int qb = seg % C::NQ;
-        const uint32_t q_base = smem_u32(sQ + qb * C::QB);
-        if (!mbar_wait_or_abort(&qfull[qb], (seg / C::NQ) & 1, ctl)) break;
-        for (int i = 0; i < sg.n_kt; ++i, ++it) {
-          const int t = it & 1;
-          const uint32_t ph = (it >> 1) & 1;
-          if (!mbar_wait_or_abort(&afull[t], ph, ctl) || !mbar_wait_or_abort(&sempty[t], ph ^ 1, ctl)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          uint32_t a_col = tmem + t * C::A_COLS;
-#pragma unroll 1
-          for (int p = 0; p < D / 64; ++p) {  // panels of 64 elements of the head dimension
-            uint64_t bd = make_sdesc(q_base + p * R * 128, 16, 1024, kLayoutSW128);
-#pragma unroll 1
-            for (int kk = 0; kk < 4; ++kk, a_col += 8, bd += 32 >> 4)
-              umma_f16_ts(tmem + C::S_COL + t * R, a_col, bd, idesc, p + kk);
-          }
+    constexpr uint32_t idesc = make_idesc_f16(128, R, BF16, false);
+    const uint32_t tm = warp_uniform(tmem);
+    int it = 0, seg = 0;
+    bool ok = true;
+    AttnWalk wk(pre, ta.nb, x0, x1);
+    AttnSeg sg;
+    for (; ok && wk.next(pre, heads, sg); ++seg) {
+      const int qb = seg % C::NQ;
+      const uint32_t q_base = smem_u32(sQ + qb * C::QB);
+      ok = __all_sync(0xffffffffu, mbar_wait_or_abort(&qfull[qb], (seg / C::NQ) & 1, ctl));
+      if (!ok) break;
+      const int n_kt = warp_uniform(sg.n_kt);
+      for (int i = 0; i < n_kt; ++i, ++it) {
+        const int t = it & 1;
+        const uint32_t ph = (it >> 1) & 1;
+        ok = mbar_wait_or_abort(&afull[t], ph, ctl) && mbar_wait_or_abort(&sempty[t], ph ^ 1, ctl);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)  // panels of 64 elements of the head dimension, 16 a step
+            umma_f16_ts(tm + C::S_COL + t * R, tm + t * C::A_COLS + kk * 8,
+                        make_sdesc(q_base + (kk >> 2) * R * 128 + (kk & 3) * 32, 16, 1024, kLayoutSW128), idesc, kk > 0);
           umma_commit(&sfull[t]);
+          if (i == n_kt - 1) umma_commit(&qempty[qb]);
         }
-        if (ok) umma_commit(&qempty[qb]);
+        __syncwarp();
       }
+    }
+    if (elect_one()) {
       umma_commit(&final_bar[0]);  // every MMA issued here has completed before TMEM is released
       mbar_wait_at(&final_bar[0], 0, ctl, kSiteAtFinal, false);
     }
+    __syncwarp();
   } else if (warp == 2) {
     // ---------------- V . P ----------------
-    if (lane == 0) {
-      constexpr uint32_t idesc = make_idesc_f16(128, 2 * R, true, true, true);
-      int it = 0;
-      bool ok = true;
-      AttnWalk wk(pre, ta.nb, x0, x1);
-      AttnSeg sg;
-      while (ok && wk.next(pre, heads, sg)) {
-        for (int i = 0; i < sg.n_kt; ++i, ++it) {
-          const int t = it & 1;
-          const uint32_t ph = (it >> 1) & 1;
-          if (!mbar_wait_or_abort(&vbfull[t], ph, ctl) || !mbar_wait_or_abort(&pfull[t], ph, ctl)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t o_tmem = tmem + C::O_COL + (C::ALT ? t * 2 * R : 0);
-          constexpr int first = C::ALT ? 1 : 0;  // the last tile of a segment that starts an accumulator
+    constexpr uint32_t idesc = make_idesc_f16(128, 2 * R, true, true, true);
+    constexpr int first = C::ALT ? 1 : 0;  // the last tile of a segment that starts an accumulator
+    const uint32_t tm = warp_uniform(tmem);
+    int it = 0;
+    bool ok = true;
+    AttnWalk wk(pre, ta.nb, x0, x1);
+    AttnSeg sg;
+    while (ok && wk.next(pre, heads, sg)) {
+      const int n_kt = warp_uniform(sg.n_kt);
+      for (int i = 0; i < n_kt; ++i, ++it) {
+        const int t = it & 1;
+        const uint32_t ph = (it >> 1) & 1;
+        ok = mbar_wait_or_abort(&vbfull[t], ph, ctl) && mbar_wait_or_abort(&pfull[t], ph, ctl);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t o_tmem = tm + C::O_COL + (C::ALT ? t * 2 * R : 0);
           const uint32_t v_base = smem_u32(sVB + t * C::VB);
           const uint32_t p_base = smem_u32(sP + t * C::PB);
           // the second 64 rows of V^T: the next panel, or zeros
           const uint32_t lbo = D == 128 ? kTile * 128 : smem_u32(smem + C::OFF_Z) - v_base;
-          uint64_t ad = make_sdesc(v_base, lbo, 1024, kLayoutSW128);
-          uint64_t bd = make_sdesc(p_base, kTile * 128, 1024, kLayoutSW128);
-#pragma unroll 1
-          for (int kk = 0; kk < kTile / 16; ++kk, ad += 2048 >> 4, bd += 2048 >> 4)
-            umma_f16(o_tmem, ad, bd, idesc, i > first || kk > 0);
+#pragma unroll
+          for (int kk = 0; kk < kTile / 16; ++kk)
+            umma_f16(o_tmem, make_sdesc(v_base + kk * 2048, lbo, 1024, kLayoutSW128),
+                     make_sdesc(p_base + kk * 2048, kTile * 128, 1024, kLayoutSW128), idesc, i > first || kk > 0);
           umma_commit(&pempty[t]);
         }
+        __syncwarp();
       }
+    }
+    if (elect_one()) {
       umma_commit(&final_bar[1]);
       mbar_wait_at(&final_bar[1], 0, ctl, kSiteAtFinal, false);
     }
+    __syncwarp();
   } else if (warp < 8) {
     // ---------------- K codes -> TMEM (thread = slot) ----------------
     const int q = warp & 3;
