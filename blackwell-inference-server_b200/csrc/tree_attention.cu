@@ -171,7 +171,7 @@ struct ACfg {
   static constexpr int OFF_Q = OFF_P + 2 * PB;
   static constexpr int OFF_RING = OFF_Q + NQ * QB;
   static constexpr int SCALES = kScaleStages * (2 * kTile * 4 + 16);
-  static constexpr int CTRL = 640 + SCALES + 2 * 4 * 32 * 4 * 2 + 2 * 3 * 32 * 4 + 4 * 64 * 4 + (2 * 256 + 32) * 4 + 2 * 64 * 8 + 64 * 4 +
+  static constexpr int CTRL = 640 + SCALES + 2 * 4 * 32 * 4 * 2 + 2 * 4 * 32 * 4 + 4 * 64 * 4 + (2 * 256 + 32) * 4 + 2 * 64 * 8 + 64 * 4 +
                               (kAttnMaxBatch + 1) * 4 + 64;
   static constexpr int ROOM = 227 * 1024 - 1024 - OFF_RING - CTRL;
   static constexpr int ST = ROOM / (2 * KV) < 6 ? ROOM / (2 * KV) : 6;  // stages of a K and a V tile
@@ -278,13 +278,34 @@ __device__ __forceinline__ void cp_async_arrive_noinc(uint64_t* bar) {
 }
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
+// Four codes -> two bf16x2 words, exactly, with half of the work on the FMA pipe (the integer pipe, at half
+// its rate, bounds the dequantisers).  u = code + 128 in the low byte of 0x4300 reads as v = 128 + u for
+// u < 128 and 2 u above, where the byte's top bit falls into the exponent.  d = v - 256 is the code there and
+// twice the code here, so code = d - relu(d / 2); every value fits bf16's 8 bits.
+__device__ __forceinline__ void codes4_bf16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  const uint32_t u = w ^ 0x80808080u;
+  uint32_t v[2];
+  asm("prmt.b32 %0, %1, %2, 0x5140;" : "=r"(v[0]) : "r"(u), "r"(0x43434343u));
+  asm("prmt.b32 %0, %1, %2, 0x5342;" : "=r"(v[1]) : "r"(u), "r"(0x43434343u));
+  uint32_t q[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint32_t r, d;
+    asm("fma.rn.relu.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(v[i]), "r"(0x3F003F00u), "r"(0xC300C300u));  // 0.5 v - 128
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(v[i]), "r"(0x3F803F80u), "r"(0xC380C380u));       // v - 256
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(q[i]) : "r"(r), "r"(0xBF80BF80u), "r"(d));                 // d - r
+  }
+  lo = q[0];
+  hi = q[1];
+}
+
 // 16 codes -> 16 fp16 or bf16 values.
 template <bool BF16>
 __device__ __forceinline__ void codes16(const uint4& v, uint32_t* o) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if constexpr (BF16) i8x4_to_bf16x4(w[i], o[2 * i], o[2 * i + 1]);
+    if constexpr (BF16) codes4_bf16(w[i], o[2 * i], o[2 * i + 1]);
     else i8x4_to_f16x4(w[i], o[2 * i], o[2 * i + 1]);
   }
 }
@@ -350,8 +371,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   float* sScale = reinterpret_cast<float*>(smem + C::OFF_CTRL + 640);  // [stages][2][128]: ks, vs
   uint32_t* sPages = reinterpret_cast<uint32_t*>(sScale + kScaleStages * 2 * kTile);  // [stages]: pages that exist
   float* wred = reinterpret_cast<float*>(smem + C::OFF_CTRL + 640 + C::SCALES);  // [2 groups][2][4 warps][32]
-  float* refs = wred + 2 * 2 * 4 * 32;                               // [2 groups][3][32]: m, its factor, sums
-  float* fin = refs + 2 * 3 * 32;                                    // [4][64]: m, sum, factors of the two streams
+  float* refs = wred + 2 * 2 * 4 * 32;                               // [2 groups][4][32]: m, its factor, sums, -m
+  float* fin = refs + 2 * 4 * 32;                                    // [4][64]: m, sum, factors of the two streams
   float* ftab = fin + 4 * 64;                                        // [2 groups][2][128], 32 zeros
   unsigned long long* rmask = reinterpret_cast<unsigned long long*>(ftab + 2 * 256 + 32);  // [2][64]
   int* rows = reinterpret_cast<int*>(rmask + 2 * 64);                // [64] node | query head of the group << 16
@@ -703,7 +724,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         const int tok8 = D == 128 ? (lane & 4 ? (lane >> 3) ^ 5 : lane >> 3) : lane >> 2;
         const int c4 = lane & 3;
         const int w0 = (((2 * c4) ^ tok8) << 4), w1 = (((2 * c4 + 1) ^ tok8) << 4);
-#pragma unroll 1
+#pragma unroll 2
         for (int k = 0; k < kTile / 32; k += D == 128 ? 1 : 2) {
           uint4 r0, r1;
           uint8_t *d0, *d1;
@@ -752,8 +773,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     const uint32_t lanes = tmem + (static_cast<uint32_t>(q * 32) << 16);
     float* gmax = wred + g * 2 * 4 * 32;
     float* gsum = gmax + 4 * 32;
-    float* mref = refs + g * 3 * 32;
+    float* mref = refs + g * 4 * 32;
     float* fac = mref + 32;
+    float* mneg = mref + 96;  // -m, as the scores' multiply-add takes it
     float* tab = ftab + g * 256;
     const float* zeros = ftab + 2 * 256;
     int it0 = 0, seg = 0;  // it0: the segment's first tile
@@ -767,7 +789,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       const int64_t keys = ctx + nodes;
       const int qb = seg % C::NQ;
       const bool got_q = mbar_wait_or_abort(&qfull[qb], (seg / C::NQ) & 1, ctl);
-      if (tid < RC) mref[tid] = kLowest;
+      if (tid < RC) {
+        mref[tid] = kLowest;
+        mneg[tid] = -kLowest;
+      }
       // A group that gives up still meets the other at the segment's end (barrier 3), where both leave.
       if (named_bar_any(bar, 128, !got_q)) ok = false;
       const unsigned long long* masks = rmask + qb * 64 + cb;
@@ -803,17 +828,17 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         int pass = 0;
 #pragma unroll 1
         for (;; ++pass) {
-          const float* m = pass == 1 ? zeros : mref;
-#pragma unroll
-          for (int c = 0; c < RC; c += 8)
-            tmem_ld8(lanes + C::S_COL + t * R + cb + c, reinterpret_cast<uint32_t*>(x) + c);
+          const float* m = pass == 1 ? zeros : mneg;
+          const uint32_t s_tmem = lanes + C::S_COL + t * R + cb;
+          if constexpr (RC == 32) tmem_ld32(s_tmem, reinterpret_cast<uint32_t(&)[32]>(x));
+          else tmem_ld16(s_tmem, reinterpret_cast<uint32_t(&)[16]>(x));
           tmem_ld_wait();
           const float2 k2 = make_float2(ks, ks);
 #pragma unroll
           for (int c = 0; c < RC; c += 4) {
             const float4 r = *reinterpret_cast<const float4*>(m + c);
-            const float2 a01 = __ffma2_rn(make_float2(x[c], x[c + 1]), k2, make_float2(-r.x, -r.y));
-            const float2 a23 = __ffma2_rn(make_float2(x[c + 2], x[c + 3]), k2, make_float2(-r.z, -r.w));
+            const float2 a01 = __ffma2_rn(make_float2(x[c], x[c + 1]), k2, make_float2(r.x, r.y));
+            const float2 a23 = __ffma2_rn(make_float2(x[c + 2], x[c + 3]), k2, make_float2(r.z, r.w));
             x[c] = a01.x;
             x[c + 1] = a01.y;
             x[c + 2] = a23.x;
@@ -826,10 +851,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           }
           if (pass == 2) break;
           if (pass == 0) {
-            float top = x[0];
+            float top[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-            for (int c = 1; c < RC; ++c) top = fmaxf(top, x[c]);
-            if (!named_bar_any(bar, 128, top > 8.f || !fine)) break;
+            for (int c = 4; c < RC; ++c) top[c & 3] = fmaxf(top[c & 3], x[c]);
+            const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            if (!named_bar_any(bar, 128, most > 8.f || !fine)) break;
             continue;
           }
           const float top = warp_columns<RC, true>(x, lane);
@@ -843,6 +869,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             const float old = mref[tid];
             const float best = fmaxf(fmaxf(fmaxf(gmax[tid], gmax[32 + tid]), fmaxf(gmax[64 + tid], gmax[96 + tid])), old);
             mref[tid] = best;
+            mneg[tid] = -best;
             fac[tid] = exp2_approx(old - best);
           }
           // the accumulator is still: its last V . P is complete, the next waits for this tile's weights
@@ -892,8 +919,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             const float2 v = __fmul2_rn(p, make_float2(vs, vs));
             const __nv_bfloat162 h = __float22bfloat162_rn(v);
             hi[e] = *reinterpret_cast<const uint32_t*>(&h);
-            const float2 left = __fadd2_rn(v, make_float2(-__uint_as_float(hi[e] << 16),
-                                                          -__uint_as_float(hi[e] & 0xFFFF0000u)));
+            const float2 left = __ffma2_rn(make_float2(__uint_as_float(hi[e] << 16), __uint_as_float(hi[e] & 0xFFFF0000u)),
+                                           make_float2(-1.f, -1.f), v);  // v - hi, exact
             const __nv_bfloat162 r = __float22bfloat162_rn(left);
             lo[e] = *reinterpret_cast<const uint32_t*>(&r);
           }
@@ -937,10 +964,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       if (tid < RH) {
         const int c = rb + tid;
         if constexpr (C::ALT) {
-          const float m0 = refs[c], m1 = refs[96 + c], top = fmaxf(m0, m1);
+          const float m0 = refs[c], m1 = refs[128 + c], top = fmaxf(m0, m1);
           const float f0 = exp2_approx(m0 - top), f1 = exp2_approx(m1 - top);
           fin[c] = top;
-          fin[64 + c] = f0 * refs[64 + c] + f1 * refs[160 + c];
+          fin[64 + c] = f0 * refs[64 + c] + f1 * refs[192 + c];
           fin[128 + c] = f0;
           fin[192 + c] = f1;
         } else {
