@@ -208,6 +208,19 @@ __device__ __forceinline__ bool mbar_wait_or_abort(uint64_t* bar, uint32_t parit
   return true;
 }
 
+// For a phase that completes soon, whatever other roles do: bounded by a number of tries (each of which waits a
+// while by itself).
+__device__ __forceinline__ void mbar_wait_tries(uint64_t* bar, uint32_t parity, WaitControl* w, int site) {
+#pragma unroll 1
+  for (uint32_t i = 0; !mbar_try_wait(bar, parity); ++i) {
+    if (i == (1u << 20)) {
+      atomicCAS(w->status, 0, site);
+      w->abort = 1;
+      return;
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------
 // thread-block clusters: distributed shared memory (every CTA loads its own TMA tiles)
 // ---------------------------------------------------------------------------

@@ -148,7 +148,7 @@ constexpr int kScaleStages = 4;   // tiles whose scales are on their way or in u
 constexpr float kLowest = -3.0e38f;  // a row's reference before any score: finite, so differences are
 constexpr int kAttnMaxBatch = 512;  // sequences of one launch (their unit ranges lie in shared memory)
 constexpr size_t kAttnCounterBytes = 4096;
-enum AttnSite : int { kSiteAtTma = 401, kSiteAtDrain = 402, kSiteAtDone = 403, kSiteAtFinal = 404 };
+enum AttnSite : int { kSiteAtTma = 401, kSiteAtDrain = 402, kSiteAtDone = 403, kSiteAtFinal = 404, kSiteAtVote = 405 };
 
 template <int D, int R>
 struct ACfg {
@@ -366,8 +366,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   uint64_t* scempty = scfull + kScaleStages;
   uint64_t* final_bar = scempty + kScaleStages;  // 2
   uint64_t* done = final_bar + 2;                // the softmax warps have no more to do
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
-  WaitControl* ctl = reinterpret_cast<WaitControl*>(done + 2);
+  uint64_t* voted = done + 1;                    // 2: a group's four warps have voted on a tile
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(voted + 2);
+  WaitControl* ctl = reinterpret_cast<WaitControl*>(voted + 3);
+  volatile int* votes = reinterpret_cast<volatile int*>(voted + 6);  // [2 groups][2 parities]
   float* sScale = reinterpret_cast<float*>(smem + C::OFF_CTRL + 640);  // [stages][2][128]: ks, vs
   uint32_t* sPages = reinterpret_cast<uint32_t*>(sScale + kScaleStages * 2 * kTile);  // [stages]: pages that exist
   float* wred = reinterpret_cast<float*>(smem + C::OFF_CTRL + 640 + C::SCALES);  // [2 groups][2][4 warps][32]
@@ -377,7 +379,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   unsigned long long* rmask = reinterpret_cast<unsigned long long*>(ftab + 2 * 256 + 32);  // [2][64]
   int* rows = reinterpret_cast<int*>(rmask + 2 * 64);                // [64] node | query head of the group << 16
   int* pre = rows + 64;                                              // [nb + 1] first unit of a sequence
-  static_assert((4 * 6 + 24 + 2 * kScaleStages) * 8 + 8 + sizeof(WaitControl) <= 640, "barriers");
+  static_assert((4 * 6 + 25 + 2 * kScaleStages) * 8 + 8 + sizeof(WaitControl) + 16 <= 640 && sizeof(WaitControl) == 24,
+                "barriers");
 
   const int warp = warp_uniform(threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
@@ -403,6 +406,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       mbar_init(&final_bar[i], 1);
     }
     mbar_init(done, 8);
+    mbar_init(&voted[0], 4);
+    mbar_init(&voted[1], 4);
+    for (int i = 0; i < 4; ++i) votes[i] = 0;
     for (int i = 0; i < kScaleStages; ++i) {
       mbar_init(&scfull[i], 33);  // each lane's copies, and the page word
       mbar_init(&scempty[i], C::GW);
@@ -779,6 +785,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     float* tab = ftab + g * 256;
     const float* zeros = ftab + 2 * 256;
     int it0 = 0, seg = 0;  // it0: the segment's first tile
+    uint32_t poll = 0;     // tiles that the group has voted on
     bool ok = true;
     AttnWalk wk(pre, ta.nb, x0, x1);
     AttnSeg sg;
@@ -807,31 +814,39 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         const int64_t j0 = static_cast<int64_t>(sg.kt0 + i) * kTile;
         const int left = static_cast<int>(min(keys - j0, static_cast<int64_t>(kTile)));  // slots of the tile
         const int sc = it % kScaleStages;
-        bool fine = mbar_wait_or_abort(&scfull[sc], (it / kScaleStages) & 1, ctl);
-        const float ks = sScale[sc * 2 * kTile + row] * a.scale_log2;
-        const float vs = sScale[sc * 2 * kTile + kTile + row];
-        const bool there = row < left && ((sPages[sc] >> (row >> 2)) & 1);
-        // a node's slot is seen by the rows whose mask names it, a context slot by all
-        const int node = row + static_cast<int>(max(j0 - ctx, static_cast<int64_t>(-kTile)));
-        const bool masked = !there || node >= 0;
-        fine = mbar_wait_or_abort(&sfull[t], ph, ctl) && fine;
+        bool fine = mbar_wait_or_abort(&sfull[t], ph, ctl);
         tc_fence_after();
         // x = score - reference, in powers of two; -inf where the row does not see the slot.  A vote
-        // over the group: does any score exceed its row's reference by more than 8?  Then once more
-        // from 0 for the rows' maxima, and again from the new references.
+        // over the group: does any score exceed its row's reference by more than 8?  The weights are
+        // worked out meanwhile; if one does, once more from 0 for the rows' maxima, and again from the
+        // new references.
         float x[RC];
+        float ks = 0.f, vs = 0.f;
         uint32_t see = 0;  // rows that see a slot that not all see
-        if (masked && there) {
-#pragma unroll 1
-          for (int c = 0; c < RC; ++c) see |= static_cast<uint32_t>((masks[c] >> node) & 1) << c;
-        }
-        int pass = 0;
+        bool masked = false;
+        int pass = i == i0 ? 1 : 0;  // (a segment's first tile has no reference yet)
+        bool got = false;
 #pragma unroll 1
         for (;; ++pass) {
           const float* m = pass == 1 ? zeros : mneg;
           const uint32_t s_tmem = lanes + C::S_COL + t * R + cb;
           if constexpr (RC == 32) tmem_ld32(s_tmem, reinterpret_cast<uint32_t(&)[32]>(x));
           else tmem_ld16(s_tmem, reinterpret_cast<uint32_t(&)[16]>(x));
+          if (!got) {  // (while the scores are on their way)
+            got = true;
+            fine = mbar_wait_or_abort(&scfull[sc], (it / kScaleStages) & 1, ctl) && fine;
+            fine = mbar_wait_or_abort(&pempty[t], ph ^ 1, ctl) && fine;
+            ks = sScale[sc * 2 * kTile + row] * a.scale_log2;
+            vs = sScale[sc * 2 * kTile + kTile + row];
+            const bool there = row < left && ((sPages[sc] >> (row >> 2)) & 1);
+            // a node's slot is seen by the rows whose mask names it, a context slot by all
+            const int node = row + static_cast<int>(max(j0 - ctx, static_cast<int64_t>(-kTile)));
+            masked = !there || node >= 0;
+            if (masked && there) {
+#pragma unroll 1
+              for (int c = 0; c < RC; ++c) see |= static_cast<uint32_t>((masks[c] >> node) & 1) << c;
+            }
+          }
           tmem_ld_wait();
           const float2 k2 = make_float2(ks, ks);
 #pragma unroll
@@ -849,13 +864,26 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             for (int c = 0; c < RC; ++c)
               if (!((see >> c) & 1)) x[c] = -INFINITY;
           }
-          if (pass == 2) break;
-          if (pass == 0) {
-            float top[4] = {x[0], x[1], x[2], x[3]};
+          if (pass != 1) {
+            if (pass == 0) {
+              float top[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-            for (int c = 4; c < RC; ++c) top[c & 3] = fmaxf(top[c & 3], x[c]);
-            const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-            if (!named_bar_any(bar, 128, most > 8.f || !fine)) break;
+              for (int c = 4; c < RC; ++c) top[c & 3] = fmaxf(top[c & 3], x[c]);
+              const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+              const bool again = __any_sync(0xffffffffu, most > 8.f || !fine);
+              if (lane == 0) {
+                if (again) votes[g * 2 + (poll & 1)] = 1;
+                mbar_arrive(&voted[g]);
+              }
+            }
+#pragma unroll
+            for (int c = 0; c < RC; ++c) x[c] = exp2_approx(x[c]);
+            if (pass == 2) break;
+            // (All four warps vote, also after a wait that ran out, so this one ends.)
+            mbar_wait_tries(&voted[g], poll & 1, ctl, kSiteAtVote);
+            const bool again = votes[g * 2 + (poll & 1)] != 0;
+            ++poll;
+            if (!again) break;
             continue;
           }
           const float top = warp_columns<RC, true>(x, lane);
@@ -865,6 +893,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             ok = false;
             break;
           }
+          if (tid == 0) votes[g * 2 + ((poll - 1) & 1)] = 0;  // all have read it
           if (tid < RC) {
             const float old = mref[tid];
             const float best = fmaxf(fmaxf(fmaxf(gmax[tid], gmax[32 + tid]), fmaxf(gmax[64 + tid], gmax[96 + tid])), old);
@@ -897,14 +926,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           }
         }
         if (!ok) break;
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&sempty[t]);
-          mbar_arrive(&scempty[sc]);
-        }
         // weights
-        if (!mbar_wait_or_abort(&pempty[t], ph ^ 1, ctl)) ctl->abort = 1;
         uint8_t* prow = sP + t * C::PB + row * 128;
 #pragma unroll
         for (int c0 = 0; c0 < RC; c0 += 8) {
@@ -912,7 +934,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int c = c0 + 2 * e;
-            const float2 p = make_float2(exp2_approx(x[c]), exp2_approx(x[c + 1]));
+            const float2 p = make_float2(x[c], x[c + 1]);
             const float2 l2 = __fadd2_rn(make_float2(l[c], l[c + 1]), p);
             l[c] = l2.x;
             l[c + 1] = l2.y;
@@ -941,47 +963,56 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           }
         }
         fence_proxy_async_smem();
+        tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&pfull[t]);
+        if (lane == 0) {
+          mbar_arrive(&pfull[t]);
+          mbar_arrive(&sempty[t]);
+          mbar_arrive(&scempty[sc]);
+        }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&qempty[qb]);  // the masks are read no more
       // ---- the segment's end: sums of the weights, output or piece ----
       const int last = it0 + i0 + (sg.n_kt - 1 - i0) / STEP * STEP;  // the group's last tile
       const bool any = i0 < sg.n_kt;
-      const bool fine = ok && (!any || mbar_wait_or_abort(&pempty[last & 1], (last >> 1) & 1, ctl));
       {
         const float sum = warp_columns<RC, false>(l, lane);
         if (lane % (32 / RC) == 0) gsum[w * 32 + lane / (32 / RC)] = sum;
       }
-      named_bar_sync(bar, 128);
-      if (tid < RC) mref[64 + tid] = ((gsum[tid] + gsum[32 + tid]) + gsum[64 + tid]) + gsum[96 + tid];
+      const bool fine = ok && (!any || mbar_wait_or_abort(&pempty[last & 1], (last >> 1) & 1, ctl));
       if (named_bar_any(3, 256, !fine || ctl->abort)) break;
       tc_fence_after();
-      if (lane == 0) mbar_arrive(&qempty[qb]);  // the masks are read no more
       const bool mine = row < D;                 // this thread's head dimension
       // From here on a group has the rows [rb, rb + RH): their references and sums, of both streams' where
       // there are two.
       const int rb = g * RH;
+      const bool split = sg.n_kt != sg.tiles;  // several CTAs share the (sequence, head)
       if (tid < RH) {
         const int c = rb + tid;
+        // (C::ALT ? both streams' sums over the four warps : the group's)
+        const float* sums = wred + 4 * 32 + (C::ALT ? c : g * 2 * 4 * 32 + tid);
+        float sum = ((sums[0] + sums[32]) + sums[64]) + sums[96];
+        float top = mref[tid], f0 = 1.f;
         if constexpr (C::ALT) {
-          const float m0 = refs[c], m1 = refs[128 + c], top = fmaxf(m0, m1);
-          const float f0 = exp2_approx(m0 - top), f1 = exp2_approx(m1 - top);
-          fin[c] = top;
-          fin[64 + c] = f0 * refs[64 + c] + f1 * refs[192 + c];
-          fin[128 + c] = f0;
+          const float m0 = refs[c], m1 = refs[4 * 32 + c];
+          sums += 2 * 4 * 32;
+          const float sum1 = ((sums[0] + sums[32]) + sums[64]) + sums[96];
+          top = fmaxf(m0, m1);
+          f0 = exp2_approx(m0 - top);
+          const float f1 = exp2_approx(m1 - top);
+          sum = f0 * sum + f1 * sum1;
           fin[192 + c] = f1;
-        } else {
-          fin[c] = mref[tid];
-          fin[64 + c] = mref[64 + tid];
-          fin[128 + c] = 1.f;
         }
+        fin[c] = top;
+        fin[64 + c] = split ? sum : inverse(sum);
+        fin[128 + c] = f0;
       }
       named_bar_sync(bar, 128);
       T* out = static_cast<T*>(a.o) + (b * a.t * a.hq + sg.h * grp) * static_cast<int64_t>(D) + row;
       constexpr int PIECE = R * D + 2 * R;
-      const int c_first = range.owner(sg.u0);
-      const int c_last = range.owner(sg.u0 + sg.tiles - 1);
-      const bool split = c_last > c_first;
+      const int c_first = split ? range.owner(sg.u0) : 0;
+      const int c_last = split ? range.owner(sg.u0 + sg.tiles - 1) : 0;
       float* piece = ta.pieces + (static_cast<int64_t>(blockIdx.x) * 2 + sg.slot) * PIECE;
       // piece p of the (sequence, head): CTA c_first + p's first segment, unless it started before
       auto piece_of = [&](int p) {
@@ -1017,12 +1048,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
               m = top;
             }
             fin[rb + tid] = m;
-            fin[64 + rb + tid] = sum;
+            fin[64 + rb + tid] = inverse(sum);
           }
-          named_bar_sync(bar, 128);
-        }
-        if (stage == 1) {
-          if (tid < RH) fin[64 + rb + tid] = inverse(fin[64 + rb + tid]);
           named_bar_sync(bar, 128);
         }
 #pragma unroll 1
@@ -1031,17 +1058,21 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 #pragma unroll
           for (int e = 0; e < 8; ++e) o[e] = 0.f;
           if (!join) {
-#pragma unroll 1
-            for (int k = 0; k < (C::ALT ? 2 : 1); ++k) {
+            constexpr int NS = C::ALT ? 2 : 1;
+            uint32_t hi[NS][8], lo[NS][8];
+#pragma unroll
+            for (int k = 0; k < NS; ++k) {
+              tmem_ld8(lanes + C::O_COL + k * 2 * R + rb + c0, hi[k]);
+              tmem_ld8(lanes + C::O_COL + k * 2 * R + R + rb + c0, lo[k]);
+            }
+            tmem_ld_wait();
+#pragma unroll
+            for (int k = 0; k < NS; ++k) {
               // (a stream without a tile has no accumulator)
               if (C::ALT && sg.n_kt == 1 && k != (it0 & 1)) continue;
-              uint32_t hi[8], lo[8];
-              tmem_ld8(lanes + C::O_COL + k * 2 * R + rb + c0, hi);
-              tmem_ld8(lanes + C::O_COL + k * 2 * R + R + rb + c0, lo);
-              tmem_ld_wait();
 #pragma unroll
               for (int e = 0; e < 8; ++e)
-                o[e] += (__uint_as_float(hi[e]) + __uint_as_float(lo[e])) * fin[128 + 64 * k + rb + c0 + e];
+                o[e] += (__uint_as_float(hi[k][e]) + __uint_as_float(lo[k][e])) * fin[128 + 64 * k + rb + c0 + e];
             }
           } else {
             // four pieces at a time: every thread's values and, by one warp, their factors on the way together
@@ -1101,8 +1132,6 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           if (gmax[0] == 0.f) break;
         }
       }
-      // mref, fac and gsum are free for the next segment once everyone is here
-      named_bar_sync(bar, 128);
     }
     if (lane == 0) mbar_arrive(done);
   }
