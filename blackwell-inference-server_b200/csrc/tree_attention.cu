@@ -147,7 +147,10 @@ static_assert(kRegsIssue + kRegsK + kRegsV + 2 * kRegsSoft == 5 * 96, "register 
 constexpr int kScaleStages = 4;   // tiles whose scales are on their way or in use
 constexpr float kLowest = -3.0e38f;  // a row's reference before any score: finite, so differences are
 constexpr int kAttnMaxBatch = 512;  // sequences of one launch (their unit ranges lie in shared memory)
+// Tickets, two per CTA, in a prefix of one size for every shape: calls of different shapes share a workspace
+// whose prefix is zeroed once.  A grid that it cannot hold (more than 32768 rows) takes attn_rows_kernel.
 constexpr size_t kAttnCounterBytes = 4096;
+constexpr int kAttnMaxGrid = kAttnCounterBytes / (2 * sizeof(int));
 enum AttnSite : int { kSiteAtTma = 401, kSiteAtDrain = 402, kSiteAtDone = 403, kSiteAtFinal = 404, kSiteAtVote = 405 };
 
 template <int D, int R>
@@ -270,6 +273,10 @@ __device__ __forceinline__ float inverse(float sum) { return sum == 0.f ? 0.f : 
 // 16 bytes global -> shared without registers; zeros, and nothing read, if !have.
 __device__ __forceinline__ void cp_async16_zfill(void* dst, const void* src, bool have) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(have ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void st_shared16(uint32_t dst, const uint32_t (&v)[4]) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
                : "memory");
 }
 // One arrival on `bar` when this thread's copies so far are complete.
@@ -877,7 +884,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
               }
             }
 #pragma unroll
-            for (int c = 0; c < RC; ++c) x[c] = exp2_approx(x[c]);
+            for (int c = 0; c < RC / 2; ++c) x[c] = exp2_approx(x[c]);  // (the other half between the conversions)
             if (pass == 2) break;
             // (All four warps vote, also after a wait that ran out, so this one ends.)
             mbar_wait_tries(&voted[g], poll & 1, ctl, kSiteAtVote);
@@ -928,13 +935,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         if (!ok) break;
         // weights
         uint8_t* prow = sP + t * C::PB + row * 128;
+        const uint32_t p_addr = smem_u32(prow) + ((row & 7) << 4);
 #pragma unroll
         for (int c0 = 0; c0 < RC; c0 += 8) {
           uint32_t hi[4], lo[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int c = c0 + 2 * e;
-            const float2 p = make_float2(x[c], x[c + 1]);
+            const float2 p = c0 < RC / 2 ? make_float2(x[c], x[c + 1]) : make_float2(exp2_approx(x[c]), exp2_approx(x[c + 1]));
             const float2 l2 = __fadd2_rn(make_float2(l[c], l[c + 1]), p);
             l[c] = l2.x;
             l[c + 1] = l2.y;
@@ -947,10 +955,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             lo[e] = *reinterpret_cast<const uint32_t*>(&r);
           }
           const int nh = cb + c0, nl = R + nh;  // columns of P
-          *reinterpret_cast<uint4*>(prow + (nh >> 6) * kTile * 128 + ((((nh & 63) >> 3) ^ (row & 7)) << 4)) =
-              make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          *reinterpret_cast<uint4*>(prow + (nl >> 6) * kTile * 128 + ((((nl & 63) >> 3) ^ (row & 7)) << 4)) =
-              make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          st_shared16((p_addr ^ ((nh & 63) << 1)) + (nh >> 6) * kTile * 128, hi);
+          st_shared16((p_addr ^ ((nl & 63) << 1)) + (nl >> 6) * kTile * 128, lo);
         }
         // What is not seen adds nothing, whatever its scale (0 times one that is not finite is not 0).
         if (masked && !(fabsf(vs) <= 3.402823466e38f)) {
@@ -1153,9 +1159,7 @@ static TilePlan tile_plan(int64_t t, int64_t grp, int64_t d) {
   p.rts = static_cast<int>((t * grp + p.r - 1) / p.r);
   p.groups = num_sms() / p.rts > 1 ? num_sms() / p.rts : 1;
   p.grid = p.groups * p.rts;
-  const size_t counters = (static_cast<size_t>(p.grid) * 2 * sizeof(int) + kAttnCounterBytes - 1) / kAttnCounterBytes *
-                          kAttnCounterBytes;
-  p.bytes = counters + static_cast<size_t>(p.grid) * 2 * (p.r * d + 2 * p.r) * sizeof(float);
+  p.bytes = kAttnCounterBytes + static_cast<size_t>(p.grid) * 2 * (p.r * d + 2 * p.r) * sizeof(float);
   return p;
 }
 // A tile is made of whole pages or lies inside one.
@@ -1188,8 +1192,7 @@ static int launch_tiles(const AttnArgs& a, const TilePlan& p, void* ws, bool qve
   ta.qvec = qvec;
   ta.counters = static_cast<int*>(ws);
   if (int s = device_wait_ptrs(&ta.status, &ta.limit)) return s;
-  ta.pieces = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + p.bytes -
-                                       static_cast<size_t>(p.grid) * 2 * (R * D + 2 * R) * sizeof(float));
+  ta.pieces = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + kAttnCounterBytes);
   for (int64_t b0 = 0; b0 < a.b; b0 += kAttnMaxBatch) {
     ta.b0 = b0;
     ta.nb = static_cast<int>(a.b - b0 < kAttnMaxBatch ? a.b - b0 : kAttnMaxBatch);
@@ -1229,15 +1232,13 @@ static int launch_tiles_d(const AttnArgs& a, const TilePlan& p, void* ws, bool q
 extern "C" size_t bw_tree_attention_int8_workspace_size(int64_t b, int64_t t, int64_t hq, int64_t heads, int64_t d) {
   if (b <= 0 || t <= 0 || t > bw::kTreeMaxNodes || heads <= 0 || hq < heads || hq > 65535 || (d != 64 && d != 128))
     return 0;
-  return bw::tile_plan(t, hq / heads, d).bytes;
+  const bw::TilePlan p = bw::tile_plan(t, hq / heads, d);
+  return p.grid <= bw::kAttnMaxGrid ? p.bytes : 0;
 }
 
 extern "C" size_t bw_tree_attention_int8_workspace_zeroed_bytes(int64_t b, int64_t t, int64_t hq, int64_t heads,
                                                                 int64_t d) {
-  const size_t all = bw_tree_attention_int8_workspace_size(b, t, hq, heads, d);
-  if (all == 0) return 0;
-  const bw::TilePlan p = bw::tile_plan(t, hq / heads, d);
-  return all - static_cast<size_t>(p.grid) * 2 * (p.r * d + 2 * p.r) * sizeof(float);
+  return bw_tree_attention_int8_workspace_size(b, t, hq, heads, d) != 0 ? bw::kAttnCounterBytes : 0;
 }
 
 extern "C" int bw_tree_attention_int8(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int dtype, void* out,
@@ -1287,10 +1288,10 @@ extern "C" int bw_tree_attention_int8(const void* q, int64_t q_sb, int64_t q_st,
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // the tensor-core kernel's units are counted in 32 bits, its cache rows addressed in them
   const int64_t units = b * heads * ((table_cols * page + kTile - 1) / kTile + 1);
-  if (tile_dims(d, page) && units < INT32_MAX && pages > 0 && pages * heads * page < INT32_MAX &&
+  const TilePlan p = tile_plan(t, hq / heads, d);
+  if (tile_dims(d, page) && p.grid <= kAttnMaxGrid && units < INT32_MAX && pages > 0 && pages * heads * page < INT32_MAX &&
       (reinterpret_cast<uintptr_t>(cache_k) | reinterpret_cast<uintptr_t>(cache_v) |
        reinterpret_cast<uintptr_t>(k_scale) | reinterpret_cast<uintptr_t>(v_scale)) % 16 == 0) {
-    const TilePlan p = tile_plan(t, hq / heads, d);
     if (workspace == nullptr || workspace_bytes < p.bytes)
       return fail(BW_ERR_WORKSPACE, "tree_attention_int8: workspace of %zu bytes required, %zu given", p.bytes,
                   workspace_bytes);

@@ -198,6 +198,29 @@ def test_long(cuda_dev, b, t, hq, h, d, page, ctx):
             assert bool((err <= bound).all()), float((err - bound).max())
 
 
+@pytest.mark.parametrize("b,t,hq,h,d,page", [
+    (700, 1, 4, 2, 64, 16),      # more sequences than one launch takes
+    (2, 1, 12000, 1, 64, 16),    # more blocks of query rows than SMs
+    (1, 3, 11200, 1, 64, 16),    # more query rows than the tickets cover
+])
+def test_many_sequences_and_heads(cuda_dev, b, t, hq, h, d, page):
+    """Shapes at the ends of the grid, with calls of an ordinary shape on the same workspace between them."""
+    from blackwell_ops.decode import tree_attention_int8
+
+    dt = torch.float16
+    small = _setup(21, 3, 2, 8, 2, 128, 16, [700, 40, 3000], dt, cuda_dev)
+    args = (small[3], small[0], _i32(small[2], cuda_dev), _i32([700, 40, 3000], cuda_dev))
+    before = tree_attention_int8(*args)
+    _check(before, small[3], small[1], small[2], [700, 40, 3000], dt)
+    rng = np.random.default_rng(22)
+    ctx = [int(x) for x in rng.integers(0, 40, b)]
+    cache, host, table, q, _ = _setup(23, b, t, hq, h, d, page, ctx, dt, cuda_dev)
+    for _ in range(2):
+        out = tree_attention_int8(q, cache, _i32(table, cuda_dev), _i32(ctx, cuda_dev))
+        _check(out, q, host, table, ctx, dt)
+        assert torch.equal(tree_attention_int8(*args), before)
+
+
 def test_offsets_past_32_bits(cuda_dev):
     from blackwell_ops.decode import KVCacheInt8, tree_attention_int8
 
