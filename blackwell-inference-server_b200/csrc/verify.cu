@@ -12,12 +12,16 @@
 // depends on a summation order, and only from a second sibling on.
 #include <stdio.h>
 
+#include <mutex>
+
 #include "kv_cache.cuh"
 
 namespace bw {
 
-constexpr int kVerifyThreads = 1024;
-constexpr int kVerifyCluster = 8;
+constexpr int kVerifyThreads = 512;
+constexpr int kVerifyStages = 3;  // steps of a row that a thread has on their way
+constexpr int kVerifySmem = kVerifyStages * 3 * kVerifyThreads * 16;
+constexpr int kVerifyCluster = 16;  // CTAs of a cluster at most
 
 struct VerifyArgs {
   const float* p;        // [b, t, v]
@@ -31,6 +35,7 @@ struct VerifyArgs {
   int64_t* out;          // [b, t]
   int64_t v;
   int t;
+  int ctas;              // of a cluster
 };
 
 // w(x) after the rejections so far at a node: with a draft distribution the recurrence over the
@@ -41,11 +46,23 @@ __device__ __forceinline__ float residual(float p, float q, const float* z, int 
   return w;
 }
 
+__device__ __forceinline__ void copy16_async(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+
+// Within 2^-23 of 1 / x for the x that are trusted below.
+__device__ __forceinline__ float approx_inverse(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float kTrustLow = 0x1p-60f, kTrustHigh = 0x1p60f;
+
 // One value of each CTA of the cluster into all of them, in the CTAs' order; `slot`s are not reused before
 // every CTA has passed another exchange.
 template <typename V>
-__device__ __forceinline__ void cluster_share(V (*slot)[kVerifyCluster], V v, int rank) {
-  if (threadIdx.x < kVerifyCluster) {
+__device__ __forceinline__ void cluster_share(V (*slot)[kVerifyCluster], V v, int rank, int ctas) {
+  if (threadIdx.x < ctas) {
     const uint32_t at = mapa_shared(smem_u32(&(*slot)[rank]), threadIdx.x);
     if constexpr (sizeof(V) == 8)
       asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(at), "l"(v) : "memory");
@@ -55,15 +72,19 @@ __device__ __forceinline__ void cluster_share(V (*slot)[kVerifyCluster], V v, in
   cluster_sync_all();
 }
 
-// One cluster per sequence, a CTA each eighth of the vocabulary.  Every CTA walks the tree on its own: the
+// One cluster per sequence, each CTA a part of the vocabulary.  Every CTA walks the tree on its own: the
 // probabilities of all drafted tokens at their parents are gathered at once, so a walk without a rejected
 // sibling before another one reads nothing more, and only then is Z summed over the row (cluster-wide, in
-// one order).  The token at the end takes one pass over the row's p, q and e: bound by their bytes where
-// sequences are many, by three dependent reads (tree, gather, row) where they are few.
+// one order).  The token at the end takes one pass over the row's p, q and e.
+// Few sequences are bound by three dependent reads (tree, gather, row), many by the bytes of the passes that
+// the unluckiest walk makes one after another.  One sequence, a chain of 5 over 151936 tokens: 7.6 us with
+// sixteen CTAs, 9.6 with eight (launch, gather and cluster barriers alone: 4.8).  32 sequences, trees of 16
+// without draft probabilities: 24 us, of which the last pass 11 (39 MB) and the sums of Z 8.
 // Scores are positive floats, whose bits order like them; with the token's complement below, the maximum of
 // the 64-bit keys is the best score at its lowest token.
 template <bool DRAFT, bool VEC>
-__global__ void __launch_bounds__(kVerifyThreads) verify_tree_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(const VerifyArgs a) {
+  extern __shared__ float4 stages[];  // [kVerifyStages][p, q, e][thread]
   __shared__ int parent[kTreeMaxNodes];
   __shared__ int64_t tok[kTreeMaxNodes];
   __shared__ int64_t dropped[kTreeMaxNodes];
@@ -75,7 +96,8 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_tree_kernel(const Verif
   __shared__ unsigned long long keys[2][kVerifyCluster];
   __shared__ int walk[4];  // node, rejections, accepted nodes, next child to try (t: the walk has ended)
   const int rank = static_cast<int>(cluster_ctarank());
-  const int64_t b = blockIdx.x / kVerifyCluster;
+  const int ctas = a.ctas;
+  const int64_t b = blockIdx.x / ctas;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int threads = blockDim.x;
   if (tid < a.t) {
@@ -93,14 +115,19 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_tree_kernel(const Verif
   }
   if (tid < 4) walk[tid] = tid == 3 ? 1 : 0;
   // this CTA's part of a row, whole groups of four
-  const int64_t per = ((a.v + kVerifyCluster - 1) / kVerifyCluster + 3) / 4 * 4;
+  const int64_t per = ((a.v + ctas - 1) / ctas + 3) / 4 * 4;
   const int64_t v0 = min(per * rank, a.v), v1 = min(v0 + per, a.v);
   __syncthreads();
   // What is left of four consecutive tokens' weights after the first r rejections.
   auto rest = [&](float4& w, const float4& qw, int64_t v, int r) {
     if (DRAFT) {
-      w = make_float4(residual(w.x, qw.x, z, r), residual(w.y, qw.y, z, r), residual(w.z, qw.z, z, r),
-                      residual(w.w, qw.w, z, r));
+      for (int i = 0; i < r; ++i) {  // (residual, of four)
+        const float zi = z[i];
+        w.x = fmaxf(__fsub_rn(w.x, __fmul_rn(zi, qw.x)), 0.f);
+        w.y = fmaxf(__fsub_rn(w.y, __fmul_rn(zi, qw.y)), 0.f);
+        w.z = fmaxf(__fsub_rn(w.z, __fmul_rn(zi, qw.z)), 0.f);
+        w.w = fmaxf(__fsub_rn(w.w, __fmul_rn(zi, qw.w)), 0.f);
+      }
     } else {
       for (int j = 0; j < r; ++j) {
         const int64_t off = dropped[j] - v;
@@ -108,6 +135,46 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_tree_kernel(const Verif
         if (VEC && off == 1) w.y = 0.f;
         if (VEC && off == 2) w.z = 0.f;
         if (VEC && off == 3) w.w = 0.f;
+      }
+    }
+  };
+  // f(four tokens of p, of q and of e, or zeros where a row is not given; the first of them) over this
+  // thread's part, in order.  Each thread copies its own groups to shared memory, kVerifyStages steps ahead
+  // (in registers they would be too few to cover the latency); rows that are no groups of four go one by one.
+  auto each = [&](const float* pr, const float* qr, const float* er, auto f) {
+    const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
+    if constexpr (VEC) {
+      const int step = threads * 4;
+      auto fetch = [&](int64_t v, int stage) {
+        if (v < v1) {
+          float4* to = stages + stage * 3 * threads + tid;
+          copy16_async(to, pr + v);
+          if (qr != nullptr) copy16_async(to + threads, qr + v);
+          if (er != nullptr) copy16_async(to + 2 * threads, er + v);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+#pragma unroll 1
+      for (int k = 0; k < kVerifyStages; ++k) fetch(v0 + tid * 4 + static_cast<int64_t>(k) * step, k);
+      int stage = 0;
+#pragma unroll 1
+      for (int64_t v = v0 + tid * 4; v < v1; v += step) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kVerifyStages - 1) : "memory");
+        const float4* from = stages + stage * 3 * threads + tid;
+        const float4 w = from[0];
+        const float4 qw = qr != nullptr ? from[threads] : none;
+        const float4 ew = er != nullptr ? from[2 * threads] : none;
+        f(w, qw, ew, v);
+        fetch(v + static_cast<int64_t>(kVerifyStages) * step, stage);
+        stage = stage + 1 == kVerifyStages ? 0 : stage + 1;
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+    } else {
+#pragma unroll 2
+      for (int64_t v = v0 + tid; v < v1; v += threads) {
+        const float4 qw = make_float4(qr != nullptr ? __ldg(qr + v) : 0.f, 0.f, 0.f, 0.f);
+        const float4 ew = make_float4(er != nullptr ? __ldg(er + v) : 0.f, 0.f, 0.f, 0.f);
+        f(make_float4(__ldg(pr + v), 0.f, 0.f, 0.f), qw, ew, v);
       }
     }
   };
@@ -152,31 +219,19 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_tree_kernel(const Verif
     const float* p = a.p + (b * a.t + cur) * a.v;
     const float* q = DRAFT ? a.q + (b * a.t + cur) * a.v : nullptr;
     float sum = 0.f;
-    if constexpr (VEC) {
-#pragma unroll 4
-      for (int64_t v = v0 + tid * 4; v < v1; v += threads * 4) {
-        float4 w = __ldg(reinterpret_cast<const float4*>(p + v));
-        const float4 qw = DRAFT ? __ldg(reinterpret_cast<const float4*>(q + v)) : make_float4(0.f, 0.f, 0.f, 0.f);
-        rest(w, qw, v, r);
-        sum += (w.x + w.y) + (w.z + w.w);
-      }
-    } else {
-#pragma unroll 4
-      for (int64_t v = v0 + tid; v < v1; v += threads) {
-        float4 w = make_float4(__ldg(p + v), 0.f, 0.f, 0.f);
-        rest(w, make_float4(DRAFT ? __ldg(q + v) : 0.f, 0.f, 0.f, 0.f), v, r);
-        sum += w.x;
-      }
-    }
+    each(p, q, nullptr, [&](float4 w, const float4& qw, const float4&, int64_t v) {
+      rest(w, qw, v, r);
+      sum += (w.x + w.y) + (w.z + w.w);
+    });
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) red[warp] = sum;
     __syncthreads();
     sum = 0.f;
     for (int k = 0; k < threads / 32; ++k) sum += red[k];
-    cluster_share(&sums[phase & 1], sum, rank);
+    cluster_share(&sums[phase & 1], sum, rank, ctas);
     if (tid == 0) {
       float s = 0.f;
-      for (int k = 0; k < kVerifyCluster; ++k) s += sums[phase & 1][k];
+      for (int k = 0; k < ctas; ++k) s += sums[phase & 1][k];
       z[r] = s;
     }
     ++phase;
@@ -198,27 +253,46 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_tree_kernel(const Verif
       }
     };
     const int rr = pass == 0 ? r : 0;
-    if constexpr (VEC) {
-#pragma unroll 4
-      for (int64_t v = v0 + tid * 4; v < v1; v += threads * 4) {
-        float4 w = __ldg(reinterpret_cast<const float4*>(p + v));
-        const float4 ew = __ldg(reinterpret_cast<const float4*>(e + v));
-        const float4 qw = DRAFT && rr > 0 ? __ldg(reinterpret_cast<const float4*>(q + v)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    auto scores = [&](auto f) {  // f(w, e, token)
+      each(p, rr > 0 ? q : nullptr, e, [&](float4 w, const float4& qw, const float4& ew, int64_t v) {
         rest(w, qw, v, rr);
-        score(w.x, ew.x, v);
-        score(w.y, ew.y, v + 1);
-        score(w.z, ew.z, v + 2);
-        score(w.w, ew.w, v + 3);
+        f(w.x, ew.x, static_cast<int>(v));
+        if (VEC) {
+          f(w.y, ew.y, static_cast<int>(v) + 1);
+          f(w.z, ew.z, static_cast<int>(v) + 2);
+          f(w.w, ew.w, static_cast<int>(v) + 3);
+        }
+      });
+    };
+    // First w times an approximate 1 / e (together within 2^-22), of which a thread keeps the best and the
+    // second best; then the rounded quotient of what comes within 2^-20 of the CTA's best, usually one
+    // token.  A thread whose second best does, and every thread where the approximation's error is not
+    // known (e or the best score outside [2^-60, 2^60]), goes through its part again with rounded
+    // quotients.
+    float top = 0.f, second = 0.f, top_w = 0.f, top_e = 1.f, e_min = 1.f, e_max = 1.f;
+    int top_v = 0;
+    scores([&](float w, float ew, int v) {
+      const float s = w * approx_inverse(ew);
+      e_min = fminf(e_min, ew);
+      e_max = fmaxf(e_max, ew);
+      second = fmaxf(second, fminf(top, s));
+      if (s > top) {
+        top = s;
+        top_w = w;
+        top_e = ew;
+        top_v = v;
       }
-    } else {
-#pragma unroll 4
-      for (int64_t v = v0 + tid; v < v1; v += threads) {
-        float4 w = make_float4(__ldg(p + v), 0.f, 0.f, 0.f);
-        const float ew = __ldg(e + v);
-        rest(w, make_float4(DRAFT && rr > 0 ? __ldg(q + v) : 0.f, 0.f, 0.f, 0.f), v, rr);
-        score(w.x, ew, v);
-      }
-    }
+    });
+    float most = top;
+    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (lane == 0) red[warp] = most;
+    const bool odd = __syncthreads_or(!(e_min >= kTrustLow && e_max <= kTrustHigh));
+    for (int k = 0; k < threads / 32; ++k) most = fmaxf(most, red[k]);
+    const float near = most * (1.f - 0x1p-20f);
+    if (odd || !(most >= kTrustLow && most <= kTrustHigh) || second >= near)
+      scores(score);
+    else if (top >= near)
+      score(top_w, top_e, top_v);
     for (int o = 16; o > 0; o >>= 1) {
       const unsigned long long k = __shfl_xor_sync(0xffffffffu, best, o);
       best = k > best ? k : best;
@@ -227,9 +301,9 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_tree_kernel(const Verif
     __syncthreads();
     best = 0;
     for (int k = 0; k < threads / 32; ++k) best = redk[k] > best ? redk[k] : best;
-    cluster_share(&keys[pass], best, rank);
+    cluster_share(&keys[pass], best, rank, ctas);
     best = 0;
-    for (int k = 0; k < kVerifyCluster; ++k) best = keys[pass][k] > best ? keys[pass][k] : best;
+    for (int k = 0; k < ctas; ++k) best = keys[pass][k] > best ? keys[pass][k] : best;
     if (best == 0 && pass == 0) continue;
     if (rank == 0) {
       if (tid == 0) {
@@ -248,19 +322,40 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_tree_kernel(const Verif
 }
 
 template <bool DRAFT, bool VEC>
-static int launch_verify(const VerifyArgs& a, int64_t b, cudaStream_t st) {
+static int launch_verify(VerifyArgs a, int64_t b, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(b * kVerifyCluster));
-  // one CTA an SM while there is an SM for each, two smaller ones where there are more
-  cfg.blockDim = dim3(b * kVerifyCluster <= num_sms() ? kVerifyThreads : kVerifyThreads / 2);
-  cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = kVerifyCluster;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  cfg.stream = st;
+  cfg.blockDim = dim3(kVerifyThreads);
+  cfg.dynamicSmemBytes = VEC ? kVerifySmem : 0;
+  auto shape = [&](int ctas) {
+    a.ctas = ctas;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(ctas);
+    cfg.gridDim = dim3(static_cast<unsigned>(b * ctas));
+  };
+  static std::once_flag once[64];
+  static cudaError_t attr_err[64];
+  static bool wide[64];
+  int dev = 0;
+  if (cudaError_t err = cudaGetDevice(&dev)) return check_cuda(err, "cudaGetDevice");
+  dev &= 63;
+  std::call_once(once[dev], [&] {
+    auto kernel = verify_tree_kernel<DRAFT, VEC>;
+    attr_err[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kVerifySmem);
+    shape(kVerifyCluster);
+    int fit = 0;
+    wide[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                cudaOccupancyMaxActiveClusters(&fit, kernel, &cfg) == cudaSuccess && fit > 0;
+    if (!wide[dev]) cudaGetLastError();
+  });
+  if (int s = check_cuda(attr_err[dev], "cudaFuncSetAttribute(verify_tree_kernel)")) return s;
+  // Few sequences: sixteen CTAs each, where the device can place such a cluster; else two CTAs an SM.
+  shape(wide[dev] && b * kVerifyCluster <= num_sms() ? kVerifyCluster : 8);
   return check_cuda(cudaLaunchKernelEx(&cfg, verify_tree_kernel<DRAFT, VEC>, a), "cudaLaunchKernelEx(verify_tree_kernel)");
 }
 
@@ -277,7 +372,7 @@ extern "C" int bw_verify_tree(const float* target, const float* draft, const int
     return fail(BW_ERR_INVALID_ARGUMENT, "verify_tree: null pointer");
   if (int s = require_sm100()) return s;
   VerifyArgs a = {target, draft, tokens, parents, accept_u, sample_e, n_accepted, path, out_tokens, v,
-                  static_cast<int>(t)};
+                  static_cast<int>(t), 0};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // rows of 16-byte groups: every row starts on one
   const bool vec = v % 4 == 0 && (reinterpret_cast<uintptr_t>(target) | reinterpret_cast<uintptr_t>(draft) |

@@ -85,6 +85,45 @@ def test_padding_ties_and_empty_residuals(cuda_dev):
     _check((p, tok, par, u, e, q), cuda_dev)
 
 
+@pytest.mark.parametrize("v", [4096, 4099, 200])
+@pytest.mark.parametrize("b", [3, 20])
+def test_scores_near_and_out_of_range(cuda_dev, b, v):
+    """The last token is the best rounded quotient, lowest token first, where quotients are equal or a few ulps apart,
+    within one thread's part and across parts, and where weights or exponentials are tiny, huge, zero, infinite or (the weights) NaN."""
+    rng = np.random.default_rng(v + b)
+    f = np.float32
+    for kind in range(9):
+        p, tok, par, u, e, q = _case(kind, b, 1, v, "chain", True)
+        if kind == 0:                                 # two to five quotients a few ulps apart near the top
+            for i in range(b):
+                at = rng.choice(v, 5, replace=False)
+                p[i, 0, at], e[i, at] = f(0.9), f(1e-3) * (1 + f(2.0**-23) * rng.integers(0, 9, 5).astype(f))
+        elif kind == 1:                               # neighbours, the same quotient from different pairs
+            p[:, 0, 8], e[:, 8] = f(0.25), f(2.0**-20)
+            p[:, 0, 9], e[:, 9] = f(0.5), f(2.0**-19)
+            p[:, 0, v - 1], e[:, v - 1] = f(0.125), f(2.0**-21)
+        elif kind == 2:
+            p *= f(1e-30)                             # all scores below the trusted range
+        elif kind == 3:
+            p *= f(1e-42)                             # subnormal weights
+        elif kind == 4:
+            e[:, 5] = f(1e-44)                        # a subnormal exponential: the quotient overflows or is huge
+        elif kind == 5:
+            e[:, 7], p[:, 0, 7] = 0.0, f(1e-3)        # infinite
+            e[:, 11], p[:, 0, 11] = 0.0, 0.0          # no candidate
+        elif kind == 6:
+            e[:, 3] = np.inf
+            p[:, 0, 6] = np.nan
+        elif kind == 7:
+            p[:, 0] = 0.0
+            p[:, 0, v // 2], e[:, v // 2] = f(1e-20), f(1e25)   # the only candidate
+        else:
+            p *= f(1e30)
+            e *= f(1e-25)
+        with np.errstate(all="ignore"):
+            _check((p, tok, par, u, e, q), cuda_dev)
+
+
 def test_strides(cuda_dev):
     from blackwell_ops.decode import verify_tree
 
