@@ -267,6 +267,19 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+// v less two bf16 numbers, one instruction each (a multiply-add of bf16 factors and an fp32 addend).
+__device__ __forceinline__ float2 sub_bf16x2(const float2& v, uint32_t h) {
+  float2 y;
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tfma.rn.f32.bf16 %0, a, %5, %3;\n\tfma.rn.f32.bf16 %1, b, %5, %4;\n\t}"
+      : "=f"(y.x), "=f"(y.y)
+      : "r"(h), "f"(v.x), "f"(v.y), "h"(static_cast<unsigned short>(0xBF80)));  // -1
+  return y;
+}
 // 1 / sum of a row's weights; 0 where it saw nothing.
 __device__ __forceinline__ float inverse(float sum) { return sum == 0.f ? 0.f : __frcp_rn(sum); }
 
@@ -364,8 +377,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   uint64_t* afull = vempty + ST;      // 2: K dequantised in TMEM
   uint64_t* vbfull = afull + 2;       // 2: V dequantised
   uint64_t* sfull = vbfull + 2;       // 2: scores (and the K tile is read)
-  uint64_t* sempty = sfull + 2;
-  uint64_t* pfull = sempty + 2;       // 2: weights
+  uint64_t* pfull = sfull + 2;        // 2: weights (and the scores are read)
   uint64_t* pempty = pfull + 2;       //    read, as is the V tile, and added to the accumulator
   uint64_t* qfull = pempty + 2;       // 2: Q and the row masks of a segment
   uint64_t* qempty = qfull + 2;
@@ -405,7 +417,6 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       mbar_init(&afull[i], 4);
       mbar_init(&vbfull[i], 4);
       mbar_init(&sfull[i], 1);
-      mbar_init(&sempty[i], C::GW);
       mbar_init(&pfull[i], C::GW);
       mbar_init(&pempty[i], 1);
       mbar_init(&qfull[i], 1);
@@ -622,7 +633,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       for (int i = 0; i < n_kt; ++i, ++it) {
         const int t = it & 1;
         const uint32_t ph = (it >> 1) & 1;
-        ok = mbar_wait_or_abort(&afull[t], ph, ctl) && mbar_wait_or_abort(&sempty[t], ph ^ 1, ctl);
+        // (once the tile's predecessor is in the accumulator, its scores and weights are read as well: the
+        // softmax warps, who see this tile's scores, need not wait for either)
+        ok = mbar_wait_or_abort(&afull[t], ph, ctl) && mbar_wait_or_abort(&pempty[t], ph ^ 1, ctl);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
@@ -842,7 +855,6 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           if (!got) {  // (while the scores are on their way)
             got = true;
             fine = mbar_wait_or_abort(&scfull[sc], (it / kScaleStages) & 1, ctl) && fine;
-            fine = mbar_wait_or_abort(&pempty[t], ph ^ 1, ctl) && fine;
             ks = sScale[sc * 2 * kTile + row] * a.scale_log2;
             vs = sScale[sc * 2 * kTile + kTile + row];
             const bool there = row < left && ((sPages[sc] >> (row >> 2)) & 1);
@@ -873,10 +885,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           }
           if (pass != 1) {
             if (pass == 0) {
-              float top[4] = {x[0], x[1], x[2], x[3]};
+            float top[2] = {x[0], x[1]};
 #pragma unroll
-              for (int c = 4; c < RC; ++c) top[c & 3] = fmaxf(top[c & 3], x[c]);
-              const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+              for (int c = 2; c < RC; c += 4) {
+                top[0] = max3(top[0], x[c], x[c + 1]);
+                if (c + 2 < RC) top[1] = max3(top[1], x[c + 2], x[c + 3]);
+              }
+              const float most = fmaxf(top[0], top[1]);
               const bool again = __any_sync(0xffffffffu, most > 8.f || !fine);
               if (lane == 0) {
                 if (again) votes[g * 2 + (poll & 1)] = 1;
@@ -949,8 +964,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             const float2 v = __fmul2_rn(p, make_float2(vs, vs));
             const __nv_bfloat162 h = __float22bfloat162_rn(v);
             hi[e] = *reinterpret_cast<const uint32_t*>(&h);
-            const float2 left = __ffma2_rn(make_float2(__uint_as_float(hi[e] << 16), __uint_as_float(hi[e] & 0xFFFF0000u)),
-                                           make_float2(-1.f, -1.f), v);  // v - hi, exact
+            const float2 left = sub_bf16x2(v, hi[e]);  // exact
             const __nv_bfloat162 r = __float22bfloat162_rn(left);
             lo[e] = *reinterpret_cast<const uint32_t*>(&r);
           }
@@ -973,7 +987,6 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(&pfull[t]);
-          mbar_arrive(&sempty[t]);
           mbar_arrive(&scempty[sc]);
         }
       }
