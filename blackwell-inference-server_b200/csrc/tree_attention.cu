@@ -123,10 +123,11 @@ __global__ void __launch_bounds__(32 * kRowWarps) attn_rows_kernel(const __grid_
 // two bf16 numbers (hi = bf16(x), lo = bf16(x - hi), 2^-17 of x left out): fp16 would be one number
 // but cannot hold w vs_j for every scale, one bf16 alone loses 2^-9.
 //
-// Softmax: one thread holds one slot's R scores, so the exponentials need no exchange; what is
-// shared is each row's reference m.  m moves only when a score exceeds it by more than 8 (in powers
-// of two): a vote decides, and only then are the row maxima taken over the 128 slots, the sums l and
-// the accumulators rescaled.  Weights stay under 2^8, sums and accumulators are fp32.
+// Softmax: one thread holds one slot's scores, so the exponentials need no exchange; what is shared is
+// each row's reference m.  m moves only when a score exceeds it by more than 8 (in powers of two): the
+// warps vote while they work out the weights, and only if one has such a score are the row maxima taken
+// over the 128 slots, the sums l and the accumulators rescaled.  Weights stay under 2^8, sums and
+// accumulators are fp32.
 //
 // Work: the (sequence, key head, tile) units, laid end to end, are split evenly over the CTAs, so
 // ragged lengths balance; with more rows than R, neighbouring CTAs take the row blocks of one range
@@ -134,9 +135,18 @@ __global__ void __launch_bounds__(32 * kRowWarps) attn_rows_kernel(const __grid_
 // is joined by its last CTA (a ticket) from the pieces in the workspace, in range order, so results
 // do not depend on timing.
 //
-// One CTA per SM, five warpgroups: 0 and 3 TMA (one box per page), scales and Q, 1 issues K.Q, 2 issues V.P;
-// 4-7 dequantise K into TMEM (thread = slot); 8-11 dequantise V into shared memory and load Q; 12-15
-// and 16-19 are two softmax groups of half the rows each.
+// One CTA per SM, five warpgroups.  Warps 0 and 3: TMA of K and of V (one box per page), scales, each
+// segment's Q and row masks; warp 0 also watches the time for all waits.  Warps 1 and 2 issue K.Q and V.P.
+// 4-7 dequantise K into TMEM (thread = slot), 8-11 V into shared memory, 12-15 and 16-19 are the two softmax
+// groups.
+//
+// What bounds it (one B200, D = 128, bf16, long contexts): with 16 rows the two dequantisers' issue slots,
+// 1.05 us a tile of 32 KB in every SM, 4.7 TB/s (fp16, whose conversion has five instructions for four codes
+// where bf16 has nine: 0.87 us, 5.7 TB/s); with 64 rows the softmax groups, 1.55 us a tile, 400 TFLOP/s;
+// with short contexts a segment's start and end, 3 us together.  Measured and not kept: 64 rows in alternate
+// tiles, whose scores are then fetched twice (a sixth slower on a tree of 64 nodes over 128k slots); row
+// blocks of equal height (690 us for 618 there: branches between the columns cost more than the columns); a
+// segment's end put off into the next one's first tiles (125 us for 116 on 64 x 4k).
 // ---------------------------------------------------------------------------
 constexpr int kTile = 128;
 constexpr int kAttnThreads = 20 * 32;
@@ -885,7 +895,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           }
           if (pass != 1) {
             if (pass == 0) {
-            float top[2] = {x[0], x[1]};
+              float top[2] = {x[0], x[1]};
 #pragma unroll
               for (int c = 2; c < RC; c += 4) {
                 top[0] = max3(top[0], x[c], x[c + 1]);
