@@ -209,7 +209,8 @@ __device__ __forceinline__ void codes16(const float* x, float sc, float rcp, uin
 template <typename T, int L, bool WRITE, bool INTER>
 __global__ void __launch_bounds__(256, WRITE ? 3 : 4) rotary_vec_kernel(const __grid_constant__ RotArgs a, int gpt) {
   constexpr int D = 16 * L;
-  __shared__ __align__(16) float2 turns_of[256];  // (cos, sin) of the CTA's tokens' pairs
+  // (cos, sin) of the CTA's tokens' pairs: 256 / (gpt L) tokens of rot / 2 <= 8 L pairs, so gpt is 8 at least
+  __shared__ __align__(16) float2 turns_of[256];
   const int j = threadIdx.x % L;
   const int64_t group = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / L;
   const int64_t tok = group / gpt;
@@ -218,6 +219,30 @@ __global__ void __launch_bounds__(256, WRITE ? 3 : 4) rotary_vec_kernel(const __
   // gpt * L is a power of two: whole tokens in a CTA, or a part of one
   const int in_cta = max(1, 256 / (gpt * L));
   const int64_t tok0 = static_cast<int64_t>(blockIdx.x) * 256 / (gpt * L);
+  const int64_t b = tok / a.t, t = tok - b * a.t;
+  const bool turns = j < a.rot / 16;
+  const int e0 = turns ? 8 * j : a.rot / 2 + 8 * j;  // (the rest starts at rot, at lane rot / 16)
+  const int e1 = turns ? a.rot / 2 + 8 * j : D / 2 + 8 * j;
+  const int hq = a.q.heads, hqk = hq + a.k.heads;
+  const int rows = tok < a.b * a.t ? hqk + a.v.heads : 0;  // (the same for a whole group: the shuffles stay inside one)
+  int64_t krow = -1;
+  if (WRITE && rows > 0 && (a.counts == nullptr || t < a.counts[b]))
+    krow = kv_row(a.cache, b, static_cast<int64_t>(a.start[b]) + t);
+  const unsigned lanes = L == 32 ? 0xffffffffu : ((1u << L) - 1u) << ((threadIdx.x & 31) / L * L);
+  // The next row is on its way while one is turned, the first while the sines are computed.  8191 tokens of 72
+  // rows: 57 us, 5.3 TB/s; two rows ahead 60, three 68 (their registers spill).  The write of 4096 tokens' 32
+  // query rows with 16 rows into the cache: 26.5 us, 3.5 TB/s, the quotients' instructions between the loads.
+  auto fetch = [&](int h, uint4 (&raw)[2]) {
+    if (h >= rows) return;
+    const int which = h < hq ? 0 : (h < hqk ? 1 : 2);
+    const int hh = which == 0 ? h : (which == 1 ? h - hq : h - hqk);
+    const RowSet& s = which == 0 ? a.q : (which == 1 ? a.k : a.v);
+    const T* x = static_cast<const T*>(s.p) + b * s.sb + t * s.st + hh * s.sh;
+    raw[0] = *reinterpret_cast<const uint4*>(x + (which == 2 ? 8 * j : e0));
+    raw[1] = *reinterpret_cast<const uint4*>(x + (which == 2 ? D / 2 + 8 * j : e1));
+  };
+  uint4 next[2];
+  fetch(g, next);
   for (int e = threadIdx.x; e < in_cta * half; e += 256) {
     const int k = e / half;
     if (tok0 + k < a.b * a.t) {
@@ -227,84 +252,58 @@ __global__ void __launch_bounds__(256, WRITE ? 3 : 4) rotary_vec_kernel(const __
     }
   }
   __syncthreads();
-  if (tok >= a.b * a.t) return;  // (a whole group at once: the shuffles below stay inside one)
-  const int64_t b = tok / a.t, t = tok - b * a.t;
-  const bool turns = j < a.rot / 16;
-  const int e0 = turns ? 8 * j : a.rot / 2 + 8 * j;  // (the rest starts at rot, at lane rot / 16)
-  const int e1 = turns ? a.rot / 2 + 8 * j : D / 2 + 8 * j;
-  const int hq = a.q.heads, hqk = hq + a.k.heads, rows = hqk + a.v.heads;
   // pairs of the lane: eight of the half layout, four of each chunk of the interleaved one
   const float4* cs0 = reinterpret_cast<const float4*>(turns_of + static_cast<int>(tok - tok0) * half) +
                       (INTER ? e0 / 4 : 4 * j);
   const float4* cs1 = INTER ? cs0 - e0 / 4 + e1 / 4 : cs0 + 2;
-  int64_t krow = -1;
-  if (WRITE && (a.counts == nullptr || t < a.counts[b])) krow = kv_row(a.cache, b, static_cast<int64_t>(a.start[b]) + t);
-  const unsigned lanes = L == 32 ? 0xffffffffu : ((1u << L) - 1u) << ((threadIdx.x & 31) / L * L);
-  // rows on their way at once (8191 tokens of 72 rows: 59 us with two, 62 with one; the write, with its
-  // codes' registers, 27 us with one, 29 with two)
-  constexpr int UNROLL = WRITE ? 1 : 2;
-  for (int h0 = g; h0 < rows; h0 += gpt * UNROLL) {
-    uint4 raw[UNROLL][2];
+#pragma unroll 1
+  for (int h = g; h < rows; h += gpt) {
+    const uint4 raw[2] = {next[0], next[1]};
+    fetch(h + gpt, next);
+    const int which = h < hq ? 0 : (h < hqk ? 1 : 2);
+    const int hh = which == 0 ? h : (which == 1 ? h - hq : h - hqk);
+    const bool plain = which == 2;  // values do not turn
+    const int f0 = plain ? 8 * j : e0, f1 = plain ? D / 2 + 8 * j : e1;
+    float v[16];
+    unpack8<T>(raw[0], v);
+    unpack8<T>(raw[1], v + 8);
+    if (turns && !plain) {
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int h = h0 + u * gpt;
-      if (h >= rows) continue;
-      const int which = h < hq ? 0 : (h < hqk ? 1 : 2);
-      const int hh = which == 0 ? h : (which == 1 ? h - hq : h - hqk);
-      const RowSet& s = which == 0 ? a.q : (which == 1 ? a.k : a.v);
-      const T* x = static_cast<const T*>(s.p) + b * s.sb + t * s.st + hh * s.sh;
-      raw[u][0] = *reinterpret_cast<const uint4*>(x + (which == 2 ? 8 * j : e0));
-      raw[u][1] = *reinterpret_cast<const uint4*>(x + (which == 2 ? D / 2 + 8 * j : e1));
-    }
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int h = h0 + u * gpt;
-      if (h >= rows) continue;
-      const int which = h < hq ? 0 : (h < hqk ? 1 : 2);
-      const int hh = which == 0 ? h : (which == 1 ? h - hq : h - hqk);
-      const bool plain = which == 2;  // values do not turn
-      const int f0 = plain ? 8 * j : e0, f1 = plain ? D / 2 + 8 * j : e1;
-      float v[16];
-      unpack8<T>(raw[u][0], v);
-      unpack8<T>(raw[u][1], v + 8);
-      if (turns && !plain) {
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {  // two pairs
-          const float4 cs = p < 2 ? cs0[p] : cs1[p - 2];
-          // half layout: elements 2 p, 2 p + 1 with their partners 8 on; interleaved: four neighbours
-          float& x0 = v[INTER ? 4 * p : 2 * p];
-          float& x1 = v[INTER ? 4 * p + 1 : 2 * p + 8];
-          float& y0 = v[INTER ? 4 * p + 2 : 2 * p + 1];
-          float& y1 = v[INTER ? 4 * p + 3 : 2 * p + 9];
-          const float u0 = x0, u1 = x1, w0 = y0, w1 = y1;
-          x0 = u0 * cs.x - u1 * cs.y;
-          x1 = u0 * cs.y + u1 * cs.x;
-          y0 = w0 * cs.z - w1 * cs.w;
-          y1 = w0 * cs.w + w1 * cs.z;
-        }
+      for (int p = 0; p < 4; ++p) {  // two pairs
+        const float4 cs = p < 2 ? cs0[p] : cs1[p - 2];
+        // half layout: elements 2 p, 2 p + 1 with their partners 8 on; interleaved: four neighbours
+        float& x0 = v[INTER ? 4 * p : 2 * p];
+        float& x1 = v[INTER ? 4 * p + 1 : 2 * p + 8];
+        float& y0 = v[INTER ? 4 * p + 2 : 2 * p + 1];
+        float& y1 = v[INTER ? 4 * p + 3 : 2 * p + 9];
+        const float u0 = x0, u1 = x1, w0 = y0, w1 = y1;
+        x0 = u0 * cs.x - u1 * cs.y;
+        x1 = u0 * cs.y + u1 * cs.x;
+        y0 = w0 * cs.z - w1 * cs.w;
+        y1 = w0 * cs.w + w1 * cs.z;
       }
-      if (!WRITE || which == 0) {
-        T* y = static_cast<T*>(which == 0 ? a.q_out : a.k_out) + (tok * (which == 0 ? hq : a.k.heads) + hh) * D;
-        *reinterpret_cast<uint4*>(y + f0) = pack8<T>(v);
-        *reinterpret_cast<uint4*>(y + f1) = pack8<T>(v + 8);
-        continue;
-      }
-      float m = 0.f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(v[i]));
-#pragma unroll
-      for (int o = L / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(lanes, m, o));
-      if (krow < 0) continue;
-      const int64_t row = krow + static_cast<int64_t>(hh) * a.cache.page;
-      const float sc = __fdiv_rn(m, 127.0f);
-      const float rcp = __frcp_rn(sc);
-      int8_t* q = (which == 1 ? a.cache.k : a.cache.v) + row * D;
-      uint2 lo, hi;
-      codes16(v, sc, rcp, lo, hi);
-      *reinterpret_cast<uint2*>(q + f0) = lo;
-      *reinterpret_cast<uint2*>(q + f1) = hi;
-      if (j == 0) (which == 1 ? a.cache.ks : a.cache.vs)[row] = sc;
     }
+    if (!WRITE || which == 0) {
+      T* y = static_cast<T*>(which == 0 ? a.q_out : a.k_out) + (tok * (which == 0 ? hq : a.k.heads) + hh) * D;
+      *reinterpret_cast<uint4*>(y + f0) = pack8<T>(v);
+      *reinterpret_cast<uint4*>(y + f1) = pack8<T>(v + 8);
+      continue;
+    }
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(v[i]));
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(lanes, m, o));
+    if (krow < 0) continue;
+    const int64_t row = krow + static_cast<int64_t>(hh) * a.cache.page;
+    const float sc = __fdiv_rn(m, 127.0f);
+    const float rcp = __frcp_rn(sc);
+    int8_t* q = (which == 1 ? a.cache.k : a.cache.v) + row * D;
+    uint2 lo, hi;
+    codes16(v, sc, rcp, lo, hi);
+    *reinterpret_cast<uint2*>(q + f0) = lo;
+    *reinterpret_cast<uint2*>(q + f1) = hi;
+    if (j == 0) (which == 1 ? a.cache.ks : a.cache.vs)[row] = sc;
   }
 }
 
