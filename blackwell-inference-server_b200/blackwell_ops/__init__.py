@@ -10,7 +10,10 @@ Drop-in names, as in the reference package:
   (reference ``src/blackwell_ops/cuda/__init__.py:89-101``)
 
 plus the fused ``blackwell_ops.cuda.lora_merge`` / ``lora_merge_requant`` and
-the column-parallel ``blackwell_ops.nsplit`` wrapper.
+the column-parallel ``blackwell_ops.nsplit`` wrapper, and in
+``blackwell_ops.decode`` the operators of a decoder step around the linears:
+rotary positions, a paged int8 KV cache, attention of drafted trees over it and
+their verification.
 """
 
 __version__ = "0.1.0+b200"

@@ -41,10 +41,24 @@ _workspaces: dict[tuple[int, int], torch.Tensor] = {}
 _stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
 
+try:  # the allocation that the compiler's generated code calls: 0.8 us where torch.empty takes 3
+    from torch._C._dynamo.guards import _empty_strided_cuda as _empty_strided
+except ImportError:
+    _empty_strided = None
 
-def _like(x: torch.Tensor) -> torch.Tensor:
-    """A contiguous tensor of x's shape, type and device (half the cost of torch.empty with a device)."""
-    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+def _new(shape: tuple, dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
+    """A contiguous tensor."""
+    n = len(shape)
+    if _empty_strided is None or n > 4 or dev.index != _current_device():
+        return torch.empty(shape, dtype=dtype, device=dev)
+    if n == 4:
+        a, b, c, d = shape
+        return _empty_strided((a, b, c, d), (b * c * d, c * d, d, 1), dtype)
+    if n == 3:
+        a, b, c = shape
+        return _empty_strided((a, b, c), (b * c, c, 1), dtype)
+    return _empty_strided(tuple(shape), (shape[1], 1) if n == 2 else (1,), dtype)
 
 
 def _call(op: str, dev: torch.device, fn, *args) -> None:
@@ -215,14 +229,14 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
     if plan.device != dev:
         raise RuntimeError("rotary: the plan is on another device")
     positions = _positions(positions, lead, dev)
-    q_out = _like(q) if len(shape) < 5 else torch.empty(shape, dtype=dt, device=dev)
+    q_out = _new(shape, dt, dev)
     k_out, hk, kb, kt, kh, kp, kop = None, 0, 0, 0, 0, None, None
     if k is not None:
         k, kshape, _, _, kb, kt, kh = _rows(k, "k", lead)
         if k.dtype is not dt or k.device != dev or kshape[-1] != d:
             raise RuntimeError("k must have q's dtype, device and head dimension")
         hk = kshape[-2]
-        k_out = _like(k) if len(kshape) < 5 else torch.empty(kshape, dtype=dt, device=dev)
+        k_out = _new(kshape, dt, dev)
         kp, kop = k.data_ptr(), k_out.data_ptr()
     if d:
         _call("rotary", dev, lib.bw_rotary, q.data_ptr(), qb, qt, qh, hq, kp, kb, kt, kh, hk, q_out.data_ptr(), kop,
@@ -340,7 +354,7 @@ def _write(q, k, v, positions, plan, cache, table, start, counts, op):
             raise RuntimeError(f"{op}: the plan must be on the cache's device with rot_dim <= D")
         positions = _positions(positions, lead, dev)
         hq = qshape[2]
-        q_out = _like(q)
+        q_out = _new(qshape, dt, dev)
         qp, qop = q.data_ptr(), q_out.data_ptr()
         pp, p64, sp = positions.data_ptr(), positions.dtype is torch.int64, plan._ptr
         mag, rot, inter = plan.magnitude, plan.rot_dim, plan.interleaved
@@ -382,8 +396,7 @@ def kv_read_int8(cache: KVCacheInt8, table: torch.Tensor, start: torch.Tensor | 
     lp = None if lens is None else _ints(lens, "lens", (b,), dev)
     layers = cache.layers
     shape = (b, n, cache.heads, cache.head_dim) if layers is None else (layers, b, n, cache.heads, cache.head_dim)
-    k = torch.empty(shape, dtype=dtype, device=dev)
-    v = _like(k)
+    k, v = _new(shape, dtype, dev), _new(shape, dtype, dev)
     _call("kv_read_int8", dev, lib.bw_kv_read_int8, *cache._ptrs, 1 if layers is None else layers, *cache._dims,
           table.data_ptr(), ld, cols, None if sp is None else sp.data_ptr(), None if lp is None else lp.data_ptr(), b, n,
           k.data_ptr(), v.data_ptr(), DTYPE_CODE[dtype])
@@ -423,8 +436,7 @@ def tree_positions(parents: torch.Tensor, ctx_lens: torch.Tensor | None = None) 
     b, t = parents.shape
     if ctx_lens is not None:
         ctx_lens = _ints(ctx_lens, "ctx_lens", (b,), dev)
-    mask = torch.empty((b, t), dtype=torch.int64, device=dev)
-    pos = torch.empty((b, t), dtype=torch.int32, device=dev)
+    mask, pos = _new((b, t), torch.int64, dev), _new((b, t), torch.int32, dev)
     _call("tree_positions", dev, lib.bw_tree_positions, parents.data_ptr(), t,
           None if ctx_lens is None else ctx_lens.data_ptr(), b, t, mask.data_ptr(), pos.data_ptr())
     return mask, pos
@@ -471,7 +483,7 @@ def tree_attention_int8(q: torch.Tensor, cache: KVCacheInt8, table: torch.Tensor
             raise RuntimeError(f"mask must be int64 [{b}, {t}] on the cache's device")
         if not mask.is_contiguous():
             mask = mask.contiguous()
-    out = _like(q)
+    out = _new(shape, dt, dev)
     if b == 0 or t == 0:
         return out
     nbytes = lib.bw_tree_attention_int8_workspace_size(b, t, hq, heads, d)
@@ -524,7 +536,7 @@ def verify_tree(target_probs: torch.Tensor, tokens: torch.Tensor, parents: torch
         draft_probs = draft_probs.contiguous()
     target_probs, tokens, parents = target_probs.contiguous(), tokens.contiguous(), parents.contiguous()
     accept_u, sample_e = accept_u.contiguous(), sample_e.contiguous()
-    n, path, out = parents.new_empty((b,)), _like(parents), _like(tokens)
+    n, path, out = _new((b,), torch.int32, dev), _new(nodes, torch.int32, dev), _new(nodes, torch.int64, dev)
     if b and not t:
         n.zero_()
     _call("verify_tree", dev, lib.bw_verify_tree, target_probs.data_ptr(),
