@@ -143,7 +143,8 @@ __global__ void __launch_bounds__(32 * kRowWarps) attn_rows_kernel(const __grid_
 // What bounds it (one B200, D = 128, bf16, long contexts): with 16 rows the two dequantisers' issue slots,
 // 1.05 us a tile of 32 KB in every SM, 4.7 TB/s (fp16, whose conversion has five instructions for four codes
 // where bf16 has nine: 0.87 us, 5.7 TB/s); with 64 rows the softmax groups, 1.55 us a tile, 400 TFLOP/s;
-// with short contexts a segment's start and end, 3 us together.  Measured and not kept: 64 rows in alternate
+// with short contexts a segment's start and end, under 3 us together; one token over 1k slots 12.3 us, of which
+// 1 us from launch to the first barrier, 2 to the first tile, 1.5 from scores to weights, 1.4 the ticket.  Measured and not kept: 64 rows in alternate
 // tiles, whose scores are then fetched twice (a sixth slower on a tree of 64 nodes over 128k slots); row
 // blocks of equal height (690 us for 618 there: branches between the columns cost more than the columns); a
 // segment's end put off into the next one's first tiles (125 us for 116 on 64 x 4k).
@@ -302,6 +303,7 @@ __device__ __forceinline__ void st_shared16(uint32_t dst, const uint32_t (&v)[4]
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
                : "memory");
 }
+__device__ __forceinline__ void fence_acq_rel_gpu() { asm volatile("fence.acq_rel.gpu;" ::: "memory"); }
 // One arrival on `bar` when this thread's copies so far are complete.
 __device__ __forceinline__ void cp_async_arrive_noinc(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -408,6 +410,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   unsigned long long* rmask = reinterpret_cast<unsigned long long*>(ftab + 2 * 256 + 32);  // [2][64]
   int* rows = reinterpret_cast<int*>(rmask + 2 * 64);                // [64] node | query head of the group << 16
   int* pre = rows + 64;                                              // [nb + 1] first unit of a sequence
+  int* cut = pre + kAttnMaxBatch + 1;                                // [NQ][2] first and last CTA of a segment's whole
   static_assert((4 * 6 + 25 + 2 * kScaleStages) * 8 + 8 + sizeof(WaitControl) + 16 <= 640 && sizeof(WaitControl) == 24,
                 "barriers");
 
@@ -465,6 +468,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     rows[r] = min(n, 0x7fff) | ((rt * R + r - n * grp) << 16);
   }
   pdl_wait();  // lengths, tables, masks, q and the cache may come from the preceding kernel
+  pdl_launch_dependents();
   // units before each sequence; one at least, so that every output row is written
   if (warp == 0) {
     const int64_t room = static_cast<int64_t>(a.c.table_cols) * a.c.page;
@@ -547,6 +551,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       for (int r = lane; r < R; r += 32) {
         const int n = rows[r] & 0xffff;
         rmask[qb * 64 + r] = n < a.t ? node_mask(a, b, n, nodes) : 0ull;
+      }
+      if (lane == 0 && q_sg.n_kt != q_sg.tiles) {
+        cut[qb * 2] = range.owner(q_sg.u0);
+        cut[qb * 2 + 1] = range.owner(q_sg.u0 + q_sg.tiles - 1);
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -1000,6 +1008,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           mbar_arrive(&scempty[sc]);
         }
       }
+      const bool split = sg.n_kt != sg.tiles;  // several CTAs share the (sequence, head)
+      const int c_first = split ? cut[qb * 2] : 0;
+      const int c_last = split ? cut[qb * 2 + 1] : 0;
       __syncwarp();
       if (lane == 0) mbar_arrive(&qempty[qb]);  // the masks are read no more
       // ---- the segment's end: sums of the weights, output or piece ----
@@ -1016,7 +1027,6 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       // From here on a group has the rows [rb, rb + RH): their references and sums, of both streams' where
       // there are two.
       const int rb = g * RH;
-      const bool split = sg.n_kt != sg.tiles;  // several CTAs share the (sequence, head)
       if (tid < RH) {
         const int c = rb + tid;
         // (C::ALT ? both streams' sums over the four warps : the group's)
@@ -1040,8 +1050,6 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       named_bar_sync(bar, 128);
       T* out = static_cast<T*>(a.o) + (b * a.t * a.hq + sg.h * grp) * static_cast<int64_t>(D) + row;
       constexpr int PIECE = R * D + 2 * R;
-      const int c_first = split ? range.owner(sg.u0) : 0;
-      const int c_last = split ? range.owner(sg.u0 + sg.tiles - 1) : 0;
       float* piece = ta.pieces + (static_cast<int64_t>(blockIdx.x) * 2 + sg.slot) * PIECE;
       // piece p of the (sequence, head): CTA c_first + p's first segment, unless it started before
       auto piece_of = [&](int p) {
@@ -1151,10 +1159,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           named_bar_sync(bar, 128);
           if (tid == 0) {
             int* cnt = ta.counters + (c_first * ta.rts + rt) * 2 + g;
-            __threadfence();  // the group's stores, seen through the barrier, come before the ticket
+            fence_acq_rel_gpu();  // the group's stores, seen through the barrier, come before the ticket
             const bool final_one = atomicAdd(cnt, 1) == c_last - c_first;
-            __threadfence();
-            if (final_one) *cnt = 0;
+            if (final_one) {
+              fence_acq_rel_gpu();  // and the others' pieces after it
+              *cnt = 0;
+            }
             gmax[0] = final_one ? 1.f : 0.f;
           }
           named_bar_sync(bar, 128);
