@@ -21,6 +21,7 @@ call before capturing a CUDA graph.
 """
 from __future__ import annotations
 
+import functools
 import math
 import threading
 
@@ -78,6 +79,12 @@ def reset_workspaces() -> None:
     with _ws_lock:
         for ws in _workspaces.values():
             ws.zero_()
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_bytes(index: int, b: int, t: int, hq: int, heads: int, d: int) -> int:
+    with torch.cuda.device(index):
+        return lib.bw_tree_attention_int8_workspace_size(b, t, hq, heads, d)
 
 
 def _workspace(dev: torch.device, nbytes: int) -> torch.Tensor:
@@ -486,7 +493,7 @@ def tree_attention_int8(q: torch.Tensor, cache: KVCacheInt8, table: torch.Tensor
     out = _new(shape, dt, dev)
     if b == 0 or t == 0:
         return out
-    nbytes = lib.bw_tree_attention_int8_workspace_size(b, t, hq, heads, d)
+    nbytes = _attention_bytes(dev.index, b, t, hq, heads, d)
     ws = _workspace(dev, nbytes) if nbytes else None
     _call("tree_attention_int8", dev, lib.bw_tree_attention_int8, q.data_ptr(), stride[0], stride[1], stride[2],
           DTYPE_CODE[dt], out.data_ptr(), *cache._ptrs, *cache._dims, table.data_ptr(), ld, cols, ctx_lens.data_ptr(),
