@@ -229,11 +229,16 @@ __device__ __forceinline__ uint32_t cluster_ctarank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-// All threads of all CTAs of the cluster; used once, right after barrier init,
-// when every CTA of the (co-scheduled) cluster is certain to arrive.
+// All threads of all CTAs of the cluster.  A CTA's shared memory may be written from outside only after
+// every CTA is known to run, so a kernel passes one such barrier before its first remote access;
+// cluster_arrive at its start and cluster_wait before that access hide the wait.
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // Address of the same shared-memory variable in CTA `rank` of the cluster.
 __device__ __forceinline__ uint32_t mapa_shared(uint32_t saddr, uint32_t rank) {
   uint32_t r;

@@ -100,6 +100,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(const Ve
   const int64_t b = blockIdx.x / ctas;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int threads = blockDim.x;
+  cluster_arrive();
   if (tid < a.t) {
     const int p = a.parents[b * a.t + tid];
     const int64_t x = a.tok[b * a.t + tid];
@@ -118,6 +119,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(const Ve
   const int64_t per = ((a.v + ctas - 1) / ctas + 3) / 4 * 4;
   const int64_t v0 = min(per * rank, a.v), v1 = min(v0 + per, a.v);
   __syncthreads();
+  cluster_wait();  // every CTA runs (the wait lies behind the gather): its shared memory may be written
   // What is left of four consecutive tokens' weights after the first r rejections.
   auto rest = [&](float4& w, const float4& qw, int64_t v, int r) {
     if (DRAFT) {
