@@ -66,6 +66,7 @@ __global__ void __launch_bounds__(kKvThreads) kv_quant_cluster_kernel(const __ha
   __shared__ float red[kKvThreads / 32];
   __shared__ float part[kKvMaxCluster];  // partial maxima of the cluster's CTAs
   const int cl = static_cast<int>(cluster_ctarank());
+  cluster_arrive();
   int nclus;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(nclus));
   const int64_t c = blockIdx.x / nclus;  // channel
@@ -85,6 +86,7 @@ __global__ void __launch_bounds__(kKvThreads) kv_quant_cluster_kernel(const __ha
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
   __syncthreads();
+  cluster_wait();  // every CTA runs: its shared memory may be written
   if (threadIdx.x == 0) {
     float mm = 0.f;
     for (int w = 0; w < kKvThreads / 32; ++w) mm = fmaxf(mm, red[w]);

@@ -21,7 +21,7 @@ def _body(text, name):
     return text[start:i]
 
 
-@pytest.mark.parametrize("file,kernel", [("verify.cu", "verify_tree_kernel")])
+@pytest.mark.parametrize("file,kernel", [("verify.cu", "verify_tree_kernel"), ("kv_quant.cu", "kv_quant_cluster_kernel")])
 def test_cluster_runs_before_remote_access(file, kernel):
     body = _body((CSRC / file).read_text(), kernel)
     first = re.search(REMOTE, body)
