@@ -101,6 +101,7 @@ SIGNATURES = {
     "bw_verify_tree": (_c.c_int, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _P, _P]),
     "bw_set_wait_limit_ns": (_c.c_int, [_c.c_uint64]),
     "bw_get_wait_limit_ns": (_c.c_int, [_c.POINTER(_c.c_uint64)]),
+    "bw_stream_capture_id": (_c.c_int, [_P, _c.POINTER(_c.c_uint64)]),
     "bw_trace_enable": (_c.c_int, [_P, _c.c_size_t]),
     "bw_trace_records": (_c.c_int, [_c.POINTER(_c.c_uint)]),
 }

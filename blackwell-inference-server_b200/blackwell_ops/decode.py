@@ -16,25 +16,24 @@ Slot s of sequence b is row ``s % page`` of page ``table[b, s // page]``.  A slo
 whose entry is no page of the cache, does not exist: it is not written, reads as zero and is not seen.
 
 Kernels run on torch's current stream of the inputs' device; outputs come from the caching allocator.
-Errors are ``RuntimeError``.  The attention keeps a workspace per (device, stream): make one warm-up
-call before capturing a CUDA graph.
+Errors are ``RuntimeError``.  The attention keeps a workspace per (device, stream), and one for each CUDA
+graph that it is captured into, whose replays need no warm-up call and may run on any stream.
 """
 from __future__ import annotations
 
 import functools
 import math
-import threading
 
 import torch
 
 from ._lib import DTYPE_CODE, check, lib
+from ._workspace import Workspaces
 
 MAX_NODES = 64      # nodes of a draft tree: one bit each
 MAX_HEAD_DIM = 256
 
 _HALF = (torch.float16, torch.bfloat16)
-_ws_lock = threading.Lock()
-_workspaces: dict[tuple[int, int], torch.Tensor] = {}
+_workspaces = Workspaces(zeroed=4096)  # the tickets, in a prefix of one size for every shape
 
 
 # These operators are called once a layer and step, so what a call costs on the host counts: the current
@@ -76,9 +75,7 @@ def _call(op: str, dev: torch.device, fn, *args) -> None:
 
 def reset_workspaces() -> None:
     """Zero every cached attention workspace (needed only after a device-side timeout)."""
-    with _ws_lock:
-        for ws in _workspaces.values():
-            ws.zero_()
+    _workspaces.reset()
 
 
 @functools.lru_cache(maxsize=4096)
@@ -88,13 +85,8 @@ def _attention_bytes(index: int, b: int, t: int, hq: int, heads: int, d: int) ->
 
 
 def _workspace(dev: torch.device, nbytes: int) -> torch.Tensor:
-    """Scratch of the current stream; its counters start, and stay, zero."""
-    key = (dev.index, _stream(dev.index))
-    ws = _workspaces.get(key)
-    if ws is None or ws.numel() < nbytes:
-        with _ws_lock:
-            ws = _workspaces[key] = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=dev)
-    return ws
+    """Scratch of the current stream; its tickets start, and stay, zero."""
+    return _workspaces.get(dev, _stream(dev.index), nbytes)
 
 
 # ---------------------------------------------------------------- rotary positions

@@ -163,6 +163,17 @@ extern "C" int bw_get_wait_limit_ns(uint64_t* ns) {
   return BW_OK;
 }
 
+extern "C" int bw_stream_capture_id(void* stream, uint64_t* id) {
+  using namespace bw;
+  if (!id) return fail(BW_ERR_INVALID_ARGUMENT, "stream_capture_id: null pointer");
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long n = 0;
+  if (int s = check_cuda(cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &n), "cudaStreamGetCaptureInfo"))
+    return s;
+  *id = status == cudaStreamCaptureStatusActive ? n : 0;
+  return BW_OK;
+}
+
 extern "C" int bw_trace_enable(void* buffer, size_t bytes) {
   using namespace bw;
   TraceState t = {nullptr, 0u, 0u};

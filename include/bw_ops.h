@@ -424,6 +424,12 @@ int bw_set_wait_limit_ns(uint64_t ns);
 int bw_get_wait_limit_ns(uint64_t* ns);
 
 /*
+ * *id = 0, or the id of the capture that `stream` is part of (unique in the process).  A CUDA graph keeps
+ * the workspaces it was captured with: give each capture its own, and clear what has to be zero inside it.
+ */
+int bw_stream_capture_id(void* stream, uint64_t* id);
+
+/*
  * Device-side phase trace for the current device (no reference counterpart;
  * the reference profiles with torch.profiler).  While a buffer is set, each
  * CTA of a traced kernel claims one 128-byte record
