@@ -38,7 +38,7 @@ class Workspaces:
     def __init__(self, zeroed: int | None = None):
         self._zeroed = zeroed
         self._lock = threading.Lock()
-        self._eager: dict[tuple[int, int], torch.Tensor] = {}
+        self.eager: dict[tuple[int, int], torch.Tensor] = {}
         self._captured: dict[tuple[int, int], tuple[int, torch.Tensor]] = {}
 
     def get(self, dev: torch.device, stream: int, nbytes: int) -> torch.Tensor:
@@ -47,10 +47,10 @@ class Workspaces:
         key = (index, stream)
         capture = capture_id(index, stream)
         if not capture:
-            ws = self._eager.get(key)
+            ws = self.eager.get(key)
             if ws is None or ws.numel() < nbytes:
                 with self._lock:
-                    ws = self._eager[key] = torch.zeros(max(nbytes, _LEAST), dtype=torch.uint8, device=dev)
+                    ws = self.eager[key] = torch.zeros(max(nbytes, _LEAST), dtype=torch.uint8, device=dev)
             return ws
         with self._lock:
             last, ws = self._captured.get(key, (0, None))
@@ -63,5 +63,5 @@ class Workspaces:
     def reset(self) -> None:
         """Zero every workspace outside graphs (a graph clears its own)."""
         with self._lock:
-            for ws in self._eager.values():
+            for ws in self.eager.values():
                 ws.zero_()

@@ -10,39 +10,28 @@ Drop-in for ``src/blackwell_ops/kernels/int8_gemm.py`` of the reference:
 
 Both run on torch's current CUDA stream and allocate outputs with the caching
 allocator, as the reference does.  Split-K scratch is a per-(device, stream)
-workspace kept by this module; make one warm-up call before capturing a CUDA
-graph so the workspace exists.
+workspace kept by this module, and one for each CUDA graph that calls are
+captured into, whose replays may run on any stream.
 """
 from __future__ import annotations
-
-import threading
 
 import torch
 
 from .._lib import DTYPE_CODE, check, lib, stream_ptr
+from .._workspace import Workspaces
 
-_ws_lock = threading.Lock()
-_workspaces: dict[tuple[int, int], torch.Tensor] = {}
+_scratch = Workspaces(zeroed=4096)  # the counters, in a prefix of one size for every shape
+_workspaces = _scratch.eager  # those outside graphs
 
 
 def _workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor | None:
-    """Per-(device, stream) split-K workspace; counters start (and stay) zero."""
-    if nbytes == 0:
-        return None
-    key = (device.index if device.index is not None else torch.cuda.current_device(), stream)
-    with _ws_lock:
-        ws = _workspaces.get(key)
-        if ws is None or ws.numel() < nbytes:
-            ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
-            _workspaces[key] = ws
-        return ws
+    """Split-K workspace of a call on ``stream``; counters start (and stay) zero."""
+    return _scratch.get(device, stream, nbytes) if nbytes else None
 
 
 def reset_workspaces() -> None:
     """Zero every cached workspace (needed only after a device-side timeout)."""
-    with _ws_lock:
-        for ws in _workspaces.values():
-            ws.zero_()
+    _scratch.reset()
 
 
 def quantize_weight_int8(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:

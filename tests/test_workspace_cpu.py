@@ -10,7 +10,7 @@ DEV = torch.device("cpu", 0)
 
 
 class Stream:
-    handle, capture = 7, 0
+    handle, capture = 7, 0  # of the class: one stream at a time
 
 
 def _attention(n):
@@ -19,11 +19,19 @@ def _attention(n):
     return decode._workspace(DEV, n)
 
 
+def _gemm(n):
+    from blackwell_ops.kernels import int8_gemm as _  # noqa: F401  (the operator; its module holds the workspaces)
+    import sys
+
+    return sys.modules["blackwell_ops.kernels.int8_gemm"]._workspace(DEV, Stream.handle, n)
+
+
 @pytest.fixture
 def stream(monkeypatch):
     from blackwell_ops import _lib, decode
 
-    s = Stream()
+    s = Stream
+    s.handle, s.capture = 7, 0
 
     def info(handle, out):
         out._obj.value = s.capture
@@ -36,7 +44,7 @@ def stream(monkeypatch):
     yield s
 
 
-@pytest.mark.parametrize("get", [_attention])
+@pytest.mark.parametrize("get", [_attention, _gemm])
 def test_a_capture_has_its_own(stream, get):
     eager = get(3 << 20)
     assert not eager.any() and get(1 << 20) is eager
@@ -54,7 +62,7 @@ def test_a_capture_has_its_own(stream, get):
     assert get(2 << 20) is eager
 
 
-@pytest.mark.parametrize("get", [_attention])
+@pytest.mark.parametrize("get", [_attention, _gemm])
 def test_growth_leaves_a_graphs_memory_alone(stream, get):
     stream.capture = 51
     held = weakref.ref(get(2 << 20))
@@ -64,7 +72,7 @@ def test_growth_leaves_a_graphs_memory_alone(stream, get):
     assert big.numel() >= 20 << 20 and not big.any()
 
 
-@pytest.mark.parametrize("get,zeroed", [(_attention, 4096)])
+@pytest.mark.parametrize("get,zeroed", [(_attention, 4096), (_gemm, 4096)])
 def test_what_a_capture_clears(stream, get, zeroed, monkeypatch):
     """The words that have to be zero are cleared by the capture itself (so by each replay), the rest is not."""
     stream.capture = 61
