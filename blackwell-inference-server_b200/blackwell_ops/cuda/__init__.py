@@ -24,32 +24,26 @@ from __future__ import annotations
 import torch
 
 from .._lib import RequantProblem, check, lib, stream_ptr
+from .._workspace import Workspaces
 
-_ws: dict[tuple[int, int], torch.Tensor] = {}
+_scratch = Workspaces()
 
 
 def _workspace(device: torch.device, nbytes: int) -> torch.Tensor | None:
-    """Requantisation scratch (grid barrier + two sets of row maxima) per (device, stream).
+    """Requantisation scratch (grid barrier + two sets of row maxima) of a call on the current stream.
 
-    Zeroed once at allocation and always passed with its full size: each call
-    clears the set of row maxima the next call uses.  A larger need replaces it
-    with a new zeroed buffer.
+    Zeroed at allocation (in a CUDA graph, which has its own, by each replay)
+    and always passed with its full size: each call clears the set of row
+    maxima the next call uses.  A larger need replaces it with a new zeroed
+    buffer.
     """
-    if nbytes == 0:
-        return None
-    key = (device.index if device.index is not None else torch.cuda.current_device(), stream_ptr(device))
-    ws = _ws.get(key)
-    if ws is None or ws.numel() < nbytes:
-        ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
-        _ws[key] = ws
-    return ws
+    return _scratch.get(device, stream_ptr(device), nbytes) if nbytes else None
 
 
 def reset_workspaces() -> None:
     """Zero every cached requantisation workspace (needed only after a device-side timeout, which
     can leave a grid barrier or a set of row maxima mid-way)."""
-    for ws in _ws.values():
-        ws.zero_()
+    _scratch.reset()
 
 
 def _check_ab(A: torch.Tensor, B: torch.Tensor) -> tuple[int, int, int]:

@@ -26,9 +26,15 @@ def _gemm(n):
     return sys.modules["blackwell_ops.kernels.int8_gemm"]._workspace(DEV, Stream.handle, n)
 
 
+def _requant(n):
+    from blackwell_ops import cuda
+
+    return cuda._workspace(DEV, n)
+
+
 @pytest.fixture
 def stream(monkeypatch):
-    from blackwell_ops import _lib, decode
+    from blackwell_ops import _lib, cuda, decode
 
     s = Stream
     s.handle, s.capture = 7, 0
@@ -41,10 +47,11 @@ def stream(monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: s.capture != 0)
     monkeypatch.setattr(_lib.lib, "bw_stream_capture_id", info, raising=False)
     monkeypatch.setattr(decode, "_stream", lambda index: s.handle)
+    monkeypatch.setattr(cuda, "stream_ptr", lambda dev: s.handle)
     yield s
 
 
-@pytest.mark.parametrize("get", [_attention, _gemm])
+@pytest.mark.parametrize("get", [_attention, _gemm, _requant])
 def test_a_capture_has_its_own(stream, get):
     eager = get(3 << 20)
     assert not eager.any() and get(1 << 20) is eager
@@ -62,7 +69,7 @@ def test_a_capture_has_its_own(stream, get):
     assert get(2 << 20) is eager
 
 
-@pytest.mark.parametrize("get", [_attention, _gemm])
+@pytest.mark.parametrize("get", [_attention, _gemm, _requant])
 def test_growth_leaves_a_graphs_memory_alone(stream, get):
     stream.capture = 51
     held = weakref.ref(get(2 << 20))
@@ -72,14 +79,14 @@ def test_growth_leaves_a_graphs_memory_alone(stream, get):
     assert big.numel() >= 20 << 20 and not big.any()
 
 
-@pytest.mark.parametrize("get,zeroed", [(_attention, 4096), (_gemm, 4096)])
+@pytest.mark.parametrize("get,zeroed", [(_attention, 4096), (_gemm, 4096), (_requant, None)])
 def test_what_a_capture_clears(stream, get, zeroed, monkeypatch):
-    """The words that have to be zero are cleared by the capture itself (so by each replay), the rest is not."""
+    """The words that have to be zero are cleared by the capture itself (so by each replay); None: all of them."""
     stream.capture = 61
     empty = torch.empty
     monkeypatch.setattr(torch, "empty", lambda *a, **k: empty(*a, **k).fill_(7))
     ws = get(2 << 20)
-    assert not ws[:zeroed].any() and bool((ws[zeroed:] == 7).all())
+    assert not ws[:zeroed].any() and (zeroed is None or bool((ws[zeroed:] == 7).all()))
 
 
 def test_capture_id_refusal():
