@@ -508,7 +508,8 @@ def verify_tree(target_probs: torch.Tensor, tokens: torch.Tensor, parents: torch
     From the root, with w = target and Z = 1, a node's children are tried in index order: child i
     with token x is taken if ``u_i * draft(x) * Z < w(x)``, else ``w = max(w - Z * draft, 0)`` (without
     drafts' distribution draft(x) = 1 and w(x) = 0) and ``Z = sum(w)``.  Where no child is taken the
-    last token is ``argmax(w / e)``, ties to the lowest.
+    last token is ``argmax(w / e)``, ties to the lowest.  Z is summed in one order for every B, so a
+    sequence's tokens do not depend on its batch.
 
     Returns ``n`` [B] int32 accepted nodes, ``path`` [B, T] int32 (the nodes, then -1) and ``out`` [B, T]
     int64 (their tokens, the last token, then -1)."""

@@ -9,7 +9,8 @@
 // cumulative sum.  Ties go to the lowest token; an empty residual falls back to p_c.
 //
 // Every product, difference and quotient is rounded separately in fp32 (no contraction); only Z
-// depends on a summation order, and only from a second sibling on.
+// depends on a summation order, and only from a second sibling on.  That order is the same for every
+// number of sequences and of CTAs, so a sequence's tokens do not depend on its batch.
 #include <stdio.h>
 
 #include <mutex>
@@ -58,21 +59,21 @@ __device__ __forceinline__ float approx_inverse(float x) {
 }
 constexpr float kTrustLow = 0x1p-60f, kTrustHigh = 0x1p60f;
 
-// One value of each CTA of the cluster into all of them, in the CTAs' order; `slot`s are not reused before
-// every CTA has passed another exchange.
+// A value of this CTA into slot `at` of all CTAs of the cluster, which have it after the next cluster_sync_all;
+// slots are not reused before every CTA has passed another one.
 template <typename V>
-__device__ __forceinline__ void cluster_share(V (*slot)[kVerifyCluster], V v, int rank, int ctas) {
+__device__ __forceinline__ void cluster_share(V (*slot)[kVerifyCluster], V v, int index, int ctas) {
   if (threadIdx.x < ctas) {
-    const uint32_t at = mapa_shared(smem_u32(&(*slot)[rank]), threadIdx.x);
+    const uint32_t at = mapa_shared(smem_u32(&(*slot)[index]), threadIdx.x);
     if constexpr (sizeof(V) == 8)
       asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(at), "l"(v) : "memory");
     else
       asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(at), "r"(__float_as_uint(v)) : "memory");
   }
-  cluster_sync_all();
 }
 
-// One cluster per sequence, each CTA a part of the vocabulary.  Every CTA walks the tree on its own: the
+// One cluster per sequence.  A row is cut into sixteen parts whatever the cluster's size, a warp's step to each
+// in turn (so that all end together); a CTA has one part, or two neighbouring ones.  Every CTA walks the tree on its own: the
 // probabilities of all drafted tokens at their parents are gathered at once, so a walk without a rejected
 // sibling before another one reads nothing more, and only then is Z summed over the row (cluster-wide, in
 // one order).  The token at the end takes one pass over the row's p, q and e.
@@ -90,7 +91,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(const Ve
   __shared__ int64_t dropped[kTreeMaxNodes];
   __shared__ float pv[kTreeMaxNodes], qv[kTreeMaxNodes], uv[kTreeMaxNodes];
   __shared__ float z[kTreeMaxNodes + 1];
-  __shared__ float red[kVerifyThreads / 32];
+  __shared__ float red[2][kVerifyThreads / 32];
   __shared__ unsigned long long redk[kVerifyThreads / 32];
   __shared__ float sums[2][kVerifyCluster];
   __shared__ unsigned long long keys[2][kVerifyCluster];
@@ -100,6 +101,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(const Ve
   const int64_t b = blockIdx.x / ctas;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int threads = blockDim.x;
+  const int two = ctas < kVerifyCluster;  // parts of this CTA, less one
   cluster_arrive();
   if (tid < a.t) {
     const int p = a.parents[b * a.t + tid];
@@ -115,9 +117,12 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(const Ve
     z[0] = 1.f;
   }
   if (tid < 4) walk[tid] = tid == 3 ? 1 : 0;
-  // this CTA's part of a row, whole groups of four
-  const int64_t per = ((a.v + ctas - 1) / ctas + 3) / 4 * 4;
-  const int64_t v0 = min(per * rank, a.v), v1 = min(v0 + per, a.v);
+  // the first token of this thread's k-th group of four (of its k-th token): k goes through the CTA's parts in turn
+  const int group0 = warp * (32 * kVerifyCluster) + (rank << two) * 32 + lane;
+  auto token = [&](int k) {
+    const int64_t group = static_cast<int64_t>(k >> two) * (threads * kVerifyCluster) + (group0 + (k & two) * 32);
+    return group * (VEC ? 4 : 1);
+  };
   __syncthreads();
   cluster_wait();  // every CTA runs (the wait lies behind the gather): its shared memory may be written
   // What is left of four consecutive tokens' weights after the first r rejections.
@@ -140,15 +145,15 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(const Ve
       }
     }
   };
-  // f(four tokens of p, of q and of e, or zeros where a row is not given; the first of them) over this
-  // thread's part, in order.  Each thread copies its own groups to shared memory, kVerifyStages steps ahead
+  // f(four tokens of p, of q and of e, or zeros where a row is not given; the first of them; which of the
+  // CTA's parts) over this thread's tokens, in order.  Each thread copies its own groups to shared memory, kVerifyStages steps ahead
   // (in registers they would be too few to cover the latency); rows that are no groups of four go one by one.
   auto each = [&](const float* pr, const float* qr, const float* er, auto f) {
     const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
     if constexpr (VEC) {
-      const int step = threads * 4;
-      auto fetch = [&](int64_t v, int stage) {
-        if (v < v1) {
+      auto fetch = [&](int k, int stage) {
+        const int64_t v = token(k);
+        if (v < a.v) {
           float4* to = stages + stage * 3 * threads + tid;
           copy16_async(to, pr + v);
           if (qr != nullptr) copy16_async(to + threads, qr + v);
@@ -157,26 +162,27 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(const Ve
         asm volatile("cp.async.commit_group;" ::: "memory");
       };
 #pragma unroll 1
-      for (int k = 0; k < kVerifyStages; ++k) fetch(v0 + tid * 4 + static_cast<int64_t>(k) * step, k);
-      int stage = 0;
+      for (int k = 0; k < kVerifyStages; ++k) fetch(k, k);
+      int stage = 0, k = 0;
 #pragma unroll 1
-      for (int64_t v = v0 + tid * 4; v < v1; v += step) {
+      for (int64_t v = token(0); v < a.v; v = token(++k)) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kVerifyStages - 1) : "memory");
         const float4* from = stages + stage * 3 * threads + tid;
         const float4 w = from[0];
         const float4 qw = qr != nullptr ? from[threads] : none;
         const float4 ew = er != nullptr ? from[2 * threads] : none;
-        f(w, qw, ew, v);
-        fetch(v + static_cast<int64_t>(kVerifyStages) * step, stage);
+        f(w, qw, ew, v, k & two);
+        fetch(k + kVerifyStages, stage);
         stage = stage + 1 == kVerifyStages ? 0 : stage + 1;
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
+      int k = 0;
 #pragma unroll 2
-      for (int64_t v = v0 + tid; v < v1; v += threads) {
+      for (int64_t v = token(0); v < a.v; v = token(++k)) {
         const float4 qw = make_float4(qr != nullptr ? __ldg(qr + v) : 0.f, 0.f, 0.f, 0.f);
         const float4 ew = make_float4(er != nullptr ? __ldg(er + v) : 0.f, 0.f, 0.f, 0.f);
-        f(make_float4(__ldg(pr + v), 0.f, 0.f, 0.f), qw, ew, v);
+        f(make_float4(__ldg(pr + v), 0.f, 0.f, 0.f), qw, ew, v, k & two);
       }
     }
   };
@@ -220,20 +226,28 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(const Ve
     const int cur = walk[0], r = walk[1];
     const float* p = a.p + (b * a.t + cur) * a.v;
     const float* q = DRAFT ? a.q + (b * a.t + cur) * a.v : nullptr;
-    float sum = 0.f;
-    each(p, q, nullptr, [&](float4 w, const float4& qw, const float4&, int64_t v) {
+    float sum[2] = {0.f, 0.f};
+    each(p, q, nullptr, [&](float4 w, const float4& qw, const float4&, int64_t v, int part) {
       rest(w, qw, v, r);
-      sum += (w.x + w.y) + (w.z + w.w);
+      const float s = (w.x + w.y) + (w.z + w.w);
+      if (part) sum[1] += s;
+      else sum[0] += s;
     });
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) red[warp] = sum;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      for (int o = 16; o > 0; o >>= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
+      if (lane == 0) red[i][warp] = sum[i];
+    }
     __syncthreads();
-    sum = 0.f;
-    for (int k = 0; k < threads / 32; ++k) sum += red[k];
-    cluster_share(&sums[phase & 1], sum, rank, ctas);
+    for (int i = 0; i <= two; ++i) {
+      float s = 0.f;
+      for (int k = 0; k < threads / 32; ++k) s += red[i][k];
+      cluster_share(&sums[phase & 1], s, (rank << two) + i, ctas);
+    }
+    cluster_sync_all();
     if (tid == 0) {
       float s = 0.f;
-      for (int k = 0; k < ctas; ++k) s += sums[phase & 1][k];
+      for (int k = 0; k < kVerifyCluster; ++k) s += sums[phase & 1][k];
       z[r] = s;
     }
     ++phase;
@@ -256,7 +270,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(const Ve
     };
     const int rr = pass == 0 ? r : 0;
     auto scores = [&](auto f) {  // f(w, e, token)
-      each(p, rr > 0 ? q : nullptr, e, [&](float4 w, const float4& qw, const float4& ew, int64_t v) {
+      each(p, rr > 0 ? q : nullptr, e, [&](float4 w, const float4& qw, const float4& ew, int64_t v, int) {
         rest(w, qw, v, rr);
         f(w.x, ew.x, static_cast<int>(v));
         if (VEC) {
@@ -287,9 +301,9 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(const Ve
     });
     float most = top;
     for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    if (lane == 0) red[warp] = most;
+    if (lane == 0) red[0][warp] = most;
     const bool odd = __syncthreads_or(!(e_min >= kTrustLow && e_max <= kTrustHigh));
-    for (int k = 0; k < threads / 32; ++k) most = fmaxf(most, red[k]);
+    for (int k = 0; k < threads / 32; ++k) most = fmaxf(most, red[0][k]);
     const float near = most * (1.f - 0x1p-20f);
     if (odd || !(most >= kTrustLow && most <= kTrustHigh) || second >= near)
       scores(score);
@@ -304,6 +318,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(const Ve
     best = 0;
     for (int k = 0; k < threads / 32; ++k) best = redk[k] > best ? redk[k] : best;
     cluster_share(&keys[pass], best, rank, ctas);
+    cluster_sync_all();
     best = 0;
     for (int k = 0; k < ctas; ++k) best = keys[pass][k] > best ? keys[pass][k] : best;
     if (best == 0 && pass == 0) continue;

@@ -398,6 +398,8 @@ int bw_tree_attention_int8(const void* q, int64_t q_sb, int64_t q_st, int64_t q_
  * [0, 1) and sample_e exponential the tokens are distributed as the target's own.
  *   n_accepted [b]; path [b, t]: accepted nodes, then -1; out_tokens [b, t]: their tokens, the last
  *   token, then -1.  A drafted token outside [0, v) is never taken.  t <= 64.
+ * Z is summed in one order for every b: a sequence's tokens do not depend on what it is batched with.
+ * (Rows that start on 16-byte groups are summed in another order than rows that do not.)
  */
 int bw_verify_tree(const float* target, const float* draft, const int64_t* tokens, const int32_t* parents,
                    const float* accept_u, const float* sample_e, int64_t b, int64_t t, int64_t v,
