@@ -93,7 +93,7 @@ class TreeSpeculativeDecoder:
         the committed tokens.  The nodes' keys and values go to slots ``ctx`` on; nothing is committed."""
         from blackwell_ops.cuda import rmsnorm
         from blackwell_ops.decode import rotary_kv_write_int8, tree_attention_int8, tree_positions
-        from blackwell_ops.kernels.int8_gemm import int8_gemm, int8_gemm_grouped, int8_gemm_swiglu
+        from blackwell_ops.kernels.int8_gemm import int8_gemm_grouped
 
         b, t = tokens.shape
         mask = None
@@ -116,12 +116,20 @@ class TreeSpeculativeDecoder:
             o = tree_attention_int8(q, cache, self.table, self.ctx, mask, softmax_scale=att.scaling)
             x = x + att.o_proj(o.view(b * t, -1))
             y = rmsnorm(x, layer.post_attention_layernorm.weight, layer.post_attention_layernorm.variance_epsilon)
-            (wg, sg), (wu, su), (wd, sd) = (p.copies[p.active] for p in (mlp.gate_proj, mlp.up_proj, mlp.down_proj))
-            x = x + int8_gemm(int8_gemm_swiglu(y, wg, sg, wu, su), wd, sd)
+            x = x + self._mlp(mlp, y)
         if not logits:
             return None
         norm = self.model.base.model.norm
         return self.model.base.lm_head(rmsnorm(x, norm.weight, norm.variance_epsilon)).view(b, t, -1)
+
+    def _mlp(self, mlp, y: torch.Tensor) -> torch.Tensor:
+        from blackwell_ops.kernels.int8_gemm import int8_gemm, int8_gemm_swiglu
+
+        proj = (mlp.gate_proj, mlp.up_proj, mlp.down_proj)
+        if any(p.bias is not None for p in proj):
+            return mlp.down_proj(torch.nn.functional.silu(mlp.gate_proj(y)) * mlp.up_proj(y))
+        (wg, sg), (wu, su), (wd, sd) = (p.copies[p.active] for p in proj)
+        return int8_gemm(int8_gemm_swiglu(y, wg, sg, wu, su), wd, sd)
 
     def _head_norm(self, x: torch.Tensor, norm) -> torch.Tensor:
         """Qwen3 normalises each head of q and k."""
