@@ -73,6 +73,7 @@ class TreeSpeculativeDecoder:
         cfg = model.base.config
         self.head_dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads
         self.heads, self.kv_heads = cfg.num_attention_heads, cfg.num_key_value_heads
+        self.swiglu = getattr(cfg, "hidden_act", None) in ("silu", "swish")  # what the fused gate and up product computes
         self.layers = model.base.model.layers
         self.dev = next(model.base.parameters()).device
         rope = dict(getattr(cfg, "rope_parameters", None) or {})
@@ -126,8 +127,8 @@ class TreeSpeculativeDecoder:
         from blackwell_ops.kernels.int8_gemm import int8_gemm, int8_gemm_swiglu
 
         proj = (mlp.gate_proj, mlp.up_proj, mlp.down_proj)
-        if any(p.bias is not None for p in proj):
-            return mlp.down_proj(torch.nn.functional.silu(mlp.gate_proj(y)) * mlp.up_proj(y))
+        if not self.swiglu or any(p.bias is not None for p in proj):
+            return mlp.down_proj(mlp.act_fn(mlp.gate_proj(y)) * mlp.up_proj(y))
         (wg, sg), (wu, su), (wd, sd) = (p.copies[p.active] for p in proj)
         return int8_gemm(int8_gemm_swiglu(y, wg, sg, wu, su), wd, sd)
 

@@ -70,3 +70,12 @@ def test_mlp_and_attention_biases(cuda_dev):
         layer.mlp.gate_proj.bias = layer.mlp.up_proj.bias = layer.mlp.down_proj.bias = None
     with torch.no_grad():
         assert _rel(twin(input_ids=ids).logits[:, 30:], want) > 0.1  # the biases matter
+
+
+@pytest.mark.parametrize("act", ["gelu", "relu"])
+def test_other_activations(cuda_dev, act):
+    mdl, twin, ids, want = _check(transformers.LlamaConfig(**SMALL, hidden_act=act), cuda_dev)
+    for layer in twin.model.layers:
+        layer.mlp.act_fn = torch.nn.SiLU()
+    with torch.no_grad():
+        assert _rel(twin(input_ids=ids).logits[:, 30:], want) > 0.05  # the activation matters
