@@ -21,7 +21,7 @@ from __future__ import annotations
 
 import torch
 
-from .lora.delta_multi import MultiDeltaLoRAModel
+from .lora.delta_multi import MultiDeltaLoRAModel, W8A16Linear
 
 
 def lookup_tree(tokens: list[int], nodes: int, branches: int = 4, ngram: int = 3) -> tuple[list[int], list[int]]:
@@ -56,6 +56,11 @@ def lookup_tree(tokens: list[int], nodes: int, branches: int = 4, ngram: int = 3
         if found:
             break
     return out, parents
+
+
+def _fusable(projections) -> bool:
+    """int8 copies and nothing else to add: one launch can take them together."""
+    return all(isinstance(p, W8A16Linear) and p.bias is None for p in projections)
 
 
 class TreeSpeculativeDecoder:
@@ -107,10 +112,10 @@ class TreeSpeculativeDecoder:
             att, mlp = layer.self_attn, layer.mlp
             y = rmsnorm(x, layer.input_layernorm.weight, layer.input_layernorm.variance_epsilon)
             proj = (att.q_proj, att.k_proj, att.v_proj)
-            if any(p.bias is not None for p in proj):
-                q, k, v = (p(y) for p in proj)
-            else:
+            if _fusable(proj):
                 q, k, v = int8_gemm_grouped(y, [p.copies[p.active] for p in proj])
+            else:
+                q, k, v = (p(y) for p in proj)
             q, k = self._head_norm(q, getattr(att, "q_norm", None)), self._head_norm(k, getattr(att, "k_norm", None))
             shape = (b, t, -1, self.head_dim)
             q = rotary_kv_write_int8(q.view(shape), k.view(shape), v.view(shape), pos, self.plan, cache, self.table, self.ctx)
@@ -127,7 +132,7 @@ class TreeSpeculativeDecoder:
         from blackwell_ops.kernels.int8_gemm import int8_gemm, int8_gemm_swiglu
 
         proj = (mlp.gate_proj, mlp.up_proj, mlp.down_proj)
-        if not self.swiglu or any(p.bias is not None for p in proj):
+        if not self.swiglu or not _fusable(proj):
             return mlp.down_proj(mlp.act_fn(mlp.gate_proj(y)) * mlp.up_proj(y))
         (wg, sg), (wu, su), (wd, sd) = (p.copies[p.active] for p in proj)
         return int8_gemm(int8_gemm_swiglu(y, wg, sg, wu, su), wd, sd)

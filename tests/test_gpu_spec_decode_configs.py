@@ -79,3 +79,9 @@ def test_other_activations(cuda_dev, act):
         layer.mlp.act_fn = torch.nn.SiLU()
     with torch.no_grad():
         assert _rel(twin(input_ids=ids).logits[:, 30:], want) > 0.05  # the activation matters
+
+
+@pytest.mark.parametrize("targets", [("q_proj", "k_proj", "v_proj", "o_proj"), ("q_proj", "up_proj")])
+def test_registry_of_some_projections(cuda_dev, targets):
+    """The projections that the registry does not hold stay the model's own fp16 linears."""
+    _check(transformers.Qwen3Config(**SMALL), cuda_dev, targets=targets)
