@@ -63,8 +63,23 @@ def _fusable(projections) -> bool:
     return all(isinstance(p, W8A16Linear) and p.bias is None for p in projections)
 
 
+def _check_attention(cfg, positions: int) -> None:
+    """Every layer attends to all of its sequence, or to a window that no position leaves."""
+    window = getattr(cfg, "sliding_window", None)
+    if not getattr(cfg, "use_sliding_window", True):
+        window = None
+    kinds = set(getattr(cfg, "layer_types", None) or (["full_attention"] if window is None else ["sliding_attention"]))
+    for kind in sorted(kinds - {"full_attention", "sliding_attention"}):
+        raise RuntimeError(f"layers of {kind} are not supported")
+    if "sliding_attention" in kinds and (window is None or window < positions):
+        raise RuntimeError(f"a window of {window} tokens is shorter than max_len and the nodes of a step, {positions}: not supported")
+
+
 class TreeSpeculativeDecoder:
-    """Decodes ``batch`` sequences of at most ``max_len`` tokens, ``nodes`` tree nodes a step (1: plain decoding)."""
+    """Decodes ``batch`` sequences of at most ``max_len`` tokens, ``nodes`` tree nodes a step (1: plain decoding).
+
+    Takes models whose layers are the module's heading's; attention windows shorter than ``max_len + nodes`` are
+    refused."""
 
     def __init__(self, model: MultiDeltaLoRAModel, batch: int, max_len: int, nodes: int = 16, page: int = 64):
         from blackwell_ops.decode import MAX_NODES, KVCacheInt8, rotary_plan
@@ -76,6 +91,7 @@ class TreeSpeculativeDecoder:
         self.model, self.batch, self.nodes = model, batch, nodes
         self.max_len = max_len
         cfg = model.base.config
+        _check_attention(cfg, max_len + nodes)
         self.head_dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads
         self.heads, self.kv_heads = cfg.num_attention_heads, cfg.num_key_value_heads
         self.swiglu = getattr(cfg, "hidden_act", None) in ("silu", "swish")  # what the fused gate and up product computes

@@ -85,3 +85,8 @@ def test_other_activations(cuda_dev, act):
 def test_registry_of_some_projections(cuda_dev, targets):
     """The projections that the registry does not hold stay the model's own fp16 linears."""
     _check(transformers.Qwen3Config(**SMALL), cuda_dev, targets=targets)
+
+
+def test_window_longer_than_the_text(cuda_dev):
+    """A window that no token of max_len leaves changes nothing."""
+    _check(transformers.MistralConfig(**SMALL, sliding_window=64), cuda_dev)
