@@ -75,6 +75,15 @@ def _check_attention(cfg, positions: int) -> None:
         raise RuntimeError(f"a window of {window} tokens is shorter than max_len and the nodes of a step, {positions}: not supported")
 
 
+def _rope(cfg) -> dict:
+    """The model's rotation as ``rotary_plan`` takes it."""
+    rope = dict(getattr(cfg, "rope_parameters", None) or {})
+    for part in (rope.get("partial_rotary_factor"), getattr(cfg, "partial_rotary_factor", None)):
+        if part is not None and part != 1:
+            raise RuntimeError(f"partial_rotary_factor {part}: heads that turn in part are not supported")
+    return rope
+
+
 class TreeSpeculativeDecoder:
     """Decodes ``batch`` sequences of at most ``max_len`` tokens, ``nodes`` tree nodes a step (1: plain decoding).
 
@@ -92,12 +101,12 @@ class TreeSpeculativeDecoder:
         self.max_len = max_len
         cfg = model.base.config
         _check_attention(cfg, max_len + nodes)
+        rope = _rope(cfg)
         self.head_dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads
         self.heads, self.kv_heads = cfg.num_attention_heads, cfg.num_key_value_heads
         self.swiglu = getattr(cfg, "hidden_act", None) in ("silu", "swish")  # what the fused gate and up product computes
         self.layers = model.base.model.layers
         self.dev = next(model.base.parameters()).device
-        rope = dict(getattr(cfg, "rope_parameters", None) or {})
         base = float(rope.get("rope_theta", getattr(cfg, "rope_theta", 10000.0)))
         self.plan = rotary_plan(self.head_dim, base, rope, device=self.dev)
         per = -(-(max_len + nodes) // page)

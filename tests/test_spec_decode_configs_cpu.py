@@ -53,3 +53,15 @@ def test_other_kinds_of_attention_are_refused():
     cfg.layer_types = ["full_attention", "chunked_attention"]
     with pytest.raises(RuntimeError, match="chunked_attention"):
         _decoder(cfg)
+
+
+def test_partial_rotation_is_refused():
+    cfg = transformers.LlamaConfig(**SMALL)
+    cfg.rope_parameters = {"rope_type": "default", "rope_theta": 1e4, "partial_rotary_factor": 0.5}
+    with pytest.raises(RuntimeError, match="partial_rotary_factor"):
+        _decoder(cfg)
+    cfg.rope_parameters = {"rope_type": "default", "rope_theta": 1e4, "partial_rotary_factor": 1.0}
+    assert _decoder(cfg)
+    cfg.partial_rotary_factor = 0.25  # where older configurations keep it
+    with pytest.raises(RuntimeError, match="partial_rotary_factor"):
+        _decoder(cfg)
