@@ -76,8 +76,10 @@ def _check_attention(cfg, positions: int) -> None:
 
 
 def _rope(cfg) -> dict:
-    """The model's rotation as ``rotary_plan`` takes it."""
-    rope = dict(getattr(cfg, "rope_parameters", None) or {})
+    """The model's rotation as ``rotary_plan`` takes it, with its ``rope_theta``: ``rope_parameters``, or the attributes
+    ``rope_scaling`` and ``rope_theta`` of older configurations."""
+    rope = dict(getattr(cfg, "rope_parameters", None) or getattr(cfg, "rope_scaling", None) or {})
+    rope.setdefault("rope_theta", getattr(cfg, "rope_theta", 10000.0))
     for part in (rope.get("partial_rotary_factor"), getattr(cfg, "partial_rotary_factor", None)):
         if part is not None and part != 1:
             raise RuntimeError(f"partial_rotary_factor {part}: heads that turn in part are not supported")
@@ -107,8 +109,7 @@ class TreeSpeculativeDecoder:
         self.swiglu = getattr(cfg, "hidden_act", None) in ("silu", "swish")  # what the fused gate and up product computes
         self.layers = model.base.model.layers
         self.dev = next(model.base.parameters()).device
-        base = float(rope.get("rope_theta", getattr(cfg, "rope_theta", 10000.0)))
-        self.plan = rotary_plan(self.head_dim, base, rope, device=self.dev)
+        self.plan = rotary_plan(self.head_dim, float(rope["rope_theta"]), rope, device=self.dev)
         per = -(-(max_len + nodes) // page)
         self.cache = KVCacheInt8.empty(batch * per, self.kv_heads, page, self.head_dim, len(self.layers), self.dev)
         self._layer_cache = [self.cache.layer(i) for i in range(len(self.layers))]

@@ -65,3 +65,49 @@ def test_partial_rotation_is_refused():
     cfg.partial_rotary_factor = 0.25  # where older configurations keep it
     with pytest.raises(RuntimeError, match="partial_rotary_factor"):
         _decoder(cfg)
+
+
+def _rotation(cfg, monkeypatch):
+    """What the decoder asks rotary_plan for: (frequencies, magnitude)."""
+    from blackwell_inference.spec_decode import TreeSpeculativeDecoder
+    from blackwell_ops import decode
+
+    asked = []
+
+    class Reached(Exception):
+        pass
+
+    def plan(rot_dim, base=10000.0, scaling=None, interleaved=False, device=None):
+        asked.append(decode.rotary_frequencies(rot_dim, base, scaling))
+        raise Reached
+
+    monkeypatch.setattr(decode, "rotary_plan", plan)
+    base = types.SimpleNamespace(config=cfg, model=types.SimpleNamespace(layers=[]), parameters=lambda: iter([torch.zeros(1)]))
+    with pytest.raises(Reached):
+        TreeSpeculativeDecoder(types.SimpleNamespace(quantize=True, base=base), 1, 100)
+    return asked[0]
+
+
+LLAMA3 = {"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0,
+          "original_max_position_embeddings": 1024}
+
+
+@pytest.mark.parametrize("scaling", [None, LLAMA3, {"type": "linear", "factor": 4.0}])
+def test_configurations_that_carry_rope_scaling(scaling, monkeypatch):
+    """Theta and scaling as attributes of their own, without rope_parameters."""
+    from blackwell_ops.decode import rotary_frequencies
+
+    cfg = types.SimpleNamespace(model_type="llama", hidden_size=256, num_attention_heads=4, num_key_value_heads=2,
+                                hidden_act="silu", rope_theta=500000.0, rope_scaling=scaling)
+    got, want = _rotation(cfg, monkeypatch), rotary_frequencies(64, 500000.0, scaling)
+    assert torch.equal(got[0], want[0]) and got[1] == want[1]
+
+
+@pytest.mark.parametrize("scaling", [{"rope_type": "default"}, LLAMA3, {"rope_type": "linear", "factor": 4.0},
+                                     {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 1024}])
+def test_rotation_of_a_configuration(scaling, monkeypatch):
+    """Frequencies (fp32 in the model: 2^-21 with its powers) and magnitude of transformers' own Llama."""
+    cfg = transformers.LlamaConfig(**SMALL, rope_parameters={**scaling, "rope_theta": 20000.0})
+    own = transformers.AutoModelForCausalLM.from_config(cfg).model.rotary_emb
+    f, mag = _rotation(cfg, monkeypatch)
+    assert torch.allclose(own.inv_freq.double(), f, rtol=2.0**-21, atol=0) and own.attention_scaling == pytest.approx(mag, rel=1e-12)
