@@ -63,6 +63,11 @@ def _fusable(projections) -> bool:
     return all(isinstance(p, W8A16Linear) and p.bias is None for p in projections)
 
 
+# Models whose layers are what `forward` computes.  Others name their modules alike and scale embeddings, residuals or
+# logits, interleave the rotated pairs, offset the norms' weights or leave layers without positions.
+MODEL_TYPES = ("llama", "mistral", "qwen2", "qwen3")
+
+
 def _check_attention(cfg, positions: int) -> None:
     """Every layer attends to all of its sequence, or to a window that no position leaves."""
     window = getattr(cfg, "sliding_window", None)
@@ -89,8 +94,8 @@ def _rope(cfg) -> dict:
 class TreeSpeculativeDecoder:
     """Decodes ``batch`` sequences of at most ``max_len`` tokens, ``nodes`` tree nodes a step (1: plain decoding).
 
-    Takes models whose layers are the module's heading's; attention windows shorter than ``max_len + nodes`` are
-    refused."""
+    Takes models of ``MODEL_TYPES``.  Attention windows shorter than ``max_len + nodes``, heads that turn in part and
+    rotations that ``rotary_frequencies`` does not know are refused."""
 
     def __init__(self, model: MultiDeltaLoRAModel, batch: int, max_len: int, nodes: int = 16, page: int = 64):
         from blackwell_ops.decode import MAX_NODES, KVCacheInt8, rotary_plan
@@ -102,6 +107,8 @@ class TreeSpeculativeDecoder:
         self.model, self.batch, self.nodes = model, batch, nodes
         self.max_len = max_len
         cfg = model.base.config
+        if cfg.model_type not in MODEL_TYPES:
+            raise RuntimeError(f"models of type {cfg.model_type!r} are not supported, only {', '.join(MODEL_TYPES)}")
         _check_attention(cfg, max_len + nodes)
         rope = _rope(cfg)
         self.head_dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads

@@ -111,3 +111,11 @@ def test_rotation_of_a_configuration(scaling, monkeypatch):
     own = transformers.AutoModelForCausalLM.from_config(cfg).model.rotary_emb
     f, mag = _rotation(cfg, monkeypatch)
     assert torch.allclose(own.inv_freq.double(), f, rtol=2.0**-21, atol=0) and own.attention_scaling == pytest.approx(mag, rel=1e-12)
+
+
+@pytest.mark.parametrize("kind", ["GraniteConfig", "CohereConfig", "GemmaConfig", "SmolLM3Config"])
+def test_models_with_other_layers_are_refused(kind):
+    """Their modules have the same names, but embeddings or residuals are scaled, pairs interleaved, norms offset or
+    layers left without positions."""
+    with pytest.raises(RuntimeError, match="not supported"):
+        _decoder(getattr(transformers, kind)(**SMALL, pad_token_id=0))
