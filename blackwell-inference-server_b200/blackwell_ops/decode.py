@@ -103,7 +103,8 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: dict | None
       ``factor``, those under ``.. / high_freq_factor`` kept, the ones between mixed linearly in their frequency;
     * ``yarn``: pairs that turn fewer than ``beta_slow`` times over the original context are stretched by
       ``factor``, those that turn more than ``beta_fast`` times kept, a linear ramp over the pairs between; the
-      magnitude is ``attention_factor``, or ``0.1 ln(factor) + 1``.
+      magnitude is ``attention_factor``, or ``g(mscale) / g(mscale_all_dim)`` where both are given (and not 0),
+      or ``g(1)``, with ``g(m) = 0.1 m ln(factor) + 1`` (1 for a factor of at most 1).
     """
     if rot_dim < 2 or rot_dim % 2:
         raise RuntimeError("rotary: rot_dim must be even and positive")
@@ -143,7 +144,11 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: dict | None
             stretch = ((i - lo) / max(hi - lo, 0.001)).clamp(0.0, 1.0)
             mag = scaling.get("attention_factor")
             if mag is None:
-                mag = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+                def grown(m: float) -> float:
+                    return 0.1 * m * math.log(factor) + 1.0 if factor > 1 else 1.0
+
+                both = scaling.get("mscale"), scaling.get("mscale_all_dim")
+                mag = grown(float(both[0])) / grown(float(both[1])) if all(both) else grown(1.0)
             return stretch * f / factor + (1 - stretch) * f, float(mag)
     except KeyError as e:
         raise RuntimeError(f"rotary: {kind} scaling needs {e.args[0]}") from None
