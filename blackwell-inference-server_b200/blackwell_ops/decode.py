@@ -102,9 +102,9 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: dict | None
     * ``llama3``: wavelengths over ``original_max_position_embeddings / low_freq_factor`` are stretched by
       ``factor``, those under ``.. / high_freq_factor`` kept, the ones between mixed linearly in their frequency;
     * ``yarn``: pairs that turn fewer than ``beta_slow`` times over the original context are stretched by
-      ``factor``, those that turn more than ``beta_fast`` times kept, a linear ramp over the pairs between; the
-      magnitude is ``attention_factor``, or ``g(mscale) / g(mscale_all_dim)`` where both are given (and not 0),
-      or ``g(1)``, with ``g(m) = 0.1 m ln(factor) + 1`` (1 for a factor of at most 1).
+      ``factor``, those that turn more than ``beta_fast`` times kept, a linear ramp over the pairs between (whose
+      ends are rounded outwards to whole pairs unless ``truncate`` is false); the magnitude is
+      ``attention_factor``, or ``g(mscale) / g(mscale_all_dim)`` where both are given (and not 0), or ``g(1)``, with ``g(m) = 0.1 m ln(factor) + 1`` (1 for a factor of at most 1).
     """
     if rot_dim < 2 or rot_dim % 2:
         raise RuntimeError("rotary: rot_dim must be even and positive")
@@ -139,8 +139,11 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: dict | None
             def pair_that_turns(n: float) -> float:
                 return rot_dim * math.log(old / (n * 2 * math.pi)) / (2 * math.log(base))
 
-            lo = max(math.floor(pair_that_turns(float(scaling.get("beta_fast") or 32.0))), 0)
-            hi = min(math.ceil(pair_that_turns(float(scaling.get("beta_slow") or 1.0))), rot_dim - 1)
+            lo = pair_that_turns(float(scaling.get("beta_fast") or 32.0))
+            hi = pair_that_turns(float(scaling.get("beta_slow") or 1.0))
+            if scaling.get("truncate", True):
+                lo, hi = math.floor(lo), math.ceil(hi)
+            lo, hi = max(lo, 0), min(hi, rot_dim - 1)
             stretch = ((i - lo) / max(hi - lo, 0.001)).clamp(0.0, 1.0)
             mag = scaling.get("attention_factor")
             if mag is None:

@@ -37,3 +37,19 @@ def test_magnitude(keys, mag):
     theirs, their_mag = _theirs({**YARN, **keys})
     assert got == pytest.approx(mag, rel=1e-14) and got == pytest.approx(their_mag, rel=1e-12)
     assert torch.allclose(theirs, f, rtol=2.0**-21, atol=0)
+
+
+@pytest.mark.parametrize("betas", [{}, {"beta_fast": 20.0, "beta_slow": 3.0}])
+def test_ends_of_the_ramp(betas):
+    """truncate False: the ramp runs between the fractional pairs that turn beta_fast and beta_slow times."""
+    from blackwell_ops.decode import rotary_frequencies
+
+    keys = {**YARN, **betas, "truncate": False}
+    f, _ = rotary_frequencies(64, 10000.0, keys)
+    plain = 10000.0 ** (-torch.arange(32, dtype=torch.float64) / 32)
+    at = [64 * math.log(1024 / (betas.get(k, d) * 2 * math.pi)) / (2 * math.log(10000.0)) for k, d in (("beta_fast", 32.0), ("beta_slow", 1.0))]
+    ramp = ((torch.arange(32, dtype=torch.float64) - at[0]) / (at[1] - at[0])).clamp(0, 1)
+    assert torch.allclose(f, plain * (1 - ramp) + plain / 4 * ramp, rtol=1e-12, atol=0)
+    assert torch.allclose(_theirs(keys)[0], f, rtol=2.0**-20, atol=0)
+    whole, _ = rotary_frequencies(64, 10000.0, {**keys, "truncate": True})
+    assert torch.equal(whole, rotary_frequencies(64, 10000.0, {**YARN, **betas})[0]) and not torch.equal(whole, f)
