@@ -90,10 +90,10 @@ def _workspace(dev: torch.device, nbytes: int) -> torch.Tensor:
 
 
 # ---------------------------------------------------------------- rotary positions
-def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: dict | None = None) -> tuple[torch.Tensor, float]:
+def rotary_frequencies(rot_dim: int, base: float | None = None, scaling: dict | None = None) -> tuple[torch.Tensor, float]:
     """Radians per position of the ``rot_dim / 2`` pairs (float64, CPU) and the magnitude of a turned pair.
 
-    ``scaling`` is a Hugging Face ``rope_scaling`` / ``rope_parameters`` mapping:
+    ``base`` defaults to the ``rope_theta`` of ``scaling``, or 10000.  ``scaling`` is a Hugging Face ``rope_scaling`` / ``rope_parameters`` mapping:
     ``rope_type`` (or ``type``) one of
 
     * ``default``;
@@ -108,9 +108,11 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: dict | None
     """
     if rot_dim < 2 or rot_dim % 2:
         raise RuntimeError("rotary: rot_dim must be even and positive")
+    scaling = scaling or {}
+    if base is None:
+        base = float(scaling.get("rope_theta") or 10000.0)
     if not (math.isfinite(base) and base > 1):
         raise RuntimeError("rotary: base must be over 1")
-    scaling = scaling or {}
     kind = scaling.get("rope_type", scaling.get("type", "default")) or "default"
     i = torch.arange(rot_dim // 2, dtype=torch.float64)
     f = base ** (-2.0 * i / rot_dim)
@@ -179,7 +181,7 @@ class RotaryPlan:
         self._ptr = self.steps.data_ptr()
 
 
-def rotary_plan(rot_dim: int, base: float = 10000.0, scaling: dict | None = None, interleaved: bool = False,
+def rotary_plan(rot_dim: int, base: float | None = None, scaling: dict | None = None, interleaved: bool = False,
                 device="cuda") -> RotaryPlan:
     """A plan for ``rotary``: see ``rotary_frequencies`` for the arguments."""
     f, mag = rotary_frequencies(rot_dim, base, scaling)
