@@ -201,6 +201,8 @@ class TreeSpeculativeDecoder:
         b, length = ids.shape
         if b != self.batch or length < 1:
             raise RuntimeError(f"ids must be [{self.batch}, L] with L >= 1")
+        if max_new_tokens < 0:
+            raise RuntimeError("max_new_tokens must not be negative")
         if length + max_new_tokens > self.max_len:
             raise RuntimeError(f"at most max_len = {self.max_len} tokens a sequence")
         self.model.set_adapter(adapter)
@@ -229,4 +231,4 @@ class TreeSpeculativeDecoder:
             for s, k, new in zip(seen, n.tolist(), out.tolist()):
                 if len(s) < length + max_new_tokens:
                     s += new[:k + 1]
-        return torch.tensor([s[length:length + max_new_tokens] for s in seen], device=self.dev)
+        return torch.tensor([s[length:length + max_new_tokens] for s in seen], dtype=torch.int64, device=self.dev)

@@ -90,3 +90,23 @@ def test_registry_of_some_projections(cuda_dev, targets):
 def test_window_longer_than_the_text(cuda_dev):
     """A window that no token of max_len leaves changes nothing."""
     _check(transformers.MistralConfig(**SMALL, sliding_window=64), cuda_dev)
+
+
+def test_qwen2(cuda_dev):
+    """Biases of q, k and v alone, no norms of the heads."""
+    _check(transformers.Qwen2Config(**SMALL), cuda_dev)
+
+
+def test_no_new_tokens(cuda_dev):
+    from blackwell_inference.spec_decode import TreeSpeculativeDecoder
+
+    mdl, _ = _pair(transformers.Qwen3Config(**SMALL), cuda_dev)
+    dec = TreeSpeculativeDecoder(mdl, batch=2, max_len=50)
+    new = dec.generate(_ids(cuda_dev), 0)
+    assert new.shape == (2, 0) and new.dtype == dec.generate(_ids(cuda_dev), 1).dtype == torch.int64
+    with pytest.raises(RuntimeError, match="max_new_tokens"):
+        dec.generate(_ids(cuda_dev), -1)
+    with pytest.raises(RuntimeError, match="max_len"):
+        dec.generate(_ids(cuda_dev), 11)
+    with pytest.raises(RuntimeError, match="ids must be"):
+        dec.generate(_ids(cuda_dev)[:1], 1)
