@@ -37,9 +37,18 @@ _workspaces = Workspaces(zeroed=4096)  # the tickets, in a prefix of one size fo
 
 
 # These operators are called once a layer and step, so what a call costs on the host counts: the current
-# stream's handle and device come without the objects around them.
-_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch._C._cuda_getDevice
+# stream's handle and device come without the objects around them.  The calls are torch's own, without a
+# promise to stay; where one is missing the public call does the same (an attention call then takes 17.2 us
+# on the host instead of 11.1).
+try:
+    from torch._C import _cuda_getCurrentRawStream as _stream
+    from torch._C import _cuda_getDevice as _current_device
+except ImportError:
+    def _stream(index: int) -> int:
+        return torch.cuda.current_stream(index).cuda_stream
+
+    def _current_device() -> int:
+        return torch.cuda.current_device()
 
 try:  # the allocation that the compiler's generated code calls: 0.8 us where torch.empty takes 3
     from torch._C._dynamo.guards import _empty_strided_cuda as _empty_strided
