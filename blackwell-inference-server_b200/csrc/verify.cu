@@ -59,12 +59,12 @@ __device__ __forceinline__ float approx_inverse(float x) {
 }
 constexpr float kTrustLow = 0x1p-60f, kTrustHigh = 0x1p60f;
 
-// A value of this CTA into slot `at` of all CTAs of the cluster, which have it after the next cluster_sync_all;
-// slots are not reused before every CTA has passed another one.
+// By one warp: a value into slot `index` of all CTAs of the cluster, which have it after the next
+// cluster_sync_all; slots are not reused before every CTA has passed another one.
 template <typename V>
 __device__ __forceinline__ void cluster_share(V (*slot)[kVerifyCluster], V v, int index, int ctas) {
-  if (threadIdx.x < ctas) {
-    const uint32_t at = mapa_shared(smem_u32(&(*slot)[index]), threadIdx.x);
+  if ((threadIdx.x & 31) < ctas) {
+    const uint32_t at = mapa_shared(smem_u32(&(*slot)[index]), threadIdx.x & 31);
     if constexpr (sizeof(V) == 8)
       asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(at), "l"(v) : "memory");
     else
@@ -72,15 +72,22 @@ __device__ __forceinline__ void cluster_share(V (*slot)[kVerifyCluster], V v, in
   }
 }
 
+__device__ __forceinline__ float sum4(const float4& v) { return (v.x + v.y) + (v.z + v.w); }
+__device__ __forceinline__ float sum16(const float* x) {
+  const float4* v = reinterpret_cast<const float4*>(x);
+  return (sum4(v[0]) + sum4(v[1])) + (sum4(v[2]) + sum4(v[3]));
+}
+
 // One cluster per sequence.  A row is cut into sixteen parts whatever the cluster's size, a warp's step to each
-// in turn (so that all end together); a CTA has one part, or two neighbouring ones.  Every CTA walks the tree on its own: the
-// probabilities of all drafted tokens at their parents are gathered at once, so a walk without a rejected
-// sibling before another one reads nothing more, and only then is Z summed over the row (cluster-wide, in
-// one order).  The token at the end takes one pass over the row's p, q and e.
+// in turn (so that all end together); a CTA has one part, or two neighbouring ones, whose sums it keeps apart:
+// the order of a sum is then the same in both (2 % of the time below).  Every CTA walks the tree on its own:
+// the probabilities of all drafted tokens at their parents are gathered at once, so a walk without a rejected
+// sibling before another one reads nothing more, and only then is Z summed over the row, cluster-wide.  The
+// token at the end takes one pass over the row's p, q and e.
 // Few sequences are bound by three dependent reads (tree, gather, row), many by the bytes of the passes that
-// the unluckiest walk makes one after another.  One sequence, a chain of 5 over 151936 tokens: 7.6 us with
+// the unluckiest walk makes one after another.  One sequence, a chain of 5 over 151936 tokens: 7.3 us with
 // sixteen CTAs, 9.6 with eight (launch, gather and cluster barriers alone: 4.8).  32 sequences, trees of 16
-// without draft probabilities: 24 us, of which the last pass 11 (39 MB) and the sums of Z 8.
+// without draft probabilities: 23 us, of which the last pass 11 (39 MB) and the sums of Z 8.
 // Scores are positive floats, whose bits order like them; with the token's complement below, the maximum of
 // the 64-bit keys is the best score at its lowest token.
 template <bool DRAFT, bool VEC>
@@ -91,9 +98,10 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(const Ve
   __shared__ int64_t dropped[kTreeMaxNodes];
   __shared__ float pv[kTreeMaxNodes], qv[kTreeMaxNodes], uv[kTreeMaxNodes];
   __shared__ float z[kTreeMaxNodes + 1];
-  __shared__ float red[2][kVerifyThreads / 32];
+  __shared__ __align__(16) float red[2][kVerifyThreads / 32];
   __shared__ unsigned long long redk[kVerifyThreads / 32];
-  __shared__ float sums[2][kVerifyCluster];
+  __shared__ __align__(16) float sums[2][kVerifyCluster];
+  static_assert(kVerifyThreads / 32 == 16 && kVerifyCluster == 16, "sum16");
   __shared__ unsigned long long keys[2][kVerifyCluster];
   __shared__ int walk[4];  // node, rejections, accepted nodes, next child to try (t: the walk has ended)
   const int rank = static_cast<int>(cluster_ctarank());
@@ -117,12 +125,12 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(const Ve
     z[0] = 1.f;
   }
   if (tid < 4) walk[tid] = tid == 3 ? 1 : 0;
-  // the first token of this thread's k-th group of four (of its k-th token): k goes through the CTA's parts in turn
-  const int group0 = warp * (32 * kVerifyCluster) + (rank << two) * 32 + lane;
-  auto token = [&](int k) {
-    const int64_t group = static_cast<int64_t>(k >> two) * (threads * kVerifyCluster) + (group0 + (k & two) * 32);
-    return group * (VEC ? 4 : 1);
-  };
+  // the first group of four tokens (the first token) of this thread, and the steps to the next ones: from an even
+  // one and from an odd one, as they go through the CTA's parts in turn
+  constexpr int kWidth = VEC ? 4 : 1;
+  const int v0 = ((warp * kVerifyCluster + (rank << two)) * 32 + lane) * kWidth;
+  const int even = (two ? 32 : threads * kVerifyCluster) * kWidth;
+  const int odd = (threads * kVerifyCluster - (two ? 32 : 0)) * kWidth;
   __syncthreads();
   cluster_wait();  // every CTA runs (the wait lies behind the gather): its shared memory may be written
   // What is left of four consecutive tokens' weights after the first r rejections.
@@ -151,8 +159,10 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(const Ve
   auto each = [&](const float* pr, const float* qr, const float* er, auto f) {
     const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
     if constexpr (VEC) {
+      int64_t ahead = v0;
       auto fetch = [&](int k, int stage) {
-        const int64_t v = token(k);
+        const int64_t v = ahead;
+        ahead += (k & 1) ? odd : even;
         if (v < a.v) {
           float4* to = stages + stage * 3 * threads + tid;
           copy16_async(to, pr + v);
@@ -163,9 +173,9 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(const Ve
       };
 #pragma unroll 1
       for (int k = 0; k < kVerifyStages; ++k) fetch(k, k);
-      int stage = 0, k = 0;
+      int stage = 0;
 #pragma unroll 1
-      for (int64_t v = token(0); v < a.v; v = token(++k)) {
+      for (int64_t v = v0, k = 0; v < a.v; v += (k++ & 1) ? odd : even) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kVerifyStages - 1) : "memory");
         const float4* from = stages + stage * 3 * threads + tid;
         const float4 w = from[0];
@@ -177,9 +187,8 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(const Ve
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
-      int k = 0;
 #pragma unroll 2
-      for (int64_t v = token(0); v < a.v; v = token(++k)) {
+      for (int64_t v = v0, k = 0; v < a.v; v += (k++ & 1) ? odd : even) {
         const float4 qw = make_float4(qr != nullptr ? __ldg(qr + v) : 0.f, 0.f, 0.f, 0.f);
         const float4 ew = make_float4(er != nullptr ? __ldg(er + v) : 0.f, 0.f, 0.f, 0.f);
         f(make_float4(__ldg(pr + v), 0.f, 0.f, 0.f), qw, ew, v, k & two);
@@ -239,17 +248,9 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(const Ve
       if (lane == 0) red[i][warp] = sum[i];
     }
     __syncthreads();
-    for (int i = 0; i <= two; ++i) {
-      float s = 0.f;
-      for (int k = 0; k < threads / 32; ++k) s += red[i][k];
-      cluster_share(&sums[phase & 1], s, (rank << two) + i, ctas);
-    }
+    if (warp <= two) cluster_share(&sums[phase & 1], sum16(red[warp]), (rank << two) + warp, ctas);
     cluster_sync_all();
-    if (tid == 0) {
-      float s = 0.f;
-      for (int k = 0; k < kVerifyCluster; ++k) s += sums[phase & 1][k];
-      z[r] = s;
-    }
+    if (tid == 0) z[r] = sum16(sums[phase & 1]);
     ++phase;
     __syncthreads();
   }
@@ -302,10 +303,10 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(const Ve
     float most = top;
     for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
     if (lane == 0) red[0][warp] = most;
-    const bool odd = __syncthreads_or(!(e_min >= kTrustLow && e_max <= kTrustHigh));
+    const bool unsure = __syncthreads_or(!(e_min >= kTrustLow && e_max <= kTrustHigh));
     for (int k = 0; k < threads / 32; ++k) most = fmaxf(most, red[0][k]);
     const float near = most * (1.f - 0x1p-20f);
-    if (odd || !(most >= kTrustLow && most <= kTrustHigh) || second >= near)
+    if (unsure || !(most >= kTrustLow && most <= kTrustHigh) || second >= near)
       scores(score);
     else if (top >= near)
       score(top_w, top_e, top_v);
@@ -317,7 +318,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(const Ve
     __syncthreads();
     best = 0;
     for (int k = 0; k < threads / 32; ++k) best = redk[k] > best ? redk[k] : best;
-    cluster_share(&keys[pass], best, rank, ctas);
+    if (warp == 0) cluster_share(&keys[pass], best, rank, ctas);
     cluster_sync_all();
     best = 0;
     for (int k = 0; k < ctas; ++k) best = keys[pass][k] > best ? keys[pass][k] : best;
