@@ -469,7 +469,11 @@ def tree_attention_int8(q: torch.Tensor, cache: KVCacheInt8, table: torch.Tensor
     nodes j whose bit is set in ``mask[b, i]`` (int64; None: nodes 0 .. i, a chain).  ``counts`` [B]
     limits a sequence's nodes: later ones are not seen and give zeros, and so does a node that sees
     nothing.  Query head h reads key head ``h // (Hq / heads)``.  T <= 64; T = 1 is ordinary decoding.
-    ``softmax_scale`` defaults to ``D ** -0.5``."""
+    ``softmax_scale`` defaults to ``D ** -0.5``.
+
+    The tensor-core kernel takes D = 64 or 128, pages of 16, 32, 64 or a multiple of 128 slots, cache tensors on
+    16-byte boundaries with fewer than 2^31 rows (pages * heads * page), and at most 32768 query rows a key head; other
+    calls go to a kernel of a CTA a query row, some 25 times slower on long batches."""
     if cache.layers is not None:
         cache._one_layer("tree_attention_int8")
     dev, dt = cache.device, q.dtype

@@ -230,8 +230,9 @@ __global__ void __launch_bounds__(256, WRITE ? 3 : 4) rotary_vec_kernel(const __
     krow = kv_row(a.cache, b, static_cast<int64_t>(a.start[b]) + t);
   const unsigned lanes = L == 32 ? 0xffffffffu : ((1u << L) - 1u) << ((threadIdx.x & 31) / L * L);
   // The next row is on its way while one is turned, the first while the sines are computed.  8191 tokens of 72
-  // rows: 57 us, 5.3 TB/s; two rows ahead 60, three 68 (their registers spill).  The write of 4096 tokens' 32
-  // query rows with 16 rows into the cache: 26.5 us, 3.5 TB/s, the quotients' instructions between the loads.
+  // rows: 56 us, 5.4 TB/s; two rows ahead 60, three 68 (their registers spill).  The write of 4096 tokens' 32
+  // query rows with 16 rows into the cache: 27 us, 3.4 TB/s (24 without any quotient: three CTAs an SM and two
+  // and a third waves more than the instructions).
   auto fetch = [&](int h, uint4 (&raw)[2]) {
     if (h >= rows) return;
     const int which = h < hq ? 0 : (h < hqk ? 1 : 2);

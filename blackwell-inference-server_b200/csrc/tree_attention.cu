@@ -143,8 +143,9 @@ __global__ void __launch_bounds__(32 * kRowWarps) attn_rows_kernel(const __grid_
 // What bounds it (one B200, D = 128, bf16, long contexts): with 16 rows the two dequantisers' issue slots,
 // 1.05 us a tile of 32 KB in every SM, 4.7 TB/s (fp16, whose conversion has five instructions for four codes
 // where bf16 has nine: 0.87 us, 5.7 TB/s); with 64 rows the softmax groups, 1.55 us a tile, 400 TFLOP/s;
-// with short contexts a segment's start and end, under 3 us together.  One token over 1k slots: 12.3 us, of
-// which 1 from launch to the first barrier, 2 to the first tile, 1.5 from scores to weights, 1.4 the ticket.
+// with short contexts a segment's start and end, under 3 us together.  One token over 1k slots: 12 us, of
+// which 1 from launch to the first barrier, 2 to the first tile, 1.5 from scores to weights, 1.4 the ticket
+// (timed one by one; the rest was not).
 // Measured and not kept: 64 rows in alternate tiles, whose scores are then fetched twice (a sixth slower on a
 // tree of 64 nodes over 128k slots); row blocks of equal height (690 us for 618 there: branches between the
 // columns cost more than the columns); a segment's end put off into the next one's first tiles (125 us for
