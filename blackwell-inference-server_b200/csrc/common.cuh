@@ -122,6 +122,17 @@ __device__ __forceinline__ void fence_mbar_init() {
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+// One arrival of a warp, after every lane has `loaded` in a register: for a slot whose reads are all that keeps it,
+// given back before anything else uses what was read.  Program order is not enough: a load is still in flight when
+// the instructions after it are issued, and an arrive there let the next copy into the slot overtake it (the fp16
+// gate and up GEMM at 128 tokens a tile had wrong rows in one of 150 to 500 calls on an idle GPU).  An asm
+// statement without an instruction keeps nothing either.  Here the arrive's address depends on every lane's
+// loads: `zero` is 0, which the compiler must not know.
+__device__ __forceinline__ void mbar_arrive_loaded(uint64_t* bar, uint32_t loaded, uint32_t zero, int lane) {
+  const uint32_t all = __ballot_sync(0xffffffffu, (loaded & zero) != 0u);
+  if (lane == 0)
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar) + all) : "memory");
+}
 __device__ __forceinline__ void mbar_arrive_expect_tx(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes)
                : "memory");
