@@ -420,6 +420,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   const int lane = threadIdx.x & 31;
   const int grp = a.hq / a.c.heads;  // query heads of a key head
   const int heads = a.c.heads;
+  const uint32_t never = static_cast<uint32_t>(a.t) >> 31;  // 0
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
@@ -729,7 +730,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       const int sw = D == 128 ? (row & 7) : ((row >> 1) & 3);
       if (!mbar_wait_or_abort(&sfull[t], ((it >> 1) & 1) ^ 1, ctl)) break;
       tc_fence_after();
-      uint32_t dep = 0;
+      uint32_t loaded = 0;
 #pragma unroll 1
       for (int c = 0; c < D / 16; c += 2) {
         const uint4 r0 = *reinterpret_cast<const uint4*>(src + ((c ^ sw) << 4));
@@ -738,11 +739,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         codes16<BF16>(r0, o);
         codes16<BF16>(r1, o + 8);
         tmem_st16(dst + t * C::A_COLS + c * 8, o);
-        dep |= o[7] | o[15];
+        loaded |= r0.w | r1.w;
       }
-      asm volatile("" ::"r"(dep));  // the last loads are complete before the slot is released
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&kempty[s]);
+      mbar_arrive_loaded(&kempty[s], loaded, never, lane);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -760,7 +759,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         if (!mbar_wait_or_abort(&pempty[t], ((it >> 1) & 1) ^ 1, ctl)) break;
         const uint8_t* src = sV + s * C::KV;
         uint8_t* dst = sVB + t * C::VB;
-        uint32_t dep = 0;
+        uint32_t loaded = 0;
         // One 16-byte chunk of codes -> chunks 2 (c % 4), 2 (c % 4) + 1 of a bf16 row of panel c / 4.
         // Two chunks a step, few steps unrolled: five roles share the instruction cache, and with the
         // loops of the dequantisers unrolled in full half of all issue slots waited for it.
@@ -794,11 +793,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           *reinterpret_cast<uint4*>(d0 + w1) = make_uint4(o[4], o[5], o[6], o[7]);
           *reinterpret_cast<uint4*>(d1 + w0) = make_uint4(o[8], o[9], o[10], o[11]);
           *reinterpret_cast<uint4*>(d1 + w1) = make_uint4(o[12], o[13], o[14], o[15]);
-          dep |= o[7] | o[15];
+          loaded |= r0.w | r1.w;
         }
-        asm volatile("" ::"r"(dep));  // the last loads are complete before the slot is released
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&vempty[s]);
+        mbar_arrive_loaded(&vempty[s], loaded, never, lane);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&vbfull[t]);
