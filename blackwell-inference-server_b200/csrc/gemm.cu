@@ -164,14 +164,6 @@ __device__ __forceinline__ float round_out(float v) {
 // its own accumulator; BM = 128 one.  A third issuer (warp 15, with the weight producer also
 // loading the activation tiles) measured slower on the Llama-3-70B MLP decode shapes (3.1 against
 // 4.0 TB/s; the single producer then issued one weight tile per ~1250 cycles) and is not kept.
-// Shared memory (KB) of the two decode rings together.
-#ifndef BW_GEMM_DEC_SMEM_KB
-#define BW_GEMM_DEC_SMEM_KB 208
-#endif
-// Activation ring depth at BM = 16 (the weight ring takes the rest of the decode rings' budget).
-#ifndef BW_GEMM_XSTAGES16
-#define BW_GEMM_XSTAGES16 16
-#endif
 // The weight producer requests this many consecutive k-blocks of the same rows back to back
 // (waiting for that many free slots), so a row's adjacent 128-byte blocks reach DRAM together.
 #ifndef BW_GEMM_W_GROUP
@@ -203,8 +195,13 @@ struct PCfg {
   // weight tiles already issued, so an activation tile must be issued with (or before) its
   // k-block's weight tile; with a shallow ring its slot frees only when an MMA completes, and the
   // tile then landed a full loaded latency after the MMA was due (one stage per ~900 cycles).
-  static constexpr int XSTAGES_DEC = BM == 16 ? BW_GEMM_XSTAGES16 : BM == 32 ? 12 : 5;
-  static constexpr int STAGES_DEC = (BW_GEMM_DEC_SMEM_KB * 1024 - XSTAGES_DEC * X_BYTES) / W_BYTES;
+  // Every ring that two groups take in turn has an even number of slots, so that a slot has one group.
+  // A group that sees only every other filling of a slot cannot wait for the next one: the parity it
+  // waits for is also that of the last filling it saw, for as long as the one between is on its way.
+  // The 70B up projection at M = 16, 32, 64: 51.4, 53.4, 59.2 us; with 9 + 16, 7 + 12 and 8 + 5 slots
+  // 51.6, 54.2, 59.4, with 10 + 12 and 8 + 10 52.2, 53.9.
+  static constexpr int XSTAGES_DEC = BM == 16 ? 16 : BM == 32 ? 8 : 4;
+  static constexpr int STAGES_DEC = 8;
   static constexpr int STAGES = BM < 128 ? STAGES_DEC : STAGES_PRE;
   static constexpr int XSTAGES = BM < 128 ? XSTAGES_DEC : STAGES_PRE;
   // TMEM: A buffers (64 columns each) between the dequantisers and the MMAs, as many as the
@@ -225,6 +222,7 @@ struct PCfg {
   static_assert(BM >= 16 && BM <= 128 && BM % 16 == 0, "UMMA N for M=128");
   static_assert(NI >= 1 && NI <= 2, "one or two MMA issuers");
   static_assert(ASTAGES >= 2, "TMEM A buffers");
+  static_assert(STAGES % 2 == 0 && ASTAGES % 2 == 0 && XSTAGES % NI == 0, "a slot has one group of dequantisers, one issuer");
   static_assert(D_COL0 + DBUF * NI * BM <= TMEM_COLS, "TMEM budget");
   static_assert(SMEM <= 232448, "shared memory budget");
   // barriers, then 32 bytes of slots (TMEM address, abort flag, ticket, epoch, trace record) and the
