@@ -259,6 +259,11 @@ __global__ void __launch_bounds__(kLsThreads, 1)
           umma_f16(tmem + db * 128, ad, bd, idesc, kk > 0 ? 1u : 0u);
         }
         umma_commit(&aempty[sa]);
+        if constexpr (MODE != kModeDelta) {
+          // The tile's W has landed as well: this thread takes every tile in turn and so sees every filling of
+          // a W slot, where a group, one of three over four slots, could mistake an earlier one for its own.
+          if (!mbar_wait(&wfull[i % SW], (i / SW) & 1, abort_flag, kSiteLsMma)) break;
+        }
         umma_commit(&dfull[db]);
         // the last tile of this row block in the CTA's range: B may be replaced once it completes
         const bool last_of_rb = i + 1 == ntile || static_cast<int>((t + 1) / n_cb) != rb;

@@ -1,4 +1,4 @@
-"""Rings whose slots are waited for by parity: which rings two consumers may take in turn.
+"""Rings whose slots are waited for by parity: which rings several consumers may take in turn.
 
 A wait for filling number n of a slot (counted from 0) passes when the slot's count of completed fillings has not the
 parity of n: for n + 1 completed, as meant, but also for n - 1.  A consumer that took filling n - 1 itself never sees that
@@ -12,11 +12,11 @@ import pytest
 CSRC = Path(__file__).resolve().parent.parent / "blackwell-inference-server_b200" / "csrc"
 
 
-def _stale_reads(slots, items, arrivals):
-    """Items that a consumer would take before they are there: two consumers take even and odd items, each as soon as its
-    wait passes; the producer fills a slot when its last item has been taken; item i arrives at arrivals[i] or later."""
+def _stale_reads(slots, items, arrivals, consumers=2):
+    """Items that a consumer would take before they are there: consumers take the items in turn, each as soon as its wait
+    passes; the producer fills a slot when its last item has been taken; item i arrives at arrivals[i] or later."""
     count, taken, issued, at = [0] * slots, set(), {}, 0
-    heads, stale = [0, 1], []
+    heads, stale = list(range(consumers)), []
     landed = set()
     for now in itertools.count():
         while at < items and (at < slots or at - slots in taken):
@@ -26,14 +26,14 @@ def _stale_reads(slots, items, arrivals):
             if i not in landed and now >= max(t, arrivals[i]):
                 landed.add(i)
                 count[i % slots] += 1
-        for c in (0, 1):
+        for c in range(consumers):
             i = heads[c]
             if i < items and count[i % slots] % 2 != (i // slots) % 2:
                 if i not in landed:
                     stale.append(i)
                     return stale
                 taken.add(i)
-                heads[c] += 2
+                heads[c] += consumers
         if all(h >= items for h in heads):
             return stale
 
@@ -46,6 +46,21 @@ def test_which_rings_two_consumers_may_share(slots):
         assert any(late), "an odd ring gives an item that is not there to the other consumer"
     else:
         assert not any(late)
+
+
+@pytest.mark.parametrize("slots,safe", [(3, True), (4, False), (6, True)])
+def test_three_consumers(slots, safe):
+    items = 4 * slots * 3
+    late = [_stale_reads(slots, items, [0 if i != slow else 10**3 for i in range(items)], 3) for slow in range(items - 1)]
+    assert any(late) != safe
+
+
+def test_the_merge_sees_every_filling():
+    """Three groups take the tiles of four W slots: the MMA thread, which takes all, waits for a tile's W before the
+    commit that the tile's group waits for."""
+    text = (CSRC / "lora.cu").read_text()
+    issuer = text[text.index("umma_commit(&aempty[sa]);"):text.index("umma_commit(&dfull[db]);")]
+    assert "mbar_wait(&wfull[i % SW], (i / SW) & 1" in issuer
 
 
 def test_the_gemm_asserts_it():
