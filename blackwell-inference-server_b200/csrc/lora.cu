@@ -1031,7 +1031,9 @@ static ReqPlan req_plan(int rp_max) {
   pl.off_ring = 2 * pl.b_bytes;
   const int staging = 4 * kReqGroups * 2048;
   const int fixed = pl.off_ring + staging + kReqBarBytes + 1024;
-  pl.stages = std::min(kReqMaxStages, (kReqSmemLimit - fixed) / pl.stage_bytes);
+  // an even number: two MMA issuers take the items in turn, and one that saw only every other filling of a
+  // slot could take an earlier one for the next (r = 33 .. 48 had seven)
+  pl.stages = std::min(kReqMaxStages, (kReqSmemLimit - fixed) / pl.stage_bytes) / 2 * 2;
   pl.off_q = pl.off_ring + pl.stages * pl.stage_bytes;
   pl.off_bar = pl.off_q + staging;
   pl.smem = pl.off_bar + kReqBarBytes + 1024;

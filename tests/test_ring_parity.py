@@ -63,6 +63,12 @@ def test_the_merge_sees_every_filling():
     assert "mbar_wait(&wfull[i % SW], (i / SW) & 1" in issuer
 
 
+def test_the_requantiser_has_an_even_ring():
+    text = (CSRC / "lora.cu").read_text()
+    assert re.search(r"pl\.stages = std::min\(kReqMaxStages, .*\) / 2 \* 2;", text)
+    assert int(re.search(r"kReqMaxStages = (\d+)", text)[1]) % 2 == 0
+
+
 def test_the_gemm_asserts_it():
     text = (CSRC / "gemm.cu").read_text()
     assert re.search(r"static_assert\(STAGES % 2 == 0 && ASTAGES % 2 == 0 && XSTAGES % NI == 0", text)
