@@ -744,12 +744,10 @@ __global__ void __launch_bounds__(kReqThreads, 1) lora_requant_coop_kernel(const
           for (int c = 0; c < 4; ++c) wv[c] = *reinterpret_cast<const uint4*>(wrow + (((4 * h + c) ^ sw) << 4));
           tmem_ld_wait();
           if (h == 1) {
+            // this warp is done with the accumulator slot and, its rows in registers, with the stage
             tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-              mbar_arrive(&dempty[d]);
-              mbar_arrive(&empty[st]);  // this warp is done with the accumulator slot and the stage
-            }
+            mbar_arrive_loaded(&empty[st], wv[0].w | wv[1].w | wv[2].w | wv[3].w, static_cast<uint32_t>(T) >> 31, lane);
+            if (lane == 0) mbar_arrive(&dempty[d]);
           }
           __half2 merged[16];
 #pragma unroll

@@ -13,8 +13,9 @@ def test_no_empty_asm(path):
     assert not re.findall(r'asm\s+(?:volatile\s*)?\(\s*""', path.read_text())
 
 
-@pytest.mark.parametrize("file,barriers", [("gemm.cu", ["empty"]), ("tree_attention.cu", ["kempty", "vempty"])])
+@pytest.mark.parametrize("file,barriers", [("gemm.cu", ["empty"]), ("lora.cu", ["empty"]),
+                                           ("tree_attention.cu", ["kempty", "vempty"])])
 def test_slots_that_are_read_into_registers(file, barriers):
     text = (CSRC / file).read_text()
     for b in barriers:
-        assert re.search(rf"mbar_arrive_loaded\(&{b}\[s\],", text) and not re.search(rf"mbar_arrive\(&{b}\[", text), b
+        assert re.search(rf"mbar_arrive_loaded\(&{b}\[\w+\],", text) and not re.search(rf"mbar_arrive\(&{b}\[", text), b
