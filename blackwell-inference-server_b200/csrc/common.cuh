@@ -122,8 +122,9 @@ __device__ __forceinline__ void fence_mbar_init() {
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-// One arrival of a warp, after every lane has `loaded` in a register: for a slot whose reads are all that keeps it,
-// given back before anything else uses what was read.  Program order is not enough: a load is still in flight when
+// One arrival of a warp, after every lane has `loaded` in a register: for a slot that TMA fills again, given back
+// before anything else uses what was read (between ordinary reads and writes the arrive's release is enough; a
+// copy by the async proxy is not ordered by it).  Program order is not enough: a load is still in flight when
 // the instructions after it are issued, and an arrive there let the next copy into the slot overtake it (the fp16
 // gate and up GEMM at 128 tokens a tile had wrong rows in one of 150 to 500 calls on an idle GPU).  An asm
 // statement without an instruction keeps nothing either.  Here the arrive's address depends on every lane's
