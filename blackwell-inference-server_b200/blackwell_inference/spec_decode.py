@@ -77,7 +77,8 @@ def _check_attention(cfg, positions: int) -> None:
     for kind in sorted(kinds - {"full_attention", "sliding_attention"}):
         raise RuntimeError(f"layers of {kind} are not supported")
     if "sliding_attention" in kinds and (window is None or window < positions):
-        raise RuntimeError(f"a window of {window} tokens is shorter than max_len and the nodes of a step, {positions}: not supported")
+        raise RuntimeError(f"a window of {window} tokens is shorter than max_len and the nodes of a step, {positions}: "
+                           "not supported")
 
 
 def _rope(cfg) -> dict:
@@ -113,7 +114,7 @@ class TreeSpeculativeDecoder:
         rope = _rope(cfg)
         self.head_dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads
         self.heads, self.kv_heads = cfg.num_attention_heads, cfg.num_key_value_heads
-        self.swiglu = getattr(cfg, "hidden_act", None) in ("silu", "swish")  # what the fused gate and up product computes
+        self.swiglu = getattr(cfg, "hidden_act", None) in ("silu", "swish")  # the fused gate and up product's
         self.layers = model.base.model.layers
         self.dev = next(model.base.parameters()).device
         self.plan = rotary_plan(self.head_dim, float(rope["rope_theta"]), rope, device=self.dev)

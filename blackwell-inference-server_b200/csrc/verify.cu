@@ -154,8 +154,9 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(const Ve
     }
   };
   // f(four tokens of p, of q and of e, or zeros where a row is not given; the first of them; which of the
-  // CTA's parts) over this thread's tokens, in order.  Each thread copies its own groups to shared memory, kVerifyStages steps ahead
-  // (in registers they would be too few to cover the latency); rows that are no groups of four go one by one.
+  // CTA's parts) over this thread's tokens, in order.  Each thread copies its own groups to shared memory,
+  // kVerifyStages steps ahead (in registers they would be too few to cover the latency); rows that are no groups
+  // of four go one by one.
   auto each = [&](const float* pr, const float* qr, const float* er, auto f) {
     const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
     if constexpr (VEC) {

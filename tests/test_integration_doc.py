@@ -1,4 +1,4 @@
-"""The bindings that INTEGRATION.md publishes: their workspaces, with the library and the GPUs played by the test."""
+"""The published ctypes bindings: their workspaces, with the library and the GPUs played by the test."""
 import contextlib
 import os
 import re
