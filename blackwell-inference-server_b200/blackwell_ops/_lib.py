@@ -88,6 +88,12 @@ SIGNATURES = {
     "bw_rotary_kv_write_int8": (_c.c_int, [_P, _I64, _I64, _I64, _c.c_int, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64,
                                            _P, _c.c_int, _I64, _I64, _P, _c.c_int, _P, _c.c_float, _I64, _c.c_int,
                                            _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _P]),
+    "bw_norm_rotary": (_c.c_int, [_P, _I64, _I64, _I64, _c.c_int, _P, _I64, _I64, _I64, _c.c_int, _P, _P, _c.c_int, _I64,
+                                  _I64, _I64, _P, _P, _c.c_float, _P, _c.c_int, _P, _c.c_float, _I64, _c.c_int, _P]),
+    "bw_norm_rotary_kv_write_int8": (_c.c_int, [_P, _I64, _I64, _I64, _c.c_int, _P, _I64, _I64, _I64, _P, _I64, _I64,
+                                                _I64, _P, _P, _c.c_int, _I64, _I64, _P, _P, _c.c_float, _P, _c.c_int,
+                                                _P, _c.c_float, _I64, _c.c_int, _P, _P, _P, _P, _I64, _I64, _I64,
+                                                _I64, _P, _I64, _I64, _P, _P, _P, _P]),
     "bw_kv_read_int8": (_c.c_int, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _I64,
                                    _P, _P, _c.c_int, _P]),
     "bw_kv_move_int8": (_c.c_int, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _P,

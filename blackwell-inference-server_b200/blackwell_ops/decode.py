@@ -3,10 +3,12 @@
 The operators of one decoder step next to the W8A16 linears:
 
 * ``rotary`` turns queries and keys by their positions (``rotary_plan``: half or interleaved pairs,
-  part of the head, frequencies scaled for long contexts);
+  part of the head, frequencies scaled for long contexts); ``norm_rotary`` normalises each of their heads first,
+  in the same pass;
 * ``KVCacheInt8`` holds int8 codes and one fp32 scale per token and head in pages;
   ``kv_write_int8`` quantises new keys and values as they are written, ``rotary_kv_write_int8``
-  rotates and writes in one launch, ``kv_read_int8`` gives values back, ``kv_move_int8`` moves the
+  rotates and writes in one launch (``norm_rotary_kv_write_int8``: normalises too, and takes packed
+  sequences of different lengths), ``kv_read_int8`` gives values back, ``kv_move_int8`` moves the
   accepted nodes of a draft tree to their final slots in every layer;
 * ``tree_attention_int8`` attends from the nodes of a draft tree (or one new token) to the cache;
   ``tree_positions`` gives a tree's masks and positions;
@@ -263,6 +265,49 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
     return q_out, k_out
 
 
+def _weight(w: torch.Tensor | None, name: str, d: int, dt: torch.dtype, dev: torch.device) -> torch.Tensor | None:
+    """A norm's contiguous weights [d], or none."""
+    if w is None:
+        return None
+    if w.dtype is not dt or w.device != dev or w.shape != (d,):
+        raise RuntimeError(f"{name} must be [{d}] of the inputs' dtype and device")
+    return w if w.is_contiguous() else w.contiguous()
+
+
+def norm_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, plan: RotaryPlan,
+                q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
+                eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """``rotary`` of queries and keys whose heads are normalised first, in one pass: each head's row x [D] becomes
+    ``w * x / sqrt(mean(x^2) + eps)`` with w = ``q_weight`` or ``k_weight`` [D] (None: its rows are only turned).
+
+    32-bit arithmetic, rounded once, behind the rotation.  Returns new contiguous tensors."""
+    lead = q.shape[:-2]
+    q, shape, b, t, qb, qt, qh = _rows(q, "q", lead)
+    dev, dt, hq, d = q.device, q.dtype, shape[-2], shape[-1]
+    if plan.rot_dim > d or d > MAX_HEAD_DIM:
+        raise RuntimeError(f"norm_rotary: need rot_dim <= D <= {MAX_HEAD_DIM}")
+    if plan.device != dev:
+        raise RuntimeError("norm_rotary: the plan is on another device")
+    if not eps >= 0:
+        raise RuntimeError("norm_rotary: eps must not be negative")
+    positions = _positions(positions, lead, dev)
+    q_weight, k_weight = _weight(q_weight, "q_weight", d, dt, dev), _weight(k_weight, "k_weight", d, dt, dev)
+    q_out = _new(shape, dt, dev)
+    k_out, hk, kb, kt, kh, kp, kop = None, 0, 0, 0, 0, None, None
+    if k is not None:
+        k, kshape, _, _, kb, kt, kh = _rows(k, "k", lead)
+        if k.dtype is not dt or k.device != dev or kshape[-1] != d:
+            raise RuntimeError("k must have q's dtype, device and head dimension")
+        hk = kshape[-2]
+        k_out = _new(kshape, dt, dev)
+        kp, kop = k.data_ptr(), k_out.data_ptr()
+    _call("norm_rotary", dev, lib.bw_norm_rotary, q.data_ptr(), qb, qt, qh, hq, kp, kb, kt, kh, hk, q_out.data_ptr(), kop,
+          DTYPE_CODE[dt], b, t, d, None if q_weight is None else q_weight.data_ptr(),
+          None if k_weight is None else k_weight.data_ptr(), eps, positions.data_ptr(), positions.dtype is torch.int64,
+          plan._ptr, plan.magnitude, plan.rot_dim, plan.interleaved)
+    return q_out, k_out
+
+
 # ---------------------------------------------------------------- the cache
 class KVCacheInt8:
     """A paged int8 KV cache: ``k``, ``v`` int8 [layers?, pages, heads, page, D] and ``k_scale``, ``v_scale``
@@ -398,6 +443,64 @@ def rotary_kv_write_int8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, posi
     The rotated keys are quantised from their 32-bit values.  Returns the rotated q (every token's,
     ``counts`` limits the write only)."""
     return _write(q, k, v, positions, plan, cache, table, start, counts, "rotary_kv_write_int8")
+
+
+def norm_rotary_kv_write_int8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+                              plan: RotaryPlan, cache: KVCacheInt8, table: torch.Tensor, start: torch.Tensor,
+                              q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
+                              eps: float = 1e-6, counts: torch.Tensor | None = None,
+                              offsets: torch.Tensor | None = None,
+                              keys: bool = False) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """``norm_rotary`` of q and k, and ``kv_write_int8`` of the normalised and rotated k and of v, in one launch.
+
+    q [B, T, Hq, D] with k, v [B, T, heads, D] as in ``rotary_kv_write_int8``; or, with ``offsets`` [B + 1] (int32, not
+    descending), packed prompts [N, .., D]: rows ``offsets[b] .. offsets[b + 1]`` are sequence b's and go to slots
+    ``start[b]`` on, other rows are not written.  The keys are quantised from their 32-bit values.  Returns the rotated q and,
+    with ``keys``, the rotated k (every row's), else None."""
+    op = "norm_rotary_kv_write_int8"
+    if cache.layers is not None:
+        cache._one_layer(op)
+    dev = cache.device
+    packed = offsets is not None
+    if k.dim() != (3 if packed else 4):
+        raise RuntimeError(f"{op}: k must be {'[N, heads, D] with offsets' if packed else '[B, T, heads, D]'}")
+    lead = k.shape[:-2]
+    q, qshape, _, _, qb, qt, qh = _rows(q, "q", lead)
+    k, kshape, b, t, kb, kt, kh = _rows(k, "k", lead)
+    v, vshape, _, _, vb, vt, vh = _rows(v, "v", lead)
+    d, dt = cache.head_dim, k.dtype
+    if kshape[-2] != cache.heads or kshape[-1] != d or vshape != kshape:
+        raise RuntimeError(f"{op}: k and v must be [.., {cache.heads}, {d}] like the cache")
+    if v.dtype is not dt or k.device != dev or v.device != dev:
+        raise RuntimeError(f"{op}: k and v must share one dtype and be on the cache's device")
+    if q.dtype is not dt or q.device != dev or qshape[-1] != d:
+        raise RuntimeError(f"{op}: q must have k's dtype, device and head dimension")
+    if plan.device != dev or plan.rot_dim > d:
+        raise RuntimeError(f"{op}: the plan must be on the cache's device with rot_dim <= D")
+    if not eps >= 0:
+        raise RuntimeError(f"{op}: eps must not be negative")
+    table, rows, ld, cols = _table(table, dev)
+    if packed:
+        if counts is not None:
+            raise RuntimeError(f"{op}: packed rows have offsets, no counts")
+        b = rows
+        offsets = _ints(offsets, "offsets", (b + 1,), dev)
+    elif rows != b:
+        raise RuntimeError(f"{op}: table must have a row for each of {b} sequences")
+    start = _ints(start, "start", (b,), dev)
+    if counts is not None:
+        counts = _ints(counts, "counts", (b,), dev)
+    positions = _positions(positions, lead, dev)
+    q_weight, k_weight = _weight(q_weight, "q_weight", d, dt, dev), _weight(k_weight, "k_weight", d, dt, dev)
+    q_out = _new(qshape, dt, dev)
+    k_out = _new(kshape, dt, dev) if keys else None
+    _call(op, dev, lib.bw_norm_rotary_kv_write_int8, q.data_ptr(), qb, qt, qh, qshape[-2], k.data_ptr(), kb, kt, kh,
+          v.data_ptr(), vb, vt, vh, q_out.data_ptr(), k_out.data_ptr() if keys else None, DTYPE_CODE[dt], b, t,
+          None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(), eps,
+          positions.data_ptr(), positions.dtype is torch.int64, plan._ptr, plan.magnitude, plan.rot_dim, plan.interleaved,
+          *cache._ptrs, *cache._dims, table.data_ptr(), ld, cols, start.data_ptr(),
+          None if counts is None else counts.data_ptr(), offsets.data_ptr() if packed else None)
+    return q_out, k_out
 
 
 def kv_read_int8(cache: KVCacheInt8, table: torch.Tensor, start: torch.Tensor | None, n: int,
@@ -569,6 +672,7 @@ def verify_tree(target_probs: torch.Tensor, tokens: torch.Tensor, parents: torch
     return n, path, out
 
 
-__all__ = ["MAX_NODES", "KVCacheInt8", "RotaryPlan", "kv_move_int8", "kv_read_int8", "kv_write_int8", "reset_workspaces",
+__all__ = ["MAX_NODES", "KVCacheInt8", "RotaryPlan", "kv_move_int8", "kv_read_int8", "kv_write_int8", "norm_rotary",
+           "norm_rotary_kv_write_int8", "reset_workspaces",
            "rotary", "rotary_frequencies", "rotary_kv_write_int8", "rotary_plan", "tree_attention_int8",
            "tree_positions", "verify_tree"]

@@ -8,6 +8,9 @@
 // pos * f_i is off by up to 4e-3 radians, this by 2e-7 (the fraction's own rounding to fp32).
 // No sine table is read; the sines cost one sincospi per pair and token.
 //
+// Norm.  Where a weight w is given, a head's row is first y = w x / sqrt(mean(x^2) + eps), over all of its
+// elements, in 32 bits; the turn and the quantiser take y as it is, unrounded.
+//
 // Quantisation.  One fp32 scale per token and head, s = max|x| / 127 (NaN ignored, 0 for a row of
 // zeros), code = clamp(rne(x / s), +-127) with the IEEE quotient (NaN -> 0).  Rotated keys are
 // quantised from their 32-bit values: rounding them to 16 bits first would add an error of the
@@ -53,7 +56,29 @@ struct RotArgs {
   KvCache cache;
   const int* start;    // [b] first slot
   const int* counts;   // [b] tokens of a sequence, or null: all t
+  const void* qw;      // [d] weights of the norms, or null: not normalised
+  const void* kw;
+  float eps;
+  const int* offsets;  // [seqs + 1]: packed rows (b is 1, t counts them), or null
+  int64_t seqs;
 };
+
+// Row of the cache (of head 0) that token t of sequence b, or packed row t, goes to; -1: none.
+__device__ __forceinline__ int64_t target_row(const RotArgs& a, int64_t b, int64_t t) {
+  if (a.offsets == nullptr) {
+    if (a.counts != nullptr && t >= a.counts[b]) return -1;
+    return kv_row(a.cache, b, static_cast<int64_t>(a.start[b]) + t);
+  }
+  // the last sequence that starts at row t or before it (one of no rows starts where the next one does)
+  int64_t lo = 0, hi = a.seqs;
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (a.offsets[mid] <= t) lo = mid + 1;
+    else hi = mid;
+  }
+  if (lo == 0 || t >= a.offsets[lo]) return -1;  // before the first sequence, or behind the last
+  return kv_row(a.cache, lo - 1, static_cast<int64_t>(a.start[lo - 1]) + t - a.offsets[lo - 1]);
+}
 
 __device__ __forceinline__ void turn(int64_t pos, unsigned long long step, float mag, float& co, float& si) {
   const unsigned long long ph = static_cast<unsigned long long>(pos) * step;
@@ -68,22 +93,23 @@ __device__ __forceinline__ int64_t position_of(const RotArgs& a, int64_t tok) {
   return a.pos64 ? static_cast<const int64_t*>(a.pos)[tok] : static_cast<int64_t>(static_cast<const int*>(a.pos)[tok]);
 }
 
-// Element e of a row, rotated if the row turns.
+// Element e of a row, rotated if the row turns.  w, r: the norm's weights and factor, or null.
 template <typename T>
-__device__ __forceinline__ float row_value(const RotArgs& a, const T* x, int e, bool turns, int64_t pos) {
-  if (!turns || e >= a.rot) return to_f32(x[e]);
+__device__ __forceinline__ float row_value(const RotArgs& a, const T* x, int e, bool turns, int64_t pos, const T* w, float r) {
+  auto value = [&](int i) { return w != nullptr ? to_f32(x[i]) * r * to_f32(w[i]) : to_f32(x[i]); };
+  if (!turns || e >= a.rot) return value(e);
   const int half = a.rot / 2;
   const int i = a.interleaved ? e >> 1 : (e < half ? e : e - half);
   const bool second = a.interleaved ? (e & 1) : (e >= half);
   const int other = a.interleaved ? (e ^ 1) : (second ? e - half : e + half);
   float co, si;
   turn(pos, a.step[i], a.mag, co, si);
-  const float x0 = to_f32(x[e]), x1 = to_f32(x[other]);
+  const float x0 = value(e), x1 = value(other);
   return second ? x1 * si + x0 * co : x0 * co - x1 * si;
 }
 
 // Any layout: one warp per (token, head) row.
-template <typename T, bool WRITE>
+template <typename T, bool WRITE, bool NORM>
 __global__ void __launch_bounds__(256) rotary_rows_kernel(const __grid_constant__ RotArgs a) {
   const int lane = threadIdx.x & 31;
   const int64_t per_tok = a.q.heads + a.k.heads + a.v.heads;
@@ -99,13 +125,21 @@ __global__ void __launch_bounds__(256) rotary_rows_kernel(const __grid_constant_
     const T* x = static_cast<const T*>(s.p) + b * s.sb + t * s.st + h * s.sh;
     const bool turns = which < 2 && a.rot > 0;
     const int64_t pos = turns ? position_of(a, tok) : 0;
-    if (!WRITE || which == 0) {
-      T* y = static_cast<T*>(which == 0 ? a.q_out : a.k_out) + (tok * s.heads + h) * a.d;
-      for (int e = lane; e < a.d; e += 32) y[e] = from_f32<T>(row_value<T>(a, x, e, turns, pos));
-      continue;
+    const T* w = NORM ? static_cast<const T*>(which == 0 ? a.qw : (which == 1 ? a.kw : nullptr)) : nullptr;
+    float norm = 1.f;
+    if (NORM && w != nullptr) {
+      float sum = 0.f;
+      for (int e = lane; e < a.d; e += 32) sum += to_f32(x[e]) * to_f32(x[e]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      norm = rsqrtf(sum / static_cast<float>(a.d) + a.eps);
     }
-    if (a.counts != nullptr && t >= a.counts[b]) continue;
-    const int64_t row0 = kv_row(a.cache, b, static_cast<int64_t>(a.start[b]) + t);
+    if (!WRITE || which == 0 || (NORM && which == 1 && a.k_out != nullptr)) {
+      T* y = static_cast<T*>(which == 0 ? a.q_out : a.k_out) + (tok * s.heads + h) * a.d;
+      for (int e = lane; e < a.d; e += 32) y[e] = from_f32<T>(row_value<T>(a, x, e, turns, pos, w, norm));
+      if (!WRITE || which == 0) continue;
+    }
+    const int64_t row0 = target_row(a, b, t);
     if (row0 < 0) continue;
     const int64_t row = row0 + static_cast<int64_t>(h) * a.cache.page;
     float v[kKvMaxDim / 32];
@@ -113,7 +147,7 @@ __global__ void __launch_bounds__(256) rotary_rows_kernel(const __grid_constant_
 #pragma unroll
     for (int i = 0; i < kKvMaxDim / 32; ++i) {
       const int e = lane + 32 * i;
-      v[i] = e < a.d ? row_value<T>(a, x, e, turns, pos) : 0.f;
+      v[i] = e < a.d ? row_value<T>(a, x, e, turns, pos, w, norm) : 0.f;
       m = fmaxf(m, fabsf(v[i]));
     }
 #pragma unroll
@@ -206,9 +240,12 @@ __device__ __forceinline__ void codes16(const float* x, float sc, float rcp, uin
 // memory; a group takes every `gpt`-th row of its token.  Bound by the bytes where tokens are many (which
 // wants many warps: with each lane's sines in its registers four warps a scheduler did not cover the
 // latency), by latency where they are few, for which the host spreads a token over more groups.
-template <typename T, int L, bool WRITE, bool INTER>
+// NORM: a row's squares are summed over its L lanes by shuffles between the read and the turn; the weights lie
+// in shared memory, four of a lane beside its neighbours' four, so that a row's reads meet no bank twice.
+template <typename T, int L, bool WRITE, bool INTER, bool NORM>
 __global__ void __launch_bounds__(256, WRITE ? 3 : 4) rotary_vec_kernel(const __grid_constant__ RotArgs a, int gpt) {
   constexpr int D = 16 * L;
+  __shared__ float4 weights_of[NORM ? 2 * D / 4 : 1];  // [q, k][a lane's four times four][lane]
   // (cos, sin) of the CTA's tokens' pairs: 256 / (gpt L) tokens of rot / 2 <= 8 L pairs, so gpt is 8 at least
   __shared__ __align__(16) float2 turns_of[256];
   const int j = threadIdx.x % L;
@@ -226,7 +263,7 @@ __global__ void __launch_bounds__(256, WRITE ? 3 : 4) rotary_vec_kernel(const __
   const int hq = a.q.heads, hqk = hq + a.k.heads;
   const int rows = tok < a.b * a.t ? hqk + a.v.heads : 0;  // (the same for a whole group: the shuffles stay inside one)
   int64_t krow = -1;
-  if (WRITE && rows > 0 && (a.counts == nullptr || t < a.counts[b]))
+  if (WRITE && !NORM && rows > 0 && (a.counts == nullptr || t < a.counts[b]))
     krow = kv_row(a.cache, b, static_cast<int64_t>(a.start[b]) + t);
   const unsigned lanes = L == 32 ? 0xffffffffu : ((1u << L) - 1u) << ((threadIdx.x & 31) / L * L);
   // The next row is on its way while one is turned, the first while the sines are computed.  8191 tokens of 72
@@ -244,6 +281,18 @@ __global__ void __launch_bounds__(256, WRITE ? 3 : 4) rotary_vec_kernel(const __
   };
   uint4 next[2];
   fetch(g, next);
+  if constexpr (NORM) {
+    if (WRITE && rows > 0) krow = target_row(a, b, t);
+    // four c of lane l: its elements 4 c .., as the rows' chunks below have them
+    for (int n = threadIdx.x; n < 2 * D; n += 256) {
+      const T* w = static_cast<const T*>(n < D ? a.qw : a.kw);
+      const int c = n % D / (4 * L), l = n % D / 4 % L, k = n % 4;
+      const bool turned = l < a.rot / 16;
+      const int e = (c < 2 ? (turned ? 8 * l : a.rot / 2 + 8 * l) : (turned ? a.rot / 2 + 8 * l : D / 2 + 8 * l)) +
+                    c % 2 * 4 + k;
+      if (w != nullptr) reinterpret_cast<float*>(weights_of)[n] = to_f32(w[e]);
+    }
+  }
   for (int e = threadIdx.x; e < in_cta * half; e += 256) {
     const int k = e / half;
     if (tok0 + k < a.b * a.t) {
@@ -268,6 +317,23 @@ __global__ void __launch_bounds__(256, WRITE ? 3 : 4) rotary_vec_kernel(const __
     float v[16];
     unpack8<T>(raw[0], v);
     unpack8<T>(raw[1], v + 8);
+    if (NORM && !plain && (which == 0 ? a.qw : a.kw) != nullptr) {
+      float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) sum = __ffma2_rn(make_float2(v[i], v[i + 1]), make_float2(v[i], v[i + 1]), sum);
+      float all = sum.x + sum.y;
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) all += __shfl_xor_sync(lanes, all, o);
+      const float r = rsqrtf(all * (1.0f / D) + a.eps);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float4 w = weights_of[which * (D / 4) + c * L + j];
+        v[4 * c] *= r * w.x;
+        v[4 * c + 1] *= r * w.y;
+        v[4 * c + 2] *= r * w.z;
+        v[4 * c + 3] *= r * w.w;
+      }
+    }
     if (turns && !plain) {
 #pragma unroll
       for (int p = 0; p < 4; ++p) {  // two pairs
@@ -284,11 +350,11 @@ __global__ void __launch_bounds__(256, WRITE ? 3 : 4) rotary_vec_kernel(const __
         y1 = w0 * cs.w + w1 * cs.z;
       }
     }
-    if (!WRITE || which == 0) {
+    if (!WRITE || which == 0 || (NORM && which == 1 && a.k_out != nullptr)) {
       T* y = static_cast<T*>(which == 0 ? a.q_out : a.k_out) + (tok * (which == 0 ? hq : a.k.heads) + hh) * D;
       *reinterpret_cast<uint4*>(y + f0) = pack8<T>(v);
       *reinterpret_cast<uint4*>(y + f1) = pack8<T>(v + 8);
-      continue;
+      if (!WRITE || which == 0) continue;
     }
     float m = 0.f;
 #pragma unroll
@@ -313,7 +379,7 @@ static bool rows_aligned(const RowSet& s) {
   return s.heads == 0 || (aligned16(s.p) && s.sb % 8 == 0 && s.st % 8 == 0 && s.sh % 8 == 0);
 }
 
-template <typename T, int L>
+template <typename T, int L, bool NORM>
 static int launch_rotary_vec(const RotArgs& a, bool write, cudaStream_t st) {
   // Row groups of a token: eight (a lane's sines then serve many rows), more where the tokens alone do not
   // fill the SMs, up to one for each row.
@@ -325,34 +391,42 @@ static int launch_rotary_vec(const RotArgs& a, bool write, cudaStream_t st) {
   if (blocks > INT32_MAX) return fail(BW_ERR_INVALID_ARGUMENT, "rotary: too many tokens");
   const unsigned grid = static_cast<unsigned>(blocks);
   if (write) {
-    if (a.interleaved) rotary_vec_kernel<T, L, true, true><<<grid, 256, 0, st>>>(a, gpt);
-    else rotary_vec_kernel<T, L, true, false><<<grid, 256, 0, st>>>(a, gpt);
+    if (a.interleaved) rotary_vec_kernel<T, L, true, true, NORM><<<grid, 256, 0, st>>>(a, gpt);
+    else rotary_vec_kernel<T, L, true, false, NORM><<<grid, 256, 0, st>>>(a, gpt);
   } else {
-    if (a.interleaved) rotary_vec_kernel<T, L, false, true><<<grid, 256, 0, st>>>(a, gpt);
-    else rotary_vec_kernel<T, L, false, false><<<grid, 256, 0, st>>>(a, gpt);
+    if (a.interleaved) rotary_vec_kernel<T, L, false, true, NORM><<<grid, 256, 0, st>>>(a, gpt);
+    else rotary_vec_kernel<T, L, false, false, NORM><<<grid, 256, 0, st>>>(a, gpt);
   }
   return check_launch("rotary_vec_kernel");
 }
 
-template <typename T>
+template <typename T, bool NORM>
 static int launch_rotary(const RotArgs& a, bool write, cudaStream_t st) {
   const int64_t rows = a.b * a.t * (a.q.heads + a.k.heads + a.v.heads);
   if (rows == 0) return BW_OK;
   if (a.rot % 16 == 0 && rows_aligned(a.q) && rows_aligned(a.k) && rows_aligned(a.v) && aligned16(a.q_out) &&
       aligned16(a.k_out) && aligned16(a.cache.k) && aligned16(a.cache.v)) {
     switch (a.d) {
-      case 32: return launch_rotary_vec<T, 2>(a, write, st);
-      case 64: return launch_rotary_vec<T, 4>(a, write, st);
-      case 128: return launch_rotary_vec<T, 8>(a, write, st);
-      case 256: return launch_rotary_vec<T, 16>(a, write, st);
+      case 32: return launch_rotary_vec<T, 2, NORM>(a, write, st);
+      case 64: return launch_rotary_vec<T, 4, NORM>(a, write, st);
+      case 128: return launch_rotary_vec<T, 8, NORM>(a, write, st);
+      case 256: return launch_rotary_vec<T, 16, NORM>(a, write, st);
       default: break;
     }
   }
   const int64_t blocks = (rows + 7) / 8;
   const int grid = static_cast<int>(blocks < 16L * num_sms() ? blocks : 16L * num_sms());
-  if (write) rotary_rows_kernel<T, true><<<grid, 256, 0, st>>>(a);
-  else rotary_rows_kernel<T, false><<<grid, 256, 0, st>>>(a);
+  if (write) rotary_rows_kernel<T, true, NORM><<<grid, 256, 0, st>>>(a);
+  else rotary_rows_kernel<T, false, NORM><<<grid, 256, 0, st>>>(a);
   return check_launch("rotary_rows_kernel");
+}
+
+// Without weights, packed rows and keys to keep it is the rotation alone, and its results are that one's.
+static int launch_norm_rotary(const RotArgs& a, int dtype, bool write, cudaStream_t st) {
+  const bool more = a.qw != nullptr || a.kw != nullptr || (write && (a.offsets != nullptr || a.k_out != nullptr));
+  if (dtype == BW_DTYPE_BF16)
+    return more ? launch_rotary<__nv_bfloat16, true>(a, write, st) : launch_rotary<__nv_bfloat16, false>(a, write, st);
+  return more ? launch_rotary<__half, true>(a, write, st) : launch_rotary<__half, false>(a, write, st);
 }
 
 static int check_rows(const RowSet& s, int64_t b, int64_t t, int d, const char* name, const char* op) {
@@ -690,7 +764,7 @@ extern "C" int bw_rotary(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh
   if ((hq > 0 && !q_out) || (hk > 0 && !k_out)) return fail(BW_ERR_INVALID_ARGUMENT, "rotary: null output pointer");
   if (int s = require_sm100()) return s;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == BW_DTYPE_BF16 ? launch_rotary<__nv_bfloat16>(a, false, st) : launch_rotary<__half>(a, false, st);
+  return dtype == BW_DTYPE_BF16 ? launch_rotary<__nv_bfloat16, false>(a, false, st) : launch_rotary<__half, false>(a, false, st);
 }
 
 extern "C" int bw_rotary_kv_write_int8(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int hq, const void* k,
@@ -725,7 +799,85 @@ extern "C" int bw_rotary_kv_write_int8(const void* q, int64_t q_sb, int64_t q_st
   if (!start || (hq > 0 && !q_out)) return fail(BW_ERR_INVALID_ARGUMENT, "kv_write_int8: null pointer");
   if (int s = require_sm100()) return s;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == BW_DTYPE_BF16 ? launch_rotary<__nv_bfloat16>(a, true, st) : launch_rotary<__half>(a, true, st);
+  return dtype == BW_DTYPE_BF16 ? launch_rotary<__nv_bfloat16, false>(a, true, st) : launch_rotary<__half, false>(a, true, st);
+}
+
+extern "C" int bw_norm_rotary(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int hq, const void* k,
+                              int64_t k_sb, int64_t k_st, int64_t k_sh, int hk, void* q_out, void* k_out, int dtype,
+                              int64_t b, int64_t t, int64_t d, const void* q_weight, const void* k_weight, float eps,
+                              const void* positions, int positions64, const uint64_t* steps, float magnitude,
+                              int64_t rot, int interleaved, void* stream) {
+  using namespace bw;
+  RotArgs a = {};
+  a.q = {q, q_sb, q_st, q_sh, hq};
+  a.k = {k, k_sb, k_st, k_sh, hk};
+  a.q_out = q_out;
+  a.k_out = k_out;
+  a.b = b;
+  a.t = t;
+  a.d = d > 0 && d <= kKvMaxDim ? static_cast<int>(d) : 0;
+  a.rot = rot >= 0 && rot <= kKvMaxDim ? static_cast<int>(rot) : -1;
+  a.interleaved = interleaved;
+  a.mag = magnitude;
+  a.pos = positions;
+  a.pos64 = positions64;
+  a.step = reinterpret_cast<const unsigned long long*>(steps);
+  a.qw = q_weight;
+  a.kw = k_weight;
+  a.eps = eps;
+  if (int s = check_rot(a, dtype, "norm_rotary")) return s;
+  if (!(eps >= 0.f)) return fail(BW_ERR_INVALID_ARGUMENT, "norm_rotary: eps must not be negative");
+  if (b == 0 || t == 0) return BW_OK;
+  if ((hq > 0 && !q_out) || (hk > 0 && !k_out)) return fail(BW_ERR_INVALID_ARGUMENT, "norm_rotary: null output pointer");
+  if (int s = require_sm100()) return s;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return launch_norm_rotary(a, dtype, false, st);
+}
+
+extern "C" int bw_norm_rotary_kv_write_int8(
+    const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int hq, const void* k, int64_t k_sb, int64_t k_st,
+    int64_t k_sh, const void* v, int64_t v_sb, int64_t v_st, int64_t v_sh, void* q_out, void* k_out, int dtype,
+    int64_t b, int64_t t, const void* q_weight, const void* k_weight, float eps, const void* positions,
+    int positions64, const uint64_t* steps, float magnitude, int64_t rot, int interleaved, int8_t* cache_k,
+    int8_t* cache_v, float* k_scale, float* v_scale, int64_t pages, int64_t heads, int64_t page, int64_t d,
+    const int32_t* table, int64_t table_ld, int64_t table_cols, const int32_t* start, const int32_t* counts,
+    const int32_t* offsets, void* stream) {
+  using namespace bw;
+  constexpr const char* op = "norm_rotary_kv_write_int8";
+  RotArgs a = {};
+  a.cache = make_cache(cache_k, cache_v, k_scale, v_scale, pages, heads, page, d, table, table_ld, table_cols);
+  if (b < 0 || b > INT32_MAX) return fail(BW_ERR_INVALID_ARGUMENT, "%s: need 0 <= b < 2^31", op);
+  if (int s = check_kv_cache(a.cache, b, op)) return s;
+  a.q = {q, q_sb, q_st, q_sh, hq};
+  a.k = {k, k_sb, k_st, k_sh, a.cache.heads};
+  a.v = {v, v_sb, v_st, v_sh, a.cache.heads};
+  a.q_out = q_out;
+  a.k_out = k_out;
+  a.b = offsets != nullptr ? 1 : b;  // packed rows are one sequence of them to what reads and turns them
+  a.t = t;
+  a.seqs = b;
+  a.offsets = offsets;
+  a.d = a.cache.d;
+  a.rot = rot >= 0 && rot <= kKvMaxDim ? static_cast<int>(rot) : -1;
+  a.interleaved = interleaved;
+  a.mag = magnitude;
+  a.pos = positions;
+  a.pos64 = positions64;
+  a.step = reinterpret_cast<const unsigned long long*>(steps);
+  a.start = start;
+  a.counts = counts;
+  a.qw = q_weight;
+  a.kw = k_weight;
+  a.eps = eps;
+  if (int s = check_rot(a, dtype, op)) return s;
+  if (!(eps >= 0.f)) return fail(BW_ERR_INVALID_ARGUMENT, "%s: eps must not be negative", op);
+  if (offsets != nullptr && counts != nullptr)
+    return fail(BW_ERR_INVALID_ARGUMENT, "%s: packed rows have offsets, no counts", op);
+  if (a.b == 0 || t == 0) return BW_OK;
+  if ((!start && b > 0) || (hq > 0 && !q_out)) return fail(BW_ERR_INVALID_ARGUMENT, "%s: null pointer", op);
+  if (int s = require_sm100()) return s;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return launch_norm_rotary(a, dtype, true, st);
 }
 
 extern "C" int bw_kv_read_int8(const int8_t* cache_k, const int8_t* cache_v, const float* k_scale,

@@ -337,6 +337,33 @@ int bw_rotary_kv_write_int8(const void* q, int64_t q_sb, int64_t q_st, int64_t q
                             int64_t table_cols, const int32_t* start, const int32_t* counts, void* stream);
 
 /*
+ * Norms of queries and keys for each head, and the rotation, in one pass: as bw_rotary, of
+ *   y = w x / sqrt(mean(x^2) + eps)   over the d elements of each head, in 32 bits, not rounded before it turns.
+ * q_weight, k_weight [d] in dtype; a NULL one leaves its rows as they are.
+ */
+int bw_norm_rotary(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int hq, const void* k, int64_t k_sb,
+                   int64_t k_st, int64_t k_sh, int hk, void* q_out, void* k_out, int dtype, int64_t b, int64_t t,
+                   int64_t d, const void* q_weight, const void* k_weight, float eps, const void* positions,
+                   int positions64, const uint64_t* steps, float magnitude, int64_t rot, int interleaved, void* stream);
+
+/*
+ * The same with the write of bw_rotary_kv_write_int8: normalised and turned keys are quantised from their 32-bit
+ * values, values as they are.  k_out [b, t, heads, d] (or NULL): the keys of all tokens, rounded to dtype.
+ * offsets == NULL: b sequences of t tokens each, counts as there.  offsets [b + 1]: the inputs are t packed rows
+ * (the strides of b are not used, positions are [t]); rows offsets[i] .. offsets[i + 1] are sequence i's and go to
+ * slots start[i] on; rows before the first and behind the last sequence are not written.  counts is then NULL.
+ */
+int bw_norm_rotary_kv_write_int8(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int hq, const void* k,
+                                 int64_t k_sb, int64_t k_st, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_st,
+                                 int64_t v_sh, void* q_out, void* k_out, int dtype, int64_t b, int64_t t,
+                                 const void* q_weight, const void* k_weight, float eps, const void* positions,
+                                 int positions64, const uint64_t* steps, float magnitude, int64_t rot,
+                                 int interleaved, int8_t* cache_k, int8_t* cache_v, float* k_scale, float* v_scale,
+                                 int64_t pages, int64_t heads, int64_t page, int64_t d, const int32_t* table,
+                                 int64_t table_ld, int64_t table_cols, const int32_t* start, const int32_t* counts,
+                                 const int32_t* offsets, void* stream);
+
+/*
  * Read slots start[b] + i, i < n, back as values: k_out, v_out [layers, b, n, heads, d] in dtype
  * (F16 | BF16) = dt(code * scale).  start == NULL: 0.  Slots i >= lens[b] (lens given) are zeros.
  */

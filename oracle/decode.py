@@ -159,3 +159,11 @@ def verify(p, tokens, parents, u, e, draft=None):
             score = np.where(w > 0, w / e[b].astype(f), f(-1))
         out[b, n[b]] = int(np.argmax(score)) if (w > 0).any() else 0
     return n, path, out
+
+
+def norm(x, w, eps):
+    """w x / sqrt(mean(x^2) + eps) over the last dimension, float64 (w None: x)."""
+    x = np.asarray(x, dtype=np.float64)
+    if w is None:
+        return x
+    return x / np.sqrt((x * x).mean(-1, keepdims=True) + eps) * np.asarray(w, dtype=np.float64)
