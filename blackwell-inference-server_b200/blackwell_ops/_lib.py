@@ -104,6 +104,9 @@ SIGNATURES = {
     "bw_tree_attention_int8": (_c.c_int, [_P, _I64, _I64, _I64, _c.c_int, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64,
                                           _P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _c.c_float, _P, _c.c_size_t,
                                           _P]),
+    "bw_prompt_attention": (_c.c_int, [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _c.c_int, _P, _P, _I64, _I64, _I64,
+                                       _I64, _I64, _c.c_float, _P]),
+    "bw_token_logprobs": (_c.c_int, [_P, _c.c_int, _I64, _P, _I64, _I64, _I64, _P, _P, _P, _P, _P]),
     "bw_verify_tree": (_c.c_int, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _P, _P]),
     "bw_set_wait_limit_ns": (_c.c_int, [_c.c_uint64]),
     "bw_get_wait_limit_ns": (_c.c_int, [_c.POINTER(_c.c_uint64)]),

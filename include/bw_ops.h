@@ -414,6 +414,29 @@ int bw_tree_attention_int8(const void* q, int64_t q_sb, int64_t q_st, int64_t q_
                            void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * Causal attention over whole prompts, packed: rows offsets[i] .. offsets[i + 1] of q [n, hq, d], k and v [n, hk, d] are
+ * sequence i's (offsets int32 [b + 1] on the device, not descending), and row r of a sequence sees its rows 0 .. r:
+ *   out_r = sum_j w_rj v_j / sum_j w_rj,  w_rj = exp(softmax_scale * q_r . k_j)
+ * out [n, hq, d] contiguous, in the inputs' dtype (F16 | BF16); rows of no sequence are zeros.  Strides are in elements,
+ * with unit stride in d; hq is a multiple of hk (query head h reads key head h / (hq / hk)); d <= 256.  Scores, sums and
+ * outputs accumulate in fp32.  Results of a sequence do not depend on the others.
+ */
+int bw_prompt_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
+                        const void* v, int64_t v_st, int64_t v_sh, int dtype, void* out, const int32_t* offsets,
+                        int64_t b, int64_t n, int64_t hq, int64_t hk, int64_t d, float softmax_scale, void* stream);
+
+/*
+ * Log probabilities of given tokens: logits [rows, v] (F16 | BF16 | F32, row stride ld), tokens [rows] int64;
+ *   logprobs[r] = x_t - ln sum_i exp(x_i) with t = tokens[r], 0 where t is outside [0, v);  entropy[r] = -sum p ln p;
+ *   top_logprobs, top_tokens [rows, top]: the `top` largest, by value and then by lowest token (top <= 32, <= v).
+ * Logits of -inf have no probability; a row of nothing else has entropy 0 and log probabilities of -inf.  A row with a
+ * NaN or +inf gives NaN, and tokens -1.  Sums in fp32, in one order.
+ */
+int bw_token_logprobs(const void* logits, int dtype, int64_t ld, const int64_t* tokens, int64_t rows, int64_t v,
+                      int64_t top, float* logprobs, float* entropy, float* top_logprobs, int64_t* top_tokens,
+                      void* stream);
+
+/*
  * Verify drafted tokens: tokens[b, i] is node i's token (node 0, the root, is the last committed
  * token), target[b, i, :] the target model's probabilities of the token after node i, draft[b, i, :]
  * the distribution from which node i's children were drawn (draft == NULL: drafts without one, as
