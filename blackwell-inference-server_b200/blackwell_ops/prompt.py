@@ -24,13 +24,26 @@ MAX_TOP = 32  # alternatives of a token
 _LOGITS = (torch.float16, torch.bfloat16, torch.float32)
 
 
+def _tiled(x: torch.Tensor, n: int, heads: int, st: int, sh: int) -> tuple[torch.Tensor, int, int]:
+    """x [n, heads, D], its strides of a row and a head; a copy unless its rows lie as the tensor-core kernel's copies
+    want them: each on a 16-byte boundary, none twice."""
+    if not (x.data_ptr() % 16 or st % 8 or sh % 8 or (st == 0 and n > 1) or (sh == 0 and heads > 1)):
+        return x, st, sh
+    x = x.clone(memory_format=torch.contiguous_format)
+    return x, *x.stride()[-3:-1]
+
+
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor,
                      softmax_scale: float | None = None) -> torch.Tensor:
     """Causal attention over packed prompts: q [N, Hq, D], k and v [N, Hk, D] (fp16 or bf16) -> [N, Hq, D].
 
     Row i of a sequence sees the sequence's rows up to itself.  ``offsets`` [B + 1] int32, not descending; rows of no
     sequence (before ``offsets[0]``, behind ``offsets[B]``) give zeros.  Query head h reads key head
-    ``h // (Hq / Hk)``.  ``softmax_scale`` defaults to ``D ** -0.5``.  A sequence's results do not depend on the others."""
+    ``h // (Hq / Hk)``.  ``softmax_scale`` defaults to ``D ** -0.5``.  A sequence's results do not depend on the others.
+
+    The tensor-core kernel takes D = 64 or 128, at most 128 query heads a key head and a positive scale (rows that do not
+    start on 16-byte boundaries are copied first); other calls go to a plain kernel, a hundred times slower on long
+    prompts."""
     if q.dim() != 3:
         raise RuntimeError("q must be [N, heads, D]")
     lead = q.shape[:-2]
@@ -53,6 +66,10 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     if offsets.dim() != 1 or offsets.shape[0] == 0:
         raise RuntimeError("offsets must be [B + 1]")
     offsets = offsets.contiguous()
+    if d in (64, 128):
+        q, qt, qh = _tiled(q, n, hq, qt, qh)
+        k, kt, kh = _tiled(k, n, hk, kt, kh)
+        v, vt, vh = _tiled(v, n, hk, vt, vh)
     out = _new(shape, dt, dev)
     _call("prompt_attention", dev, lib.bw_prompt_attention, q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
           DTYPE_CODE[dt], out.data_ptr(), offsets.data_ptr(), offsets.shape[0] - 1, n, hq, hk, d,

@@ -3,8 +3,8 @@
     python blackwell-inference-server_b200/csrc/build.py [--verbose]
 
 Compiles every ``*.cu`` here with nvcc for ``-gencode arch=compute_100a,code=sm_100a``
-(relocatable device code, so the kernels share one device status word; one file is a
-whole program and gets the word's address), links
+(relocatable device code, so the kernels share one device status word; the files of
+``WHOLE_PROGRAM`` are whole programs and get the word's address), links
 them into ``blackwell_ops/_lib/libbw_ops.so`` next to the Python package, and
 skips objects whose sources and headers are unchanged.  No ``--use_fast_math``:
 the quantiser and merge must use IEEE division and round-to-nearest-even.
@@ -30,7 +30,7 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CFLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-O2", "-I", str(INCLUDE)]
 # Compiled on its own: ptxas ignores setmaxnreg in relocatable device code.  Such a file defines
 # BW_WHOLE_PROGRAM and gets the shared status word's address from the host.
-WHOLE_PROGRAM = {"tree_attention.cu"}
+WHOLE_PROGRAM = {"tree_attention.cu", "prompt_attention.cu"}
 
 
 def nvcc() -> str:

@@ -127,6 +127,25 @@ int make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dt, uin
   return BW_OK;
 }
 
+int make_tmap_3d(CUtensorMap* map, const void* base, CUtensorMapDataType dt, const uint64_t (&dims)[3],
+                 const uint64_t (&strides_bytes)[2], const uint32_t (&box)[3], CUtensorMapSwizzle swz) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(BW_ERR_UNSUPPORTED, "cuTensorMapEncodeTiled is unavailable from the driver");
+  const cuuint64_t gdim[3] = {dims[0], dims[1], dims[2]};
+  const cuuint64_t gstride[2] = {strides_bytes[0], strides_bytes[1]};
+  const cuuint32_t gbox[3] = {box[0], box[1], box[2]};
+  const cuuint32_t estride[3] = {1, 1, 1};
+  const CUresult r = fn(map, dt, 3, const_cast<void*>(base), gdim, gstride, gbox, estride,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(BW_ERR_INVALID_ARGUMENT,
+                "cuTensorMapEncodeTiled failed (%d): %llux%llux%llu strides %llu, %llu box %ux%ux%u base=%p", (int)r,
+                (unsigned long long)dims[0], (unsigned long long)dims[1], (unsigned long long)dims[2],
+                (unsigned long long)strides_bytes[0], (unsigned long long)strides_bytes[1], box[0], box[1], box[2], base);
+  return BW_OK;
+}
+
 }  // namespace bw
 
 extern "C" const char* bw_status_string(int status) {

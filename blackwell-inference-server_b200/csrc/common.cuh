@@ -354,6 +354,15 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, u
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "l"(policy)
       : "memory");
 }
+// 3-D tiled load global -> this CTA's shared memory, completion counted on `bar`.
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z,
+                                            uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4, %5}], [%2], %6;" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "l"(policy)
+      : "memory");
+}
 // 1-D bulk copy global -> this CTA's shared memory (both addresses 16-byte
 // aligned, `bytes` a multiple of 16), completion counted on `bar`.
 __device__ __forceinline__ void bulk_load_1d(void* dst, const void* src, uint32_t bytes, uint64_t* bar,
@@ -531,9 +540,27 @@ __host__ __device__ constexpr uint32_t make_idesc_f16(int M, int N, bool bf16, b
          ((b_mn_major ? 1u : 0u) << 16) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
 
+// Registers of a warpgroup's threads, given back or taken (all of its warps; whole-program files only).
+template <int N>
+__device__ __forceinline__ void setmaxnreg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void setmaxnreg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+
 // ---------------------------------------------------------------------------
 // small numeric helpers
 // ---------------------------------------------------------------------------
+// 2^x to 2 ulps; 0 for -inf and below the normal range.
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
 // Four int8 codes (one 32-bit word) -> two f16x2 words, exactly.  Each byte is
 // biased to u = q + 128 in [1, 255], placed in the mantissa of 1024.0
 // (0x6400 | u == 1024 + u) and 1152 = 1024 + 128 is subtracted.
@@ -590,6 +617,9 @@ int dtype_size(int dtype);
 // `ld_bytes`, box box_rows x box_cols, 128-byte swizzle.
 int make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dt, uint64_t rows, uint64_t cols,
                  uint64_t ld_bytes, uint32_t box_rows, uint32_t box_cols, CUtensorMapSwizzle swz);
+// The same in three dimensions, the first contiguous; strides of the second and third, box sizes in elements.
+int make_tmap_3d(CUtensorMap* map, const void* base, CUtensorMapDataType dt, const uint64_t (&dims)[3],
+                 const uint64_t (&strides_bytes)[2], const uint32_t (&box)[3], CUtensorMapSwizzle swz);
 int num_sms();
 // Device addresses of the current device's status word and wait limit.
 int device_wait_ptrs(int** status, const long long** limit);

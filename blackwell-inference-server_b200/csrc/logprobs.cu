@@ -31,11 +31,6 @@ struct LogprobArgs {
   int v, top;
 };
 
-__device__ __forceinline__ float lp_exp2(float x) {  // 2^x to 2 ulps, 0 for -inf
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kNoWeight = -200.f;  // a power of two that is 0, finite: 0 times it is 0
 
@@ -46,7 +41,7 @@ struct LpSums {
 __device__ __forceinline__ LpSums lp_join(const LpSums& a, const LpSums& b) {
   const float m = fmaxf(a.m, b.m);
   const float da = fmaxf((a.m - m) * kLog2e, kNoWeight), db = fmaxf((b.m - m) * kLog2e, kNoWeight);
-  const float fa = lp_exp2(da), fb = lp_exp2(db);
+  const float fa = exp2_approx(da), fb = exp2_approx(db);
   return {m, fa * a.s + fb * b.s, fa * (a.t + da * a.s) + fb * (b.t + db * b.s)};
 }
 
@@ -171,7 +166,7 @@ __global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(const Logpro
 #pragma unroll
     for (int e = 2; e < 8; ++e) top = fmaxf(top, f[e]);
     if (top > sum.m) {
-      const float d = fmaxf((sum.m - top) * kLog2e, kNoWeight), w = lp_exp2(d);
+      const float d = fmaxf((sum.m - top) * kLog2e, kNoWeight), w = exp2_approx(d);
       sum.t = w * (sum.t + d * sum.s);
       sum.s *= w;
       sum.m = top;
@@ -184,7 +179,7 @@ __global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(const Logpro
     for (int e = 0; e < 8; e += 2) {
       // the difference first: times log2 e a 16-bit type's lowest value would pass the range
       const float2 z = __fmul2_rn(__fadd2_rn(make_float2(f[e], f[e + 1]), m2), c2);
-      const float2 w = make_float2(lp_exp2(z.x), lp_exp2(z.y));
+      const float2 w = make_float2(exp2_approx(z.x), exp2_approx(z.y));
       s = __fadd2_rn(s, w);
       t = __ffma2_rn(w, make_float2(fmaxf(z.x, kNoWeight), fmaxf(z.y, kNoWeight)), t);
     }

@@ -10,7 +10,9 @@
 #include <stdio.h>
 
 #include <mutex>
+#include <type_traits>
 
+#define BW_WHOLE_PROGRAM
 #include "kv_cache.cuh"
 
 namespace bw {
@@ -36,9 +38,8 @@ __device__ __forceinline__ int64_t prompt_edge(const PromptArgs& a, int i) {  //
   const int64_t e = a.offsets[i - 1];
   return e < 0 ? 0 : (e < a.n ? e : a.n);
 }
-// Block number `slot`; the last blocks of a sequence, which see most keys, come first.
-template <int P>
-__device__ __forceinline__ bool prompt_block(const PromptArgs& a, int64_t slot, PromptBlock& blk) {
+// Block number `slot` of P rows; the last blocks of a sequence, which see most keys, come first.
+__device__ __forceinline__ bool prompt_block(const PromptArgs& a, int P, int64_t slot, PromptBlock& blk) {
   int lo = 0, hi = a.b + 1;  // the last segment whose numbers start at `slot` or before
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -71,7 +72,7 @@ __global__ void __launch_bounds__(128) prompt_rows_kernel(const PromptArgs a) {
   float* sv = sk + kRowsK * ld;   // [32][d]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   PromptBlock blk;
-  if (!prompt_block<kRowsQ>(a, blockIdx.x, blk)) return;
+  if (!prompt_block(a, kRowsQ, blockIdx.x, blk)) return;
   const int rows = static_cast<int>(blk.row1 - blk.row0);
   const int h = blockIdx.y, hk = h / (a.hq / a.hk);
   T* out = static_cast<T*>(a.o);
@@ -165,6 +166,627 @@ static int launch_rows(const PromptArgs& a, cudaStream_t st) {
   return check_launch("prompt_rows_kernel");
 }
 
+// ---------------------------------------------------------------------------
+// tensor-core kernel (head dimensions 64 and 128)
+//
+// A tile is 128 rows of queries: P = 128 / group positions with the query heads that read one key head, row = position *
+// group + head.  A CTA takes two neighbouring tiles A and B of a key head and walks their sequence's keys, 128 at a time:
+//   S [128 x 128 keys] = Q [128 x D] (shared memory) . K^T (shared memory)        fp32, in TMEM
+//   O [128 x D]       += P [128 x 128 keys] (TMEM, over S) . V (shared memory)    fp32, in TMEM
+// Each K and V tile in shared memory serves both query tiles, and while one tile's softmax runs, the other's products do.
+//
+// Softmax: thread = row, so nothing is exchanged.  The reference m moves only when a score exceeds it by more than 8 (in
+// powers of two); only then are the sum and the accumulator rescaled.  Weights 2^(s - m + 7) go to the tensor core in
+// the inputs' type: rounded by half an ulp like the inputs themselves, at most 2^15, and the 7 keeps fp16's subnormal steps
+// at 2^-32 of a row's largest weight.  Their sum and the accumulator are fp32 and have the same factor.
+//
+// Keys that a row does not see have weight 0, but 0 times a value that is not finite is not 0.  So a warp looks through
+// every V tile that some row of the block does not see all of: rows behind the block's last position become zeros,
+// values that are not finite become 0 and are added at the end to the rows that do see them.
+//
+// Blocks are handed out by the hardware: a CTA that nears its end takes the next one that has not started
+// (clusterlaunchcontrol), so the schedule is dynamic without a counter in memory.
+//
+// Twelve warps: 0-3 and 4-7 the softmax of A and B (their TMEM lanes are the rows), 8 TMA loads and watches the time, 9
+// issues the products, 10 looks through V, 11 finds the blocks.
+// ---------------------------------------------------------------------------
+constexpr int kPromptThreads = 384;
+constexpr int kPromptKeys = 128;
+// Registers of a thread of the three warpgroups after setmaxnreg: three times the 168 that a thread of 384 has.
+constexpr int kPromptRegsSoft = 208, kPromptRegsRest = 88;
+static_assert(2 * kPromptRegsSoft + kPromptRegsRest == 3 * 168, "register split");
+constexpr float kPromptSlack = 8.f, kPromptShift = 7.f;
+constexpr float kPromptLowest = -3.0e38f;  // a row's reference without any score: finite, so differences are
+enum PromptSite : int {
+  kSitePrBlock = 501, kSitePrQ = 502, kSitePrK = 503, kSitePrV = 504, kSitePrDrain = 505, kSitePrDone = 506,
+  kSitePrFinal = 507, kSitePrNext = 508
+};
+
+template <int D>
+struct PCfg {
+  static constexpr int TB = D / 64 * kPromptKeys * 128;  // bytes of a tile of Q, K or V: panels of 64 elements
+  static constexpr int KST = D == 128 ? 3 : 4, VST = D == 128 ? 2 : 4;
+  static constexpr int OFF_K = 2 * TB;
+  static constexpr int OFF_V = OFF_K + KST * TB;
+  static constexpr int OFF_CTRL = OFF_V + VST * TB;
+  static constexpr int CTRL = 1024;
+  static constexpr int SMEM = OFF_CTRL + CTRL + 1024;
+  static constexpr int S_COL = 0, O_COL = 256, COLS = 512;
+  static_assert(SMEM <= 227 * 1024, "shared memory");
+};
+
+struct PromptTiles {
+  PromptArgs a;
+  int grp, pos;     // query heads of a key head, positions of a tile
+  int* status;
+  const long long* limit;
+};
+
+// A block as the roles read it; positions relative to the sequence's first row.
+struct PromptInfo {
+  int first, row0, row1, head, n[2], valid;
+};
+
+__device__ __forceinline__ void clc_try_cancel(void* response, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_u32(response)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+// The block taken, or -1: none was left.
+__device__ __forceinline__ int clc_block(const void* response) {
+  int x;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t.reg .b32 y, z, w;\n\t"
+      "ld.shared.b128 r, [%1];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "mov.b32 %0, -1;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, y, z, w}, r;\n\t}\n"
+      : "=r"(x)
+      : "r"(smem_u32(response))
+      : "memory");
+  return x;
+}
+
+// Bits of a packed pair of 16-bit values that are set where one of them is not finite.
+template <typename T>
+__device__ __forceinline__ uint32_t not_finite2(uint32_t w) {
+  if constexpr (std::is_same<T, __half>::value) return ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
+  else return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float2 v) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __float22half2_rn(v);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __float22bfloat162_rn(v);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+template <int D, typename T>
+__global__ void __launch_bounds__(kPromptThreads, 1)
+    prompt_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PromptTiles ta) {
+  using C = PCfg<D>;
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int KEYS = kPromptKeys;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* sQ = smem;
+  uint8_t* sK = smem + C::OFF_K;
+  uint8_t* sV = smem + C::OFF_V;
+  uint64_t* tfull = reinterpret_cast<uint64_t*>(smem + C::OFF_CTRL);  // 2: a block's numbers are there
+  uint64_t* tempty = tfull + 2;        //    all roles are done with them
+  uint64_t* qfull = tempty + 2;        // [A, B]
+  uint64_t* qempty = qfull + 2;
+  uint64_t* kfull = qempty + 2;
+  uint64_t* kempty = kfull + C::KST;
+  uint64_t* vfull = kempty + C::KST;
+  uint64_t* vready = vfull + C::VST;   // looked through
+  uint64_t* vempty = vready + C::VST;
+  uint64_t* sfull = vempty + C::VST;   // [A, B] scores
+  uint64_t* phalf = sfull + 2;         // weights of the first 64 keys, of all
+  uint64_t* pfull = phalf + 2;
+  uint64_t* pvdone = pfull + 2;        // V . P complete
+  uint64_t* oempty = pvdone + 2;       // accumulator read
+  uint64_t* ckfull = oempty + 2;       // 2: a block's values that are not finite are known
+  uint64_t* next_bar = ckfull + 2;
+  uint64_t* done = next_bar + 1;
+  uint64_t* final_bar = done + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(final_bar + 1);
+  WaitControl* ctl = reinterpret_cast<WaitControl*>(final_bar + 2);
+  PromptInfo* info = reinterpret_cast<PromptInfo*>(smem + C::OFF_CTRL + 512);  // [2]
+  uint32_t* odd = reinterpret_cast<uint32_t*>(smem + C::OFF_CTRL + 640);       // [2][3 tiles][128 bits]
+  void* response = smem + C::OFF_CTRL + 768;
+  static_assert((27 + 2 * C::KST + 3 * C::VST) * 8 + 8 + sizeof(WaitControl) <= 512 && sizeof(PromptInfo) <= 64, "control");
+
+  const PromptArgs& a = ta.a;
+  const int warp = warp_uniform(threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  const int P = ta.pos;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tfull[i], 1);
+      mbar_init(&tempty[i], 11);  // loads, products, the look through V, eight softmax warps
+      mbar_init(&qfull[i], 1);
+      mbar_init(&qempty[i], 1);
+      mbar_init(&sfull[i], 1);
+      mbar_init(&phalf[i], 4);
+      mbar_init(&pfull[i], 4);
+      mbar_init(&pvdone[i], 1);
+      mbar_init(&oempty[i], 4);
+      mbar_init(&ckfull[i], 1);
+    }
+    for (int i = 0; i < C::KST; ++i) {
+      mbar_init(&kfull[i], 1);
+      mbar_init(&kempty[i], 1);
+    }
+    for (int i = 0; i < C::VST; ++i) {
+      mbar_init(&vfull[i], 1);
+      mbar_init(&vready[i], 1);
+      mbar_init(&vempty[i], 1);
+    }
+    mbar_init(next_bar, 1);
+    mbar_init(done, 8);
+    mbar_init(final_bar, 1);
+    ctl->abort = 0;
+    ctl->status = ta.status;
+    ctl->limit = ta.limit;
+    fence_mbar_init();
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, C::COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp >= 8) {
+    setmaxnreg_dec<kPromptRegsRest>();
+    if (warp == 8) {
+      // ---------------- TMA ----------------
+      const uint64_t pol = l2_policy_evict_normal();
+      uint32_t qn[2] = {0u, 0u}, kn = 0, vn = 0;  // loads so far
+      auto load = [&](uint8_t* dst, const CUtensorMap* tm, uint64_t* full, uint32_t bytes, int head, int row) {
+        if (elect_one()) {
+          mbar_arrive_expect_tx(full, bytes);
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c) tma_load_3d(dst + c * KEYS * 128, tm, full, c * 64, head, row, pol);
+        }
+        __syncwarp();
+      };
+      const uint32_t q_bytes = static_cast<uint32_t>(P * ta.grp * D * 2);
+      bool ok = true;
+      for (uint32_t n = 0; ok; ++n) {
+        const int sl = n & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait_at(&tfull[sl], (n >> 1) & 1, ctl, kSitePrBlock));
+        if (!ok) break;
+        const PromptInfo t = info[sl];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tempty[sl]);
+        if (!t.valid) break;
+        auto load_q = [&](int w) {
+          if (t.n[w] == 0) return true;
+          const bool fine = mbar_wait_at(&qempty[w], (qn[w] & 1) ^ 1, ctl, kSitePrQ);
+          if (!__all_sync(0xffffffffu, fine)) return false;
+          load(sQ + w * C::TB, &tm_q, &qfull[w], q_bytes, t.head * ta.grp, t.first + t.row0 + w * P);
+          ++qn[w];
+          return true;
+        };
+        const int tiles = max(t.n[0], t.n[1]);
+        ok = load_q(0);
+        for (int i = 0; ok && i < tiles; ++i) {
+          const int ks = kn % C::KST, vs = vn % C::VST;
+          ok = __all_sync(0xffffffffu, mbar_wait_at(&kempty[ks], ((kn / C::KST) & 1) ^ 1, ctl, kSitePrK));
+          if (!ok) break;
+          load(sK + ks * C::TB, &tm_k, &kfull[ks], C::TB, t.head, t.first + i * KEYS);
+          ++kn;
+          if (i == 0) ok = load_q(1);
+          ok = ok && __all_sync(0xffffffffu, mbar_wait_at(&vempty[vs], ((vn / C::VST) & 1) ^ 1, ctl, kSitePrV));
+          if (!ok) break;
+          load(sV + vs * C::TB, &tm_v, &vfull[vs], C::TB, t.head, t.first + i * KEYS);
+          ++vn;
+        }
+      }
+      if (ok) {
+        mbar_wait_at(done, 0, ctl, kSitePrDone);
+      } else {  // wait (bounded) for the copies still in flight into this CTA's shared memory
+        for (uint32_t i = kn > C::KST ? kn - C::KST : 0; i < kn; ++i)
+          mbar_wait_at(&kfull[i % C::KST], (i / C::KST) & 1, ctl, kSitePrDrain, false);
+        for (uint32_t i = vn > C::VST ? vn - C::VST : 0; i < vn; ++i)
+          mbar_wait_at(&vfull[i % C::VST], (i / C::VST) & 1, ctl, kSitePrDrain, false);
+        for (int w = 0; w < 2; ++w)
+          if (qn[w] > 0) mbar_wait_at(&qfull[w], (qn[w] - 1) & 1, ctl, kSitePrDrain, false);
+      }
+    } else if (warp == 9) {
+      // ---------------- products ----------------
+      constexpr uint32_t idesc_s = make_idesc_f16(128, KEYS, BF16, false);
+      constexpr uint32_t idesc_o = make_idesc_f16(128, D, BF16, true);
+      const uint32_t tm = warp_uniform(tmem);
+      const uint32_t q0 = smem_u32(sQ), k0 = smem_u32(sK), v0 = smem_u32(sV);
+      uint32_t kn = 0, vn = 0, seen = 0;               // K tiles begun, V tiles, blocks of A or B
+      uint32_t pn[2] = {0u, 0u}, bn[2] = {0u, 0u};     // V . P and blocks so far
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        ok = ok && __all_sync(0xffffffffu, mbar_wait_or_abort(bar, parity & 1, ctl));
+        return ok;
+      };
+      for (; ok; ++seen) {
+        const int sl = seen & 1;
+        if (!wait(&tfull[sl], seen >> 1)) break;
+        const int nt[2] = {warp_uniform(info[sl].n[0]), warp_uniform(info[sl].n[1])};
+        const int valid = warp_uniform(info[sl].valid);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tempty[sl]);
+        if (!valid) break;
+        const int tiles = max(nt[0], nt[1]);
+        const int last_w = nt[1] > 0 ? 1 : 0;  // the tile that needs a K or V tile last
+        // scores of K tile i for query tile w
+        auto scores = [&](int w, int i) {
+          const uint32_t kt = kn + i;
+          const uint32_t ks = kt % C::KST;
+          if (i == 0 && !wait(&qfull[w], bn[w])) return;
+          if ((w == 0 || i >= nt[0]) && !wait(&kfull[ks], kt / C::KST)) return;
+          // the weights over which the scores go have been read (products of different accumulators are not ordered)
+          if (pn[w] > 0 && !wait(&pvdone[w], pn[w] - 1)) return;
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t at = (kk >> 2) * KEYS * 128 + (kk & 3) * 32;
+              umma_f16(tm + C::S_COL + w * KEYS, make_sdesc(q0 + w * C::TB + at, 16, 1024, kLayoutSW128),
+                       make_sdesc(k0 + ks * C::TB + at, 16, 1024, kLayoutSW128), idesc_s, kk > 0);
+            }
+            umma_commit(&sfull[w]);
+            if (w == last_w) umma_commit(&kempty[ks]);
+            if (i == nt[w] - 1) umma_commit(&qempty[w]);
+          }
+          __syncwarp();
+        };
+        for (int w = 0; ok && w < 2; ++w)
+          if (nt[w] > 0) scores(w, 0);
+        for (int i = 0; ok && i < tiles; ++i, ++vn) {
+          const uint32_t vs = vn % C::VST;
+          if (!wait(&vready[vs], vn / C::VST)) break;
+          for (int w = 0; ok && w < 2; ++w) {
+            if (i >= nt[w]) continue;
+            const uint32_t o = tm + C::O_COL + w * D, p = tm + C::S_COL + w * KEYS, v = v0 + vs * C::TB;
+            if (i == 0 && bn[w] > 0 && !wait(&oempty[w], bn[w] - 1)) break;
+            if (!wait(&phalf[w], pn[w])) break;
+            tc_fence_after();
+            if (elect_one()) {
+#pragma unroll
+              for (int kk = 0; kk < KEYS / 32; ++kk)
+                umma_f16_ts(o, p + kk * 8, make_sdesc(v + kk * 2048, KEYS * 128, 1024, kLayoutSW128), idesc_o, i > 0 || kk > 0);
+            }
+            __syncwarp();
+            if (!wait(&pfull[w], pn[w])) break;
+            tc_fence_after();
+            if (elect_one()) {
+#pragma unroll
+              for (int kk = KEYS / 32; kk < KEYS / 16; ++kk)
+                umma_f16_ts(o, p + kk * 8, make_sdesc(v + kk * 2048, KEYS * 128, 1024, kLayoutSW128), idesc_o, 1);
+              umma_commit(&pvdone[w]);
+              if (w == last_w) umma_commit(&vempty[vs]);
+            }
+            __syncwarp();
+            ++pn[w];
+            if (i + 1 < nt[w]) scores(w, i + 1);
+          }
+        }
+        kn += tiles;
+        for (int w = 0; w < 2; ++w) bn[w] += nt[w] > 0;
+      }
+      if (elect_one()) {
+        umma_commit(final_bar);  // every MMA issued here has completed before TMEM is released
+        mbar_wait_at(final_bar, 0, ctl, kSitePrFinal, false);
+      }
+      __syncwarp();
+    } else if (warp == 10) {
+      // ---------------- V tiles that are not seen as a whole ----------------
+      uint32_t vn = 0;
+      for (uint32_t n = 0;; ++n) {
+        const int sl = n & 1;
+        if (!__all_sync(0xffffffffu, mbar_wait_or_abort(&tfull[sl], (n >> 1) & 1, ctl))) break;
+        const PromptInfo t = info[sl];
+        __syncwarp();
+        if (!t.valid) break;
+        const int tiles = max(t.n[0], t.n[1]);
+        const int from = (t.row0 + 1) / KEYS;  // the first tile with a key behind the block's first position
+        bool ok = true;
+        for (int i = 0; i < tiles; ++i, ++vn) {
+          const uint32_t vs = vn % C::VST;
+          ok = __all_sync(0xffffffffu, mbar_wait_or_abort(&vfull[vs], (vn / C::VST) & 1, ctl));
+          if (!ok) break;
+          if (i >= from) {
+            uint8_t* tile = sV + vs * C::TB;
+            const int have = t.row1 - i * KEYS;  // keys up to the block's last position
+#pragma unroll 1
+            for (int q = 0; q < 4; ++q) {
+              uint8_t* row = tile + (q * 32 + lane) * 128;
+              uint32_t bad = 0;
+              if (q * 32 + lane < have) {
+#pragma unroll 8
+                for (int c = 0; c < D / 8; ++c) {  // (the chunks of 16 bytes in an order without bank conflicts)
+                  const uint4 x = *reinterpret_cast<const uint4*>(row + (c >> 3) * KEYS * 128 + (((c ^ lane) & 7) << 4));
+                  bad |= not_finite2<T>(x.x) | not_finite2<T>(x.y) | not_finite2<T>(x.z) | not_finite2<T>(x.w);
+                }
+              } else {
+#pragma unroll 1
+                for (int c = 0; c < D / 8; ++c)
+                  *reinterpret_cast<uint4*>(row + (c >> 3) * KEYS * 128 + (((c ^ lane) & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+              }
+              const uint32_t word = __ballot_sync(0xffffffffu, bad != 0);
+              if (bad != 0) {
+#pragma unroll 1
+                for (int c = 0; c < D / 2; ++c) {
+                  uint32_t* x = reinterpret_cast<uint32_t*>(row + (c >> 5) * KEYS * 128 + (c & 31) * 4);
+                  const uint32_t b = not_finite2<T>(*x);
+                  if (b & 0x8000u) *x &= 0xFFFF0000u;
+                  if (b & 0x80000000u) *x &= 0x0000FFFFu;
+                }
+              }
+              if (lane == 0) odd[sl * 12 + (i - from) * 4 + q] = word;
+            }
+            fence_proxy_async_smem();
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&vready[vs]);
+        }
+        if (!ok) break;
+        if (lane == 0) {
+          for (int i = max(tiles - from, 0) * 4; i < 12; ++i) odd[sl * 12 + i] = 0u;
+          mbar_arrive(&ckfull[sl]);
+          mbar_arrive(&tempty[sl]);
+        }
+      }
+    } else {
+      // ---------------- blocks ----------------
+      uint32_t n = 0;
+      bool ok = true;
+      int block = blockIdx.x;
+      for (uint32_t k = 0;; ++k) {
+        if (elect_one()) {  // the next block, while this one's rows are looked up
+          mbar_arrive_expect_tx(next_bar, 16);
+          clc_try_cancel(response, next_bar);
+        }
+        __syncwarp();
+        const int slot = block / a.hk, head = block - slot * a.hk;
+        PromptBlock blk;
+        if (prompt_block(a, 2 * P, slot, blk)) {
+          if (!blk.real) {  // rows of no sequence: zeros
+            const int64_t per = static_cast<int64_t>(ta.grp) * D / 8;  // 16-byte chunks of a row
+            const int64_t chunks = (blk.row1 - blk.row0) * per;
+            uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.o) + (blk.row0 * a.hq + head * ta.grp) * D);
+            for (int64_t e = lane; e < chunks; e += 32)
+              out[e / per * (static_cast<int64_t>(a.hq) * D / 8) + e % per] = make_uint4(0u, 0u, 0u, 0u);
+          } else {
+            const int sl = n & 1;
+            ok = __all_sync(0xffffffffu, mbar_wait_or_abort(&tempty[sl], ((n >> 1) & 1) ^ 1, ctl));
+            if (lane == 0 && ok) {
+              PromptInfo t;
+              t.first = static_cast<int>(blk.first);
+              t.row0 = static_cast<int>(blk.row0 - blk.first);
+              t.row1 = static_cast<int>(blk.row1 - blk.first);
+              t.head = head;
+              t.n[0] = (min(t.row0 + P, t.row1) - 1) / KEYS + 1;
+              t.n[1] = t.row0 + P < t.row1 ? (t.row1 - 1) / KEYS + 1 : 0;
+              t.valid = 1;
+              info[sl] = t;
+              mbar_arrive(&tfull[sl]);
+            }
+            ++n;
+          }
+        }
+        mbar_wait_tries(next_bar, k & 1, ctl, kSitePrNext);
+        block = clc_block(response);
+        fence_proxy_async_smem();  // read before the next answer is written
+        __syncwarp();
+        if (!ok || block < 0 || ctl->abort) break;
+      }
+      const int sl = n & 1;
+      ok = ok && __all_sync(0xffffffffu, mbar_wait_or_abort(&tempty[sl], ((n >> 1) & 1) ^ 1, ctl));
+      if (lane == 0 && ok) {
+        info[sl].valid = 0;
+        mbar_arrive(&tfull[sl]);
+      }
+      __syncwarp();
+    }
+  } else {
+    // ---------------- softmax: thread = row ----------------
+    setmaxnreg_inc<kPromptRegsSoft>();
+    const int w = warp >> 2;  // query tile
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t s_tm = lanes + C::S_COL + w * KEYS, o_tm = lanes + C::O_COL + w * D;
+    const int p = row / ta.grp, g = row - p * ta.grp;
+    const float sc = a.scale_log2;
+    uint32_t it = 0;  // score tiles so far
+    for (uint32_t n = 0;; ++n) {
+      const int sl = n & 1;
+      if (!__all_sync(0xffffffffu, mbar_wait_or_abort(&tfull[sl], (n >> 1) & 1, ctl))) break;
+      const PromptInfo t = info[sl];
+      if (!t.valid) break;
+      if (t.n[w] == 0) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tempty[sl]);
+        continue;
+      }
+      const int pos0 = t.row0 + w * P;  // the tile's first position
+      const int pos = pos0 + p;
+      float m = kPromptLowest;
+      float2 l2 = make_float2(0.f, 0.f);
+      bool ok = true;
+#pragma unroll 1
+      for (int i = 0; i < t.n[w]; ++i, ++it) {
+        ok = __all_sync(0xffffffffu, mbar_wait_or_abort(&sfull[w], it & 1, ctl));
+        if (!ok) break;
+        tc_fence_after();
+        float x[128];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(s_tm + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&x[c * 32]));
+        tmem_ld_wait();
+        if (i * KEYS + KEYS - 1 > pos0) {  // keys that some row does not see
+          const int see = pos - i * KEYS + 1;
+#pragma unroll
+          for (int c = 0; c < 128; ++c) x[c] = c < see ? x[c] : -INFINITY;
+        }
+        float top[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          top[c] = fmaxf(x[c * 32], x[c * 32 + 1]);
+#pragma unroll
+          for (int e = 2; e < 32; e += 2) top[c] = max3(top[c], x[c * 32 + e], x[c * 32 + e + 1]);
+        }
+        const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sc;
+        if (i == 0) {
+          m = fmaxf(best, kPromptLowest);
+        } else if (__any_sync(0xffffffffu, best > m + kPromptSlack)) {
+          // the accumulator is still: these scores were issued behind its last product
+          const float to = best > m + kPromptSlack ? best : m;
+          const float f = exp2_approx(m - to);
+          m = to;
+          l2.x *= f;
+          l2.y *= f;
+#pragma unroll 1
+          for (int c = 0; c < D; c += 16) {
+            uint32_t o[16];
+            tmem_ld16(o_tm + c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tmem_st16(o_tm + c, o);
+          }
+          tmem_st_wait();
+        }
+        const float2 sc2 = make_float2(sc, sc), m2 = make_float2(kPromptShift - m, kPromptShift - m);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t packed[32];
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            const int e = h * 64 + 2 * c;
+            const float2 z = __ffma2_rn(make_float2(x[e], x[e + 1]), sc2, m2);
+            const float2 v = make_float2(exp2_approx(z.x), exp2_approx(z.y));
+            l2 = __fadd2_rn(l2, v);
+            packed[c] = pack2<T>(v);
+          }
+          tmem_st32(s_tm + h * 32, packed);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(h == 0 ? &phalf[w] : &pfull[w]);
+        }
+      }
+      if (!ok) break;
+      // ---- the block's end ----
+      ok = __all_sync(0xffffffffu, mbar_wait_or_abort(&pvdone[w], (it - 1) & 1, ctl) &&
+                                       mbar_wait_or_abort(&ckfull[sl], (n >> 1) & 1, ctl));
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t any = 0;
+#pragma unroll
+      for (int k = 0; k < 12; ++k) any |= odd[sl * 12 + k];
+      const float sum = l2.x + l2.y;
+      const float inv = sum == 0.f ? 0.f : __frcp_rn(sum);
+      const bool store = p < P && pos < t.row1;
+      T* out = static_cast<T*>(a.o) + ((static_cast<int64_t>(t.first) + pos) * a.hq + t.head * ta.grp + g) * D;
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        uint32_t o[32];
+        tmem_ld32(o_tm + c, o);
+        tmem_ld_wait();
+        float y[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) y[e] = __uint_as_float(o[e]) * inv;
+        if (any != 0 && store) {
+          // values that are not finite, of the keys that this row sees among those that not all see
+          const int from = (t.row0 + 1) / KEYS * KEYS;
+          const T* v = static_cast<const T*>(a.v) + static_cast<int64_t>(t.first) * a.v_st + t.head * a.v_sh + c;
+#pragma unroll 1
+          for (int k = 0; k < 12; ++k) {
+#pragma unroll 1
+            for (uint32_t word = odd[sl * 12 + k]; word != 0; word &= word - 1) {
+              const int key = from + k * 32 + __ffs(word) - 1;
+              if (key > pos) continue;
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                const float z = to_f32(v[key * a.v_st + e]);
+                if (!(fabsf(z) <= 3.402823466e38f)) y[e] += z;
+              }
+            }
+          }
+        }
+        if (store) {
+          uint4* to = reinterpret_cast<uint4*>(out + c);
+#pragma unroll
+          for (int e = 0; e < 32; e += 8)
+            to[e / 8] = make_uint4(pack2<T>(make_float2(y[e], y[e + 1])), pack2<T>(make_float2(y[e + 2], y[e + 3])),
+                                   pack2<T>(make_float2(y[e + 4], y[e + 5])), pack2<T>(make_float2(y[e + 6], y[e + 7])));
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&oempty[w]);
+        mbar_arrive(&tempty[sl]);
+      }
+    }
+    if (lane == 0) mbar_arrive(done);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) tmem_dealloc(tmem, C::COLS);
+}
+
+static bool tma_rows(const void* p, int64_t st, int64_t sh) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && st % 8 == 0 && sh % 8 == 0 && st > 0 && sh > 0 &&
+         st < (int64_t{1} << 38) && sh < (int64_t{1} << 38);
+}
+
+template <int D, typename T>
+static int launch_tiles(const PromptArgs& a, cudaStream_t st) {
+  using C = PCfg<D>;
+  static std::once_flag once[64];
+  static cudaError_t attr_err[64];
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev)) return check_cuda(e, "cudaGetDevice");
+  dev &= 63;
+  std::call_once(once[dev], [&] {
+    attr_err[dev] = cudaFuncSetAttribute(prompt_tile_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  });
+  if (int s = check_cuda(attr_err[dev], "cudaFuncSetAttribute(prompt_tile_kernel)")) return s;
+  PromptTiles ta = {};
+  ta.a = a;
+  ta.grp = a.hq / a.hk;
+  ta.pos = 128 / ta.grp;
+  if (int s = device_wait_ptrs(&ta.status, &ta.limit)) return s;
+  const CUtensorMapDataType dt =
+      std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  CUtensorMap tq, tk, tv;
+  auto map = [&](CUtensorMap* m, const void* p, int64_t s_tok, int64_t s_head, int heads, uint32_t box_h, uint32_t box_n) {
+    const uint64_t dims[3] = {static_cast<uint64_t>(D), static_cast<uint64_t>(heads), static_cast<uint64_t>(a.n)};
+    const uint64_t strides[2] = {static_cast<uint64_t>(s_head) * 2, static_cast<uint64_t>(s_tok) * 2};
+    const uint32_t box[3] = {64, box_h, box_n};
+    return make_tmap_3d(m, p, dt, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  };
+  if (int s = map(&tq, a.q, a.q_st, a.q_sh, a.hq, ta.grp, ta.pos)) return s;
+  if (int s = map(&tk, a.k, a.k_st, a.k_sh, a.hk, 1, kPromptKeys)) return s;
+  if (int s = map(&tv, a.v, a.v_st, a.v_sh, a.hk, 1, kPromptKeys)) return s;
+  const int64_t slots = a.n / (2 * ta.pos) + a.b + 2;
+  prompt_tile_kernel<D, T><<<static_cast<unsigned>(slots * a.hk), kPromptThreads, C::SMEM, st>>>(tq, tk, tv, ta);
+  return check_launch("prompt_tile_kernel");
+}
+
 }  // namespace bw
 
 extern "C" int bw_prompt_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
@@ -203,5 +825,20 @@ extern "C" int bw_prompt_attention(const void* q, int64_t q_st, int64_t q_sh, co
   a.d = static_cast<int>(d);
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // The tensor-core kernel: rows that TMA can copy, a positive scale (it takes maxima before it scales), and blocks that
+  // a grid can number.  (A dimension of one has any stride.)
+  if (hq == 1) a.q_sh = d;
+  if (hk == 1) a.k_sh = a.v_sh = d;
+  if (n == 1) {
+    a.q_st = a.q_sh * hq;
+    a.k_st = a.k_sh * hk;
+    a.v_st = a.v_sh * hk;
+  }
+  if ((d == 64 || d == 128) && hq / hk <= 128 && softmax_scale > 0.f && softmax_scale <= 3.402823466e38f &&
+      tma_rows(q, a.q_st, a.q_sh) && tma_rows(k, a.k_st, a.k_sh) && tma_rows(v, a.v_st, a.v_sh) &&
+      reinterpret_cast<uintptr_t>(out) % 16 == 0 && (n / (2 * (128 / (hq / hk))) + b + 2) * hk <= INT32_MAX) {
+    if (dtype == BW_DTYPE_BF16) return d == 128 ? launch_tiles<128, __nv_bfloat16>(a, st) : launch_tiles<64, __nv_bfloat16>(a, st);
+    return d == 128 ? launch_tiles<128, __half>(a, st) : launch_tiles<64, __half>(a, st);
+  }
   return dtype == BW_DTYPE_BF16 ? launch_rows<__nv_bfloat16>(a, st) : launch_rows<__half>(a, st);
 }

@@ -268,23 +268,6 @@ __device__ __forceinline__ int seq_nodes(const AttnArgs& a, int64_t b) {
 }
 __device__ __forceinline__ int64_t seq_ctx(const AttnArgs& a, int64_t b) { return a.ctx[b] > 0 ? a.ctx[b] : 0; }
 
-template <int N>
-__device__ __forceinline__ void setmaxnreg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void setmaxnreg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-
-// 2^x to 2 ulps; 0 for -inf and below the normal range.
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float y;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-  return y;
-}
 // v less two bf16 numbers, one instruction each (a multiply-add of bf16 factors and an fp32 addend).
 __device__ __forceinline__ float2 sub_bf16x2(const float2& v, uint32_t h) {
   float2 y;
