@@ -38,13 +38,17 @@ __device__ __forceinline__ int64_t prompt_edge(const PromptArgs& a, int i) {  //
   const int64_t e = a.offsets[i - 1];
   return e < 0 ? 0 : (e < a.n ? e : a.n);
 }
-// Block number `slot` of P rows; the last blocks of a sequence, which see most keys, come first.
-__device__ __forceinline__ bool prompt_block(const PromptArgs& a, int P, int64_t slot, PromptBlock& blk) {
-  int lo = 0, hi = a.b + 1;  // the last segment whose numbers start at `slot` or before
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (prompt_edge(a, mid) / P + mid <= slot) lo = mid;
-    else hi = mid - 1;
+// Block number `slot` of P rows, by a whole warp; the last blocks of a sequence, which see most keys, come first.
+__device__ __forceinline__ bool prompt_block(const PromptArgs& a, int P, int slot, PromptBlock& blk) {
+  // the last segment whose numbers start at `slot` or before: 32 of the segments lo .. hi - 1 at a time
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = a.b + 2;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32, i = lo + lane * step;
+    const bool before = i < hi && static_cast<int>(prompt_edge(a, i)) / P + i <= slot;
+    const int last = 31 - __clz(__ballot_sync(0xffffffffu, before) | 1u);
+    hi = min(hi, lo + (last + 1) * step);
+    lo += last * step;
   }
   const int64_t e0 = prompt_edge(a, lo), e1 = prompt_edge(a, lo + 1);
   const int64_t blocks = e1 > e0 ? (e1 - e0 + P - 1) / P : 0;
@@ -175,10 +179,12 @@ static int launch_rows(const PromptArgs& a, cudaStream_t st) {
 //   O [128 x D]       += P [128 x 128 keys] (TMEM, over S) . V (shared memory)    fp32, in TMEM
 // Each K and V tile in shared memory serves both query tiles, and while one tile's softmax runs, the other's products do.
 //
-// Softmax: thread = row, so nothing is exchanged.  The reference m moves only when a score exceeds it by more than 8 (in
-// powers of two); only then are the sum and the accumulator rescaled.  Weights 2^(s - m + 7) go to the tensor core in
-// the inputs' type: rounded by half an ulp like the inputs themselves, at most 2^15, and the 7 keeps fp16's subnormal steps
-// at 2^-32 of a row's largest weight.  Their sum and the accumulator are fp32 and have the same factor.
+// Softmax: thread = row, so nothing is exchanged.  Weights are 2^(s - m + 7) with a row's reference m, at first the
+// largest score of the first tile.  It moves only when 64 weights come to 2^15 or more, which takes a score two powers
+// over it: then the weights are worked out again from the largest score, and the sum and the accumulator rescaled.  So a
+// tile needs no maximum, the sum tells.  Weights go to the tensor core in the inputs' type: rounded by half an ulp like
+// the inputs themselves, under 2^15, and the 7 keeps fp16's subnormal steps at 2^-32 of a row's largest weight.  Their
+// sum and the accumulator are fp32 and have the same factor.
 //
 // Keys that a row does not see have weight 0, but 0 times a value that is not finite is not 0.  So a warp looks through
 // every V tile that some row of the block does not see all of: rows behind the block's last position become zeros,
@@ -187,15 +193,19 @@ static int launch_rows(const PromptArgs& a, cudaStream_t st) {
 // Blocks are handed out by the hardware: a CTA that nears its end takes the next one that has not started
 // (clusterlaunchcontrol), so the schedule is dynamic without a counter in memory.
 //
-// Twelve warps: 0-3 and 4-7 the softmax of A and B (their TMEM lanes are the rows), 8 TMA loads and watches the time, 9
-// issues the products, 10 looks through V, 11 finds the blocks.
+// Twelve warps: 0-3 and 4-7 the softmax of A and B (their TMEM lanes are the rows), 8 finds the blocks, loads and watches
+// the time, 9 issues the products, 10 and 11 look through V.
 // ---------------------------------------------------------------------------
 constexpr int kPromptThreads = 384;
 constexpr int kPromptKeys = 128;
 // Registers of a thread of the three warpgroups after setmaxnreg: three times the 168 that a thread of 384 has.
 constexpr int kPromptRegsSoft = 208, kPromptRegsRest = 88;
 static_assert(2 * kPromptRegsSoft + kPromptRegsRest == 3 * 168, "register split");
+// A CTA takes its next block when it loads the last but third key tile of the one it has: a block taken earlier is out of
+// other CTAs' reach for longer, one taken later is not there in time.
+constexpr int kPromptAhead = 4;
 constexpr float kPromptSlack = 8.f, kPromptShift = 7.f;
+constexpr float kPromptMost = 32768.f;  // what 64 weights may sum to: four times what they come to at a new reference
 constexpr float kPromptLowest = -3.0e38f;  // a row's reference without any score: finite, so differences are
 enum PromptSite : int {
   kSitePrBlock = 501, kSitePrQ = 502, kSitePrK = 503, kSitePrV = 504, kSitePrDrain = 505, kSitePrDone = 506,
@@ -205,10 +215,12 @@ enum PromptSite : int {
 template <int D>
 struct PCfg {
   static constexpr int TB = D / 64 * kPromptKeys * 128;  // bytes of a tile of Q, K or V: panels of 64 elements
-  static constexpr int KST = D == 128 ? 3 : 4, VST = D == 128 ? 2 : 4;
+  static constexpr int KST = D == 128 ? 2 : 4, VST = D == 128 ? 2 : 4;
+  static constexpr int OB = 32 * 128;  // bytes of a softmax warp's part of the output on its way out
   static constexpr int OFF_K = 2 * TB;
   static constexpr int OFF_V = OFF_K + KST * TB;
-  static constexpr int OFF_CTRL = OFF_V + VST * TB;
+  static constexpr int OFF_O = OFF_V + VST * TB;
+  static constexpr int OFF_CTRL = OFF_O + 8 * OB;
   static constexpr int CTRL = 1024;
   static constexpr int SMEM = OFF_CTRL + CTRL + 1024;
   static constexpr int S_COL = 0, O_COL = 256, COLS = 512;
@@ -255,6 +267,23 @@ __device__ __forceinline__ uint32_t not_finite2(uint32_t w) {
   else return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
 }
 
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {  // NaN if one is
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+__device__ __forceinline__ float max64(const float* x, float y) {
+  float top[4] = {y, x[0], x[1], x[2]};
+#pragma unroll
+  for (int e = 3; e < 59; e += 8) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) top[c] = max3_nan(top[c], x[e + 2 * c], x[e + 2 * c + 1]);
+  }
+  top[0] = max3_nan(top[0], x[59], x[60]);
+  top[1] = max3_nan(top[1], x[61], x[62]);
+  return max3_nan(max3_nan(top[0], top[1], top[2]), top[3], x[63]);
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float2 v) {
   if constexpr (std::is_same<T, __half>::value) {
@@ -278,6 +307,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   uint8_t* sQ = smem;
   uint8_t* sK = smem + C::OFF_K;
   uint8_t* sV = smem + C::OFF_V;
+  uint8_t* sO = smem + C::OFF_O;
   uint64_t* tfull = reinterpret_cast<uint64_t*>(smem + C::OFF_CTRL);  // 2: a block's numbers are there
   uint64_t* tempty = tfull + 2;        //    all roles are done with them
   uint64_t* qfull = tempty + 2;        // [A, B]
@@ -290,10 +320,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   uint64_t* sfull = vempty + C::VST;   // [A, B] scores
   uint64_t* phalf = sfull + 2;         // weights of the first 64 keys, of all
   uint64_t* pfull = phalf + 2;
-  uint64_t* pvdone = pfull + 2;        // V . P complete
+  uint64_t* pvdone = pfull + 2;        //    P . V complete
   uint64_t* oempty = pvdone + 2;       // accumulator read
   uint64_t* ckfull = oempty + 2;       // 2: a block's values that are not finite are known
-  uint64_t* next_bar = ckfull + 2;
+  uint64_t* next_bar = ckfull + 2;     // a block from the hardware
   uint64_t* done = next_bar + 1;
   uint64_t* final_bar = done + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(final_bar + 1);
@@ -311,7 +341,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tfull[i], 1);
-      mbar_init(&tempty[i], 11);  // loads, products, the look through V, eight softmax warps
+      mbar_init(&tempty[i], 11);  // products, two warps that look through V, eight softmax warps
       mbar_init(&qfull[i], 1);
       mbar_init(&qempty[i], 1);
       mbar_init(&sfull[i], 1);
@@ -319,7 +349,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       mbar_init(&pfull[i], 4);
       mbar_init(&pvdone[i], 1);
       mbar_init(&oempty[i], 4);
-      mbar_init(&ckfull[i], 1);
+      mbar_init(&ckfull[i], 2);
     }
     for (int i = 0; i < C::KST; ++i) {
       mbar_init(&kfull[i], 1);
@@ -327,7 +357,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
     for (int i = 0; i < C::VST; ++i) {
       mbar_init(&vfull[i], 1);
-      mbar_init(&vready[i], 1);
+      mbar_init(&vready[i], 2);
       mbar_init(&vempty[i], 1);
     }
     mbar_init(next_bar, 1);
@@ -353,9 +383,54 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   if (warp >= 8) {
     setmaxnreg_dec<kPromptRegsRest>();
     if (warp == 8) {
-      // ---------------- TMA ----------------
+      // ---------------- blocks and TMA ----------------
       const uint64_t pol = l2_policy_evict_normal();
       uint32_t qn[2] = {0u, 0u}, kn = 0, vn = 0;  // loads so far
+      uint32_t asked = 0, got = 0;                // answers to try_cancel
+      auto ask = [&]() {
+        if (elect_one()) {
+          mbar_arrive_expect_tx(next_bar, 16);
+          clc_try_cancel(response, next_bar);
+        }
+        __syncwarp();
+        ++asked;
+      };
+      auto answer = [&]() {
+        mbar_wait_tries(next_bar, got & 1, ctl, kSitePrNext);
+        ++got;
+        const int x = clc_block(response);
+        fence_proxy_async_smem();  // read before the next answer is written
+        __syncwarp();
+        return x;
+      };
+      PromptInfo t;
+      // Block number `x`, or the next one that has rows of a sequence; false: none is left.
+      auto find = [&](int x) {
+        while (x >= 0 && !ctl->abort) {
+          const int slot = x / a.hk, head = x - slot * a.hk;
+          PromptBlock blk;
+          if (prompt_block(a, 2 * P, slot, blk)) {
+            if (blk.real) {
+              t.first = static_cast<int>(blk.first);
+              t.row0 = static_cast<int>(blk.row0 - blk.first);
+              t.row1 = static_cast<int>(blk.row1 - blk.first);
+              t.head = head;
+              t.n[0] = (min(t.row0 + P, t.row1) - 1) / KEYS + 1;
+              t.n[1] = t.row0 + P < t.row1 ? (t.row1 - 1) / KEYS + 1 : 0;
+              return true;
+            }
+            // rows of no sequence: zeros
+            const int64_t per = static_cast<int64_t>(ta.grp) * D / 8;  // 16-byte chunks of a row
+            const int64_t chunks = (blk.row1 - blk.row0) * per;
+            uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.o) + (blk.row0 * a.hq + head * ta.grp) * D);
+            for (int64_t e = lane; e < chunks; e += 32)
+              out[e / per * (static_cast<int64_t>(a.hq) * D / 8) + e % per] = make_uint4(0u, 0u, 0u, 0u);
+          }
+          ask();
+          x = answer();
+        }
+        return false;
+      };
       auto load = [&](uint8_t* dst, const CUtensorMap* tm, uint64_t* full, uint32_t bytes, int head, int row) {
         if (elect_one()) {
           mbar_arrive_expect_tx(full, bytes);
@@ -365,15 +440,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         __syncwarp();
       };
       const uint32_t q_bytes = static_cast<uint32_t>(P * ta.grp * D * 2);
-      bool ok = true;
-      for (uint32_t n = 0; ok; ++n) {
+      bool ok = true, have = find(blockIdx.x);
+      for (uint32_t n = 0;; ++n) {
         const int sl = n & 1;
-        ok = __all_sync(0xffffffffu, mbar_wait_at(&tfull[sl], (n >> 1) & 1, ctl, kSitePrBlock));
+        ok = __all_sync(0xffffffffu, mbar_wait_at(&tempty[sl], ((n >> 1) & 1) ^ 1, ctl, kSitePrBlock));
         if (!ok) break;
-        const PromptInfo t = info[sl];
+        if (lane == 0) {
+          t.valid = have;
+          info[sl] = t;
+          mbar_arrive(&tfull[sl]);
+        }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&tempty[sl]);
-        if (!t.valid) break;
+        if (!have) break;
         auto load_q = [&](int w) {
           if (t.n[w] == 0) return true;
           const bool fine = mbar_wait_at(&qempty[w], (qn[w] & 1) ^ 1, ctl, kSitePrQ);
@@ -385,6 +463,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         const int tiles = max(t.n[0], t.n[1]);
         ok = load_q(0);
         for (int i = 0; ok && i < tiles; ++i) {
+          if (i == max(tiles - kPromptAhead, 0)) ask();
           const int ks = kn % C::KST, vs = vn % C::VST;
           ok = __all_sync(0xffffffffu, mbar_wait_at(&kempty[ks], ((kn / C::KST) & 1) ^ 1, ctl, kSitePrK));
           if (!ok) break;
@@ -396,10 +475,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           load(sV + vs * C::TB, &tm_v, &vfull[vs], C::TB, t.head, t.first + i * KEYS);
           ++vn;
         }
+        if (!ok) break;
+        have = find(answer());
       }
       if (ok) {
         mbar_wait_at(done, 0, ctl, kSitePrDone);
-      } else {  // wait (bounded) for the copies still in flight into this CTA's shared memory
+      } else {  // wait (bounded) for what is still on its way into this CTA's shared memory
+        if (asked > got) mbar_wait_tries(next_bar, got & 1, ctl, kSitePrNext);
         for (uint32_t i = kn > C::KST ? kn - C::KST : 0; i < kn; ++i)
           mbar_wait_at(&kfull[i % C::KST], (i / C::KST) & 1, ctl, kSitePrDrain, false);
         for (uint32_t i = vn > C::VST ? vn - C::VST : 0; i < vn; ++i)
@@ -409,90 +491,108 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       }
     } else if (warp == 9) {
       // ---------------- products ----------------
-      constexpr uint32_t idesc_s = make_idesc_f16(128, KEYS, BF16, false);
-      constexpr uint32_t idesc_o = make_idesc_f16(128, D, BF16, true);
-      const uint32_t tm = warp_uniform(tmem);
-      const uint32_t q0 = smem_u32(sQ), k0 = smem_u32(sK), v0 = smem_u32(sV);
-      uint32_t kn = 0, vn = 0, seen = 0;               // K tiles begun, V tiles, blocks of A or B
-      uint32_t pn[2] = {0u, 0u}, bn[2] = {0u, 0u};     // V . P and blocks so far
-      bool ok = true;
-      auto wait = [&](uint64_t* bar, uint32_t parity) {
-        ok = ok && __all_sync(0xffffffffu, mbar_wait_or_abort(bar, parity & 1, ctl));
-        return ok;
-      };
-      for (; ok; ++seen) {
-        const int sl = seen & 1;
-        if (!wait(&tfull[sl], seen >> 1)) break;
-        const int nt[2] = {warp_uniform(info[sl].n[0]), warp_uniform(info[sl].n[1])};
-        const int valid = warp_uniform(info[sl].valid);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&tempty[sl]);
-        if (!valid) break;
-        const int tiles = max(nt[0], nt[1]);
-        const int last_w = nt[1] > 0 ? 1 : 0;  // the tile that needs a K or V tile last
-        // scores of K tile i for query tile w
-        auto scores = [&](int w, int i) {
-          const uint32_t kt = kn + i;
-          const uint32_t ks = kt % C::KST;
-          if (i == 0 && !wait(&qfull[w], bn[w])) return;
-          if ((w == 0 || i >= nt[0]) && !wait(&kfull[ks], kt / C::KST)) return;
-          // the weights over which the scores go have been read (products of different accumulators are not ordered)
-          if (pn[w] > 0 && !wait(&pvdone[w], pn[w] - 1)) return;
+      {
+        const uint32_t tm = warp_uniform(tmem);
+        constexpr uint32_t idesc_s = make_idesc_f16(128, KEYS, BF16, false);
+        constexpr uint32_t idesc_o = make_idesc_f16(128, D, BF16, true);
+        const uint32_t q0 = smem_u32(sQ), k0 = smem_u32(sK), v0 = smem_u32(sV);
+        uint32_t ks = 0, kp = 0, vs = 0, vp = 0;  // stage and parity of the next K and V tile
+        uint32_t sp = 0, bp = 0;                  // parities of the next tile (bit w) and the next block of A and B
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t parity) {
+          ok = ok && __all_sync(0xffffffffu, mbar_wait_or_abort(bar, parity & 1u, ctl));
+          return ok;
+        };
+        // Scores of the next K tile, once the weights over which they go have been read (products of different
+        // accumulators are not ordered).
+        auto scores = [&](int w, bool give_k, bool give_q) {
+          if (!wait(&pvdone[w], (sp >> w) ^ 1u)) return;
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-              const uint32_t at = (kk >> 2) * KEYS * 128 + (kk & 3) * 32;
-              umma_f16(tm + C::S_COL + w * KEYS, make_sdesc(q0 + w * C::TB + at, 16, 1024, kLayoutSW128),
-                       make_sdesc(k0 + ks * C::TB + at, 16, 1024, kLayoutSW128), idesc_s, kk > 0);
-            }
-            umma_commit(&sfull[w]);
-            if (w == last_w) umma_commit(&kempty[ks]);
-            if (i == nt[w] - 1) umma_commit(&qempty[w]);
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t at = (kk >> 2) * KEYS * 128 + (kk & 3) * 32;
+            umma_f16(tm + C::S_COL + w * KEYS, make_sdesc(q0 + w * C::TB + at, 16, 1024, kLayoutSW128),
+                     make_sdesc(k0 + ks * C::TB + at, 16, 1024, kLayoutSW128), idesc_s, kk > 0);
+          }
+          umma_commit(&sfull[w]);
+          if (give_k) umma_commit(&kempty[ks]);
+          if (give_q) umma_commit(&qempty[w]);
           }
           __syncwarp();
         };
-        for (int w = 0; ok && w < 2; ++w)
-          if (nt[w] > 0) scores(w, 0);
-        for (int i = 0; ok && i < tiles; ++i, ++vn) {
-          const uint32_t vs = vn % C::VST;
-          if (!wait(&vready[vs], vn / C::VST)) break;
-          for (int w = 0; ok && w < 2; ++w) {
-            if (i >= nt[w]) continue;
-            const uint32_t o = tm + C::O_COL + w * D, p = tm + C::S_COL + w * KEYS, v = v0 + vs * C::TB;
-            if (i == 0 && bn[w] > 0 && !wait(&oempty[w], bn[w] - 1)) break;
-            if (!wait(&phalf[w], pn[w])) break;
-            tc_fence_after();
-            if (elect_one()) {
+        auto weighted = [&](int w, bool first, bool give_v) {
+          const uint32_t o = tm + C::O_COL + w * D, p = tm + C::S_COL + w * KEYS, v = v0 + vs * C::TB;
+          const uint32_t parity = sp >> w;
+          if (!wait(&phalf[w], parity)) return;
+          tc_fence_after();
+          if (elect_one()) {
 #pragma unroll
-              for (int kk = 0; kk < KEYS / 32; ++kk)
-                umma_f16_ts(o, p + kk * 8, make_sdesc(v + kk * 2048, KEYS * 128, 1024, kLayoutSW128), idesc_o, i > 0 || kk > 0);
-            }
-            __syncwarp();
-            if (!wait(&pfull[w], pn[w])) break;
-            tc_fence_after();
-            if (elect_one()) {
-#pragma unroll
-              for (int kk = KEYS / 32; kk < KEYS / 16; ++kk)
-                umma_f16_ts(o, p + kk * 8, make_sdesc(v + kk * 2048, KEYS * 128, 1024, kLayoutSW128), idesc_o, 1);
-              umma_commit(&pvdone[w]);
-              if (w == last_w) umma_commit(&vempty[vs]);
-            }
-            __syncwarp();
-            ++pn[w];
-            if (i + 1 < nt[w]) scores(w, i + 1);
+          for (int kk = 0; kk < KEYS / 32; ++kk)
+            umma_f16_ts(o, p + kk * 8, make_sdesc(v + kk * 2048, KEYS * 128, 1024, kLayoutSW128), idesc_o, !first || kk > 0);
           }
+          __syncwarp();
+          if (!wait(&pfull[w], parity)) return;
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+          for (int kk = KEYS / 32; kk < KEYS / 16; ++kk)
+            umma_f16_ts(o, p + kk * 8, make_sdesc(v + kk * 2048, KEYS * 128, 1024, kLayoutSW128), idesc_o, 1);
+          umma_commit(&pvdone[w]);
+          if (give_v) umma_commit(&vempty[vs]);
+          }
+          __syncwarp();
+          sp ^= 1u << w;
+        };
+        auto next_k = [&]() {
+          if (++ks == C::KST) {
+            ks = 0;
+            kp ^= 1;
+          }
+        };
+        for (uint32_t n = 0; ok; ++n) {
+          const int sl = n & 1;
+          if (!wait(&tfull[sl], n >> 1)) break;
+          const int na = warp_uniform(info[sl].n[0]), nb = warp_uniform(info[sl].n[1]), valid = warp_uniform(info[sl].valid);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&tempty[sl]);
+          if (!valid) break;
+          const int tiles = max(na, nb);
+          const bool both = nb > 0;  // (B then needs every K and V tile, and last)
+          if (!wait(&qfull[0], bp) || !wait(&kfull[ks], kp)) break;
+          scores(0, !both, na == 1);
+          if (both && wait(&qfull[1], bp >> 1)) scores(1, true, nb == 1);
+          next_k();
+          for (int i = 0; ok && i < tiles; ++i) {
+            if (!wait(&vready[vs], vp)) break;
+            const bool more = i + 1 < tiles;
+            if (i < na) {
+              if (i == 0 && !wait(&oempty[0], bp ^ 1u)) break;  // the block before has been read
+              weighted(0, i == 0, !both);
+              if (ok && i + 1 < na && wait(&kfull[ks], kp)) scores(0, !both, i + 2 == na);
+            }
+            if (i < nb) {
+              if (i == 0 && !wait(&oempty[1], (bp >> 1) ^ 1u)) break;
+              if (ok) weighted(1, i == 0, true);
+              if (ok && more && (i + 1 < na || wait(&kfull[ks], kp))) scores(1, true, i + 2 == nb);
+            }
+            if (more) next_k();
+            if (++vs == C::VST) {
+              vs = 0;
+              vp ^= 1;
+            }
+          }
+          bp ^= both ? 3u : 1u;
         }
-        kn += tiles;
-        for (int w = 0; w < 2; ++w) bn[w] += nt[w] > 0;
-      }
-      if (elect_one()) {
-        umma_commit(final_bar);  // every MMA issued here has completed before TMEM is released
-        mbar_wait_at(final_bar, 0, ctl, kSitePrFinal, false);
+        if (elect_one()) {
+          umma_commit(final_bar);  // every MMA issued here has completed before TMEM is released
+          mbar_wait_at(final_bar, 0, ctl, kSitePrFinal, false);
+        }
       }
       __syncwarp();
-    } else if (warp == 10) {
-      // ---------------- V tiles that are not seen as a whole ----------------
+    } else {
+      // ---------------- V tiles that are not seen as a whole: 64 rows a warp ----------------
+      const int part = warp - 10;
       uint32_t vn = 0;
       for (uint32_t n = 0;; ++n) {
         const int sl = n & 1;
@@ -510,18 +610,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           if (i >= from) {
             uint8_t* tile = sV + vs * C::TB;
             const int have = t.row1 - i * KEYS;  // keys up to the block's last position
-#pragma unroll 1
-            for (int q = 0; q < 4; ++q) {
+#pragma unroll
+            for (int q = part * 2; q < part * 2 + 2; ++q) {
               uint8_t* row = tile + (q * 32 + lane) * 128;
               uint32_t bad = 0;
               if (q * 32 + lane < have) {
-#pragma unroll 8
+#pragma unroll
                 for (int c = 0; c < D / 8; ++c) {  // (the chunks of 16 bytes in an order without bank conflicts)
                   const uint4 x = *reinterpret_cast<const uint4*>(row + (c >> 3) * KEYS * 128 + (((c ^ lane) & 7) << 4));
                   bad |= not_finite2<T>(x.x) | not_finite2<T>(x.y) | not_finite2<T>(x.z) | not_finite2<T>(x.w);
                 }
               } else {
-#pragma unroll 1
+#pragma unroll
                 for (int c = 0; c < D / 8; ++c)
                   *reinterpret_cast<uint4*>(row + (c >> 3) * KEYS * 128 + (((c ^ lane) & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
               }
@@ -544,62 +644,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         }
         if (!ok) break;
         if (lane == 0) {
-          for (int i = max(tiles - from, 0) * 4; i < 12; ++i) odd[sl * 12 + i] = 0u;
+          for (int i = max(tiles - from, 0) * 4 + part * 2; i < 12; i += 4) odd[sl * 12 + i] = odd[sl * 12 + i + 1] = 0u;
           mbar_arrive(&ckfull[sl]);
           mbar_arrive(&tempty[sl]);
         }
       }
-    } else {
-      // ---------------- blocks ----------------
-      uint32_t n = 0;
-      bool ok = true;
-      int block = blockIdx.x;
-      for (uint32_t k = 0;; ++k) {
-        if (elect_one()) {  // the next block, while this one's rows are looked up
-          mbar_arrive_expect_tx(next_bar, 16);
-          clc_try_cancel(response, next_bar);
-        }
-        __syncwarp();
-        const int slot = block / a.hk, head = block - slot * a.hk;
-        PromptBlock blk;
-        if (prompt_block(a, 2 * P, slot, blk)) {
-          if (!blk.real) {  // rows of no sequence: zeros
-            const int64_t per = static_cast<int64_t>(ta.grp) * D / 8;  // 16-byte chunks of a row
-            const int64_t chunks = (blk.row1 - blk.row0) * per;
-            uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.o) + (blk.row0 * a.hq + head * ta.grp) * D);
-            for (int64_t e = lane; e < chunks; e += 32)
-              out[e / per * (static_cast<int64_t>(a.hq) * D / 8) + e % per] = make_uint4(0u, 0u, 0u, 0u);
-          } else {
-            const int sl = n & 1;
-            ok = __all_sync(0xffffffffu, mbar_wait_or_abort(&tempty[sl], ((n >> 1) & 1) ^ 1, ctl));
-            if (lane == 0 && ok) {
-              PromptInfo t;
-              t.first = static_cast<int>(blk.first);
-              t.row0 = static_cast<int>(blk.row0 - blk.first);
-              t.row1 = static_cast<int>(blk.row1 - blk.first);
-              t.head = head;
-              t.n[0] = (min(t.row0 + P, t.row1) - 1) / KEYS + 1;
-              t.n[1] = t.row0 + P < t.row1 ? (t.row1 - 1) / KEYS + 1 : 0;
-              t.valid = 1;
-              info[sl] = t;
-              mbar_arrive(&tfull[sl]);
-            }
-            ++n;
-          }
-        }
-        mbar_wait_tries(next_bar, k & 1, ctl, kSitePrNext);
-        block = clc_block(response);
-        fence_proxy_async_smem();  // read before the next answer is written
-        __syncwarp();
-        if (!ok || block < 0 || ctl->abort) break;
-      }
-      const int sl = n & 1;
-      ok = ok && __all_sync(0xffffffffu, mbar_wait_or_abort(&tempty[sl], ((n >> 1) & 1) ^ 1, ctl));
-      if (lane == 0 && ok) {
-        info[sl].valid = 0;
-        mbar_arrive(&tfull[sl]);
-      }
-      __syncwarp();
     }
   } else {
     // ---------------- softmax: thread = row ----------------
@@ -698,41 +747,59 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       for (int k = 0; k < 12; ++k) any |= odd[sl * 12 + k];
       const float sum = l2.x + l2.y;
       const float inv = sum == 0.f ? 0.f : __frcp_rn(sum);
-      const bool store = p < P && pos < t.row1;
-      T* out = static_cast<T*>(a.o) + ((static_cast<int64_t>(t.first) + pos) * a.hq + t.head * ta.grp + g) * D;
+      const bool mine = p < P && pos < t.row1;
+      // 64 elements of the rows at a time through shared memory, so that a store has 128 bytes of each of four rows: 16
+      // bytes of 32 rows each took a quarter of the time of 24 prompts of up to 1021 tokens.
+      T* out = static_cast<T*>(a.o) + ((static_cast<int64_t>(t.first) + pos0) * a.hq + t.head * ta.grp) * D;
+      const int at = mine ? (p * a.hq + g) * D : -1;  // of this lane's row
+      uint8_t* stage = sO + warp * C::OB;
 #pragma unroll 1
-      for (int c = 0; c < D; c += 32) {
-        uint32_t o[32];
-        tmem_ld32(o_tm + c, o);
-        tmem_ld_wait();
-        float y[32];
+      for (int c0 = 0; c0 < D; c0 += 64) {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) y[e] = __uint_as_float(o[e]) * inv;
-        if (any != 0 && store) {
-          // values that are not finite, of the keys that this row sees among those that not all see
-          const int from = (t.row0 + 1) / KEYS * KEYS;
-          const T* v = static_cast<const T*>(a.v) + static_cast<int64_t>(t.first) * a.v_st + t.head * a.v_sh + c;
-#pragma unroll 1
-          for (int k = 0; k < 12; ++k) {
-#pragma unroll 1
-            for (uint32_t word = odd[sl * 12 + k]; word != 0; word &= word - 1) {
-              const int key = from + k * 32 + __ffs(word) - 1;
-              if (key > pos) continue;
+        for (int c = 0; c < 64; c += 32) {
+          uint32_t o[32];
+          tmem_ld32(o_tm + c0 + c, o);
+          tmem_ld_wait();
+          float y[32];
 #pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                const float z = to_f32(v[key * a.v_st + e]);
-                if (!(fabsf(z) <= 3.402823466e38f)) y[e] += z;
+          for (int e = 0; e < 32; ++e) y[e] = __uint_as_float(o[e]) * inv;
+          if (any != 0 && mine) {
+            // values that are not finite, of the keys that this row sees among those that not all see
+            const int from = (t.row0 + 1) / KEYS * KEYS;
+            const T* v = static_cast<const T*>(a.v) + static_cast<int64_t>(t.first) * a.v_st + t.head * a.v_sh + c0 + c;
+#pragma unroll 1
+            for (int k = 0; k < 12; ++k) {
+#pragma unroll 1
+              for (uint32_t word = odd[sl * 12 + k]; word != 0; word &= word - 1) {
+                const int key = from + k * 32 + __ffs(word) - 1;
+                if (key > pos) continue;
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                  const float z = to_f32(v[key * a.v_st + e]);
+                  if (!(fabsf(z) <= 3.402823466e38f)) y[e] += z;
+                }
               }
             }
           }
-        }
-        if (store) {
-          uint4* to = reinterpret_cast<uint4*>(out + c);
 #pragma unroll
           for (int e = 0; e < 32; e += 8)
-            to[e / 8] = make_uint4(pack2<T>(make_float2(y[e], y[e + 1])), pack2<T>(make_float2(y[e + 2], y[e + 3])),
-                                   pack2<T>(make_float2(y[e + 4], y[e + 5])), pack2<T>(make_float2(y[e + 6], y[e + 7])));
+            *reinterpret_cast<uint4*>(stage + lane * 128 + ((((c + e) >> 3) ^ (lane & 7)) << 4)) =
+                make_uint4(pack2<T>(make_float2(y[e], y[e + 1])), pack2<T>(make_float2(y[e + 2], y[e + 3])),
+                           pack2<T>(make_float2(y[e + 4], y[e + 5])), pack2<T>(make_float2(y[e + 6], y[e + 7])));
         }
+        __syncwarp();
+        uint4 line[8];
+        int to[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int r = 4 * k + (lane >> 3);
+          to[k] = __shfl_sync(0xffffffffu, at, r);
+          line[k] = *reinterpret_cast<const uint4*>(stage + r * 128 + (((lane ^ r) & 7) << 4));
+        }
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (to[k] >= 0) *reinterpret_cast<uint4*>(out + to[k] + c0 + (lane & 7) * 8) = line[k];
       }
       tc_fence_before();
       __syncwarp();
