@@ -174,17 +174,26 @@ static int launch_rows(const PromptArgs& a, cudaStream_t st) {
 // tensor-core kernel (head dimensions 64 and 128)
 //
 // A tile is 128 rows of queries: P = 128 / group positions with the query heads that read one key head, row = position *
-// group + head.  A CTA takes two neighbouring tiles A and B of a key head and walks their sequence's keys, 128 at a time:
+// group + head.  A CTA takes two neighbouring tiles A and B of a key head (or, of few rows, one) and walks their
+// sequence's keys, 128 at a time:
 //   S [128 x 128 keys] = Q [128 x D] (shared memory) . K^T (shared memory)        fp32, in TMEM
 //   O [128 x D]       += P [128 x 128 keys] (TMEM, over S) . V (shared memory)    fp32, in TMEM
 // Each K and V tile in shared memory serves both query tiles, and while one tile's softmax runs, the other's products do.
 //
-// Softmax: thread = row, so nothing is exchanged.  Weights are 2^(s - m + 7) with a row's reference m, at first the
-// largest score of the first tile.  It moves only when 64 weights come to 2^15 or more, which takes a score two powers
-// over it: then the weights are worked out again from the largest score, and the sum and the accumulator rescaled.  So a
-// tile needs no maximum, the sum tells.  Weights go to the tensor core in the inputs' type: rounded by half an ulp like
-// the inputs themselves, under 2^15, and the 7 keeps fp16's subnormal steps at 2^-32 of a row's largest weight.  Their
-// sum and the accumulator are fp32 and have the same factor.
+// What bounds it (one B200, bf16, D = 128): the products.  16383 tokens, 16 / 8 heads: 0.84 ms, 1310 TFLOP/s; 0.72 with
+// the softmax left out, 0.68 with the scores issued without waiting for the product before them.  A K . Q product of
+// 128 x 128 x 16 reads 8 KB of shared memory in its 64 cycles, all that there is, next to V's 4 KB and the copies; two SMs
+// that share a tile's other operand would halve that.  D = 64 (0.76 PFLOP/s at 8192 tokens): the exponentials, 9 to 10
+// cycles each in a warp.  Short prompts: a block's start and end, 2 us of which its neighbours hide a part.
+// Measured and not kept, of 16383 tokens: two warps that issue the products, by kind or by query tile (0.91 and 1.03 ms:
+// the tiles' softmax phases drift onto each other, where the one warp's order keeps them apart); two threads a row (1.4);
+// a quarter of the exponentials as polynomials (0.88); weights checked by their sum in place of the maximum (0.86); one
+// hand-over of the weights in place of two (0.87); the next block's first scores issued before the last of B (0.85).
+//
+// Softmax: thread = row, so nothing is exchanged.  The reference m moves only when a score exceeds it by more than 8 (in
+// powers of two); only then are the sum and the accumulator rescaled.  Weights 2^(s - m + 7) go to the tensor core in
+// the inputs' type: rounded by half an ulp like the inputs themselves, at most 2^15, and the 7 keeps fp16's subnormal steps
+// at 2^-32 of a row's largest weight.  Their sum and the accumulator are fp32 and have the same factor.
 //
 // Keys that a row does not see have weight 0, but 0 times a value that is not finite is not 0.  So a warp looks through
 // every V tile that some row of the block does not see all of: rows behind the block's last position become zeros,
@@ -230,6 +239,7 @@ struct PCfg {
 struct PromptTiles {
   PromptArgs a;
   int grp, pos;     // query heads of a key head, positions of a tile
+  int block;        // positions of a block: of one tile or of two
   int* status;
   const long long* limit;
 };
@@ -265,23 +275,6 @@ template <typename T>
 __device__ __forceinline__ uint32_t not_finite2(uint32_t w) {
   if constexpr (std::is_same<T, __half>::value) return ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
   else return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
-}
-
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {  // NaN if one is
-  float y;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-  return y;
-}
-__device__ __forceinline__ float max64(const float* x, float y) {
-  float top[4] = {y, x[0], x[1], x[2]};
-#pragma unroll
-  for (int e = 3; e < 59; e += 8) {
-#pragma unroll
-    for (int c = 0; c < 4; ++c) top[c] = max3_nan(top[c], x[e + 2 * c], x[e + 2 * c + 1]);
-  }
-  top[0] = max3_nan(top[0], x[59], x[60]);
-  top[1] = max3_nan(top[1], x[61], x[62]);
-  return max3_nan(max3_nan(top[0], top[1], top[2]), top[3], x[63]);
 }
 
 template <typename T>
@@ -409,7 +402,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         while (x >= 0 && !ctl->abort) {
           const int slot = x / a.hk, head = x - slot * a.hk;
           PromptBlock blk;
-          if (prompt_block(a, 2 * P, slot, blk)) {
+          if (prompt_block(a, ta.block, slot, blk)) {
             if (blk.real) {
               t.first = static_cast<int>(blk.first);
               t.row0 = static_cast<int>(blk.row0 - blk.first);
@@ -673,7 +666,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const int pos0 = t.row0 + w * P;  // the tile's first position
       const int pos = pos0 + p;
       float m = kPromptLowest;
-      float2 l2 = make_float2(0.f, 0.f);
+      float2 l2[2] = {};
       bool ok = true;
 #pragma unroll 1
       for (int i = 0; i < t.n[w]; ++i, ++it) {
@@ -689,14 +682,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll
           for (int c = 0; c < 128; ++c) x[c] = c < see ? x[c] : -INFINITY;
         }
-        float top[4];
+        float top[8];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          top[c] = fmaxf(x[c * 32], x[c * 32 + 1]);
+        for (int c = 0; c < 8; ++c) top[c] = fmaxf(x[c * 16], x[c * 16 + 1]);
 #pragma unroll
-          for (int e = 2; e < 32; e += 2) top[c] = max3(top[c], x[c * 32 + e], x[c * 32 + e + 1]);
-        }
-        const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sc;
+        for (int e = 2; e < 16; e += 2)
+#pragma unroll
+          for (int c = 0; c < 8; ++c) top[c] = max3(top[c], x[c * 16 + e], x[c * 16 + e + 1]);
+        const float best = fmaxf(max3(max3(top[0], top[1], top[2]), top[3], top[4]), max3(top[5], top[6], top[7])) * sc;
         if (i == 0) {
           m = fmaxf(best, kPromptLowest);
         } else if (__any_sync(0xffffffffu, best > m + kPromptSlack)) {
@@ -704,8 +697,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           const float to = best > m + kPromptSlack ? best : m;
           const float f = exp2_approx(m - to);
           m = to;
-          l2.x *= f;
-          l2.y *= f;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) l2[e] = __fmul2_rn(l2[e], make_float2(f, f));
 #pragma unroll 1
           for (int c = 0; c < D; c += 16) {
             uint32_t o[16];
@@ -726,7 +719,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             const int e = h * 64 + 2 * c;
             const float2 z = __ffma2_rn(make_float2(x[e], x[e + 1]), sc2, m2);
             const float2 v = make_float2(exp2_approx(z.x), exp2_approx(z.y));
-            l2 = __fadd2_rn(l2, v);
+            l2[c % 2] = __fadd2_rn(l2[c % 2], v);
             packed[c] = pack2<T>(v);
           }
           tmem_st32(s_tm + h * 32, packed);
@@ -745,7 +738,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       uint32_t any = 0;
 #pragma unroll
       for (int k = 0; k < 12; ++k) any |= odd[sl * 12 + k];
-      const float sum = l2.x + l2.y;
+      const float2 l4 = __fadd2_rn(l2[0], l2[1]);
+      const float sum = l4.x + l4.y;
       const float inv = sum == 0.f ? 0.f : __frcp_rn(sum);
       const bool mine = p < P && pos < t.row1;
       // 64 elements of the rows at a time through shared memory, so that a store has 128 bytes of each of four rows: 16
@@ -836,6 +830,11 @@ static int launch_tiles(const PromptArgs& a, cudaStream_t st) {
   ta.a = a;
   ta.grp = a.hq / a.hk;
   ta.pos = 128 / ta.grp;
+  // Few rows: blocks of one tile, so that twice as many SMs share them and each walks its keys faster (1.4 us for 128 keys,
+  // 1.75 with two tiles); once two-tile blocks fill the SMs, those.  16 / 8 heads of 128, one prompt, us with one tile and
+  // with two: 1024 tokens 18.3 and 20.5, 2048 (128 two-tile blocks) 30.9 and 34.2, 3000 (188) 60.7 and 46.1.
+  const bool few = (a.n / (2 * ta.pos) + a.b) * a.hk <= num_sms();
+  ta.block = few ? ta.pos : 2 * ta.pos;
   if (int s = device_wait_ptrs(&ta.status, &ta.limit)) return s;
   const CUtensorMapDataType dt =
       std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
@@ -849,7 +848,7 @@ static int launch_tiles(const PromptArgs& a, cudaStream_t st) {
   if (int s = map(&tq, a.q, a.q_st, a.q_sh, a.hq, ta.grp, ta.pos)) return s;
   if (int s = map(&tk, a.k, a.k_st, a.k_sh, a.hk, 1, kPromptKeys)) return s;
   if (int s = map(&tv, a.v, a.v_st, a.v_sh, a.hk, 1, kPromptKeys)) return s;
-  const int64_t slots = a.n / (2 * ta.pos) + a.b + 2;
+  const int64_t slots = a.n / ta.block + a.b + 2;
   prompt_tile_kernel<D, T><<<static_cast<unsigned>(slots * a.hk), kPromptThreads, C::SMEM, st>>>(tq, tk, tv, ta);
   return check_launch("prompt_tile_kernel");
 }
@@ -903,7 +902,7 @@ extern "C" int bw_prompt_attention(const void* q, int64_t q_st, int64_t q_sh, co
   }
   if ((d == 64 || d == 128) && hq / hk <= 128 && softmax_scale > 0.f && softmax_scale <= 3.402823466e38f &&
       tma_rows(q, a.q_st, a.q_sh) && tma_rows(k, a.k_st, a.k_sh) && tma_rows(v, a.v_st, a.v_sh) &&
-      reinterpret_cast<uintptr_t>(out) % 16 == 0 && (n / (2 * (128 / (hq / hk))) + b + 2) * hk <= INT32_MAX) {
+      reinterpret_cast<uintptr_t>(out) % 16 == 0 && (n / (128 / (hq / hk)) + b + 2) * hk <= INT32_MAX) {
     if (dtype == BW_DTYPE_BF16) return d == 128 ? launch_tiles<128, __nv_bfloat16>(a, st) : launch_tiles<64, __nv_bfloat16>(a, st);
     return d == 128 ? launch_tiles<128, __half>(a, st) : launch_tiles<64, __half>(a, st);
   }
