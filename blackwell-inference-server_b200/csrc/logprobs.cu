@@ -2,23 +2,27 @@
 //
 // With m = max x, S = sum exp(x - m), T = sum (x - m) exp(x - m) over a row x of logits:
 //   log p(i) = x_i - m - ln S,   H = -sum p ln p = ln S - T / S   (both terms of H are >= 0: nothing cancels).
-// A thread keeps m, S and T (in powers of two) of what it has seen and rescales S and T where m moves; the joins
-// are made in one order, so results do not depend on timing.
+// A thread keeps m, S and T (in powers of two) of what it has seen and rescales S and T where m moves.  A row is
+// cut into four parts, one group of eight logits a thread to each in turn; a cluster of one, two or four CTAs has a
+// row, and a thread's sums of the four parts are joined first, then the threads': the order of a sum is the same
+// for every cluster and every number of rows, so a row's results depend on neither.
 //
-// The alternatives cost the pass nothing but where each thread's maximum is.  A thread sees every 512th group of
-// eight logits; the k largest logits (by value, then by lowest index: a total order) lie in the k threads whose
+// The alternatives cost the pass nothing but where each thread's maximum is.  A thread sees every 256th group of
+// its CTA's; the k largest logits (by value, then by lowest index: a total order) lie in the k threads whose
 // maxima are largest by (value, group), for if one lay elsewhere, k maxima would come before it.  So the k best
 // threads are found (a sort of 32 in each warp, merges of sorted lists), and only their groups are read again,
-// one 512th of the row each, from L2: k lists of some 300 logits, of which those before the k-th maximum are candidates.
+// one 256th of the CTA's each, from L2: lists of some 300 logits, of which those before the k-th maximum are candidates.
+#include <mutex>
 #include <type_traits>
 
 #include "common.cuh"
 
 namespace bw {
 
-constexpr int kLpThreads = 512;
+constexpr int kLpThreads = 256;
 constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kLpTop = 32;  // alternatives at most: a list is a warp's
+constexpr int kLpParts = 4;
 
 struct LogprobArgs {
   const void* x;        // [rows, v], row stride ld
@@ -129,17 +133,44 @@ __device__ __forceinline__ float lp_to_f32(float x) { return x; }
 __device__ __forceinline__ float lp_to_f32(__half x) { return __half2float(x); }
 __device__ __forceinline__ float lp_to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// One CTA a row.
+__device__ __forceinline__ void copy16_async(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void lp_send(uint32_t addr, const LpSums& x) {
+  st_shared_cluster_f32(addr, x.m);
+  st_shared_cluster_f32(addr + 4, x.s);
+  st_shared_cluster_f32(addr + 8, x.t);
+}
+
+// Steps of four groups that a thread has on their way in shared memory, and CTAs of an SM.  16-bit logits: three, 192 KB an SM,
+// which registers have no room for (2047 rows of 151936: 125 us, from registers 141).  fp32 logits have 128 bytes a thread in a
+// step as it is, from registers (2047 rows of 50257: 85 us, through shared memory 112).
 template <typename T>
-__global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(const LogprobArgs a) {
-  constexpr int U = 8 / sizeof(T);  // groups of a thread on their way
+struct LpRing {
+  static constexpr int STAGES = sizeof(T) == 4 ? 0 : 3, CTAS = sizeof(T) == 4 ? 3 : 4;
+  static constexpr int BYTES = STAGES * kLpParts * kLpThreads * 16;
+};
+
+// A cluster of kLpParts / OWN CTAs a row.
+template <typename T, int OWN>
+__global__ void __launch_bounds__(kLpThreads, LpRing<T>::CTAS) token_logprobs_kernel(const LogprobArgs a) {
+  constexpr int U = kLpParts / OWN;  // groups of a part in a step
+  constexpr int STAGES = LpRing<T>::STAGES;
+  extern __shared__ uint4 ring[];    // [stage][group of a step][thread]
   __shared__ unsigned long long lists[kLpWarps][32];
-  __shared__ LpSums part[kLpWarps];
-  __shared__ LpSums whole;
-  const int64_t row = blockIdx.x;
+  __shared__ unsigned long long firsts[32];              // the k best threads
+  __shared__ unsigned long long from[kLpParts][32];      // at rank 0: the CTAs' lists
+  __shared__ LpSums sent[kLpParts][kLpThreads];          //            their threads' sums
+  __shared__ float tops[kLpWarps];
+  __shared__ float2 part[kLpWarps];
+  constexpr int ctas = kLpParts / OWN, own = OWN;  // CTAs of the row, parts of this one
+  const int rank = ctas > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  if (ctas > 1) cluster_arrive();
+  const int64_t row = blockIdx.x / ctas;
   const T* x = static_cast<const T*>(a.x) + row * a.ld;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   // Groups lie on 32-byte (16-bit types: 16-byte) boundaries of memory: index i of group c is 8 c - shift + i.
+  // Group c is thread c % 256's of part c / 256 % 4.
   const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(x) / sizeof(T) & 7);
   const int groups = static_cast<int>((static_cast<int64_t>(a.v) + shift + 7) >> 3);
   const int whole_lo = shift ? 1 : 0, whole_hi = static_cast<int>((static_cast<int64_t>(a.v) + shift) >> 3);
@@ -155,22 +186,26 @@ __global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(const Logpro
       }
     }
   };
-  const int64_t tok = tid == 0 ? a.tok[row] : -1;
+  const int64_t tok = tid == 0 && rank == 0 ? a.tok[row] : -1;
   const bool given = tok >= 0 && tok < a.v;
   const float x_tok = given ? lp_to_f32(x[tok]) : 0.f;
 
-  LpSums sum = {-INFINITY, 0.f, 0.f};
-  int best = tid;  // the first group with the thread's maximum
-  auto take = [&](int c, const float(&f)[8]) {
-    float top = fmaxf(f[0], f[1]);
+  LpSums sum[OWN];                              // of the parts
 #pragma unroll
-    for (int e = 2; e < 8; ++e) top = fmaxf(top, f[e]);
+  for (int p = 0; p < OWN; ++p) sum[p] = {-INFINITY, 0.f, 0.f};
+  float most = -INFINITY;                       // the thread's maximum, and the first of its groups that has it
+  int best = rank * own * kLpThreads + tid;
+  auto take = [&](int c, const float(&f)[8], LpSums& sum) {
+    const float top = fmaxf(max3(max3(f[0], f[1], f[2]), f[3], f[4]), max3(f[5], f[6], f[7]));
     if (top > sum.m) {
       const float d = fmaxf((sum.m - top) * kLog2e, kNoWeight), w = exp2_approx(d);
       sum.t = w * (sum.t + d * sum.s);
       sum.s *= w;
       sum.m = top;
-      best = c;
+      if (top > most || (top == most && c < best)) {
+        most = top;
+        best = c;
+      }
     }
     const float m = sum.m == -INFINITY ? 0.f : sum.m;  // (-inf alone weighs nothing)
     const float2 m2 = make_float2(-m, -m), c2 = make_float2(kLog2e, kLog2e);
@@ -187,77 +222,122 @@ __global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(const Logpro
     sum.t += t.x + t.y;
   };
   {
+    // four groups at a time, whatever the cluster: of one part, of two or of four
+    constexpr int step = kLpParts * kLpThreads;
+    const int c0 = rank * own * kLpThreads + tid;
     float f[8];
-    if (tid == 0 && shift) {
+    if (c0 == 0 && shift) {
       load(0, f);
-      take(0, f);
+      take(0, f, sum[0]);
     }
-    int c = tid < whole_lo ? tid + kLpThreads : tid;
-    for (; c < whole_hi; c += U * kLpThreads) {
-      LpRaw<T> raw[U];
+    if constexpr (LpRing<T>::STAGES == 0) {
+      for (int k = 0; c0 + k < whole_hi; k += U * step) {
+        LpRaw<T> raw[kLpParts];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (c + u * kLpThreads < whole_hi) raw[u] = lp_fetch<T>(at(c + u * kLpThreads));
+        for (int n = 0; n < kLpParts; ++n) {
+          const int c = c0 + k + n % OWN * kLpThreads + n / OWN * step;
+          if (c >= whole_lo && c < whole_hi) raw[n] = lp_fetch<T>(at(c));
+        }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (c + u * kLpThreads < whole_hi) {
-          lp_unpack<T>(raw[u], f);
-          take(c + u * kLpThreads, f);
+        for (int n = 0; n < kLpParts; ++n) {
+          const int c = c0 + k + n % OWN * kLpThreads + n / OWN * step;
+          if (c >= whole_lo && c < whole_hi) {
+            lp_unpack<T>(raw[n], f);
+            take(c, f, sum[n % OWN]);
+          }
         }
       }
+    } else {
+      // Each thread copies its own groups to shared memory, three steps of four ahead (nobody else reads them: no barrier).
+      auto fetch = [&](int k, int stage) {
+#pragma unroll
+        for (int n = 0; n < kLpParts; ++n) {
+          const int c = c0 + k + n % OWN * kLpThreads + n / OWN * step;
+          if (c >= whole_lo && c < whole_hi)
+            copy16_async(&ring[(stage * kLpParts + n) * kLpThreads + tid], at(c));
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+#pragma unroll
+      for (int i = 0; i < STAGES; ++i) fetch(i * U * step, i);
+      int stage = 0;
+      for (int k = 0; c0 + k < whole_hi; k += U * step) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+#pragma unroll
+        for (int n = 0; n < kLpParts; ++n) {
+          const int c = c0 + k + n % OWN * kLpThreads + n / OWN * step;
+          if (c >= whole_lo && c < whole_hi) {
+            LpRaw<T> raw;
+            raw.w[0] = ring[(stage * kLpParts + n) * kLpThreads + tid];
+            lp_unpack<T>(raw, f);
+            take(c, f, sum[n % OWN]);
+          }
+        }
+        fetch(k + STAGES * U * step, stage);
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
     }
     const int last = groups - 1;  // a group that the row ends in
-    if (last >= whole_hi && (last > 0 || !shift) && tid == last % kLpThreads) {
-      load(last, f);
-      take(last, f);
+    if (last >= whole_hi && (last > 0 || !shift)) {
+#pragma unroll
+      for (int p = 0; p < OWN; ++p)
+        if (c0 + p * kLpThreads == last % step) {
+          load(last, f);
+          take(last, f, sum[p]);
+        }
     }
   }
-  const unsigned long long mine = tid < groups ? lp_key(sum.m, best) : 0ull;  // 0: a thread without groups
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    LpSums other;
-    other.m = __shfl_xor_sync(0xffffffffu, sum.m, o);
-    other.s = __shfl_xor_sync(0xffffffffu, sum.s, o);
-    other.t = __shfl_xor_sync(0xffffffffu, sum.t, o);
-    sum = lane & o ? lp_join(other, sum) : lp_join(sum, other);
+  LpSums all = sum[0];  // (0 + 1) + (2 + 3), or what the CTA has of it
+  if constexpr (OWN >= 2) all = lp_join(sum[0], sum[1]);
+  if constexpr (OWN == 4) all = lp_join(all, lp_join(sum[2], sum[3]));
+  const bool any = rank * own * kLpThreads + tid < groups;  // the thread has a group
+  unsigned long long mine = any ? lp_key(most, best) : 0ull;
+  if (ctas > 1) {
+    cluster_wait();  // every CTA runs: its shared memory may be written
+    if (rank != 0) lp_send(mapa_shared(smem_u32(&sent[rank][tid]), 0), all);
   }
-  if (lane == 0) part[warp] = sum;
-  __syncthreads();
-  if (tid == 0) {
-    LpSums all = part[0];
+  // the k best threads of the CTA, then the CTA's k best
+  unsigned long long list = 0ull;  // the warp's best so far, descending
+  if (a.top > 0) {
+    unsigned long long limit;  // the k-th maximum: what comes behind it is not among the k
+    if (a.top == 1) {
 #pragma unroll
-    for (int w = 1; w < kLpWarps; ++w) all = lp_join(all, part[w]);
-    whole = all;
-    const float log_s = log2f(all.s) * kLn2;
-    const bool bad = !(all.s <= 3.402823466e38f), none = all.m == -INFINITY;
-    a.logp[row] = !given ? 0.f : (bad ? NAN : (none ? -INFINITY : (x_tok - all.m) - log_s));
-    a.entropy[row] = bad ? NAN : (none ? 0.f : log_s - all.t / all.s * kLn2);
-  }
-  if (a.top == 0) return;
-  lp_merge_warps(lists, lp_sort(mine, lane), warp, lane);
-  const unsigned long long limit = lists[0][a.top - 1];  // the k-th maximum: what comes behind it is not among the k
-  unsigned long long list = 0ull;                        // the warp's best so far, descending
-  unsigned long long first[2];                           // this warp's threads to read again: the warp-th and so on
-  static_assert(kLpTop <= 2 * kLpWarps, "two a warp");
+      for (int o = 16; o > 0; o >>= 1) mine = lp_max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+      if (lane == 0) lists[warp][0] = mine;
+      __syncthreads();
+      limit = lists[lane % kLpWarps][0];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) first[k] = warp + k * kLpWarps < a.top ? lists[0][warp + k * kLpWarps] : 0ull;
-  __syncthreads();
-#pragma unroll 1
-  for (int k = 0; k < 2; ++k) {
-    if (first[k] == 0ull) break;
-    const int column = static_cast<int>((0xffffffffu - static_cast<uint32_t>(first[k])) % kLpThreads);
-    for (int c0 = column; c0 < groups; c0 += 32 * kLpThreads) {
-      const int c = c0 + lane * kLpThreads;
+      for (int o = kLpWarps / 2; o > 0; o >>= 1) limit = lp_max(limit, __shfl_xor_sync(0xffffffffu, limit, o));
+      if (tid == 0) firsts[0] = limit;
+    } else {
+      lp_merge_warps(lists, lp_sort(mine, lane), warp, lane);
+      limit = lists[0][a.top - 1];
+      if (warp == 0) firsts[lane] = lists[0][lane];
+    }
+    __syncthreads();
+    // The k threads' groups, `each` of one at most, one a lane.  They are few: most lanes find nothing before the limit.
+    const int each = (groups + kLpParts * kLpThreads - 1) / (kLpParts * kLpThreads) * own;
+    for (int q0 = warp * 32; q0 < a.top * each; q0 += kLpThreads) {
+      const int k = (q0 + lane) / each, j = q0 + lane - k * each;
+      const unsigned long long first = k < a.top ? firsts[k] : 0ull;
+      const int column = static_cast<int>((0xffffffffu - static_cast<uint32_t>(first)) % kLpThreads);
+      const int c = (j / own * kLpParts + rank * own + j % own) * kLpThreads + column;
       float f[8];
-      if (c < groups) load(c, f);
+      bool has = false;
+      if (first != 0ull && c < groups) {
+        load(c, f);
+        has = lp_key(fmaxf(max3(max3(f[0], f[1], f[2]), f[3], f[4]), max3(f[5], f[6], f[7])), c) >= limit;
+      }
+      if (!__any_sync(0xffffffffu, has)) continue;
 #pragma unroll 1
       for (int e = 0; e < 8; ++e) {
         const int64_t i = static_cast<int64_t>(c) * 8 - shift + e;
         unsigned long long key = 0ull;
-        if (c < groups && i >= 0 && i < a.v) {
+        if (has && i >= 0 && i < a.v) {
           float v = f[0];
 #pragma unroll
-          for (int j = 1; j < 8; ++j) v = e == j ? f[j] : v;
+          for (int n = 1; n < 8; ++n) v = e == n ? f[n] : v;
           if (lp_key(v, c) >= limit) key = lp_key(v, static_cast<uint32_t>(i));
         }
         unsigned todo = __ballot_sync(0xffffffffu, key > __shfl_sync(0xffffffffu, list, 31));
@@ -270,23 +350,97 @@ __global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(const Logpro
         }
       }
     }
+    lp_merge_warps(lists, list, warp, lane);  // (at top 1, any warp may have the one)
+    if (warp == 0) list = lists[0][lane];
+    if (ctas > 1 && rank != 0 && warp == 0) {
+      const uint32_t to = mapa_shared(smem_u32(&from[rank][lane]), 0);
+      asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(to), "l"(list) : "memory");
+    }
   }
-  lp_merge_warps(lists, list, warp, lane);
-  if (tid < a.top) {
-    const unsigned long long key = lists[0][tid];
-    const LpSums all = whole;
-    const bool bad = !(all.s <= 3.402823466e38f);
-    const float log_s = log2f(all.s) * kLn2;
-    const float v = lp_value(static_cast<uint32_t>(key >> 32));
-    a.top_logp[row * a.top + tid] = bad ? NAN : (v == -INFINITY ? -INFINITY : (v - all.m) - log_s);
-    a.top_tok[row * a.top + tid] = bad ? -1 : static_cast<int64_t>(0xffffffffu - static_cast<uint32_t>(key));
+  if (ctas > 1) {
+    cluster_sync_all();  // (no CTA is written to after this)
+    if (rank != 0) return;
+    all = ctas == 2 ? lp_join(all, sent[1][tid]) : lp_join(lp_join(all, sent[1][tid]), lp_join(sent[2][tid], sent[3][tid]));
   }
+  // the maximum of all threads, then their sums relative to it
+  float top = all.m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) tops[warp] = top;
+  __syncthreads();
+  top = tops[lane % kLpWarps];
+#pragma unroll
+  for (int o = kLpWarps / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  {
+    const float d = fmaxf((all.m - top) * kLog2e, kNoWeight), w = exp2_approx(d);
+    all.t = w * (all.t + d * all.s);
+    all.s *= w;
+    all.m = top;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    all.s += __shfl_xor_sync(0xffffffffu, all.s, o);
+    all.t += __shfl_xor_sync(0xffffffffu, all.t, o);
+  }
+  if (lane == 0) part[warp] = make_float2(all.s, all.t);
+  __syncthreads();
+  if (warp != 0) return;
+  all.s = part[lane % kLpWarps].x;
+  all.t = part[lane % kLpWarps].y;
+#pragma unroll
+  for (int o = kLpWarps / 2; o > 0; o >>= 1) {
+    all.s += __shfl_xor_sync(0xffffffffu, all.s, o);
+    all.t += __shfl_xor_sync(0xffffffffu, all.t, o);
+  }
+  const float log_s = log2f(all.s) * kLn2;
+  const bool bad = !(all.s <= 3.402823466e38f), none = all.m == -INFINITY;
+  if (tid == 0) {
+    a.logp[row] = !given ? 0.f : (bad ? NAN : (none ? -INFINITY : (x_tok - all.m) - log_s));
+    a.entropy[row] = bad ? NAN : (none ? 0.f : log_s - all.t / all.s * kLn2);
+  }
+  if (a.top == 0) return;
+  for (int r = 1; r < ctas; ++r) list = lp_merge(list, from[r][31 - lane], lane);
+  if (lane < a.top) {
+    const float v = lp_value(static_cast<uint32_t>(list >> 32));
+    a.top_logp[row * a.top + lane] = bad ? NAN : (v == -INFINITY ? -INFINITY : (v - all.m) - log_s);
+    a.top_tok[row * a.top + lane] = bad ? -1 : static_cast<int64_t>(0xffffffffu - static_cast<uint32_t>(list));
+  }
+}
+
+template <typename T, int OWN>
+static int launch_logprobs_own(const LogprobArgs& a, int64_t rows, cudaStream_t st) {
+  static std::once_flag once[64];
+  static cudaError_t attr_err[64];
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev)) return check_cuda(e, "cudaGetDevice");
+  dev &= 63;
+  std::call_once(once[dev], [&] {
+    attr_err[dev] = cudaFuncSetAttribute(token_logprobs_kernel<T, OWN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         LpRing<T>::BYTES);
+  });
+  if (int s = check_cuda(attr_err[dev], "cudaFuncSetAttribute(token_logprobs_kernel)")) return s;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kLpParts / OWN;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cfg.stream = st;
+  cfg.gridDim = dim3(static_cast<unsigned>(rows * (kLpParts / OWN)));
+  cfg.blockDim = dim3(kLpThreads);
+  cfg.dynamicSmemBytes = LpRing<T>::BYTES;
+  return check_cuda(cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, OWN>, a), "cudaLaunchKernelEx(token_logprobs_kernel)");
 }
 
 template <typename T>
 static int launch_logprobs(const LogprobArgs& a, int64_t rows, cudaStream_t st) {
-  token_logprobs_kernel<T><<<static_cast<unsigned>(rows), kLpThreads, 0, st>>>(a);
-  return check_launch("token_logprobs_kernel");
+  // Few rows: clusters, as long as two CTAs an SM hold them.  Us with one, two and four CTAs a row: 64 rows of 128256, top 5:
+  // 22, 16 and 14; 148 rows: 22, 19 and 27; 333 rows of 151936, top 1: 36, 39 and 45.
+  const int ctas = rows * 4 <= 2 * num_sms() ? 4 : (rows * 2 <= 2 * num_sms() ? 2 : 1);
+  if (ctas == 4) return launch_logprobs_own<T, 1>(a, rows, st);
+  return ctas == 2 ? launch_logprobs_own<T, 2>(a, rows, st) : launch_logprobs_own<T, 4>(a, rows, st);
 }
 
 }  // namespace bw
