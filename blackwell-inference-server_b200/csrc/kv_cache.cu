@@ -240,12 +240,13 @@ __device__ __forceinline__ void codes16(const float* x, float sc, float rcp, uin
 // memory; a group takes every `gpt`-th row of its token.  Bound by the bytes where tokens are many (which
 // wants many warps: with each lane's sines in its registers four warps a scheduler did not cover the
 // latency), by latency where they are few, for which the host spreads a token over more groups.
-// NORM: a row's squares are summed over its L lanes by shuffles between the read and the turn; the weights lie
-// in shared memory, four of a lane beside its neighbours' four, so that a row's reads meet no bank twice.
+// NORM: a row's squares are summed over its L lanes by shuffles between the read and the turn; a lane has its weights
+// in registers, as they are, while a token's queries last, and then its keys' (read from shared memory as fp32 for every
+// row, that memory was the bound: 8191 tokens of 40 rows 39.7 us for 36.0, 4.7 TB/s).
 template <typename T, int L, bool WRITE, bool INTER, bool NORM>
 __global__ void __launch_bounds__(256, WRITE ? 3 : 4) rotary_vec_kernel(const __grid_constant__ RotArgs a, int gpt) {
   constexpr int D = 16 * L;
-  __shared__ float4 weights_of[NORM ? 2 * D / 4 : 1];  // [q, k][a lane's four times four][lane]
+  __shared__ __align__(16) T weights_of[NORM ? 2 * D : 8];  // [q, k][a lane's first eight, second eight][lane]
   // (cos, sin) of the CTA's tokens' pairs: 256 / (gpt L) tokens of rot / 2 <= 8 L pairs, so gpt is 8 at least (NORM: 4)
   __shared__ __align__(16) float2 turns_of[NORM ? 512 : 256];
   const int j = threadIdx.x % L;
@@ -283,14 +284,12 @@ __global__ void __launch_bounds__(256, WRITE ? 3 : 4) rotary_vec_kernel(const __
   fetch(g, next);
   if constexpr (NORM) {
     if (WRITE && rows > 0) krow = target_row(a, b, t);
-    // four c of lane l: its elements 4 c .., as the rows' chunks below have them
     for (int n = threadIdx.x; n < 2 * D; n += 256) {
       const T* w = static_cast<const T*>(n < D ? a.qw : a.kw);
-      const int c = n % D / (4 * L), l = n % D / 4 % L, k = n % 4;
+      const int c = n % D / (8 * L), l = n % D / 8 % L;
       const bool turned = l < a.rot / 16;
-      const int e = (c < 2 ? (turned ? 8 * l : a.rot / 2 + 8 * l) : (turned ? a.rot / 2 + 8 * l : D / 2 + 8 * l)) +
-                    c % 2 * 4 + k;
-      if (w != nullptr) reinterpret_cast<float*>(weights_of)[n] = to_f32(w[e]);
+      const int e = (c == 0 ? (turned ? 8 * l : a.rot / 2 + 8 * l) : (turned ? a.rot / 2 + 8 * l : D / 2 + 8 * l)) + n % 8;
+      if (w != nullptr) weights_of[n] = w[e];
     }
   }
   for (int e = threadIdx.x; e < in_cta * half; e += 256) {
@@ -306,6 +305,8 @@ __global__ void __launch_bounds__(256, WRITE ? 3 : 4) rotary_vec_kernel(const __
   const float4* cs0 = reinterpret_cast<const float4*>(turns_of + static_cast<int>(tok - tok0) * half) +
                       (INTER ? e0 / 4 : 4 * j);
   const float4* cs1 = INTER ? cs0 - e0 / 4 + e1 / 4 : cs0 + 2;
+  uint4 w01[2];  // NORM: the lane's weights, of q or of k
+  int has = -1;
 #pragma unroll 1
   for (int h = g; h < rows; h += gpt) {
     const uint4 raw[2] = {next[0], next[1]};
@@ -325,13 +326,17 @@ __global__ void __launch_bounds__(256, WRITE ? 3 : 4) rotary_vec_kernel(const __
 #pragma unroll
       for (int o = L / 2; o > 0; o >>= 1) all += __shfl_xor_sync(lanes, all, o);
       const float r = rsqrtf(all * (1.0f / D) + a.eps);
+      if (WRITE || which != has) {  // (the write's codes leave no registers for them)
+        has = which;
+        w01[0] = *reinterpret_cast<const uint4*>(weights_of + which * D + 8 * j);
+        w01[1] = *reinterpret_cast<const uint4*>(weights_of + which * D + 8 * L + 8 * j);
+      }
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float4 w = weights_of[which * (D / 4) + c * L + j];
-        v[4 * c] *= r * w.x;
-        v[4 * c + 1] *= r * w.y;
-        v[4 * c + 2] *= r * w.z;
-        v[4 * c + 3] *= r * w.w;
+      for (int c = 0; c < 2; ++c) {
+        float w[8];
+        unpack8<T>(w01[c], w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[8 * c + i] *= r * w[i];
       }
     }
     if (turns && !plain) {
@@ -382,8 +387,8 @@ static bool rows_aligned(const RowSet& s) {
 template <typename T, int L, bool NORM>
 static int launch_rotary_vec(const RotArgs& a, bool write, cudaStream_t st) {
   // Row groups of a token: eight (a lane's sines then serve many rows), more where the tokens alone do not
-  // fill the SMs, up to one for each row.  With norms, whose weights a CTA fetches as well, four: 8191 tokens of 40 rows
-  // 39.7 us, 4.2 TB/s (41.6 with eight, 39.7 with two).
+  // fill the SMs, up to one for each row.  With norms, whose weights a CTA fetches as well, four (a twentieth faster on
+  // 8191 tokens of 40 rows than eight; two are as fast as four).
   const int rows = a.q.heads + a.k.heads + a.v.heads;
   const int64_t tokens = a.b * a.t;
   int gpt = NORM ? 4 : 8;
