@@ -16,6 +16,15 @@ their final slots, and the last token is the next tree's root.
     mdl = MultiDeltaLoRAModel(model, device="cuda")
     dec = TreeSpeculativeDecoder(mdl, batch=1, max_len=4096)
     new = dec.generate(ids, max_new_tokens=64, adapter="a")
+
+Whole prompts of different lengths go through one pass over their packed tokens (``score``, ``prefill_packed``, and
+``generate`` with ``packed=True``), whose layers normalise and rotate queries and keys in one launch, which writes the
+cache too, and attend with ``prompt_attention`` to the 16-bit keys and values:
+
+    norm_rotary_kv_write_int8 (score: norm_rotary) -> prompt_attention.
+
+    for s in dec.score([first, second], top=5):  # log probabilities of each prompt's tokens, as a server returns them
+        print(s.logprobs, s.top_tokens)
 """
 from __future__ import annotations
 
@@ -96,9 +105,14 @@ class TreeSpeculativeDecoder:
     """Decodes ``batch`` sequences of at most ``max_len`` tokens, ``nodes`` tree nodes a step (1: plain decoding).
 
     Takes models of ``MODEL_TYPES``.  Attention windows shorter than ``max_len + nodes``, heads that turn in part and
-    rotations that ``rotary_frequencies`` does not know are refused."""
+    rotations that ``rotary_frequencies`` does not know are refused.
 
-    def __init__(self, model: MultiDeltaLoRAModel, batch: int, max_len: int, nodes: int = 16, page: int = 64):
+    ``packed``: ``generate`` takes its prompts in one pass (``prefill_packed``) and every step normalises queries and keys
+    in the launch that rotates them.  Without it prompts go in chains of 64 through the decoding step, which rounds the
+    normalised queries and keys to 16 bits and attends to the int8 cache: the two differ by those roundings."""
+
+    def __init__(self, model: MultiDeltaLoRAModel, batch: int, max_len: int, nodes: int = 16, page: int = 64,
+                 packed: bool = False):
         from blackwell_ops.decode import MAX_NODES, KVCacheInt8, rotary_plan
 
         if not model.quantize:
@@ -106,7 +120,7 @@ class TreeSpeculativeDecoder:
         if not 1 <= nodes <= MAX_NODES:
             raise RuntimeError(f"1 to {MAX_NODES} nodes a step")
         self.model, self.batch, self.nodes = model, batch, nodes
-        self.max_len = max_len
+        self.max_len, self.packed = max_len, packed
         cfg = model.base.config
         if cfg.model_type not in MODEL_TYPES:
             raise RuntimeError(f"models of type {cfg.model_type!r} are not supported, only {', '.join(MODEL_TYPES)}")
@@ -132,8 +146,8 @@ class TreeSpeculativeDecoder:
         """Logits [B, T, V] after each node of a tree ``tokens``, ``parents`` [B, T] (None: a chain) that follows
         the committed tokens.  The nodes' keys and values go to slots ``ctx`` on; nothing is committed."""
         from blackwell_ops.cuda import rmsnorm
-        from blackwell_ops.decode import rotary_kv_write_int8, tree_attention_int8, tree_positions
-        from blackwell_ops.kernels.int8_gemm import int8_gemm_grouped
+        from blackwell_ops.decode import (norm_rotary_kv_write_int8, rotary_kv_write_int8, tree_attention_int8,
+                                          tree_positions)
 
         b, t = tokens.shape
         mask = None
@@ -144,15 +158,15 @@ class TreeSpeculativeDecoder:
         x = self.model.base.model.embed_tokens(tokens).reshape(b * t, -1)
         for layer, cache in zip(self.layers, self._layer_cache):
             att, mlp = layer.self_attn, layer.mlp
-            y = rmsnorm(x, layer.input_layernorm.weight, layer.input_layernorm.variance_epsilon)
-            proj = (att.q_proj, att.k_proj, att.v_proj)
-            if _fusable(proj):
-                q, k, v = int8_gemm_grouped(y, [p.copies[p.active] for p in proj])
-            else:
-                q, k, v = (p(y) for p in proj)
-            q, k = self._head_norm(q, getattr(att, "q_norm", None)), self._head_norm(k, getattr(att, "k_norm", None))
+            q, k, v = self._qkv(layer, x)
             shape = (b, t, -1, self.head_dim)
-            q = rotary_kv_write_int8(q.view(shape), k.view(shape), v.view(shape), pos, self.plan, cache, self.table, self.ctx)
+            if self.packed:
+                q, _ = norm_rotary_kv_write_int8(q.view(shape), k.view(shape), v.view(shape), pos, self.plan, cache,
+                                                 self.table, self.ctx, **self._norms(att))
+            else:
+                q, k = self._head_norm(q, getattr(att, "q_norm", None)), self._head_norm(k, getattr(att, "k_norm", None))
+                q = rotary_kv_write_int8(q.view(shape), k.view(shape), v.view(shape), pos, self.plan, cache, self.table,
+                                         self.ctx)
             o = tree_attention_int8(q, cache, self.table, self.ctx, mask, softmax_scale=att.scaling)
             x = x + att.o_proj(o.view(b * t, -1))
             y = rmsnorm(x, layer.post_attention_layernorm.weight, layer.post_attention_layernorm.variance_epsilon)
@@ -161,6 +175,60 @@ class TreeSpeculativeDecoder:
             return None
         norm = self.model.base.model.norm
         return self.model.base.lm_head(rmsnorm(x, norm.weight, norm.variance_epsilon)).view(b, t, -1)
+
+    def _qkv(self, layer, x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        from blackwell_ops.cuda import rmsnorm
+        from blackwell_ops.kernels.int8_gemm import int8_gemm_grouped
+
+        y = rmsnorm(x, layer.input_layernorm.weight, layer.input_layernorm.variance_epsilon)
+        proj = (layer.self_attn.q_proj, layer.self_attn.k_proj, layer.self_attn.v_proj)
+        if _fusable(proj):
+            return tuple(int8_gemm_grouped(y, [p.copies[p.active] for p in proj]))
+        return tuple(p(y) for p in proj)
+
+    def _norms(self, att) -> dict:
+        """What ``norm_rotary`` takes: a layer without norms of its heads has no weights."""
+        q, k = getattr(att, "q_norm", None), getattr(att, "k_norm", None)
+        if q is None and k is None:
+            return {}
+        return {"q_weight": None if q is None else q.weight, "k_weight": None if k is None else k.weight,
+                "eps": (k if q is None else q).variance_epsilon}
+
+    def _prompts(self, tokens: torch.Tensor, lens: list[int], write: bool) -> tuple[torch.Tensor, torch.Tensor]:
+        """Hidden states [N, hidden] of packed prompts ``tokens`` [N] of ``lens``, and their offsets.  ``write``: their keys
+        and values go to the cache's slots from 0 on."""
+        from blackwell_ops.cuda import rmsnorm
+        from blackwell_ops.decode import norm_rotary, norm_rotary_kv_write_int8
+        from blackwell_ops.prompt import prompt_attention
+
+        n = sum(lens)
+        ends = torch.tensor([0, *lens]).cumsum(0)
+        pos = torch.arange(n) - ends[:-1].repeat_interleave(torch.tensor(lens))
+        offsets, pos = ends.to(self.dev, torch.int32), pos.to(self.dev, torch.int32)
+        start = torch.zeros_like(self.ctx)
+        x = self.model.base.model.embed_tokens(tokens)
+        for layer, cache in zip(self.layers, self._layer_cache):
+            att = layer.self_attn
+            q, k, v = (y.view(n, -1, self.head_dim) for y in self._qkv(layer, x))
+            if write:
+                q, k = norm_rotary_kv_write_int8(q, k, v, pos, self.plan, cache, self.table, start, offsets=offsets,
+                                                 keys=True, **self._norms(att))
+            else:
+                q, k = norm_rotary(q, k, pos, self.plan, **self._norms(att))
+            x = x + att.o_proj(prompt_attention(q, k, v, offsets, softmax_scale=att.scaling).view(n, -1))
+            y = rmsnorm(x, layer.post_attention_layernorm.weight, layer.post_attention_layernorm.variance_epsilon)
+            x = x + self._mlp(layer.mlp, y)
+        return x, offsets
+
+    def _pack(self, prompts) -> tuple[torch.Tensor, list[int]]:
+        """Prompts, one behind the other on the device, and their lengths."""
+        prompts = [torch.as_tensor(p, dtype=torch.int64) for p in prompts]
+        if any(p.dim() != 1 for p in prompts):
+            raise RuntimeError("a prompt must be a list of tokens")
+        lens = [p.numel() for p in prompts]
+        if max(lens, default=0) > self.max_len:
+            raise RuntimeError(f"at most max_len = {self.max_len} tokens a sequence")
+        return torch.cat([p.to(self.dev) for p in prompts] or [torch.empty(0, dtype=torch.int64, device=self.dev)]), lens
 
     def _mlp(self, mlp, y: torch.Tensor) -> torch.Tensor:
         from blackwell_ops.kernels.int8_gemm import int8_gemm, int8_gemm_swiglu
@@ -194,6 +262,48 @@ class TreeSpeculativeDecoder:
             self.ctx += part.shape[1]
 
     @torch.no_grad()
+    def prefill_packed(self, prompts) -> None:
+        """Start afresh and commit one prompt a sequence, of different lengths (none, too), in one pass."""
+        tokens, lens = self._pack(prompts)
+        if len(lens) != self.batch:
+            raise RuntimeError(f"need a prompt for each of {self.batch} sequences")
+        self.reset()
+        if tokens.numel():
+            self._prompts(tokens, lens, write=True)
+            self.ctx = torch.tensor(lens, dtype=torch.int32, device=self.dev)
+
+    @torch.no_grad()
+    def score(self, prompts, adapter: str | None = None, top: int = 0, rows: int = 2048) -> list:
+        """Log probabilities of prompts' tokens after those before them, in one pass over all prompts.
+
+        ``prompts``: any number of lists of at most ``max_len`` tokens.  Returns a ``TokenLogprobs`` for each, of its
+        tokens from the second on (log probability, entropy, the ``top`` most likely tokens there).  ``rows``: logits
+        held at a time.  The decoder's sequences and cache are left alone."""
+        from blackwell_ops.cuda import rmsnorm
+        from blackwell_ops.prompt import TokenLogprobs, token_logprobs
+
+        tokens, lens = self._pack(prompts)
+        n = sum(lens)
+        if rows < 1:
+            raise RuntimeError("rows must be positive")
+        self.model.set_adapter(adapter)
+        if n:
+            x, _ = self._prompts(tokens, lens, write=False)
+            norm, nxt = self.model.base.model.norm, torch.cat([tokens[1:], tokens[:1]])
+            parts = []
+            for at in range(0, n, rows):
+                logits = self.model.base.lm_head(rmsnorm(x[at:at + rows], norm.weight, norm.variance_epsilon))
+                parts.append(token_logprobs(logits, nxt[at:at + rows], top))
+            every = [torch.cat(y) for y in zip(*parts)]
+        else:
+            every = token_logprobs(torch.zeros((0, max(top, 1)), device=self.dev), tokens, top)
+        out, at = [], 0
+        for m in lens:
+            out.append(TokenLogprobs(*(y[at:at + max(m - 1, 0)] for y in every)))
+            at += m
+        return out
+
+    @torch.no_grad()
     def generate(self, ids: torch.Tensor, max_new_tokens: int, adapter: str | None = None, temperature: float = 0.0,
                  generator: torch.Generator | None = None) -> torch.Tensor:
         """The new tokens [B, max_new_tokens] after the prompts ``ids`` [B, L]; ``temperature`` 0 is greedy."""
@@ -209,7 +319,10 @@ class TreeSpeculativeDecoder:
         self.model.set_adapter(adapter)
         self.reset()
         ids = ids.to(self.dev)
-        self.prefill(ids[:, :-1])
+        if self.packed:
+            self.prefill_packed(ids[:, :-1])
+        else:
+            self.prefill(ids[:, :-1])
         seen = ids.tolist()
         while min(len(s) for s in seen) < length + max_new_tokens:
             # (a sequence that has its tokens goes on with its root alone, whose place is kept)

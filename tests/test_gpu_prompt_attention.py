@@ -47,8 +47,8 @@ def _check(q, k, v, offsets, scale=None, got=None):
     return got
 
 
-HEADS = [(1, 1, 128), (16, 8, 128), (32, 8, 128), (28, 4, 64), (12, 1, 128), (8, 8, 64), (64, 8, 64), (5, 1, 64)]
-ODD = [(4, 2, 80), (3, 3, 96), (2, 1, 256), (2, 2, 1), (6, 2, 33), (130, 1, 32), (4, 4, 192)]
+HEADS = [(1, 1, 128), (128, 1, 64), (100, 1, 128), (16, 8, 128), (32, 8, 128), (28, 4, 64), (12, 1, 128), (8, 8, 64), (64, 8, 64), (5, 1, 64)]
+ODD = [(4, 2, 80), (3, 3, 96), (2, 1, 256), (2, 2, 1), (6, 2, 33), (130, 1, 32), (130, 1, 64), (4, 4, 192)]
 LENS = [[1], [17], [0, 1, 2, 0, 3], [128], [127, 129], [16, 15, 14, 13, 33], [300, 0, 513], [64] * 9]
 
 
