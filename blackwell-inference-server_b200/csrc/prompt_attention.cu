@@ -177,14 +177,17 @@ static int launch_rows(const PromptArgs& a, cudaStream_t st) {
 // group + head.  A CTA takes two neighbouring tiles A and B of a key head (or, of few rows, one) and walks their
 // sequence's keys, 128 at a time:
 //   S [128 x 128 keys] = Q [128 x D] (shared memory) . K^T (shared memory)        fp32, in TMEM
-//   O [128 x D]       += P [128 x 128 keys] (TMEM, over S) . V (shared memory)    fp32, in TMEM
+//   O [128 x D]       += P [128 x 128 keys] (TMEM) . V (shared memory)            fp32, in TMEM
+// At D = 128 the accumulators leave no room for P but over S, so a tile's next scores wait for its weights' product; at
+// D = 64 P lies beside them, and the next scores come as soon as the softmax has these in registers.
 // Each K and V tile in shared memory serves both query tiles, and while one tile's softmax runs, the other's products do.
 //
 // What bounds it (one B200, bf16, D = 128): the products.  16383 tokens, 16 / 8 heads: 0.84 ms, 1310 TFLOP/s; 0.72 with
 // the softmax left out, 0.68 with the scores issued without waiting for the product before them.  A K . Q product of
 // 128 x 128 x 16 reads 8 KB of shared memory in its 64 cycles, all that there is, next to V's 4 KB and the copies; two SMs
-// that share a tile's other operand would halve that.  D = 64 (0.76 PFLOP/s at 8192 tokens): the exponentials, 9 to 10
-// cycles each in a warp.  Short prompts: a block's start and end, 2 us of which its neighbours hide a part.
+// that share a tile's other operand would halve that.  D = 64: the softmax warps, 1.5 us for two tiles, of which the
+// special-function unit works 1.05; 16384 tokens, 32 / 8 heads: 1.34 ms, 820 TFLOP/s (1.40 with the weights over the
+// scores, as at D = 128; 1.02 without the softmax).  Short prompts: a block's start and end, of which its neighbours hide a part.
 // Measured and not kept, of 16383 tokens: two warps that issue the products, by kind or by query tile (0.91 and 1.03 ms:
 // the tiles' softmax phases drift onto each other, where the one warp's order keeps them apart); two threads a row (1.4);
 // a quarter of the exponentials as polynomials (0.88); weights checked by their sum in place of the maximum (0.86); one
@@ -223,6 +226,7 @@ enum PromptSite : int {
 
 template <int D>
 struct PCfg {
+  static constexpr int KEYS_COLS = kPromptKeys;
   static constexpr int TB = D / 64 * kPromptKeys * 128;  // bytes of a tile of Q, K or V: panels of 64 elements
   static constexpr int KST = D == 128 ? 2 : 4, VST = D == 128 ? 2 : 4;
   static constexpr int OB = 32 * 128;  // bytes of a softmax warp's part of the output on its way out
@@ -233,6 +237,9 @@ struct PCfg {
   static constexpr int CTRL = 1024;
   static constexpr int SMEM = OFF_CTRL + CTRL + 1024;
   static constexpr int S_COL = 0, O_COL = 256, COLS = 512;
+  // D = 64: accumulators of half the size leave room for the weights beside the scores.
+  static constexpr bool APART = D == 64;
+  static constexpr int P_COL = APART ? 384 : S_COL, P_STEP = APART ? 64 : KEYS_COLS;  // of A; from A to B
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
@@ -311,7 +318,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   uint64_t* vready = vfull + C::VST;   // looked through
   uint64_t* vempty = vready + C::VST;
   uint64_t* sfull = vempty + C::VST;   // [A, B] scores
-  uint64_t* phalf = sfull + 2;         // weights of the first 64 keys, of all
+  uint64_t* sread = sfull + 2;         //        in registers (APART)
+  uint64_t* phalf = sread + 2;         // weights of the first 64 keys, of all
   uint64_t* pfull = phalf + 2;
   uint64_t* pvdone = pfull + 2;        //    P . V complete
   uint64_t* oempty = pvdone + 2;       // accumulator read
@@ -338,6 +346,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       mbar_init(&qfull[i], 1);
       mbar_init(&qempty[i], 1);
       mbar_init(&sfull[i], 1);
+      mbar_init(&sread[i], 4);
       mbar_init(&phalf[i], 4);
       mbar_init(&pfull[i], 4);
       mbar_init(&pvdone[i], 1);
@@ -496,10 +505,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           ok = ok && __all_sync(0xffffffffu, mbar_wait_or_abort(bar, parity & 1u, ctl));
           return ok;
         };
+        uint32_t rp = 0;                          // parity of the next scores of A and B
         // Scores of the next K tile, once the weights over which they go have been read (products of different
-        // accumulators are not ordered).
+        // accumulators are not ordered); APART: once the scores before them have.
         auto scores = [&](int w, bool give_k, bool give_q) {
-          if (!wait(&pvdone[w], (sp >> w) ^ 1u)) return;
+          if (!wait(C::APART ? &sread[w] : &pvdone[w], ((C::APART ? rp : sp) >> w) ^ 1u)) return;
+          rp ^= 1u << w;
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
@@ -515,7 +526,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           __syncwarp();
         };
         auto weighted = [&](int w, bool first, bool give_v) {
-          const uint32_t o = tm + C::O_COL + w * D, p = tm + C::S_COL + w * KEYS, v = v0 + vs * C::TB;
+          const uint32_t o = tm + C::O_COL + w * D, p = tm + C::P_COL + w * C::P_STEP, v = v0 + vs * C::TB;
           const uint32_t parity = sp >> w;
           if (!wait(&phalf[w], parity)) return;
           tc_fence_after();
@@ -556,23 +567,47 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           scores(0, !both, na == 1);
           if (both && wait(&qfull[1], bp >> 1)) scores(1, true, nb == 1);
           next_k();
-          for (int i = 0; ok && i < tiles; ++i) {
-            if (!wait(&vready[vs], vp)) break;
-            const bool more = i + 1 < tiles;
-            if (i < na) {
-              if (i == 0 && !wait(&oempty[0], bp ^ 1u)) break;  // the block before has been read
-              weighted(0, i == 0, !both);
-              if (ok && i + 1 < na && wait(&kfull[ks], kp)) scores(0, !both, i + 2 == na);
-            }
-            if (i < nb) {
-              if (i == 0 && !wait(&oempty[1], (bp >> 1) ^ 1u)) break;
-              if (ok) weighted(1, i == 0, true);
-              if (ok && more && (i + 1 < na || wait(&kfull[ks], kp))) scores(1, true, i + 2 == nb);
-            }
-            if (more) next_k();
+          auto next_v = [&]() {
             if (++vs == C::VST) {
               vs = 0;
               vp ^= 1;
+            }
+          };
+          if constexpr (C::APART) {
+            // The scores of tile i + 1 while the softmax works on tile i, and the weights of B a tile behind those of A.
+            for (int i = 0; ok && i <= tiles; ++i) {
+              const bool more = i + 1 < tiles;
+              if (i + 1 < na && wait(&kfull[ks], kp)) scores(0, !both, i + 2 == na);
+              if (ok && i >= 1 && i - 1 < nb) {
+                if (i - 1 >= na && !wait(&vready[vs], vp)) break;
+                if (i == 1 && !wait(&oempty[1], (bp >> 1) ^ 1u)) break;  // the block before has been read
+                weighted(1, i == 1, true);
+              }
+              if (i >= 1) next_v();
+              if (ok && i + 1 < nb && (i + 1 < na || wait(&kfull[ks], kp))) scores(1, true, i + 2 == nb);
+              if (more) next_k();
+              if (ok && i < na) {
+                if (!wait(&vready[vs], vp)) break;
+                if (i == 0 && !wait(&oempty[0], bp ^ 1u)) break;
+                weighted(0, i == 0, !both);
+              }
+            }
+          } else {
+            for (int i = 0; ok && i < tiles; ++i) {
+              if (!wait(&vready[vs], vp)) break;
+              const bool more = i + 1 < tiles;
+              if (i < na) {
+                if (i == 0 && !wait(&oempty[0], bp ^ 1u)) break;  // the block before has been read
+                weighted(0, i == 0, !both);
+                if (ok && i + 1 < na && wait(&kfull[ks], kp)) scores(0, !both, i + 2 == na);
+              }
+              if (i < nb) {
+                if (i == 0 && !wait(&oempty[1], (bp >> 1) ^ 1u)) break;
+                if (ok) weighted(1, i == 0, true);
+                if (ok && more && (i + 1 < na || wait(&kfull[ks], kp))) scores(1, true, i + 2 == nb);
+              }
+              if (more) next_k();
+              next_v();
             }
           }
           bp ^= both ? 3u : 1u;
@@ -650,6 +685,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t s_tm = lanes + C::S_COL + w * KEYS, o_tm = lanes + C::O_COL + w * D;
+    const uint32_t p_tm = lanes + C::P_COL + w * C::P_STEP;
     const int p = row / ta.grp, g = row - p * ta.grp;
     const float sc = a.scale_log2;
     uint32_t it = 0;  // score tiles so far
@@ -677,6 +713,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(s_tm + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&x[c * 32]));
         tmem_ld_wait();
+        if constexpr (C::APART) {  // the next scores may come
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sread[w]);
+        }
         if (i * KEYS + KEYS - 1 > pos0) {  // keys that some row does not see
           const int see = pos - i * KEYS + 1;
 #pragma unroll
@@ -690,10 +731,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll
           for (int c = 0; c < 8; ++c) top[c] = max3(top[c], x[c * 16 + e], x[c * 16 + e + 1]);
         const float best = fmaxf(max3(max3(top[0], top[1], top[2]), top[3], top[4]), max3(top[5], top[6], top[7])) * sc;
+        if constexpr (C::APART) {  // the weights before have been read
+          ok = __all_sync(0xffffffffu, mbar_wait_or_abort(&pvdone[w], (it & 1) ^ 1, ctl));
+          if (!ok) break;
+          tc_fence_after();
+        }
         if (i == 0) {
           m = fmaxf(best, kPromptLowest);
         } else if (__any_sync(0xffffffffu, best > m + kPromptSlack)) {
-          // the accumulator is still: these scores were issued behind its last product
+          // the accumulator is still: these scores were issued behind its last product (APART: which is waited for)
           const float to = best > m + kPromptSlack ? best : m;
           const float f = exp2_approx(m - to);
           m = to;
@@ -722,7 +768,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             l2[c % 2] = __fadd2_rn(l2[c % 2], v);
             packed[c] = pack2<T>(v);
           }
-          tmem_st32(s_tm + h * 32, packed);
+          tmem_st32(p_tm + h * 32, packed);
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
