@@ -22,21 +22,19 @@ struct PromptArgs {
   int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;  // strides of a token and a head
   void* o;                                     // [n, hq, d] contiguous
   const int* offsets;                          // [b + 1]
-  int64_t n;
-  int b, hq, hk, d;
+  int n, b, hq, hk, d;
   float scale_log2;
 };
 
 // A block of at most P rows of one segment: rows [row0, row1), its sequence's first row, and whether it is a sequence's.
 struct PromptBlock {
-  int64_t first, row0, row1;
+  int first, row0, row1;
   bool real;
 };
-__device__ __forceinline__ int64_t prompt_edge(const PromptArgs& a, int i) {  // segment i's first row
+__device__ __forceinline__ int prompt_edge(const PromptArgs& a, int i) {  // segment i's first row
   if (i == 0) return 0;
   if (i == a.b + 2) return a.n;
-  const int64_t e = a.offsets[i - 1];
-  return e < 0 ? 0 : (e < a.n ? e : a.n);
+  return min(max(a.offsets[i - 1], 0), a.n);
 }
 // Block number `slot` of P rows, by a whole warp; the last blocks of a sequence, which see most keys, come first.
 __device__ __forceinline__ bool prompt_block(const PromptArgs& a, int P, int slot, PromptBlock& blk) {
@@ -45,18 +43,18 @@ __device__ __forceinline__ bool prompt_block(const PromptArgs& a, int P, int slo
   int lo = 0, hi = a.b + 2;
   while (hi - lo > 1) {
     const int step = (hi - lo + 31) / 32, i = lo + lane * step;
-    const bool before = i < hi && static_cast<int>(prompt_edge(a, i)) / P + i <= slot;
+    const bool before = i < hi && prompt_edge(a, i) / P + i <= slot;
     const int last = 31 - __clz(__ballot_sync(0xffffffffu, before) | 1u);
     hi = min(hi, lo + (last + 1) * step);
     lo += last * step;
   }
-  const int64_t e0 = prompt_edge(a, lo), e1 = prompt_edge(a, lo + 1);
-  const int64_t blocks = e1 > e0 ? (e1 - e0 + P - 1) / P : 0;
-  const int64_t i = slot - (e0 / P + lo);
+  const int e0 = prompt_edge(a, lo), e1 = prompt_edge(a, lo + 1);
+  const int blocks = e1 > e0 ? (e1 - e0 + P - 1) / P : 0;
+  const int i = slot - (e0 / P + lo);
   if (i >= blocks) return false;
   blk.first = e0;
   blk.row0 = e0 + (blocks - 1 - i) * P;
-  blk.row1 = blk.row0 + P < e1 ? blk.row0 + P : e1;
+  blk.row1 = min(blk.row0 + P, e1);
   blk.real = lo >= 1 && lo <= a.b;
   return true;
 }
@@ -77,12 +75,12 @@ __global__ void __launch_bounds__(128) prompt_rows_kernel(const PromptArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   PromptBlock blk;
   if (!prompt_block(a, kRowsQ, blockIdx.x, blk)) return;
-  const int rows = static_cast<int>(blk.row1 - blk.row0);
+  const int rows = blk.row1 - blk.row0;
   const int h = blockIdx.y, hk = h / (a.hq / a.hk);
   T* out = static_cast<T*>(a.o);
   if (!blk.real) {
     for (int e = threadIdx.x; e < rows * d; e += 128)
-      out[((blk.row0 + e / d) * a.hq + h) * d + e % d] = from_f32<T>(0.f);
+      out[(static_cast<int64_t>(blk.row0 + e / d) * a.hq + h) * d + e % d] = from_f32<T>(0.f);
     return;
   }
   const T* q = static_cast<const T*>(a.q) + h * a.q_sh;
@@ -98,8 +96,8 @@ __global__ void __launch_bounds__(128) prompt_rows_kernel(const PromptArgs a) {
 #pragma unroll
     for (int i = 0; i < kKvMaxDim / 32; ++i) o[r][i] = 0.f;
   }
-  for (int64_t j0 = blk.first; j0 < blk.row1; j0 += kRowsK) {
-    const int keys = static_cast<int>(blk.row1 - j0 < kRowsK ? blk.row1 - j0 : kRowsK);
+  for (int j0 = blk.first; j0 < blk.row1; j0 += kRowsK) {
+    const int keys = min(blk.row1 - j0, kRowsK);
     __syncthreads();
     for (int e = threadIdx.x; e < keys * d; e += 128) {
       const int j = e / d, c = e - j * d;
@@ -112,8 +110,7 @@ __global__ void __launch_bounds__(128) prompt_rows_kernel(const PromptArgs a) {
       const int row = warp * 4 + r;
       if (row >= rows) continue;
       // keys of this tile that the query sees, one at least in a sequence's first tile
-      const int64_t past = blk.row0 + row - j0 + 1;
-      const int see = static_cast<int>(past < keys ? past : keys);
+      const int see = min(blk.row0 + row - j0 + 1, keys);
       if (see <= 0) continue;
       float s = -INFINITY;
       if (lane < see) {
@@ -148,7 +145,7 @@ __global__ void __launch_bounds__(128) prompt_rows_kernel(const PromptArgs a) {
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
     for (int i = 0; i < kKvMaxDim / 32; ++i)
-      if (lane + 32 * i < d) out[((blk.row0 + row) * a.hq + h) * d + lane + 32 * i] = from_f32<T>(o[r][i] * inv);
+      if (lane + 32 * i < d) out[(static_cast<int64_t>(blk.row0 + row) * a.hq + h) * d + lane + 32 * i] = from_f32<T>(o[r][i] * inv);
   }
 }
 
@@ -413,20 +410,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           PromptBlock blk;
           if (prompt_block(a, ta.block, slot, blk)) {
             if (blk.real) {
-              t.first = static_cast<int>(blk.first);
-              t.row0 = static_cast<int>(blk.row0 - blk.first);
-              t.row1 = static_cast<int>(blk.row1 - blk.first);
+              t.first = blk.first;
+              t.row0 = blk.row0 - blk.first;
+              t.row1 = blk.row1 - blk.first;
               t.head = head;
               t.n[0] = (min(t.row0 + P, t.row1) - 1) / KEYS + 1;
               t.n[1] = t.row0 + P < t.row1 ? (t.row1 - 1) / KEYS + 1 : 0;
               return true;
             }
             // rows of no sequence: zeros
-            const int64_t per = static_cast<int64_t>(ta.grp) * D / 8;  // 16-byte chunks of a row
-            const int64_t chunks = (blk.row1 - blk.row0) * per;
-            uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.o) + (blk.row0 * a.hq + head * ta.grp) * D);
-            for (int64_t e = lane; e < chunks; e += 32)
-              out[e / per * (static_cast<int64_t>(a.hq) * D / 8) + e % per] = make_uint4(0u, 0u, 0u, 0u);
+            const int per = ta.grp * D / 8;  // 16-byte chunks of a row
+            for (int r = blk.row0; r < blk.row1; ++r) {
+              uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.o) + (static_cast<int64_t>(r) * a.hq + head * ta.grp) * D);
+              for (int e = lane; e < per; e += 32) out[e] = make_uint4(0u, 0u, 0u, 0u);
+            }
           }
           ask();
           x = answer();
@@ -442,9 +439,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         __syncwarp();
       };
       const uint32_t q_bytes = static_cast<uint32_t>(P * ta.grp * D * 2);
-      bool ok = true, have = find(blockIdx.x);
+      bool ok = true;
+      int x = blockIdx.x;
       for (uint32_t n = 0;; ++n) {
         const int sl = n & 1;
+        const bool have = find(x);
         ok = __all_sync(0xffffffffu, mbar_wait_at(&tempty[sl], ((n >> 1) & 1) ^ 1, ctl, kSitePrBlock));
         if (!ok) break;
         if (lane == 0) {
@@ -478,7 +477,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           ++vn;
         }
         if (!ok) break;
-        have = find(answer());
+        x = answer();
       }
       if (ok) {
         mbar_wait_at(done, 0, ctl, kSitePrDone);
@@ -563,10 +562,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           if (!valid) break;
           const int tiles = max(na, nb);
           const bool both = nb > 0;  // (B then needs every K and V tile, and last)
-          if (!wait(&qfull[0], bp) || !wait(&kfull[ks], kp)) break;
-          scores(0, !both, na == 1);
-          if (both && wait(&qfull[1], bp >> 1)) scores(1, true, nb == 1);
-          next_k();
+          // (Two copies of each product's instructions, which share a cache with the other roles'; with one, whose addresses
+          // are worked out on the way, long prompts take 3 % longer, with six short ones.)
+          // Tile i + 1's scores: the first of A and B to come to them waits for the K tile.
+          auto scores_of = [&](int w, int i, bool& have_k) {
+            if (i + 1 == 0 && !wait(&qfull[w], bp >> w)) return;
+            if (!have_k && !wait(&kfull[ks], kp)) return;
+            have_k = true;
+            scores(w, w == 1 || !both, i + 2 == (w ? nb : na));
+          };
+          auto weights_of = [&](int w, int i, bool& have_v) {
+            if (!have_v && !wait(&vready[vs], vp)) return;
+            have_v = true;
+            if (i == 0 && !wait(&oempty[w], (bp >> w) ^ 1u)) return;  // the block before has been read
+            weighted(w, i == 0, w == 1 || !both);
+          };
           auto next_v = [&]() {
             if (++vs == C::VST) {
               vs = 0;
@@ -575,39 +585,34 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           };
           if constexpr (C::APART) {
             // The scores of tile i + 1 while the softmax works on tile i, and the weights of B a tile behind those of A.
-            for (int i = 0; ok && i <= tiles; ++i) {
-              const bool more = i + 1 < tiles;
-              if (i + 1 < na && wait(&kfull[ks], kp)) scores(0, !both, i + 2 == na);
-              if (ok && i >= 1 && i - 1 < nb) {
-                if (i - 1 >= na && !wait(&vready[vs], vp)) break;
-                if (i == 1 && !wait(&oempty[1], (bp >> 1) ^ 1u)) break;  // the block before has been read
-                weighted(1, i == 1, true);
+            bool have_v = false;
+#pragma unroll 1
+            for (int i = -1; ok && i <= tiles; ++i) {
+              bool have_k = false;
+#pragma unroll
+              for (int w = 0; w < 2; ++w) {
+                if (i + 1 < (w ? nb : na)) scores_of(w, i, have_k);
+                const int j = i - 1 + w, u = 1 - w;  // B's of tile i - 1, then A's of tile i
+                if (ok && j >= 0 && j < (u ? nb : na)) weights_of(u, j, have_v);
+                if (w == 0 && i >= 1) {
+                  next_v();
+                  have_v = false;
+                }
               }
-              if (i >= 1) next_v();
-              if (ok && i + 1 < nb && (i + 1 < na || wait(&kfull[ks], kp))) scores(1, true, i + 2 == nb);
-              if (more) next_k();
-              if (ok && i < na) {
-                if (!wait(&vready[vs], vp)) break;
-                if (i == 0 && !wait(&oempty[0], bp ^ 1u)) break;
-                weighted(0, i == 0, !both);
-              }
+              if (i + 1 < tiles) next_k();
             }
           } else {
-            for (int i = 0; ok && i < tiles; ++i) {
-              if (!wait(&vready[vs], vp)) break;
-              const bool more = i + 1 < tiles;
-              if (i < na) {
-                if (i == 0 && !wait(&oempty[0], bp ^ 1u)) break;  // the block before has been read
-                weighted(0, i == 0, !both);
-                if (ok && i + 1 < na && wait(&kfull[ks], kp)) scores(0, !both, i + 2 == na);
+#pragma unroll 1
+            for (int i = -1; ok && i < tiles; ++i) {
+              bool have_k = false, have_v = false;
+#pragma unroll
+              for (int w = 0; w < 2; ++w) {
+                const int mine = w ? nb : na;
+                if (i >= 0 && i < mine) weights_of(w, i, have_v);
+                if (ok && i + 1 < mine) scores_of(w, i, have_k);
               }
-              if (i < nb) {
-                if (i == 0 && !wait(&oempty[1], (bp >> 1) ^ 1u)) break;
-                if (ok) weighted(1, i == 0, true);
-                if (ok && more && (i + 1 < na || wait(&kfull[ks], kp))) scores(1, true, i + 2 == nb);
-              }
-              if (more) next_k();
-              next_v();
+              if (i + 1 < tiles) next_k();
+              if (i >= 0) next_v();
             }
           }
           bp ^= both ? 3u : 1u;
@@ -638,7 +643,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           if (i >= from) {
             uint8_t* tile = sV + vs * C::TB;
             const int have = t.row1 - i * KEYS;  // keys up to the block's last position
-#pragma unroll
+#pragma unroll 1
             for (int q = part * 2; q < part * 2 + 2; ++q) {
               uint8_t* row = tile + (q * 32 + lane) * 128;
               uint32_t bad = 0;
@@ -803,29 +808,30 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           float y[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) y[e] = __uint_as_float(o[e]) * inv;
-          if (any != 0 && mine) {
-            // values that are not finite, of the keys that this row sees among those that not all see
-            const int from = (t.row0 + 1) / KEYS * KEYS;
-            const T* v = static_cast<const T*>(a.v) + static_cast<int64_t>(t.first) * a.v_st + t.head * a.v_sh + c0 + c;
-#pragma unroll 1
-            for (int k = 0; k < 12; ++k) {
-#pragma unroll 1
-              for (uint32_t word = odd[sl * 12 + k]; word != 0; word &= word - 1) {
-                const int key = from + k * 32 + __ffs(word) - 1;
-                if (key > pos) continue;
-#pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                  const float z = to_f32(v[key * a.v_st + e]);
-                  if (!(fabsf(z) <= 3.402823466e38f)) y[e] += z;
-                }
-              }
-            }
-          }
 #pragma unroll
           for (int e = 0; e < 32; e += 8)
             *reinterpret_cast<uint4*>(stage + lane * 128 + ((((c + e) >> 3) ^ (lane & 7)) << 4)) =
                 make_uint4(pack2<T>(make_float2(y[e], y[e + 1])), pack2<T>(make_float2(y[e + 2], y[e + 3])),
                            pack2<T>(make_float2(y[e + 4], y[e + 5])), pack2<T>(make_float2(y[e + 6], y[e + 7])));
+        }
+        if (any != 0 && mine) {
+          // values that are not finite, of the keys that this row sees among those that not all see
+          const int from = (t.row0 + 1) / KEYS * KEYS;
+          const T* v = static_cast<const T*>(a.v) + static_cast<int64_t>(t.first) * a.v_st + t.head * a.v_sh + c0;
+#pragma unroll 1
+          for (int k = 0; k < 12; ++k) {
+#pragma unroll 1
+            for (uint32_t word = odd[sl * 12 + k]; word != 0; word &= word - 1) {
+              const int key = from + k * 32 + __ffs(word) - 1;
+              if (key > pos) continue;
+#pragma unroll 1
+              for (int e = 0; e < 64; ++e) {
+                const float z = to_f32(v[key * a.v_st + e]);
+                T* y = reinterpret_cast<T*>(stage + lane * 128 + (((e >> 3) ^ (lane & 7)) << 4)) + (e & 7);
+                if (!(fabsf(z) <= 3.402823466e38f)) *y = from_f32<T>(to_f32(*y) + z);
+              }
+            }
+          }
         }
         __syncwarp();
         uint4 line[8];
@@ -930,7 +936,7 @@ extern "C" int bw_prompt_attention(const void* q, int64_t q_st, int64_t q_sh, co
   a.v_sh = v_sh;
   a.o = out;
   a.offsets = offsets;
-  a.n = n;
+  a.n = static_cast<int>(n);
   a.b = static_cast<int>(b);
   a.hq = static_cast<int>(hq);
   a.hk = static_cast<int>(hk);
