@@ -228,7 +228,13 @@ class TreeSpeculativeDecoder:
         lens = [p.numel() for p in prompts]
         if max(lens, default=0) > self.max_len:
             raise RuntimeError(f"at most max_len = {self.max_len} tokens a sequence")
-        return torch.cat([p.to(self.dev) for p in prompts] or [torch.empty(0, dtype=torch.int64, device=self.dev)]), lens
+        tokens = torch.cat([p.to(self.dev) for p in prompts] or [torch.empty(0, dtype=torch.int64, device=self.dev)])
+        vocab = self.model.base.model.embed_tokens.weight.shape[0]
+        if tokens.numel():  # (the embedding's kernel would end the process' use of the GPU)
+            least, most = torch.stack(torch.aminmax(tokens)).tolist()
+            if least < 0 or most >= vocab:
+                raise RuntimeError(f"tokens must be 0 to {vocab - 1}")
+        return tokens, lens
 
     def _mlp(self, mlp, y: torch.Tensor) -> torch.Tensor:
         from blackwell_ops.kernels.int8_gemm import int8_gemm, int8_gemm_swiglu

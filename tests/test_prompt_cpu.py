@@ -117,3 +117,20 @@ def test_messages_on_the_host():
         P.prompt_attention(x, x, x, torch.zeros(2, dtype=torch.int32))
     with pytest.raises(RuntimeError, match="logits must be CUDA"):
         P.token_logprobs(x[0], torch.zeros(2, dtype=torch.int64))
+
+
+def test_prompts_of_the_decoder():
+    """What packing refuses: tokens outside the vocabulary (which would fault in the embedding), long and nested prompts."""
+    from types import SimpleNamespace
+
+    from blackwell_inference.spec_decode import TreeSpeculativeDecoder
+
+    dec = TreeSpeculativeDecoder.__new__(TreeSpeculativeDecoder)
+    dec.dev, dec.max_len = torch.device("cpu"), 4
+    dec.model = SimpleNamespace(base=SimpleNamespace(model=SimpleNamespace(embed_tokens=torch.nn.Embedding(10, 2))))
+    tokens, lens = dec._pack([[0, 9], [], torch.tensor([3], dtype=torch.int32)])
+    assert tokens.tolist() == [0, 9, 3] and lens == [2, 0, 1]
+    assert dec._pack([])[0].numel() == 0 and dec._pack([[]])[1] == [0]
+    for match, prompts in [("0 to 9", [[1], [10]]), ("0 to 9", [[-1, 2]]), ("max_len = 4", [[1] * 5]), ("list of tokens", [[[1]]])]:
+        with pytest.raises(RuntimeError, match=match):
+            dec._pack(prompts)
