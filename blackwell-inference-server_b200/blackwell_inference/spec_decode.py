@@ -276,7 +276,7 @@ class TreeSpeculativeDecoder:
         self.reset()
         if tokens.numel():
             self._prompts(tokens, lens, write=True)
-            self.ctx = torch.tensor(lens, dtype=torch.int32, device=self.dev)
+            self.ctx.copy_(torch.tensor(lens, dtype=torch.int32))  # in place, as everywhere: a captured step reads it there
 
     @torch.no_grad()
     def score(self, prompts, adapter: str | None = None, top: int = 0, rows: int = 2048) -> list:
