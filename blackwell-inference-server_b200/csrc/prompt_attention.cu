@@ -193,7 +193,7 @@ static int launch_rows(const PromptArgs& a, cudaStream_t st) {
 // Softmax: thread = row, so nothing is exchanged.  The reference m moves only when a score exceeds it by more than 8 (in
 // powers of two); only then are the sum and the accumulator rescaled.  Weights 2^(s - m + 7) go to the tensor core in
 // the inputs' type: rounded by half an ulp like the inputs themselves, at most 2^15, and the 7 keeps fp16's subnormal steps
-// at 2^-32 of a row's largest weight.  Their sum and the accumulator are fp32 and have the same factor.
+// at 2^-31 of a row's largest weight at most.  Their sum and the accumulator are fp32 and have the same factor.
 //
 // Keys that a row does not see have weight 0, but 0 times a value that is not finite is not 0.  So a warp looks through
 // every V tile that some row of the block does not see all of: rows behind the block's last position become zeros,
@@ -214,7 +214,6 @@ static_assert(2 * kPromptRegsSoft + kPromptRegsRest == 3 * 168, "register split"
 // other CTAs' reach for longer, one taken later is not there in time.
 constexpr int kPromptAhead = 4;
 constexpr float kPromptSlack = 8.f, kPromptShift = 7.f;
-constexpr float kPromptMost = 32768.f;  // what 64 weights may sum to: four times what they come to at a new reference
 constexpr float kPromptLowest = -3.0e38f;  // a row's reference without any score: finite, so differences are
 enum PromptSite : int {
   kSitePrBlock = 501, kSitePrQ = 502, kSitePrK = 503, kSitePrV = 504, kSitePrDrain = 505, kSitePrDone = 506,
