@@ -271,17 +271,33 @@ __global__ void __launch_bounds__(256, WRITE ? 3 : 4) rotary_vec_kernel(const __
   // rows: 56 us, 5.4 TB/s; two rows ahead 60, three 68 (their registers spill).  The write of 4096 tokens' 32
   // query rows with 16 rows into the cache: 27 us, 3.4 TB/s (24 without any quotient: three CTAs an SM and two
   // and a third waves more than the instructions).
-  auto fetch = [&](int h, uint4 (&raw)[2]) {
-    if (h >= rows) return;
-    const int which = h < hq ? 0 : (h < hqk ? 1 : 2);
-    const int hh = which == 0 ? h : (which == 1 ? h - hq : h - hqk);
-    const RowSet& s = which == 0 ? a.q : (which == 1 ? a.k : a.v);
-    const T* x = static_cast<const T*>(s.p) + b * s.sb + t * s.st + hh * s.sh;
-    raw[0] = *reinterpret_cast<const uint4*>(x + (which == 2 ? 8 * j : e0));
-    raw[1] = *reinterpret_cast<const uint4*>(x + (which == 2 ? D / 2 + 8 * j : e1));
+  // NORM's write has two rows ahead in shared memory, each lane's chunks in places of its own (no barrier), which leaves
+  // the codes their registers: 21000 tokens of 36 heads of 64 in 44.9 us for 48.0, of 56 of 128 131.5 for 135.3.
+  constexpr int RING = WRITE && NORM ? 2 : 0;
+  __shared__ uint4 ring[RING > 0 ? RING * 512 : 1];  // [row ahead][chunk][thread]
+  auto fetch = [&](int h, int place, uint4 (&raw)[2]) {
+    if (h < rows) {
+      const int which = h < hq ? 0 : (h < hqk ? 1 : 2);
+      const int hh = which == 0 ? h : (which == 1 ? h - hq : h - hqk);
+      const RowSet& s = which == 0 ? a.q : (which == 1 ? a.k : a.v);
+      const T* x = static_cast<const T*>(s.p) + b * s.sb + t * s.st + hh * s.sh;
+      const uint4* c0 = reinterpret_cast<const uint4*>(x + (which == 2 ? 8 * j : e0));
+      const uint4* c1 = reinterpret_cast<const uint4*>(x + (which == 2 ? D / 2 + 8 * j : e1));
+      if constexpr (RING > 0) {
+        const uint32_t to = smem_u32(&ring[place * 512 + threadIdx.x]);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(c0) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 4096u), "l"(c1) : "memory");
+      } else {
+        raw[0] = *c0;
+        raw[1] = *c1;
+      }
+    }
+    if constexpr (RING > 0) asm volatile("cp.async.commit_group;" ::: "memory");
   };
   uint4 next[2];
-  fetch(g, next);
+  fetch(g, 0, next);
+  if constexpr (RING > 0) fetch(g + gpt, 1, next);
+  int place = 0;
   if constexpr (NORM) {
     if (WRITE && rows > 0) krow = target_row(a, b, t);
     for (int n = threadIdx.x; n < 2 * D; n += 256) {
@@ -309,8 +325,18 @@ __global__ void __launch_bounds__(256, WRITE ? 3 : 4) rotary_vec_kernel(const __
   int has = -1;
 #pragma unroll 1
   for (int h = g; h < rows; h += gpt) {
-    const uint4 raw[2] = {next[0], next[1]};
-    fetch(h + gpt, next);
+    uint4 raw[2];
+    if constexpr (RING > 0) {
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      raw[0] = ring[place * 512 + threadIdx.x];
+      raw[1] = ring[place * 512 + 256 + threadIdx.x];
+      fetch(h + RING * gpt, place, next);
+      place ^= 1;
+    } else {
+      raw[0] = next[0];
+      raw[1] = next[1];
+      fetch(h + gpt, 0, next);
+    }
     const int which = h < hq ? 0 : (h < hqk ? 1 : 2);
     const int hh = which == 0 ? h : (which == 1 ? h - hq : h - hqk);
     const bool plain = which == 2;  // values do not turn
@@ -388,11 +414,17 @@ template <typename T, int L, bool NORM>
 static int launch_rotary_vec(const RotArgs& a, bool write, cudaStream_t st) {
   // Row groups of a token: eight (a lane's sines then serve many rows), more where the tokens alone do not
   // fill the SMs, up to one for each row.  With norms, whose weights a CTA fetches as well, four (a twentieth faster on
-  // 8191 tokens of 40 rows than eight; two are as fast as four).
+  // 8191 tokens of 40 rows than eight; two are as fast as four), and more only as long as all CTAs run at once.  Us so, and with
+  // up to twice the CTAs that run at once, as for the rotation: 512 tokens of 32 rows written 6.5 and 8.5, 1500 10.2 and
+  // 11.9, 2500 of 48 21.8 and 21.0; turned alone, 1000 of 40 7.9 and 9.2, 4607 of 24 14.8 and 16.2, 2500 of 40 17.2 and 16.4.
   const int rows = a.q.heads + a.k.heads + a.v.heads;
   const int64_t tokens = a.b * a.t;
   int gpt = NORM ? 4 : 8;
-  while (gpt < rows && tokens * gpt * L < 1024L * num_sms()) gpt *= 2;
+  if (NORM) {
+    while (gpt < rows && 2 * tokens * gpt * L <= (write ? 768L : 1024L) * num_sms()) gpt *= 2;
+  } else {
+    while (gpt < rows && tokens * gpt * L < 1024L * num_sms()) gpt *= 2;
+  }
   const int64_t blocks = (tokens * gpt * L + 255) / 256;
   if (blocks > INT32_MAX) return fail(BW_ERR_INVALID_ARGUMENT, "rotary: too many tokens");
   const unsigned grid = static_cast<unsigned>(blocks);
