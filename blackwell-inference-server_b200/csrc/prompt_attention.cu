@@ -122,7 +122,8 @@ __global__ void __launch_bounds__(128) prompt_rows_kernel(const PromptArgs a) {
       for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
       top = fmaxf(top, m[r]);
       const float base = top == -INFINITY ? 0.f : top;  // (scores of -inf alone: no weight)
-      const float f = exp2f(m[r] - base), p = lane < see ? exp2f(s - base) : 0.f;
+      // (2^-16: sums over as many keys of values near bf16's largest stay finite)
+      const float f = exp2f(m[r] - base), p = lane < see ? exp2f(s - base - 16.f) : 0.f;
       m[r] = top;
       l[r] = l[r] * f + p;  // the lane's keys
 #pragma unroll
@@ -191,9 +192,10 @@ static int launch_rows(const PromptArgs& a, cudaStream_t st) {
 // hand-over of the weights in place of two (0.87); the next block's first scores issued before the last of B (0.85).
 //
 // Softmax: thread = row, so nothing is exchanged.  The reference m moves only when a score exceeds it by more than 8 (in
-// powers of two); only then are the sum and the accumulator rescaled.  Weights 2^(s - m + 7) go to the tensor core in
-// the inputs' type: rounded by half an ulp like the inputs themselves, at most 2^15, and the 7 keeps fp16's subnormal steps
-// at 2^-31 of a row's largest weight at most.  Their sum and the accumulator are fp32 and have the same factor.
+// powers of two); only then are the sum and the accumulator rescaled.  Weights 2^(s - m + shift) go to the tensor core in
+// the inputs' type: rounded by half an ulp like the inputs themselves.  fp16: a shift of 7, so at most 2^15, and the type's
+// subnormal steps are at most 2^-31 of a row's largest weight.  bf16, whose values reach fp32's range: -16, so that the
+// sum over 2^16 keys of values near the largest stays finite (2^8 where scores have gone 8 above the reference).  Their sum and the accumulator are fp32 and have the same factor.
 //
 // Keys that a row does not see have weight 0, but 0 times a value that is not finite is not 0.  So a warp looks through
 // every V tile that some row of the block does not see all of: rows behind the block's last position become zeros,
@@ -213,7 +215,9 @@ static_assert(2 * kPromptRegsSoft + kPromptRegsRest == 3 * 168, "register split"
 // A CTA takes its next block when it loads the last but third key tile of the one it has: a block taken earlier is out of
 // other CTAs' reach for longer, one taken later is not there in time.
 constexpr int kPromptAhead = 4;
-constexpr float kPromptSlack = 8.f, kPromptShift = 7.f;
+constexpr float kPromptSlack = 8.f;
+template <typename T>
+constexpr float kPromptShift = std::is_same<T, __half>::value ? 7.f : -16.f;
 constexpr float kPromptLowest = -3.0e38f;  // a row's reference without any score: finite, so differences are
 enum PromptSite : int {
   kSitePrBlock = 501, kSitePrQ = 502, kSitePrK = 503, kSitePrV = 504, kSitePrDrain = 505, kSitePrDone = 506,
@@ -760,7 +764,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           }
           tmem_st_wait();
         }
-        const float2 sc2 = make_float2(sc, sc), m2 = make_float2(kPromptShift - m, kPromptShift - m);
+        const float2 sc2 = make_float2(sc, sc), m2 = make_float2(kPromptShift<T> - m, kPromptShift<T> - m);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t packed[32];

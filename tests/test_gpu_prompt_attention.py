@@ -125,6 +125,16 @@ def test_scores_that_grow(cuda_dev, d, dt):
         _check(qq, kk, v, _off([n - 260, 260], cuda_dev))
 
 
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hq,hk,d", [(4, 2, 128), (4, 2, 64), (4, 2, 80)])
+def test_the_largest_and_smallest_values(cuda_dev, hq, hk, d, dt):
+    """Values up to half the type's largest, whose mean is in range where their sum is not; and tiny ones."""
+    q, k = (_randn(s, (700, h, d), dt, cuda_dev) for s, h in ((1, hq), (2, hk)))
+    v = torch.rand((700, hk, d), generator=torch.Generator().manual_seed(3)).to(cuda_dev) * 0.5 + 0.5
+    _check(q, k, (v * (torch.finfo(dt).max / 2)).to(dt), _off([1, 2, 97, 600], cuda_dev))
+    _check(q, k, (v * 2.0**-14).to(dt), _off([1, 2, 97, 600], cuda_dev))
+
+
 def test_scales(cuda_dev):
     q, k, v = (_randn(s, (300, h, 128), torch.bfloat16, cuda_dev) for s, h in ((1, 8), (2, 2), (3, 2)))
     off = _off([300], cuda_dev)
