@@ -436,9 +436,14 @@ static int launch_logprobs_own(const LogprobArgs& a, int64_t rows, cudaStream_t 
 
 template <typename T>
 static int launch_logprobs(const LogprobArgs& a, int64_t rows, cudaStream_t st) {
-  // Few rows: clusters, as long as two CTAs an SM hold them.  Us with one, two and four CTAs a row: 64 rows of 128256, top 5:
-  // 22, 16 and 14; 148 rows: 22, 19 and 27; 333 rows of 151936, top 1: 36, 39 and 45.
-  const int ctas = rows * 4 <= 2 * num_sms() ? 4 : (rows * 2 <= 2 * num_sms() ? 2 : 1);
+  // Long rows, and few: clusters.  A CTA costs some 5 us whatever its part of the row, the cluster's exchange 1, and one that
+  // waits for a place all of that again, so the more CTAs an SM has, the longer the rows must be.  Us with one, two and four CTAs
+  // a row: 8 rows of 8000 (bf16, top 5) 6.3, 7.0 and 7.2, of 32000 9.0, 8.5 and 7.8; 80 of 32000 9.4, 9.7 and 11.4; 64 of 50257
+  // (fp32, top 8) 14.0, 11.4 and 10.6; 90 14.5, 12.5 and 12.6; 90 of 128256 (bf16, top 5) 21.8, 17.6 and 15.4, 111 22.3, 18.3 and
+  // 22.7, 222 27.5, 23.2 and 35.5, 240 27.5, 33.3 and 37.2.
+  int ctas = 1;
+  if (a.v >= 16384 && rows * 4 * 25000 <= static_cast<int64_t>(num_sms()) * (a.v < 62500 ? a.v : 62500)) ctas = 4;
+  else if (a.v >= 32768 && rows * 2 <= 3 * num_sms()) ctas = 2;
   if (ctas == 4) return launch_logprobs_own<T, 1>(a, rows, st);
   return ctas == 2 ? launch_logprobs_own<T, 2>(a, rows, st) : launch_logprobs_own<T, 4>(a, rows, st);
 }

@@ -139,6 +139,22 @@ def test_rows_alone_and_together(cuda_dev):
                 assert all(torch.equal(a, b) for a, b in zip(token_logprobs(x, t, top), want))
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("rows,v", [(2, 16383), (2, 16384), (20, 16391), (28, 16400), (30, 16385), (50, 32767), (100, 32768), (120, 33001),
+                                    (222, 32773), (223, 32770), (92, 62501), (93, 62500)])
+def test_rows_of_one_two_and_four_ctas(cuda_dev, rows, v, dt):
+    """At the lengths and numbers of rows where a row's CTAs change: ties across them, masked parts, a NaN in the last group."""
+    x = _logits(rows + v, rows, v, dt, cuda_dev)
+    x[0] = (torch.arange(v, device=cuda_dev) % 5).to(dt)
+    x[1] = -float("inf")
+    x[1, v - 3:] = 1.0
+    x[rows // 2, :v - v // 4] = torch.finfo(dt).min
+    if rows > 2:
+        x[rows - 1, v - 1] = float("nan")
+    _check(x, _tokens(v, rows, v, cuda_dev), 1)
+    _check(x, _tokens(v, rows, v, cuda_dev), 20)
+
+
 def test_many_rows(cuda_dev):
     """More rows than a grid's second dimension; offsets past 2^31 elements."""
     from blackwell_ops.prompt import token_logprobs
