@@ -139,7 +139,8 @@ __global__ void __launch_bounds__(256) rotary_rows_kernel(const __grid_constant_
       for (int e = lane; e < a.d; e += 32) y[e] = from_f32<T>(row_value<T>(a, x, e, turns, pos, w, norm));
       if (!WRITE || which == 0) continue;
     }
-    const int64_t row0 = target_row(a, b, t);
+    if (!NORM && a.counts != nullptr && t >= a.counts[b]) continue;
+    const int64_t row0 = NORM ? target_row(a, b, t) : kv_row(a.cache, b, static_cast<int64_t>(a.start[b]) + t);
     if (row0 < 0) continue;
     const int64_t row = row0 + static_cast<int64_t>(h) * a.cache.page;
     float v[kKvMaxDim / 32];
