@@ -229,12 +229,16 @@ class TreeSpeculativeDecoder:
         if max(lens, default=0) > self.max_len:
             raise RuntimeError(f"at most max_len = {self.max_len} tokens a sequence")
         tokens = torch.cat([p.to(self.dev) for p in prompts] or [torch.empty(0, dtype=torch.int64, device=self.dev)])
+        self._check_tokens(tokens)
+        return tokens, lens
+
+    def _check_tokens(self, tokens: torch.Tensor) -> None:
+        """Refuses tokens outside the vocabulary (the embedding's kernel would end the process' use of the GPU)."""
         vocab = self.model.base.model.embed_tokens.weight.shape[0]
-        if tokens.numel():  # (the embedding's kernel would end the process' use of the GPU)
+        if tokens.numel():
             least, most = torch.stack(torch.aminmax(tokens)).tolist()
             if least < 0 or most >= vocab:
                 raise RuntimeError(f"tokens must be 0 to {vocab - 1}")
-        return tokens, lens
 
     def _mlp(self, mlp, y: torch.Tensor) -> torch.Tensor:
         from blackwell_ops.kernels.int8_gemm import int8_gemm, int8_gemm_swiglu
@@ -322,6 +326,7 @@ class TreeSpeculativeDecoder:
             raise RuntimeError("max_new_tokens must not be negative")
         if length + max_new_tokens > self.max_len:
             raise RuntimeError(f"at most max_len = {self.max_len} tokens a sequence")
+        self._check_tokens(ids)
         self.model.set_adapter(adapter)
         self.reset()
         ids = ids.to(self.dev)
