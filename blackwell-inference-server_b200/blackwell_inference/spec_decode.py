@@ -288,7 +288,7 @@ class TreeSpeculativeDecoder:
 
         ``prompts``: any number of lists of at most ``max_len`` tokens.  Returns a ``TokenLogprobs`` for each, of its
         tokens from the second on (log probability, entropy, the ``top`` most likely tokens there).  ``rows``: logits
-        held at a time.  The decoder's sequences and cache are left alone."""
+        held at a time.  The decoder's sequences, its cache and the model's current adapter are left as they are."""
         from blackwell_ops.cuda import rmsnorm
         from blackwell_ops.prompt import TokenLogprobs, token_logprobs
 
@@ -296,17 +296,21 @@ class TreeSpeculativeDecoder:
         n = sum(lens)
         if rows < 1:
             raise RuntimeError("rows must be positive")
+        before = self.model.current_adapter
         self.model.set_adapter(adapter)
-        if n:
-            x, _ = self._prompts(tokens, lens, write=False)
-            norm, nxt = self.model.base.model.norm, torch.cat([tokens[1:], tokens[:1]])
-            parts = []
-            for at in range(0, n, rows):
-                logits = self.model.base.lm_head(rmsnorm(x[at:at + rows], norm.weight, norm.variance_epsilon))
-                parts.append(token_logprobs(logits, nxt[at:at + rows], top))
-            every = [torch.cat(y) for y in zip(*parts)]
-        else:
-            every = token_logprobs(torch.zeros((0, max(top, 1)), device=self.dev), tokens, top)
+        try:
+            if n:
+                x, _ = self._prompts(tokens, lens, write=False)
+                norm, nxt = self.model.base.model.norm, torch.cat([tokens[1:], tokens[:1]])
+                parts = []
+                for at in range(0, n, rows):
+                    logits = self.model.base.lm_head(rmsnorm(x[at:at + rows], norm.weight, norm.variance_epsilon))
+                    parts.append(token_logprobs(logits, nxt[at:at + rows], top))
+                every = [torch.cat(y) for y in zip(*parts)]
+            else:
+                every = token_logprobs(torch.zeros((0, max(top, 1)), device=self.dev), tokens, top)
+        finally:  # the decoder's sequences go on with theirs
+            self.model.set_adapter(before)
         out, at = [], 0
         for m in lens:
             out.append(TokenLogprobs(*(y[at:at + max(m - 1, 0)] for y in every)))

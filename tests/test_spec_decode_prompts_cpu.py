@@ -37,3 +37,37 @@ def test_generate_refuses_tokens_outside_the_vocabulary(ids, packed):
     with pytest.raises(RuntimeError, match="tokens must be 0 to 9"):
         dec.generate(torch.tensor(ids), 2, adapter="a")
     assert dec.model.switches == [] and int(dec.ctx[0]) == 5  # a refused call changes nothing
+
+
+def test_scores_leave_the_adapter_as_it_was(monkeypatch):
+    """Steps that go on behind a score have the adapter that their sequences began with, also where the score fails."""
+    import blackwell_ops.cuda
+    import blackwell_ops.prompt as P
+
+    dec = _decoder()
+    dec.model.set_adapter("mine")
+    dec.model.base.model.norm = SimpleNamespace(weight=None, variance_epsilon=1e-6)
+    dec.model.base.lm_head = lambda x: x
+    used = []
+
+    def prompts(tokens, lens, **kw):
+        used.append(dec.model.current_adapter)
+        return torch.zeros((tokens.numel(), 10)), None
+
+    monkeypatch.setattr(dec, "_prompts", prompts)
+    monkeypatch.setattr(blackwell_ops.cuda, "rmsnorm", lambda x, w, eps: x)
+    none = lambda logits, tokens, top: P.TokenLogprobs(*(torch.zeros((len(tokens), *shape)) for shape in ((), (), (top,), (top,))))  # noqa: E731
+    monkeypatch.setattr(P, "token_logprobs", none)
+    for adapter in (None, "other"):
+        assert [len(s.logprobs) for s in dec.score([[1, 2, 3], [], [4]], adapter=adapter, rows=2)] == [2, 0, 0]
+        assert used.pop() == adapter and dec.model.current_adapter == "mine"
+        dec.score([], adapter=adapter)
+        assert dec.model.current_adapter == "mine"
+
+    def fails(*args, **kw):
+        raise RuntimeError("no memory")
+
+    monkeypatch.setattr(dec, "_prompts", fails)
+    with pytest.raises(RuntimeError, match="no memory"):
+        dec.score([[1, 2]], adapter="other")
+    assert dec.model.current_adapter == "mine"
