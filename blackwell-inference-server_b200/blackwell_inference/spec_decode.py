@@ -356,7 +356,7 @@ class TreeSpeculativeDecoder:
             full = torch.tensor([len(s) >= length + max_new_tokens for s in seen], device=self.dev)
             before = self.ctx.clone()
             self.commit(path, n)
-            self.ctx = torch.where(full, before, self.ctx)
+            self.ctx.copy_(torch.where(full, before, self.ctx))  # in place: a captured step reads it there
             for s, k, new in zip(seen, n.tolist(), out.tolist()):
                 if len(s) < length + max_new_tokens:
                     s += new[:k + 1]

@@ -71,3 +71,31 @@ def test_scores_leave_the_adapter_as_it_was(monkeypatch):
     with pytest.raises(RuntimeError, match="no memory"):
         dec.score([[1, 2]], adapter="other")
     assert dec.model.current_adapter == "mine"
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_generate_keeps_the_lengths_in_place(monkeypatch, packed):
+    """A captured step reads the sequences' lengths where they were when it was captured."""
+    import blackwell_ops.decode as D
+
+    dec = _decoder(batch=2, max_len=20, packed=packed)
+    ctx, at = dec.ctx, []
+
+    def forward(tokens, parents=None, logits=True):
+        at.append((tokens.shape[1], ctx.tolist()))
+        return torch.zeros((*tokens.shape, 10)) if logits else None
+
+    def commit(path, taken):
+        dec.ctx += taken + 1
+
+    def verify(probs, tokens, parents, u, e):  # the root's best token, and nothing drafted
+        return torch.zeros(2, dtype=torch.int32), None, torch.full((2, 1), 7)
+
+    monkeypatch.setattr(dec, "forward", forward)
+    monkeypatch.setattr(dec, "commit", commit)
+    monkeypatch.setattr(dec, "_prompts", lambda *a, **kw: None)
+    monkeypatch.setattr(D, "verify_tree", verify)
+    for n in (0, 1, 3):
+        assert dec.generate(torch.tensor([[1, 2, 3], [4, 5, 6]]), n).tolist() == [[7] * n] * 2
+        assert dec.ctx is ctx and ctx.tolist() == [2 + n] * 2
+    assert at[-3:] == [(1, [2, 2]), (1, [3, 3]), (1, [4, 4])]
