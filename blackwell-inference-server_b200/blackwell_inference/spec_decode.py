@@ -18,8 +18,9 @@ their final slots, and the last token is the next tree's root.
     new = dec.generate(ids, max_new_tokens=64, adapter="a")
 
 Whole prompts of different lengths go through one pass over their packed tokens (``score``, ``prefill_packed``, and
-``generate`` with ``packed=True``), whose layers normalise and rotate queries and keys in one launch, which writes the
-cache too, and attend with ``prompt_attention`` to the 16-bit keys and values:
+``generate`` with ``packed=True``; many prompts through passes of a bounded size), whose layers normalise and rotate
+queries and keys in one launch, which writes the cache too, and attend with ``prompt_attention`` to the 16-bit keys and
+values:
 
     norm_rotary_kv_write_int8 (score: norm_rotary) -> prompt_attention.
 
@@ -111,6 +112,10 @@ class TreeSpeculativeDecoder:
     in the launch that rotates them.  Without it prompts go in chains of 64 through the decoding step, which rounds the
     normalised queries and keys to 16 bits and attends to the int8 cache: the two differ by those roundings."""
 
+    # Tokens of packed prompts that pass the layers together at most; a longer prompt goes alone.  A pass holds a few rows of
+    # the hidden size and one of the MLP's for each of them, so this bounds its memory; its products fill the GPU long before.
+    pass_tokens = 32768
+
     def __init__(self, model: MultiDeltaLoRAModel, batch: int, max_len: int, nodes: int = 16, page: int = 64,
                  packed: bool = False):
         from blackwell_ops.decode import MAX_NODES, KVCacheInt8, rotary_plan
@@ -194,9 +199,20 @@ class TreeSpeculativeDecoder:
         return {"q_weight": None if q is None else q.weight, "k_weight": None if k is None else k.weight,
                 "eps": (k if q is None else q).variance_epsilon}
 
-    def _prompts(self, tokens: torch.Tensor, lens: list[int], write: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    def _passes(self, lens: list[int]):
+        """Prompts i .. j - 1, whose tokens are a .. b - 1 of the packed ones, for each pass (i, j, a, b) that has tokens."""
+        i = a = b = 0
+        for j, n in enumerate(lens):
+            if b > a and b + n - a > self.pass_tokens:
+                yield i, j, a, b
+                i, a = j, b
+            b += n
+        if b > a:
+            yield i, len(lens), a, b
+
+    def _prompts(self, tokens: torch.Tensor, lens: list[int], write: bool, first: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
         """Hidden states [N, hidden] of packed prompts ``tokens`` [N] of ``lens``, and their offsets.  ``write``: their keys
-        and values go to the cache's slots from 0 on."""
+        and values go to the cache's slots from 0 on, of the sequences from ``first`` on."""
         from blackwell_ops.cuda import rmsnorm
         from blackwell_ops.decode import norm_rotary, norm_rotary_kv_write_int8
         from blackwell_ops.prompt import prompt_attention
@@ -205,13 +221,13 @@ class TreeSpeculativeDecoder:
         ends = torch.tensor([0, *lens]).cumsum(0)
         pos = torch.arange(n) - ends[:-1].repeat_interleave(torch.tensor(lens))
         offsets, pos = ends.to(self.dev, torch.int32), pos.to(self.dev, torch.int32)
-        start = torch.zeros_like(self.ctx)
+        table, start = self.table[first:first + len(lens)], torch.zeros_like(self.ctx[first:first + len(lens)])
         x = self.model.base.model.embed_tokens(tokens)
         for layer, cache in zip(self.layers, self._layer_cache):
             att = layer.self_attn
             q, k, v = (y.view(n, -1, self.head_dim) for y in self._qkv(layer, x))
             if write:
-                q, k = norm_rotary_kv_write_int8(q, k, v, pos, self.plan, cache, self.table, start, offsets=offsets,
+                q, k = norm_rotary_kv_write_int8(q, k, v, pos, self.plan, cache, table, start, offsets=offsets,
                                                  keys=True, **self._norms(att))
             else:
                 q, k = norm_rotary(q, k, pos, self.plan, **self._norms(att))
@@ -273,18 +289,20 @@ class TreeSpeculativeDecoder:
 
     @torch.no_grad()
     def prefill_packed(self, prompts) -> None:
-        """Start afresh and commit one prompt a sequence, of different lengths (none, too), in one pass."""
+        """Start afresh and commit one prompt a sequence, of different lengths (none, too), in passes of at most
+        ``pass_tokens`` tokens."""
         tokens, lens = self._pack(prompts)
         if len(lens) != self.batch:
             raise RuntimeError(f"need a prompt for each of {self.batch} sequences")
         self.reset()
+        for i, j, a, b in self._passes(lens):
+            self._prompts(tokens[a:b], lens[i:j], write=True, first=i)
         if tokens.numel():
-            self._prompts(tokens, lens, write=True)
             self.ctx.copy_(torch.tensor(lens, dtype=torch.int32))  # in place, as everywhere: a captured step reads it there
 
     @torch.no_grad()
     def score(self, prompts, adapter: str | None = None, top: int = 0, rows: int = 2048) -> list:
-        """Log probabilities of prompts' tokens after those before them, in one pass over all prompts.
+        """Log probabilities of prompts' tokens after those before them, in passes of at most ``pass_tokens`` tokens.
 
         ``prompts``: any number of lists of at most ``max_len`` tokens.  Returns a ``TokenLogprobs`` for each, of its
         tokens from the second on (log probability, entropy, the ``top`` most likely tokens there).  ``rows``: logits
@@ -293,22 +311,20 @@ class TreeSpeculativeDecoder:
         from blackwell_ops.prompt import TokenLogprobs, token_logprobs
 
         tokens, lens = self._pack(prompts)
-        n = sum(lens)
         if rows < 1:
             raise RuntimeError("rows must be positive")
         before = self.model.current_adapter
         self.model.set_adapter(adapter)
         try:
-            if n:
-                x, _ = self._prompts(tokens, lens, write=False)
-                norm, nxt = self.model.base.model.norm, torch.cat([tokens[1:], tokens[:1]])
-                parts = []
-                for at in range(0, n, rows):
+            parts = [token_logprobs(torch.zeros((0, max(top, 1)), device=self.dev), tokens[:0], top)]
+            norm = self.model.base.model.norm
+            for i, j, a, b in self._passes(lens):
+                x, _ = self._prompts(tokens[a:b], lens[i:j], write=False)
+                nxt = torch.cat([tokens[a + 1:b], tokens[a:a + 1]])
+                for at in range(0, b - a, rows):
                     logits = self.model.base.lm_head(rmsnorm(x[at:at + rows], norm.weight, norm.variance_epsilon))
                     parts.append(token_logprobs(logits, nxt[at:at + rows], top))
-                every = [torch.cat(y) for y in zip(*parts)]
-            else:
-                every = token_logprobs(torch.zeros((0, max(top, 1)), device=self.dev), tokens, top)
+            every = [torch.cat(y) for y in zip(*(parts[1:] or parts))]
         finally:  # the decoder's sequences go on with theirs
             self.model.set_adapter(before)
         out, at = [], 0

@@ -99,3 +99,49 @@ def test_generate_keeps_the_lengths_in_place(monkeypatch, packed):
         assert dec.generate(torch.tensor([[1, 2, 3], [4, 5, 6]]), n).tolist() == [[7] * n] * 2
         assert dec.ctx is ctx and ctx.tolist() == [2 + n] * 2
     assert at[-3:] == [(1, [2, 2]), (1, [3, 3]), (1, [4, 4])]
+
+
+def test_prompts_go_in_passes_of_bounded_size(monkeypatch):
+    """No pass has more tokens than ``pass_tokens`` but a single prompt's; every prompt is in one pass, in its own place."""
+    import blackwell_ops.cuda
+    import blackwell_ops.prompt as P
+
+    lens = [3, 0, 5, 1, 0, 9, 2, 2, 4, 0]
+    prompts = [[(i + 1) % 10] * n for i, n in enumerate(lens)]
+    dec = _decoder(batch=len(lens), max_len=9)
+    dec.model.base.model.norm = SimpleNamespace(weight=None, variance_epsilon=1e-6)
+    dec.model.base.lm_head = lambda x: x
+    for most in (1, 4, 8, 9, 13, 1000):
+        dec.pass_tokens = most
+        for write in (False, True):
+            seen = [None] * len(lens)
+            sizes = []
+
+            def one(tokens, part, write=write, first=None):
+                assert tokens.numel() == sum(part) and (sum(part) <= most or sum(n > 0 for n in part) == 1)
+                sizes.append(sum(part))
+                at = 0
+                for k, n in enumerate(part):
+                    if write:
+                        assert seen[first + k] is None
+                        seen[first + k] = tokens[at:at + n].tolist()
+                    at += n
+                return torch.nn.functional.one_hot(tokens, 10).float(), None
+
+            monkeypatch.setattr(dec, "_prompts", one)
+            monkeypatch.setattr(blackwell_ops.cuda, "rmsnorm", lambda x, w, eps: x)
+
+            def logprobs(logits, tokens, top):  # the token that the row stands for
+                rows = logits.argmax(-1).float() if len(logits) else torch.zeros(0)
+                return P.TokenLogprobs(rows, tokens.float(), torch.zeros((len(tokens), top)), torch.zeros((len(tokens), top)))
+
+            monkeypatch.setattr(P, "token_logprobs", logprobs)
+            if write:
+                dec.prefill_packed(prompts)
+                assert [x or [] for x in seen] == prompts and dec.ctx.tolist() == lens
+            else:
+                for s, p in zip(dec.score(prompts, rows=2), prompts):
+                    assert s.logprobs.tolist() == p[:-1] and s.entropy.tolist() == p[1:]
+            assert sum(sizes) == sum(lens) and min(sizes) > 0
+            if most == 1000:
+                assert len(sizes) == 1
