@@ -196,6 +196,9 @@ class TreeSpeculativeDecoder:
         q, k = getattr(att, "q_norm", None), getattr(att, "k_norm", None)
         if q is None and k is None:
             return {}
+        if q is not None and k is not None and q.variance_epsilon != k.variance_epsilon:
+            raise RuntimeError(f"norms of queries and keys with different epsilons ({q.variance_epsilon} and "
+                               f"{k.variance_epsilon}) are not supported")
         return {"q_weight": None if q is None else q.weight, "k_weight": None if k is None else k.weight,
                 "eps": (k if q is None else q).variance_epsilon}
 

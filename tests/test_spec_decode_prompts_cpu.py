@@ -145,3 +145,15 @@ def test_prompts_go_in_passes_of_bounded_size(monkeypatch):
             assert sum(sizes) == sum(lens) and min(sizes) > 0
             if most == 1000:
                 assert len(sizes) == 1
+
+
+def test_norms_of_queries_and_keys_have_one_epsilon():
+    """One launch takes both with one epsilon: layers that differ are refused, not normalised with the queries'."""
+    dec = _decoder()
+    norm = lambda eps: SimpleNamespace(weight=torch.ones(2), variance_epsilon=eps)  # noqa: E731
+    with pytest.raises(RuntimeError, match="different epsilons"):
+        dec._norms(SimpleNamespace(q_norm=norm(1e-6), k_norm=norm(1e-5)))
+    assert dec._norms(SimpleNamespace(q_norm=norm(1e-5), k_norm=norm(1e-5)))["eps"] == 1e-5
+    one = dec._norms(SimpleNamespace(k_norm=norm(1e-5)))
+    assert one["eps"] == 1e-5 and one["q_weight"] is None
+    assert dec._norms(SimpleNamespace()) == {}
