@@ -280,7 +280,9 @@ def norm_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor
     """``rotary`` of queries and keys whose heads are normalised first, in one pass: each head's row x [D] becomes
     ``w * x / sqrt(mean(x^2) + eps)`` with w = ``q_weight`` or ``k_weight`` [D] (None: its rows are only turned).
 
-    32-bit arithmetic, rounded once, behind the rotation.  Returns new contiguous tensors."""
+    32-bit arithmetic, rounded once, behind the rotation.  The sum of squares is 32-bit, too: a bf16 row where it passes
+    the range (values from 1.6e18 on, for D = 128) gives zeros, and with ``eps`` 0 one of values under 1e-19 is undefined.
+    Returns new contiguous tensors."""
     lead = q.shape[:-2]
     q, shape, b, t, qb, qt, qh = _rows(q, "q", lead)
     dev, dt, hq, d = q.device, q.dtype, shape[-2], shape[-1]

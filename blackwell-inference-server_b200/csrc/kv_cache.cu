@@ -9,7 +9,9 @@
 // No sine table is read; the sines cost one sincospi per pair and token.
 //
 // Norm.  Where a weight w is given, a head's row is first y = w x / sqrt(mean(x^2) + eps), over all of its
-// elements, in 32 bits; the turn and the quantiser take y as it is, unrounded.
+// elements, in 32 bits; the turn and the quantiser take y as it is, unrounded.  The squares' sum has fp32's range: beyond
+// it (bf16 values from 1.6e18 on, at 128 elements) the factor is 0 and so is the row.  A power of two taken out of such rows first
+// costs every other one: 8191 tokens of 40 rows 40 us for 36 without a branch, 41 to 43 with rows that are done again.
 //
 // Quantisation.  One fp32 scale per token and head, s = max|x| / 127 (NaN ignored, 0 for a row of
 // zeros), code = clamp(rne(x / s), +-127) with the IEEE quotient (NaN -> 0).  Rotated keys are

@@ -339,7 +339,9 @@ int bw_rotary_kv_write_int8(const void* q, int64_t q_sb, int64_t q_st, int64_t q
 /*
  * Norms of queries and keys for each head, and the rotation, in one pass: as bw_rotary, of
  *   y = w x / sqrt(mean(x^2) + eps)   over the d elements of each head, in 32 bits, not rounded before it turns.
- * q_weight, k_weight [d] in dtype; a NULL one leaves its rows as they are.
+ * q_weight, k_weight [d] in dtype; a NULL one leaves its rows as they are.  The squares are summed in fp32: a bf16 row
+ * whose sum passes its range (values from 1.6e18 on, for d = 128) gives zeros, and without eps one whose sum is under the
+ * normal numbers (values under 1e-19) is undefined.
  */
 int bw_norm_rotary(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int hq, const void* k, int64_t k_sb,
                    int64_t k_st, int64_t k_sh, int hk, void* q_out, void* k_out, int dtype, int64_t b, int64_t t,
