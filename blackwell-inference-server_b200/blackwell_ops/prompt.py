@@ -90,7 +90,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
 
     A token outside [0, V) (padding) is not scored: 0.  Ties go to the lowest token.  Logits of -inf have no
     probability; a row of nothing else has entropy 0 and log probabilities of -inf.  A row with a NaN or +inf gives NaN,
-    and tokens -1.  32-bit sums in one order: a row's results do not depend on the others."""
+    and tokens -1.  32-bit sums in one order: a row's results depend neither on the others nor on where it lies."""
     if not logits.is_cuda:
         raise RuntimeError("logits must be CUDA")
     if logits.dtype not in _LOGITS:

@@ -5,7 +5,10 @@
 // A thread keeps m, S and T (in powers of two) of what it has seen and rescales S and T where m moves.  A row is
 // cut into four parts, one group of eight logits a thread to each in turn; a cluster of one, two or four CTAs has a
 // row, and a thread's sums of the four parts are joined first, then the threads': the order of a sum is the same
-// for every cluster and every number of rows, so a row's results depend on neither.
+// for every cluster and every number of rows, so a row's results depend on neither.  Nor do they on where in memory the
+// row starts: groups go by the logits' numbers, and a row that starts on no 16-byte boundary (every second row of an odd
+// vocabulary and more) is still read by wide loads: fp32 groups by the widest that their place allows, 16-bit ones in
+// 16-byte pieces, two for a group.
 //
 // The alternatives cost the pass nothing but where each thread's maximum is.  A thread sees every 256th group of
 // its CTA's; the k largest logits (by value, then by lowest index: a total order) lie in the k threads whose
@@ -96,17 +99,39 @@ __device__ __forceinline__ void lp_merge_warps(unsigned long long (*lists)[32], 
   }
 }
 
-// Eight logits of a group that lies in the row and on 16-byte boundaries.
+// Eight logits of a group.
 template <typename T>
 struct LpRaw {
   uint4 w[sizeof(T) / 2];
 };
-template <typename T>
-__device__ __forceinline__ LpRaw<T> lp_fetch(const T* group) {
-  LpRaw<T> r;
-#pragma unroll
-  for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r.w[i] = __ldg(reinterpret_cast<const uint4*>(group) + i);
-  return r;
+// fp32, `Q` words behind a 16-byte boundary.
+template <int Q>
+__device__ __forceinline__ LpRaw<float> lp_words(const float* p) {
+  const uint32_t* u = reinterpret_cast<const uint32_t*>(p);
+  auto two = [&](int i) { return __ldg(reinterpret_cast<const uint2*>(u + i)); };
+  auto four = [&](int i) { return __ldg(reinterpret_cast<const uint4*>(u + i)); };
+  if constexpr (Q == 0) {
+    return {{four(0), four(4)}};
+  } else if constexpr (Q == 1) {
+    const uint32_t a = __ldg(u), d = __ldg(u + 7);
+    const uint2 b = two(1);
+    const uint4 c = four(3);
+    return {{make_uint4(a, b.x, b.y, c.x), make_uint4(c.y, c.z, c.w, d)}};
+  } else if constexpr (Q == 2) {
+    const uint2 a = two(0), c = two(6);
+    const uint4 b = four(2);
+    return {{make_uint4(a.x, a.y, b.x, b.y), make_uint4(b.z, b.w, c.x, c.y)}};
+  } else {
+    const uint32_t a = __ldg(u), d = __ldg(u + 7);
+    const uint4 b = four(1);
+    const uint2 c = two(5);
+    return {{make_uint4(a, b.x, b.y, b.z), make_uint4(b.w, c.x, c.y, d)}};
+  }
+}
+// 16-bit, from the five words that they lie in: from the first's lower half on, or its upper (__byte_perm's selectors).
+__device__ __forceinline__ uint4 lp_halves(const uint32_t (&x)[5], uint32_t halves) {
+  return make_uint4(__byte_perm(x[0], x[1], halves), __byte_perm(x[1], x[2], halves), __byte_perm(x[2], x[3], halves),
+                    __byte_perm(x[3], x[4], halves));
 }
 template <typename T>
 __device__ __forceinline__ void lp_unpack(const LpRaw<T>& r, float (&f)[8]) {
@@ -142,13 +167,15 @@ __device__ __forceinline__ void lp_send(uint32_t addr, const LpSums& x) {
   st_shared_cluster_f32(addr + 8, x.t);
 }
 
-// Steps of four groups that a thread has on their way in shared memory, and CTAs of an SM.  16-bit logits: three, 192 KB an SM,
-// which registers have no room for (2047 rows of 151936: 125 us, from registers 141).  fp32 logits have 128 bytes a thread in a
-// step as it is, from registers (2047 rows of 50257: 85 us, through shared memory 112).
+// Steps of four groups that a thread has on their way in shared memory, and CTAs of an SM.  16-bit logits: three, 198 KB an SM,
+// which registers have no room for (2047 rows of 151936: 125 us, from registers 141); CTAs of a cluster hold the others' sums,
+// too, and an SM three of them.  fp32 logits have 128 bytes a thread in a step as it is, from registers (2047 rows of
+// 50256: 86 us; through shared memory, rows of 50257, 112 us).
 template <typename T>
 struct LpRing {
   static constexpr int STAGES = sizeof(T) == 4 ? 0 : 3, CTAS = sizeof(T) == 4 ? 3 : 4;
-  static constexpr int BYTES = STAGES * kLpParts * kLpThreads * 16;
+  static constexpr int ROW = 33;  // pieces of a warp's 32 groups: one more, into which the last one's logits may reach
+  static constexpr int BYTES = STAGES * kLpParts * kLpWarps * ROW * 16;
 };
 
 // A cluster of kLpParts / OWN CTAs a row.
@@ -156,7 +183,7 @@ template <typename T, int OWN>
 __global__ void __launch_bounds__(kLpThreads, LpRing<T>::CTAS) token_logprobs_kernel(const LogprobArgs a) {
   constexpr int U = kLpParts / OWN;  // groups of a part in a step
   constexpr int STAGES = LpRing<T>::STAGES;
-  extern __shared__ uint4 ring[];    // [stage][group of a step][thread]
+  extern __shared__ uint4 ring[];    // [stage][group of a step][warp][LpRing::ROW]
   __shared__ unsigned long long lists[kLpWarps][32];
   __shared__ unsigned long long firsts[32];              // the k best threads
   __shared__ unsigned long long from[kLpParts][32];      // at rank 0: the CTAs' lists
@@ -169,20 +196,38 @@ __global__ void __launch_bounds__(kLpThreads, LpRing<T>::CTAS) token_logprobs_ke
   const int64_t row = blockIdx.x / ctas;
   const T* x = static_cast<const T*>(a.x) + row * a.ld;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // Groups lie on 32-byte (16-bit types: 16-byte) boundaries of memory: index i of group c is 8 c - shift + i.
-  // Group c is thread c % 256's of part c / 256 % 4.
-  const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(x) / sizeof(T) & 7);
-  const int groups = static_cast<int>((static_cast<int64_t>(a.v) + shift + 7) >> 3);
-  const int whole_lo = shift ? 1 : 0, whole_hi = static_cast<int>((static_cast<int64_t>(a.v) + shift) >> 3);
-  auto at = [&](int c) { return x + (static_cast<int64_t>(c) * 8 - shift); };
+  // Group c has the logits 8 c to 8 c + 7 and is thread c % 256's of part c / 256 % 4.  The row starts `shift` logits behind a
+  // 16-byte boundary.  Where a 16-bit one does, group c lies in the pieces c and c + 1 from that boundary on: pieces 1 .. hi - 1
+  // lie in the row as a whole, and so do all of the groups lo .. whole - 1.  Groups before and behind those are read one by one.
+  constexpr int PIECE = 16 / sizeof(T);
+  const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(x) / sizeof(T)) & (PIECE - 1);
+  const bool apart = sizeof(T) == 2 && shift != 0;
+  const int word = sizeof(T) == 4 ? shift : shift >> 1;  // that a group starts in, behind a boundary
+  const uint32_t halves = shift & 1 ? 0x5432 : 0x3210;
+  const uint4* piece = reinterpret_cast<const uint4*>(x - shift);
+  const int groups = static_cast<int>((static_cast<int64_t>(a.v) + 7) >> 3);
+  const int hi = static_cast<int>((static_cast<int64_t>(a.v) + shift) >> 3);
+  const int lo = apart ? 1 : 0, whole = apart ? hi - 1 : a.v >> 3;  // (may be -1)
   auto load = [&](int c, float(&f)[8]) {
-    if (c >= whole_lo && c < whole_hi) {
-      lp_unpack<T>(lp_fetch<T>(at(c)), f);
+    if (c >= lo && c < whole && (sizeof(T) == 2 || shift == 0)) {
+      LpRaw<T> raw;
+      if constexpr (sizeof(T) == 4) {
+        raw = lp_words<0>(x + static_cast<int64_t>(c) * 8);
+      } else if (!apart) {
+        raw.w[0] = __ldg(piece + c);
+      } else {
+        const uint32_t* from = reinterpret_cast<const uint32_t*>(piece + c) + word;
+        uint32_t y[5];
+#pragma unroll
+        for (int i = 0; i < 5; ++i) y[i] = __ldg(from + i);
+        raw.w[0] = lp_halves(y, halves);
+      }
+      lp_unpack<T>(raw, f);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int64_t i = static_cast<int64_t>(c) * 8 - shift + e;
-        f[e] = i >= 0 && i < a.v ? lp_to_f32(x[i]) : -INFINITY;
+        const int64_t i = static_cast<int64_t>(c) * 8 + e;
+        f[e] = i < a.v ? lp_to_f32(x[i]) : -INFINITY;
       }
     }
   };
@@ -222,70 +267,116 @@ __global__ void __launch_bounds__(kLpThreads, LpRing<T>::CTAS) token_logprobs_ke
     sum.t += t.x + t.y;
   };
   {
-    // four groups at a time, whatever the cluster: of one part, of two or of four
+    // four groups at a time, whatever the cluster: of one part, two or four
     constexpr int step = kLpParts * kLpThreads;
     const int c0 = rank * own * kLpThreads + tid;
+    auto place = [&](int n) { return n % OWN * kLpThreads + n / OWN * step; };
     float f[8];
-    if (c0 == 0 && shift) {
-      load(0, f);
-      take(0, f, sum[0]);
-    }
-    if constexpr (LpRing<T>::STAGES == 0) {
-      for (int k = 0; c0 + k < whole_hi; k += U * step) {
-        LpRaw<T> raw[kLpParts];
+    // Copies of the pass, for 2047 rows of 50257 in us (in brackets with groups that go by the boundaries): fp32, one for each
+    // word that a row may start at 89 (87.5), two and selections 97; 16-bit, one for rows on a boundary and one for those between
+    // 68 (63), selections in place of shared memory's words 73, one for each word, more code than its cache holds, 76.
+    auto pass = [&](auto start, auto between) {
+      constexpr int Q = decltype(start)::value;
+      constexpr bool APART = decltype(between)::value;
+      if constexpr (LpRing<T>::STAGES == 0) {
+        for (int k = 0; c0 + k < whole; k += U * step) {
+          LpRaw<T> raw[kLpParts];
 #pragma unroll
-        for (int n = 0; n < kLpParts; ++n) {
-          const int c = c0 + k + n % OWN * kLpThreads + n / OWN * step;
-          if (c >= whole_lo && c < whole_hi) raw[n] = lp_fetch<T>(at(c));
-        }
+          for (int n = 0; n < kLpParts; ++n) {
+            const int c = c0 + k + place(n);
+            if (c < whole) raw[n] = lp_words<Q>(x + static_cast<int64_t>(c) * 8);
+          }
 #pragma unroll
-        for (int n = 0; n < kLpParts; ++n) {
-          const int c = c0 + k + n % OWN * kLpThreads + n / OWN * step;
-          if (c >= whole_lo && c < whole_hi) {
-            lp_unpack<T>(raw[n], f);
-            take(c, f, sum[n % OWN]);
+          for (int n = 0; n < kLpParts; ++n) {
+            const int c = c0 + k + place(n);
+            if (c < whole) {
+              lp_unpack<T>(raw[n], f);
+              take(c, f, sum[n % OWN]);
+            }
           }
         }
+      } else {
+        // Each lane copies its own groups' pieces to shared memory, three steps of four ahead.  APART: a lane reads its neighbour's
+        // piece, too (the last one's neighbour is an additional piece of its own), so a warp's lanes go on together.
+        constexpr int ROW = APART ? LpRing<T>::ROW : 32, GROUP = kLpWarps * ROW;
+        uint4* mine = ring + warp * ROW + lane;
+        const int begin = APART ? c0 - lane : c0;
+        auto fetch = [&](int k, int stage) {
+#pragma unroll
+          for (int n = 0; n < kLpParts; ++n) {
+            const int c = c0 + k + place(n);
+            uint4* to = mine + (stage * kLpParts + n) * GROUP;
+            if ((!APART || c > 0) && c < hi) copy16_async(to, piece + c);
+            if (APART && lane == 31 && c + 1 < hi) copy16_async(to + 1, piece + c + 1);
+          }
+          asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+#pragma unroll
+        for (int i = 0; i < STAGES; ++i) fetch(i * U * step, i);
+        if (APART && c0 == 0) {
+          load(0, f);
+          take(0, f, sum[0]);
+        }
+        int stage = 0;
+        for (int k = 0; begin + k < whole; k += U * step) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+          if (APART) __syncwarp();  // the neighbour's, too
+#pragma unroll
+          for (int n = 0; n < kLpParts; ++n) {
+            const int c = c0 + k + place(n);
+            if ((!APART || c > 0) && c < whole) {
+              const uint4* from = mine + (stage * kLpParts + n) * GROUP;
+              LpRaw<T> raw;
+              if constexpr (APART) {
+                uint32_t y[5];
+#pragma unroll
+                for (int i = 0; i < 5; ++i) y[i] = reinterpret_cast<const uint32_t*>(from)[word + i];
+                raw.w[0] = lp_halves(y, halves);
+              } else {
+                raw.w[0] = from[0];
+              }
+              lp_unpack<T>(raw, f);
+              take(c, f, sum[n % OWN]);
+            }
+          }
+          if (APART) __syncwarp();  // read by both
+          fetch(k + STAGES * U * step, stage);
+          stage = stage + 1 == STAGES ? 0 : stage + 1;
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+      }
+    };
+    using std::integral_constant;
+    if constexpr (sizeof(T) == 4) {
+      if (word == 0) pass(integral_constant<int, 0>{}, std::false_type{});
+      else if (word == 1) pass(integral_constant<int, 1>{}, std::false_type{});
+      else if (word == 2) pass(integral_constant<int, 2>{}, std::false_type{});
+      else pass(integral_constant<int, 3>{}, std::false_type{});
+    } else if (apart) {
+      pass(integral_constant<int, 0>{}, std::true_type{});
+    } else {
+      pass(integral_constant<int, 0>{}, std::false_type{});
+    }
+    // the groups that the row ends in: two at most (fp32: one), each its thread's last
+    if constexpr (sizeof(T) == 4) {
+      for (int c = whole; c < groups; ++c) {
+#pragma unroll
+        for (int p = 0; p < OWN; ++p)
+          if (c0 + p * kLpThreads == c % step) {
+            load(c, f);
+            take(c, f, sum[p]);
+          }
       }
     } else {
-      // Each thread copies its own groups to shared memory, three steps of four ahead (nobody else reads them: no barrier).
-      auto fetch = [&](int k, int stage) {
+      const int end = max(whole, lo);
 #pragma unroll
-        for (int n = 0; n < kLpParts; ++n) {
-          const int c = c0 + k + n % OWN * kLpThreads + n / OWN * step;
-          if (c >= whole_lo && c < whole_hi)
-            copy16_async(&ring[(stage * kLpParts + n) * kLpThreads + tid], at(c));
+      for (int p = 0; p < OWN; ++p) {
+        const int c = end + ((c0 + p * kLpThreads - end) & (step - 1));
+        if (c < groups) {
+          load(c, f);
+          take(c, f, sum[p]);
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-      };
-#pragma unroll
-      for (int i = 0; i < STAGES; ++i) fetch(i * U * step, i);
-      int stage = 0;
-      for (int k = 0; c0 + k < whole_hi; k += U * step) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
-#pragma unroll
-        for (int n = 0; n < kLpParts; ++n) {
-          const int c = c0 + k + n % OWN * kLpThreads + n / OWN * step;
-          if (c >= whole_lo && c < whole_hi) {
-            LpRaw<T> raw;
-            raw.w[0] = ring[(stage * kLpParts + n) * kLpThreads + tid];
-            lp_unpack<T>(raw, f);
-            take(c, f, sum[n % OWN]);
-          }
-        }
-        fetch(k + STAGES * U * step, stage);
-        stage = stage + 1 == STAGES ? 0 : stage + 1;
       }
-      asm volatile("cp.async.wait_all;" ::: "memory");
-    }
-    const int last = groups - 1;  // a group that the row ends in
-    if (last >= whole_hi && (last > 0 || !shift)) {
-#pragma unroll
-      for (int p = 0; p < OWN; ++p)
-        if (c0 + p * kLpThreads == last % step) {
-          load(last, f);
-          take(last, f, sum[p]);
-        }
     }
   }
   LpSums all = sum[0];  // (0 + 1) + (2 + 3), or what the CTA has of it
@@ -332,9 +423,9 @@ __global__ void __launch_bounds__(kLpThreads, LpRing<T>::CTAS) token_logprobs_ke
       if (!__any_sync(0xffffffffu, has)) continue;
 #pragma unroll 1
       for (int e = 0; e < 8; ++e) {
-        const int64_t i = static_cast<int64_t>(c) * 8 - shift + e;
+        const int64_t i = static_cast<int64_t>(c) * 8 + e;
         unsigned long long key = 0ull;
-        if (has && i >= 0 && i < a.v) {
+        if (has && i < a.v) {
           float v = f[0];
 #pragma unroll
           for (int n = 1; n < 8; ++n) v = e == n ? f[n] : v;

@@ -432,7 +432,8 @@ int bw_prompt_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k
  *   logprobs[r] = x_t - ln sum_i exp(x_i) with t = tokens[r], 0 where t is outside [0, v);  entropy[r] = -sum p ln p;
  *   top_logprobs, top_tokens [rows, top]: the `top` largest, by value and then by lowest token (top <= 32, <= v).
  * Logits of -inf have no probability; a row of nothing else has entropy 0 and log probabilities of -inf.  A row with a
- * NaN or +inf gives NaN, and tokens -1.  Sums in fp32, in one order.
+ * NaN or +inf gives NaN, and tokens -1.  Sums in fp32, in one order of the logits, whatever the number of rows and
+ * wherever a row starts.
  */
 int bw_token_logprobs(const void* logits, int dtype, int64_t ld, const int64_t* tokens, int64_t rows, int64_t v,
                       int64_t top, float* logprobs, float* entropy, float* top_logprobs, int64_t* top_tokens,
