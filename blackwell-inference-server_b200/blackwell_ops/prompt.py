@@ -40,6 +40,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     Row i of a sequence sees the sequence's rows up to itself.  ``offsets`` [B + 1] int32, not descending; rows of no
     sequence (before ``offsets[0]``, behind ``offsets[B]``) give zeros.  Query head h reads key head
     ``h // (Hq / Hk)``.  ``softmax_scale`` defaults to ``D ** -0.5``.  A sequence's results do not depend on the others.
+    Infinite and NaN elements of v go to that element of every row that sees them, whatever their weight.
 
     The tensor-core kernel takes D = 64 or 128, at most 128 query heads a key head and a positive scale (rows that do not
     start on 16-byte boundaries are copied first); other calls go to a plain kernel, a hundred times slower on long

@@ -7,6 +7,11 @@
 // i's blocks are numbered from offset_i / P + i on (whole division): ceil(length / P) of them always fit before the
 // next segment's, at most one number a segment is left without a block, and n / P + b + 2 numbers are enough for all.
 // Offsets are clamped to [0, n]: where they descend, results are undefined but nothing outside is read or written.
+//
+// Values that are not finite.  An element of v that is infinite or NaN goes to that element of every row that sees it, whatever
+// its weight: the rows' element is the sum of such values (infinities of one sign: this infinity).  The formula says so for
+// every weight over 0, and all weights are; as a product, a weight that underflows would make it NaN, and whether it
+// does would go by the tiles.
 #include <stdio.h>
 
 #include <mutex>
@@ -59,6 +64,8 @@ __device__ __forceinline__ bool prompt_block(const PromptArgs& a, int P, int slo
   return true;
 }
 
+__device__ __forceinline__ bool is_finite(float x) { return fabsf(x) <= 3.402823466e38f; }
+
 // ---------------------------------------------------------------------------
 // any head dimension up to 256, any strides: a CTA has 16 queries of one head, its four warps four each, and 32 keys
 // at a time in shared memory (lane = key for the scores, lane = element for the output)
@@ -99,12 +106,15 @@ __global__ void __launch_bounds__(128) prompt_rows_kernel(const PromptArgs a) {
   for (int j0 = blk.first; j0 < blk.row1; j0 += kRowsK) {
     const int keys = min(blk.row1 - j0, kRowsK);
     __syncthreads();
+    bool bad = false;
     for (int e = threadIdx.x; e < keys * d; e += 128) {
       const int j = e / d, c = e - j * d;
+      const float y = to_f32(v[(j0 + j) * a.v_st + c]);
       sk[j * ld + c] = to_f32(k[(j0 + j) * a.k_st + c]);
-      sv[j * d + c] = to_f32(v[(j0 + j) * a.v_st + c]);
+      sv[j * d + c] = y;
+      bad |= !is_finite(y);
     }
-    __syncthreads();
+    const bool odd = __syncthreads_or(bad);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int row = warp * 4 + r;
@@ -127,12 +137,16 @@ __global__ void __launch_bounds__(128) prompt_rows_kernel(const PromptArgs a) {
       m[r] = top;
       l[r] = l[r] * f + p;  // the lane's keys
 #pragma unroll
-      for (int i = 0; i < kKvMaxDim / 32; ++i) o[r][i] *= f;
+      for (int i = 0; i < kKvMaxDim / 32; ++i) o[r][i] *= fmaxf(f, 1.17549435e-38f);  // (an infinity stays one)
       for (int j = 0; j < see; ++j) {
         const float pj = __shfl_sync(0xffffffffu, p, j);
 #pragma unroll
         for (int i = 0; i < kKvMaxDim / 32; ++i)
-          if (lane + 32 * i < d) o[r][i] += pj * sv[j * d + lane + 32 * i];
+          if (lane + 32 * i < d) {
+            const float y = sv[j * d + lane + 32 * i];
+            if (odd && !is_finite(y)) o[r][i] += y;
+            else o[r][i] += pj * y;
+          }
       }
     }
   }
@@ -143,7 +157,7 @@ __global__ void __launch_bounds__(128) prompt_rows_kernel(const PromptArgs a) {
     float sum = l[r];
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const float inv = sum == 0.f ? 1.f : 1.f / sum;  // (scores of -inf alone: 0, or what is not finite)
 #pragma unroll
     for (int i = 0; i < kKvMaxDim / 32; ++i)
       if (lane + 32 * i < d) out[(static_cast<int64_t>(blk.row0 + row) * a.hq + h) * d + lane + 32 * i] = from_f32<T>(o[r][i] * inv);
@@ -199,7 +213,10 @@ static int launch_rows(const PromptArgs& a, cudaStream_t st) {
 //
 // Keys that a row does not see have weight 0, but 0 times a value that is not finite is not 0.  So a warp looks through
 // every V tile that some row of the block does not see all of: rows behind the block's last position become zeros,
-// values that are not finite become 0 and are added at the end to the rows that do see them.
+// values that are not finite become 0 and are added at the end to the rows that do see them.  The tiles before, which all
+// rows see, go into the product as they are.  Where that leaves something that is not finite, the block's end sums those
+// tiles' values that are not finite from memory and puts the sum in place of what the weights have made of them: which
+// tiles are looked through goes by the block, so by the other sequences, and the results must not.
 //
 // Blocks are handed out by the hardware: a CTA that nears its end takes the next one that has not started
 // (clusterlaunchcontrol), so the schedule is dynamic without a counter in memory.
@@ -803,6 +820,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       uint8_t* stage = sO + warp * C::OB;
 #pragma unroll 1
       for (int c0 = 0; c0 < D; c0 += 64) {
+        float2 zero = make_float2(0.f, 0.f);  // NaN as soon as an element is not finite
 #pragma unroll
         for (int c = 0; c < 64; c += 32) {
           uint32_t o[32];
@@ -812,15 +830,45 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll
           for (int e = 0; e < 32; ++e) y[e] = __uint_as_float(o[e]) * inv;
 #pragma unroll
+          for (int e = 0; e < 32; e += 2) zero = __ffma2_rn(make_float2(y[e], y[e + 1]), make_float2(0.f, 0.f), zero);
+#pragma unroll
           for (int e = 0; e < 32; e += 8)
             *reinterpret_cast<uint4*>(stage + lane * 128 + ((((c + e) >> 3) ^ (lane & 7)) << 4)) =
                 make_uint4(pack2<T>(make_float2(y[e], y[e + 1])), pack2<T>(make_float2(y[e + 2], y[e + 3])),
                            pack2<T>(make_float2(y[e + 4], y[e + 5])), pack2<T>(make_float2(y[e + 6], y[e + 7])));
         }
+        const int from = (t.row0 + 1) / KEYS * KEYS;  // keys before it are in tiles that all rows see
+        const T* v = static_cast<const T*>(a.v) + static_cast<int64_t>(t.first) * a.v_st + t.head * a.v_sh + c0;
+        if (__builtin_expect(from > 0 && __any_sync(0xffffffffu, mine && sum == sum && !(zero.x + zero.y == 0.f)), 0)) {
+          // their values that are not finite: lane = two elements, eight keys at a time (more code here makes all blocks slower:
+          // 24 prompts of up to 1021 tokens 99.4 us without any of this, 100.9 so, 101.5 with 32 keys)
+          float2 z = make_float2(0.f, 0.f);
+#pragma unroll 1
+          for (int key = 0; key < from; key += 8) {
+            uint32_t x[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) x[u] = *reinterpret_cast<const uint32_t*>(v + (key + u) * a.v_st + 2 * lane);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+              const uint32_t b = not_finite2<T>(x[u]);
+              const T* h = reinterpret_cast<const T*>(&x[u]);
+              if (b & 0x8000u) z.x += to_f32(h[0]);
+              if (b & 0x80000000u) z.y += to_f32(h[1]);
+            }
+          }
+          const uint32_t nan_rows = __ballot_sync(0xffffffffu, sum != sum);  // (of scores, not of values)
+          __syncwarp();
+#pragma unroll 1
+          for (int r = 0; r < 32; ++r) {
+            T* y = reinterpret_cast<T*>(stage + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+            if (nan_rows >> r & 1) continue;
+            if (z.x != 0.f) y[0] = from_f32<T>(z.x);
+            if (z.y != 0.f) y[1] = from_f32<T>(z.y);
+          }
+          __syncwarp();
+        }
         if (any != 0 && mine) {
           // values that are not finite, of the keys that this row sees among those that not all see
-          const int from = (t.row0 + 1) / KEYS * KEYS;
-          const T* v = static_cast<const T*>(a.v) + static_cast<int64_t>(t.first) * a.v_st + t.head * a.v_sh + c0;
 #pragma unroll 1
           for (int k = 0; k < 12; ++k) {
 #pragma unroll 1
@@ -831,7 +879,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
               for (int e = 0; e < 64; ++e) {
                 const float z = to_f32(v[key * a.v_st + e]);
                 T* y = reinterpret_cast<T*>(stage + lane * 128 + (((e >> 3) ^ (lane & 7)) << 4)) + (e & 7);
-                if (!(fabsf(z) <= 3.402823466e38f)) *y = from_f32<T>(to_f32(*y) + z);
+                if (!is_finite(z)) *y = from_f32<T>(to_f32(*y) + z);
               }
             }
           }

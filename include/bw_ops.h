@@ -421,7 +421,9 @@ int bw_tree_attention_int8(const void* q, int64_t q_sb, int64_t q_st, int64_t q_
  *   out_r = sum_j w_rj v_j / sum_j w_rj,  w_rj = exp(softmax_scale * q_r . k_j)
  * out [n, hq, d] contiguous, in the inputs' dtype (F16 | BF16); rows of no sequence are zeros.  Strides are in elements,
  * with unit stride in d; hq is a multiple of hk (query head h reads key head h / (hq / hk)); d <= 256.  Scores, sums and
- * outputs accumulate in fp32.  Results of a sequence do not depend on the others.
+ * outputs accumulate in fp32.  Results of a sequence do not depend on the others.  Elements of v that are infinite or NaN
+ * go to that element of every row that sees them, whatever their weight (their sum; NaN from infinities of both signs);
+ * a row whose scores are all -inf has no other weight and is 0 otherwise.
  */
 int bw_prompt_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
                         const void* v, int64_t v_st, int64_t v_sh, int dtype, void* out, const int32_t* offsets,
