@@ -418,7 +418,18 @@ __global__ void __launch_bounds__(kLpThreads, LpRing<T>::CTAS) token_logprobs_ke
       float f[8];
       bool has = false;
       if (first != 0ull && c < groups) {
-        load(c, f);
+        if constexpr (sizeof(T) == 4) {
+          // (the widest loads here, too: 600 rows of 50257, top 20, 47 us for 50 one by one; inside `load`, where the
+          // row's last group would have them as well, registers spill)
+          const T* from = x + static_cast<int64_t>(c) * 8;
+          if (c >= whole) load(c, f);
+          else if (word == 0) lp_unpack<T>(lp_words<0>(from), f);
+          else if (word == 1) lp_unpack<T>(lp_words<1>(from), f);
+          else if (word == 2) lp_unpack<T>(lp_words<2>(from), f);
+          else lp_unpack<T>(lp_words<3>(from), f);
+        } else {
+          load(c, f);
+        }
         has = lp_key(fmaxf(max3(max3(f[0], f[1], f[2]), f[3], f[4]), max3(f[5], f[6], f[7])), c) >= limit;
       }
       if (!__any_sync(0xffffffffu, has)) continue;
