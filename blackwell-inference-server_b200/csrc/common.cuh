@@ -566,6 +566,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
+// NaN if one of them is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
 // Four int8 codes (one 32-bit word) -> two f16x2 words, exactly.  Each byte is
 // biased to u = q + 128 in [1, 255], placed in the mantissa of 1024.0
 // (0x6400 | u == 1024 + u) and 1152 = 1024 + 128 is subtracted.

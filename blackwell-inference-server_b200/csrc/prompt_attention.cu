@@ -312,6 +312,22 @@ __device__ __forceinline__ uint32_t pack2(float2 v) {
   }
 }
 
+// A packed pair with infinities of the type's largest value in their place (a NaN stays one).
+template <typename T>
+__device__ __forceinline__ uint32_t finite2(uint32_t w) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 top = __half2half2(__ushort_as_half(0x7BFF));
+    const __half2 h = __hmax2_nan(__hmin2_nan(*reinterpret_cast<const __half2*>(&w), top), __hneg2(top));
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 top = __bfloat162bfloat162(__ushort_as_bfloat16(0x7F7F));
+    const __nv_bfloat162 h = __hmax2_nan(__hmin2_nan(*reinterpret_cast<const __nv_bfloat162*>(&w), top), __hneg2(top));
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+template <typename T>
+constexpr float kPromptTop = std::is_same<T, __half>::value ? 65504.f : 3.38953139e38f;  // the type's largest value
+
 template <int D, typename T>
 __global__ void __launch_bounds__(kPromptThreads, 1)
     prompt_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -820,7 +836,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       uint8_t* stage = sO + warp * C::OB;
 #pragma unroll 1
       for (int c0 = 0; c0 < D; c0 += 64) {
-        float2 zero = make_float2(0.f, 0.f);  // NaN as soon as an element is not finite
+        float most = 0.f;  // of the row's elements; NaN if one is
 #pragma unroll
         for (int c = 0; c < 64; c += 32) {
           uint32_t o[32];
@@ -830,7 +846,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll
           for (int e = 0; e < 32; ++e) y[e] = __uint_as_float(o[e]) * inv;
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) zero = __ffma2_rn(make_float2(y[e], y[e + 1]), make_float2(0.f, 0.f), zero);
+          for (int e = 0; e < 32; e += 2) most = max3_nan(most, fabsf(y[e]), fabsf(y[e + 1]));
 #pragma unroll
           for (int e = 0; e < 32; e += 8)
             *reinterpret_cast<uint4*>(stage + lane * 128 + ((((c + e) >> 3) ^ (lane & 7)) << 4)) =
@@ -839,9 +855,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         }
         const int from = (t.row0 + 1) / KEYS * KEYS;  // keys before it are in tiles that all rows see
         const T* v = static_cast<const T*>(a.v) + static_cast<int64_t>(t.first) * a.v_st + t.head * a.v_sh + c0;
-        if (__builtin_expect(from > 0 && __any_sync(0xffffffffu, mine && sum == sum && !(zero.x + zero.y == 0.f)), 0)) {
-          // their values that are not finite: lane = two elements, eight keys at a time (more code here makes all blocks slower:
-          // 24 prompts of up to 1021 tokens 99.4 us without any of this, 100.9 so, 101.5 with 32 keys)
+        if (__builtin_expect(__any_sync(0xffffffffu, mine && !(most <= kPromptTop<T>)), 0)) {
+          // (The code here is kept small: more of it makes all blocks slower, 24 prompts of up to 1021 tokens 101.5 us for 100.9
+          // with 32 keys at a time below.)
+          // A mean of values near the type's largest that the weights' rounding has carried past it: their sum takes them unrounded.
+#pragma unroll 1
+          for (int c = 0; c < 32; ++c) {
+            uint32_t* x = reinterpret_cast<uint32_t*>(stage + lane * 128 + c * 4);
+            *x = finite2<T>(*x);
+          }
+          __syncwarp();
+        }
+        if (__builtin_expect(from > 0 && __any_sync(0xffffffffu, mine && sum == sum && !(most <= 3.402823466e38f)), 0)) {
+          // values that are not finite, of the keys that all rows see: lane = two elements, eight keys at a time
           float2 z = make_float2(0.f, 0.f);
 #pragma unroll 1
           for (int key = 0; key < from; key += 8) {
@@ -857,7 +883,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             }
           }
           const uint32_t nan_rows = __ballot_sync(0xffffffffu, sum != sum);  // (of scores, not of values)
-          __syncwarp();
 #pragma unroll 1
           for (int r = 0; r < 32; ++r) {
             T* y = reinterpret_cast<T*>(stage + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
