@@ -10,12 +10,13 @@
 // vocabulary and more) is still read by wide loads: fp32 groups by the widest that their place allows, 16-bit ones in
 // 16-byte pieces, two for a group.
 //
-// The alternatives cost the pass itself nothing but where each thread's maximum is; their search behind it, with none
-// of the next row's logits on their way, costs 9 us with one and 57 with twenty of 2047 rows of 151936, which take 124
-// without.  A thread sees every 256th group of its CTA's; the k largest logits (by value, then by lowest index: a total order) lie in the k threads whose
-// maxima are largest by (value, group), for if one lay elsewhere, k maxima would come before it.  So the k best
-// threads are found (a sort of 32 in each warp, merges of sorted lists), and only their groups are read again,
-// one 256th of the CTA's each, from L2: lists of some 300 logits, of which those before the k-th maximum are candidates.
+// The alternatives cost the pass itself nothing but where each thread's maximum is; their search behind it, with
+// none of the next row's logits on their way, costs 9 us with one and 57 with twenty of 2047 rows of 151936, which
+// take 124 without.  A thread sees every 256th group of its CTA's; the k largest logits (by value, then by lowest
+// index: a total order) lie in the k threads whose maxima are largest by (value, group), for if one lay elsewhere,
+// k maxima would come before it.  So the k best threads are found (a sort of 32 in each warp, merges of sorted
+// lists), and only their groups are read again, one 256th of the CTA's each, from L2: lists of some 300 logits, of
+// which those before the k-th maximum are candidates.
 #include <mutex>
 #include <type_traits>
 

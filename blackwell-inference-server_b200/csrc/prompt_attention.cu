@@ -206,10 +206,11 @@ static int launch_rows(const PromptArgs& a, cudaStream_t st) {
 // hand-over of the weights in place of two (0.87); the next block's first scores issued before the last of B (0.85).
 //
 // Softmax: thread = row, so nothing is exchanged.  The reference m moves only when a score exceeds it by more than 8 (in
-// powers of two); only then are the sum and the accumulator rescaled (a published way of rescaling less often).  Weights 2^(s - m + shift) go to the tensor core in
-// the inputs' type: rounded by half an ulp like the inputs themselves.  fp16: a shift of 7, so at most 2^15, and the type's
-// subnormal steps are at most 2^-31 of a row's largest weight.  bf16, whose values reach fp32's range: -16, so that the
-// sum over 2^16 keys of values near the largest stays finite (2^8 where scores have gone 8 above the reference).  Their sum and the accumulator are fp32 and have the same factor.
+// powers of two); only then are the sum and the accumulator rescaled (a published way of rescaling less often).  Weights
+// 2^(s - m + shift) go to the tensor core in the inputs' type: rounded by half an ulp like the inputs themselves.  fp16: a
+// shift of 7, so at most 2^15, and the type's subnormal steps are at most 2^-31 of a row's largest weight.  bf16, whose
+// values reach fp32's range: -16, so that the sum over 2^16 keys of values near the largest stays finite (2^8 where scores
+// have gone 8 above the reference).  Their sum and the accumulator are fp32 and have the same factor.
 //
 // Keys that a row does not see have weight 0, but 0 times a value that is not finite is not 0.  So a warp looks through
 // every V tile that some row of the block does not see all of: rows behind the block's last position become zeros,
